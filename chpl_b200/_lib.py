@@ -27,6 +27,16 @@ CHPL_OP_T = 1
 CHPL_GEN_CHPL = 0
 CHPL_GEN_PHILOX = 1
 
+CHPL_TYPE_BF16 = 0
+CHPL_TYPE_F16 = 1
+CHPL_TYPE_F32 = 2
+
+CHPL_ACT_NONE = 0
+CHPL_ACT_RELU = 1
+CHPL_ACT_GELU = 2
+CHPL_ACT_GELU_TANH = 3
+CHPL_ACT_SILU = 4
+
 _i64 = ctypes.c_int64
 _u64 = ctypes.c_uint64
 _sz = ctypes.c_size_t
@@ -47,6 +57,23 @@ class HplResult(ctypes.Structure):
     _fields_ = [("time_s", _dbl), ("tflops", _dbl), ("resid", _dbl), ("passed", _int), ("matgen_s", _dbl),
                 ("phase_s", _dbl * 8), ("n_emulated", _i64), ("n_launches", _i64), ("gemm_launches", _i64),
                 ("gemm_kernel_s", _dbl), ("gemm_int8_ops", _dbl), ("gemm_fp64eq_flops", _dbl), ("schedule", _int)]
+
+
+class Ckpt8(ctypes.Structure):
+    _fields_ = [("codes", _vp), ("scales", _vp), ("ldc", _i64), ("lds", _i64)]
+
+
+class LinearFwd(ctypes.Structure):
+    _fields_ = [("type", _int), ("act", _int), ("tokens", _i64), ("n", _i64), ("k", _i64), ("x", _vp), ("ldx", _i64),
+                ("w", _vp), ("ldw", _i64), ("bias", _vp), ("residual", _vp), ("ldr", _i64), ("y", _vp), ("ldy", _i64),
+                ("z", _vp), ("ldz", _i64), ("z8", Ckpt8)]
+
+
+class LinearBwd(ctypes.Structure):
+    _fields_ = [("type", _int), ("act", _int), ("in_act", _int), ("grad_type", _int), ("accumulate", _int),
+                ("tokens", _i64), ("n", _i64), ("k", _i64), ("dy", _vp), ("lddy", _i64), ("w", _vp), ("ldw", _i64),
+                ("x", _vp), ("ldx", _i64), ("x8", Ckpt8), ("z", _vp), ("ldz", _i64), ("z8", Ckpt8), ("add", _vp),
+                ("ldadd", _i64), ("dx", _vp), ("lddx", _i64), ("dw", _vp), ("lddw", _i64), ("db", _vp)]
 
 
 # name -> (restype, argtypes); every function declared in include/chpl.h
@@ -88,6 +115,12 @@ SIGNATURES = {
     "chpl_hpl_default_config": (None, [ctypes.POINTER(HplConfig)]),
     "chpl_hpl_run": (_int, [ctypes.POINTER(HplConfig), ctypes.POINTER(HplResult), _vp]),
     "chpl_hpl_run_host": (_int, [ctypes.POINTER(HplConfig), _vp, _sz, _int, ctypes.POINTER(HplResult), _vp]),
+    "chpl_ckpt8_pack": (_int, [_vp, _int, _i64, _i64, _vp, _i64, ctypes.POINTER(Ckpt8)]),
+    "chpl_ckpt8_unpack": (_int, [_vp, _int, _i64, _i64, ctypes.POINTER(Ckpt8), _vp, _i64]),
+    "chpl_linear_forward_worksize": (_int, [ctypes.POINTER(LinearFwd), ctypes.POINTER(_sz)]),
+    "chpl_linear_forward": (_int, [_vp, ctypes.POINTER(LinearFwd), _vp, _sz]),
+    "chpl_linear_backward_worksize": (_int, [ctypes.POINTER(LinearBwd), ctypes.POINTER(_sz)]),
+    "chpl_linear_backward": (_int, [_vp, ctypes.POINTER(LinearBwd), _vp, _sz]),
     "chpl_grid_unique_id": (_int, [_vp, _sz]),
     "chpl_grid_create": (_int, [_int, _int, _int, _vp, _sz, _dbl, ctypes.POINTER(_vp)]),
     "chpl_grid_run": (_int, [_vp, ctypes.POINTER(HplConfig), ctypes.POINTER(HplResult), _vp]),

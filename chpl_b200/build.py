@@ -27,7 +27,9 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVFLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
                   "--expt-relaxed-constexpr", "-I", INCLUDE, "-I", CSRC]
 LIB_SOURCES = ["capi.cu", "oz2.cu", "oz2_noalloc.cu", "oz1.cu", "fp64.cu", "hpl_kernels.cu", "panel.cu", "hpl_single.cu",
-               "hpl_grid.cu", "diag.cu"]
+               "hpl_grid.cu", "diag.cu", "ckpt8.cu", "linear.cu", "linear_gemm.cu"]
+
+
 def _nccl_dir() -> str:
     """NCCL bundled with torch (the same library torch.distributed loads), so
     one NCCL lives in the process; falls back to the system copy."""

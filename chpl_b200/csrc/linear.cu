@@ -1,0 +1,420 @@
+// Linear layers of a model: argument checks, workspace layout, the elementwise
+// kernels around the products, and the C entry points chpl_linear_forward /
+// chpl_linear_backward.
+//
+// Forward: one product.  Backward: G = dY * act'(Z) and its column sums (one
+// pass over dY and Z), the layer's input out of its checkpoint, then the two
+// products dX = G W and dW = G^T Xv.
+#include "linear.h"
+
+#include <algorithm>
+
+#include "linear_epilogue.cuh"
+
+namespace chpl {
+namespace linear {
+
+// ----------------------------------------------------------------------------
+// checks
+// ----------------------------------------------------------------------------
+int check_size(const char* who, const char* what, int64_t v)
+{
+    if (v < 0) { set_error("%s: %s = %lld is negative", who, what, (long long)v); return CHPL_ERR_INVALID; }
+    if (v > kMaxSize) { set_error("%s: %s = %lld exceeds %lld", who, what, (long long)v, (long long)kMaxSize); return CHPL_ERR_UNSUPPORTED; }
+    return CHPL_OK;
+}
+
+int check_operand(const char* who, const char* what, const void* p, int64_t ld, int64_t width, int elt)
+{
+    if (!p) { set_error("%s: %s is NULL", who, what); return CHPL_ERR_INVALID; }
+    if (reinterpret_cast<uintptr_t>(p) % elt) { set_error("%s: %s is not aligned to its elements", who, what); return CHPL_ERR_INVALID; }
+    if (ld < width) { set_error("%s: row distance of %s is %lld, below its %lld columns", who, what, (long long)ld, (long long)width); return CHPL_ERR_INVALID; }
+    if (ld > kMaxLd) { set_error("%s: row distance of %s is %lld, above %lld", who, what, (long long)ld, (long long)kMaxLd); return CHPL_ERR_UNSUPPORTED; }
+    return CHPL_OK;
+}
+
+int check_ckpt(const char* who, const char* what, const chpl_ckpt8& c, int64_t width)
+{
+    CHPL_TRY(check_operand(who, what, c.codes, c.ldc, width, 1));
+    return check_operand(who, "its scales", c.scales, c.lds, (width + kCkptGroup - 1) / kCkptGroup, 1);
+}
+
+static int check_type(const char* who, int type)
+{
+    if (type == CHPL_TYPE_BF16 || type == CHPL_TYPE_F16) return CHPL_OK;
+    set_error("%s: type %d is not BF16 or F16", who, type);
+    return CHPL_ERR_INVALID;
+}
+
+static int check_act(const char* who, int act)
+{
+    if (act >= CHPL_ACT_NONE && act <= CHPL_ACT_SILU) return CHPL_OK;
+    set_error("%s: unknown activation %d", who, act);
+    return CHPL_ERR_INVALID;
+}
+
+static int check_work(const char* who, const void* work, size_t have, size_t need)
+{
+    if (have < need || (need && !work)) { set_error("%s: workspace of %zu bytes, %zu are needed", who, work ? have : (size_t)0, need); return CHPL_ERR_WORKSPACE; }
+    if (need && reinterpret_cast<uintptr_t>(work) % 256) { set_error("%s: workspace is not 256-byte aligned", who); return CHPL_ERR_INVALID; }
+    return CHPL_OK;
+}
+
+unsigned grid_for(int64_t items, int64_t per_block)
+{
+    const int64_t want = (items + per_block - 1) / per_block;
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(want, 148 * 16));
+}
+
+// ----------------------------------------------------------------------------
+// elementwise kernels
+// ----------------------------------------------------------------------------
+constexpr int kEltThreads = 256;
+
+// rows x cols, out = act(in), in 16-bit or a checkpoint: rows that TMA can read
+template <typename T, bool CKPT>
+__global__ void __launch_bounds__(kEltThreads) expand_kernel(const T* __restrict__ x, int64_t ldx, chpl_ckpt8 c, int act,
+                                                             int64_t rows, int cols, T* __restrict__ out, int64_t ldo)
+{
+    const int64_t total = rows * cols, step = (int64_t)gridDim.x * kEltThreads;
+    for (int64_t i = (int64_t)blockIdx.x * kEltThreads + threadIdx.x; i < total; i += step) {
+        const int64_t t = i / cols;
+        const int j = (int)(i - t * cols);
+        if (!CKPT && act == CHPL_ACT_NONE) {  // a plain copy keeps every bit
+            out[t * ldo + j] = x[t * ldx + j];
+            continue;
+        }
+        float v = CKPT ? (float)c.codes[t * c.ldc + j] * ckpt_step(c.scales[t * c.lds + j / kCkptGroup])
+                       : to_f32(x[t * ldx + j]);
+        with_act(act, [&](auto tag) { v = activate<decltype(tag)::value>(v); });
+        out[t * ldo + j] = from_f32<T>(v);
+    }
+}
+
+// G = dY * act'(Z) into g (where given), and the sums of its columns over each
+// chunk of kSumRows rows into part[chunk][n]
+constexpr int kSumRows = 64;
+
+template <typename T, bool CKPT>
+__global__ void __launch_bounds__(kEltThreads) grad_act_kernel(const T* __restrict__ dy, int64_t lddy,
+                                                               const T* __restrict__ z, int64_t ldz, chpl_ckpt8 z8,
+                                                               int act, int rows, int n, T* __restrict__ g, int64_t ldg,
+                                                               float* __restrict__ part)
+{
+    const int j = blockIdx.x * kEltThreads + threadIdx.x;
+    if (j >= n) return;
+    const int chunks = (rows + kSumRows - 1) / kSumRows;
+    for (int ch = blockIdx.y; ch < chunks; ch += gridDim.y) {
+        float sum = 0.0f;
+        const int end = min(rows, (ch + 1) * kSumRows);
+        for (int t = ch * kSumRows; t < end; ++t) {
+            float v = to_f32(dy[t * lddy + j]);
+            if (act != CHPL_ACT_NONE) {
+                const float zv = CKPT ? (float)z8.codes[t * z8.ldc + j] * ckpt_step(z8.scales[t * z8.lds + j / kCkptGroup])
+                                      : to_f32(z[t * ldz + j]);
+                with_act(act, [&](auto tag) {
+                    float slope, value;
+                    slope_and_value<decltype(tag)::value>(zv, slope, value);
+                    v *= slope;
+                });
+            }
+            if (g) g[t * ldg + j] = from_f32<T>(v);
+            sum += v;
+        }
+        if (part) part[(int64_t)ch * n + j] = sum;
+    }
+}
+
+// db[j] (+)= sum of part[0..chunks)[j], in order
+template <typename T>
+__global__ void __launch_bounds__(kEltThreads) sum_chunks_kernel(const float* __restrict__ part, int chunks, int n,
+                                                                 T* __restrict__ db, int accumulate)
+{
+    const int j = blockIdx.x * kEltThreads + threadIdx.x;
+    if (j >= n) return;
+    float sum = 0.0f;
+    for (int ch = 0; ch < chunks; ++ch) sum += part[(int64_t)ch * n + j];
+    db[j] = from_f32<T>(accumulate ? to_f32(db[j]) + sum : sum);
+}
+
+// ----------------------------------------------------------------------------
+// layout
+// ----------------------------------------------------------------------------
+// TMA reads rows whose base and distance are multiples of 16 bytes; a single
+// row has no distance
+static bool tma_rows(const void* p, int64_t ld, int64_t rows)
+{
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || ld % 8 == 0);
+}
+
+static int64_t padded(int64_t width) { return (int64_t)round_up((size_t)width, 8); }
+
+struct Arena {
+    size_t used = 0;
+    size_t take(size_t bytes)
+    {
+        const size_t at = used;
+        used += round_up(bytes, 256);
+        return at;
+    }
+};
+
+// A 16-bit matrix as a product reads it: in place, or at `at` in the workspace
+struct Staged {
+    bool copy = false;
+    size_t at = 0;
+    int64_t ld = 0;
+};
+
+static Staged stage(Arena& a, bool copy, int64_t ld, int64_t rows, int64_t cols)
+{
+    Staged s;
+    s.copy = copy;
+    s.ld = copy || rows <= 1 ? padded(cols) : ld;
+    if (copy) s.at = a.take((size_t)rows * s.ld * 2);
+    return s;
+}
+
+static const void* at(const Staged& s, const void* in_place, void* work)
+{
+    return s.copy ? static_cast<char*>(work) + s.at : in_place;
+}
+
+struct ForwardPlan {
+    Staged x, w;
+    size_t bytes;
+};
+
+static ForwardPlan plan(const chpl_linear_fwd& a)
+{
+    Arena m;
+    ForwardPlan p;
+    const bool any = a.tokens > 0 && a.n > 0 && a.k > 0;
+    p.x = stage(m, any && !tma_rows(a.x, a.ldx, a.tokens), a.ldx, a.tokens, a.k);
+    p.w = stage(m, any && !tma_rows(a.w, a.ldw, a.n), a.ldw, a.n, a.k);
+    p.bytes = m.used;
+    return p;
+}
+
+struct BackwardPlan {
+    Staged g, w, x;
+    bool need_xv;   // Xv is not X as it stands
+    size_t part;
+    int chunks;
+    size_t bytes;
+};
+
+static BackwardPlan plan(const chpl_linear_bwd& a)
+{
+    Arena m;
+    BackwardPlan p;
+    const bool any = a.tokens > 0 && a.n > 0;
+    const bool products = any && (a.dx || a.dw) && a.k > 0;
+    p.g = stage(m, products && (a.act != CHPL_ACT_NONE || !tma_rows(a.dy, a.lddy, a.tokens)), a.lddy, a.tokens, a.n);
+    p.w = stage(m, products && a.dx && !tma_rows(a.w, a.ldw, a.n), a.ldw, a.n, a.k);
+    p.need_xv = a.x8.codes || a.in_act != CHPL_ACT_NONE || !tma_rows(a.x, a.ldx, a.tokens);
+    p.x = stage(m, products && a.dw && p.need_xv, a.ldx, a.tokens, a.k);
+    p.chunks = (int)((a.tokens + kSumRows - 1) / kSumRows);
+    p.part = a.db && a.n > 0 ? m.take((size_t)p.chunks * a.n * 4) : 0;
+    p.bytes = m.used;
+    return p;
+}
+
+static int check(const char* who, const chpl_linear_fwd* a, bool pointers)
+{
+    if (!a) { set_error("%s: arguments are NULL", who); return CHPL_ERR_INVALID; }
+    CHPL_TRY(check_type(who, a->type));
+    CHPL_TRY(check_act(who, a->act));
+    CHPL_TRY(check_size(who, "tokens", a->tokens));
+    CHPL_TRY(check_size(who, "n", a->n));
+    CHPL_TRY(check_size(who, "k", a->k));
+    if (!pointers || a->tokens == 0 || a->n == 0) return CHPL_OK;
+    if (a->k > 0) {
+        CHPL_TRY(check_operand(who, "x", a->x, a->ldx, a->k, 2));
+        CHPL_TRY(check_operand(who, "w", a->w, a->ldw, a->k, 2));
+    }
+    CHPL_TRY(check_operand(who, "y", a->y, a->ldy, a->n, 2));
+    if (a->bias) CHPL_TRY(check_operand(who, "bias", a->bias, a->n, a->n, 2));
+    if (a->residual) CHPL_TRY(check_operand(who, "residual", a->residual, a->ldr, a->n, 2));
+    if (a->z) CHPL_TRY(check_operand(who, "z", a->z, a->ldz, a->n, 2));
+    if (a->z8.codes) CHPL_TRY(check_ckpt(who, "z8", a->z8, a->n));
+    if (a->y == a->residual && a->ldy != a->ldr) { set_error("%s: y is residual with another row distance", who); return CHPL_ERR_INVALID; }
+    return CHPL_OK;
+}
+
+static int check(const char* who, const chpl_linear_bwd* a, bool pointers)
+{
+    if (!a) { set_error("%s: arguments are NULL", who); return CHPL_ERR_INVALID; }
+    CHPL_TRY(check_type(who, a->type));
+    CHPL_TRY(check_act(who, a->act));
+    CHPL_TRY(check_act(who, a->in_act));
+    if (a->grad_type != a->type && a->grad_type != CHPL_TYPE_F32) {
+        set_error("%s: grad_type %d is neither the operands' type nor F32", who, a->grad_type);
+        return CHPL_ERR_INVALID;
+    }
+    CHPL_TRY(check_size(who, "tokens", a->tokens));
+    CHPL_TRY(check_size(who, "n", a->n));
+    CHPL_TRY(check_size(who, "k", a->k));
+    if (!pointers) return CHPL_OK;
+    const int ge = a->grad_type == CHPL_TYPE_F32 ? 4 : 2;
+    if (a->dx && a->tokens > 0 && a->k > 0) {
+        CHPL_TRY(check_operand(who, "dx", a->dx, a->lddx, a->k, 2));
+        if (a->n > 0) CHPL_TRY(check_operand(who, "w", a->w, a->ldw, a->k, 2));
+        if (a->add) CHPL_TRY(check_operand(who, "add", a->add, a->ldadd, a->k, 2));
+        if (a->dx == a->add && a->lddx != a->ldadd) { set_error("%s: dx is add with another row distance", who); return CHPL_ERR_INVALID; }
+    }
+    if (a->dw && a->n > 0 && a->k > 0) CHPL_TRY(check_operand(who, "dw", a->dw, a->lddw, a->k, ge));
+    if (a->db && a->n > 0) CHPL_TRY(check_operand(who, "db", a->db, a->n, a->n, ge));
+    const bool any = a->tokens > 0 && a->n > 0 && (a->dx || a->dw || a->db);
+    if (any) {
+        CHPL_TRY(check_operand(who, "dy", a->dy, a->lddy, a->n, 2));
+        if (a->act != CHPL_ACT_NONE) {
+            if (a->z8.codes) CHPL_TRY(check_ckpt(who, "z8", a->z8, a->n));
+            else CHPL_TRY(check_operand(who, "z", a->z, a->ldz, a->n, 2));
+        }
+    }
+    if (a->tokens > 0 && a->k > 0 && (a->dw ? a->n > 0 : a->dx && a->in_act != CHPL_ACT_NONE)) {
+        if (a->x8.codes) CHPL_TRY(check_ckpt(who, "x8", a->x8, a->k));
+        else CHPL_TRY(check_operand(who, "x", a->x, a->ldx, a->k, 2));
+    }
+    return CHPL_OK;
+}
+
+// ----------------------------------------------------------------------------
+// the two passes
+// ----------------------------------------------------------------------------
+template <typename T>
+static int expand(cudaStream_t st, const void* x, int64_t ldx, const chpl_ckpt8& c, int act, int64_t rows, int64_t cols,
+                  void* out, int64_t ldo)
+{
+    const unsigned grid = grid_for(rows * cols, kEltThreads);
+    if (c.codes)
+        expand_kernel<T, true><<<grid, kEltThreads, 0, st>>>(nullptr, 0, c, act, rows, (int)cols, static_cast<T*>(out), ldo);
+    else
+        expand_kernel<T, false><<<grid, kEltThreads, 0, st>>>(static_cast<const T*>(x), ldx, c, act, rows, (int)cols,
+                                                              static_cast<T*>(out), ldo);
+    CHPL_CUDA(cudaGetLastError());
+    return CHPL_OK;
+}
+
+static const chpl_ckpt8 kNoCkpt = {nullptr, nullptr, 0, 0};
+
+template <typename T>
+static int forward(cudaStream_t st, const chpl_linear_fwd& a, void* work)
+{
+    const ForwardPlan p = plan(a);
+    if (p.x.copy) CHPL_TRY(expand<T>(st, a.x, a.ldx, kNoCkpt, CHPL_ACT_NONE, a.tokens, a.k, static_cast<char*>(work) + p.x.at, p.x.ld));
+    if (p.w.copy) CHPL_TRY(expand<T>(st, a.w, a.ldw, kNoCkpt, CHPL_ACT_NONE, a.n, a.k, static_cast<char*>(work) + p.w.at, p.w.ld));
+    Epilogue e = {};
+    e.m = (int)a.n;
+    e.n = (int)a.tokens;
+    e.act = a.act;
+    e.out = a.y;
+    e.ldo = a.ldy;
+    e.bias = a.bias;
+    e.add = a.residual;
+    e.ldadd = a.ldr;
+    e.z = a.z;
+    e.ldz = a.ldz;
+    e.z8 = a.z8;
+    return gemm(st, a.type, kForward, {at(p.w, a.w, work), p.w.ld, true}, {at(p.x, a.x, work), p.x.ld, true}, a.k, e);
+}
+
+template <typename T>
+static int backward(cudaStream_t st, const chpl_linear_bwd& a, void* work)
+{
+    const BackwardPlan p = plan(a);
+    char* wk = static_cast<char*>(work);
+    if (a.n > 0 && (p.g.copy || a.db)) {
+        float* part = a.db ? reinterpret_cast<float*>(wk + p.part) : nullptr;
+        T* g = p.g.copy ? reinterpret_cast<T*>(wk + p.g.at) : nullptr;
+        if (a.tokens > 0) {
+            const dim3 grid((unsigned)((a.n + kEltThreads - 1) / kEltThreads), (unsigned)std::min(p.chunks, 65535));
+            if (a.z8.codes)
+                grad_act_kernel<T, true><<<grid, kEltThreads, 0, st>>>(static_cast<const T*>(a.dy), a.lddy, nullptr, 0, a.z8,
+                                                                       a.act, (int)a.tokens, (int)a.n, g, p.g.ld, part);
+            else
+                grad_act_kernel<T, false><<<grid, kEltThreads, 0, st>>>(static_cast<const T*>(a.dy), a.lddy,
+                                                                        static_cast<const T*>(a.z), a.ldz, a.z8, a.act,
+                                                                        (int)a.tokens, (int)a.n, g, p.g.ld, part);
+            CHPL_CUDA(cudaGetLastError());
+        }
+        if (a.db) {
+            const unsigned blocks = (unsigned)((a.n + kEltThreads - 1) / kEltThreads);
+            if (a.grad_type == CHPL_TYPE_F32)
+                sum_chunks_kernel<float><<<blocks, kEltThreads, 0, st>>>(part, p.chunks, (int)a.n, static_cast<float*>(a.db), a.accumulate);
+            else
+                sum_chunks_kernel<T><<<blocks, kEltThreads, 0, st>>>(part, p.chunks, (int)a.n, static_cast<T*>(a.db), a.accumulate);
+            CHPL_CUDA(cudaGetLastError());
+        }
+    }
+    if (a.k == 0) return CHPL_OK;
+    const Operand g_rows = {at(p.g, a.dy, work), p.g.ld, true}, g_cols = {g_rows.p, p.g.ld, false};
+    if (p.x.copy) CHPL_TRY(expand<T>(st, a.x, a.ldx, a.x8, a.in_act, a.tokens, a.k, wk + p.x.at, p.x.ld));
+    if (a.dx) {
+        if (p.w.copy) CHPL_TRY(expand<T>(st, a.w, a.ldw, kNoCkpt, CHPL_ACT_NONE, a.n, a.k, wk + p.w.at, p.w.ld));
+        Epilogue e = {};
+        e.m = (int)a.k;
+        e.n = (int)a.tokens;
+        e.act = a.in_act;
+        e.out = a.dx;
+        e.ldo = a.lddx;
+        e.add = a.add;
+        e.ldadd = a.ldadd;
+        e.z = const_cast<void*>(a.x);
+        e.ldz = a.ldx;
+        e.z8 = a.x8;
+        CHPL_TRY(gemm(st, a.type, kGradInput, {at(p.w, a.w, work), p.w.ld, false}, g_rows, a.n, e));
+    }
+    if (a.dw && (a.tokens > 0 || !a.accumulate)) {
+        Epilogue e = {};
+        e.m = (int)a.k;
+        e.n = (int)a.n;
+        e.out_f32 = a.grad_type == CHPL_TYPE_F32;
+        e.accumulate = a.accumulate;
+        e.out = a.dw;
+        e.ldo = a.lddw;
+        CHPL_TRY(gemm(st, a.type, kGradWeight, {at(p.x, a.x, work), p.x.ld, false}, g_cols, a.tokens, e));
+    }
+    return CHPL_OK;
+}
+
+}  // namespace linear
+}  // namespace chpl
+
+extern "C" int chpl_linear_forward_worksize(const chpl_linear_fwd* a, size_t* work_bytes)
+{
+    using namespace chpl::linear;
+    CHPL_TRY(check("linear_forward_worksize", a, false));
+    if (!work_bytes) { chpl::set_error("linear_forward_worksize: work_bytes is NULL"); return CHPL_ERR_INVALID; }
+    *work_bytes = plan(*a).bytes;
+    return CHPL_OK;
+}
+
+extern "C" int chpl_linear_forward(void* stream, const chpl_linear_fwd* a, void* work, size_t work_bytes)
+{
+    using namespace chpl::linear;
+    CHPL_TRY(check("linear_forward", a, true));
+    if (a->tokens == 0 || a->n == 0) return CHPL_OK;
+    CHPL_TRY(check_work("linear_forward", work, work_bytes, plan(*a).bytes));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return a->type == CHPL_TYPE_BF16 ? forward<__nv_bfloat16>(st, *a, work) : forward<__half>(st, *a, work);
+}
+
+extern "C" int chpl_linear_backward_worksize(const chpl_linear_bwd* a, size_t* work_bytes)
+{
+    using namespace chpl::linear;
+    CHPL_TRY(check("linear_backward_worksize", a, false));
+    if (!work_bytes) { chpl::set_error("linear_backward_worksize: work_bytes is NULL"); return CHPL_ERR_INVALID; }
+    *work_bytes = plan(*a).bytes;
+    return CHPL_OK;
+}
+
+extern "C" int chpl_linear_backward(void* stream, const chpl_linear_bwd* a, void* work, size_t work_bytes)
+{
+    using namespace chpl::linear;
+    CHPL_TRY(check("linear_backward", a, true));
+    CHPL_TRY(check_work("linear_backward", work, work_bytes, plan(*a).bytes));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return a->type == CHPL_TYPE_BF16 ? backward<__nv_bfloat16>(st, *a, work) : backward<__half>(st, *a, work);
+}

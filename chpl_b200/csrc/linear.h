@@ -1,0 +1,64 @@
+// Internal interface of the linear-layer module (linear.cu, linear_gemm.cu, ckpt8.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "chpl.h"
+
+namespace chpl {
+namespace linear {
+
+// Sizes fit the kernels' int32 coordinates with room for a tile; row distances
+// are below TMA's 2^40 bytes and keep every 64-bit offset in range.
+constexpr int64_t kMaxSize = (int64_t)1 << 30;
+constexpr int64_t kMaxLd = (int64_t)1 << 32;
+
+// what a product's epilogue does with the accumulators D[f][t] (f: the output's
+// contiguous dimension, t: its row)
+enum Kind {
+    kForward = 0,     // Y[t][f] = act(D + bias[f]) + add[t][f]; z / z8 keep D + bias
+    kGradInput = 1,   // dX[t][f] = D * act'(z[t][f]) + add[t][f]; z comes in 16 bits or as z8; xv keeps act(z)
+    kGradWeight = 2,  // dW[t][f] (+)= D
+};
+
+struct Epilogue {
+    int m, n;        // f < m, t < n
+    int act;
+    int out_f32;     // out is FP32 (kGradWeight), else of the operands' type
+    int accumulate;  // out += (kGradWeight)
+    void* out;
+    int64_t ldo;
+    const void* bias;
+    const void* add;
+    int64_t ldadd;
+    void* z;         // 16-bit z: written by kForward, read by kGradInput
+    int64_t ldz;
+    chpl_ckpt8 z8;   // 8-bit z: written by kForward, read by kGradInput
+    void* xv;        // kGradInput: act(z), of the operands' type
+    int64_t ldxv;
+};
+
+// One operand of a product over c: element (i, c) at p[i * ld + c] when
+// k_major, else at p[c * ld + i].  16-bit, base and rows on 16-byte boundaries.
+struct Operand {
+    const void* p;
+    int64_t ld;
+    bool k_major;
+};
+
+// D[f][t] = sum_{c < k} A(f, c) B(t, c), handed to the epilogue; type BF16 or F16
+int gemm(cudaStream_t st, int type, Kind kind, const Operand& a, const Operand& b, int64_t k, const Epilogue& e);
+
+int check_size(const char* who, const char* what, int64_t v);
+int check_operand(const char* who, const char* what, const void* p, int64_t ld, int64_t width, int elt);
+int check_ckpt(const char* who, const char* what, const chpl_ckpt8& c, int64_t width);
+
+// blocks for `items` units of work at `per_block` each: enough to fill the GPU several times over
+unsigned grid_for(int64_t items, int64_t per_block);
+
+int read_clear_status(int* st);
+
+}  // namespace linear
+}  // namespace chpl

@@ -1,0 +1,67 @@
+"""A model's feed-forward block, Y = act(X W1^T + b1) W2^T + b2 [+ X], trained from 8-bit checkpoints.
+
+Between the passes the block holds X and the pre-activation Z in 8 bits (2.06 bytes per token for each pair of an input
+and a hidden feature, where X, Z and act(Z) in 16 bits hold 6): the forward products code Z in their epilogue, and the
+backward ones take act(Z), act'(Z) and X from the codes.  The gradients are those of the block at the checkpointed X and Z.
+
+    y, saved = ffn.forward(x, w1, b1, w2, b2, act="gelu", residual=True, save=True)
+    dx, dw1, db1, dw2, db2 = ffn.backward(dy, saved, w1, w2)
+
+``block`` wraps the two for torch's autograd.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import ckpt8, linear
+
+
+class Saved(NamedTuple):
+    x: ckpt8.Ckpt8
+    z: ckpt8.Ckpt8
+    act: str
+    residual: bool
+
+
+def forward(x, w1, b1, w2, b2, *, act: str = "gelu", residual: bool = False, save: bool = False, stream=None):
+    """Y, or with save=True (Y, what backward needs).  b1 and b2 may be None."""
+    if not save:
+        h = linear.forward(x, w1, b1, act=act, stream=stream)
+        return linear.forward(h, w2, b2, residual=x if residual else None, stream=stream)
+    x8 = ckpt8.pack(x, stream=stream)
+    h, z8 = linear.forward(x, w1, b1, act=act, save="z8", stream=stream)
+    y = linear.forward(h, w2, b2, residual=x if residual else None, stream=stream)
+    return y, Saved(x8, z8, act, residual)
+
+
+def backward(dy, saved: Saved, w1, w2, *, need_dx: bool = True, need_db: bool = True, grad_dtype=None, stream=None):
+    """(dx, dw1, db1, dw2, db2) of the block from dy; with need_db=False db1 and db2 are None."""
+    dz, dw2, db2 = linear.backward(dy, saved.z, w2, in_act=saved.act, need_db=need_db, grad_dtype=grad_dtype, stream=stream)
+    dx, dw1, db1 = linear.backward(dz, saved.x, w1, add=dy if saved.residual else None, need_dx=need_dx, need_db=need_db,
+                                   grad_dtype=grad_dtype, stream=stream)
+    return dx, dw1, db1, dw2, db2
+
+
+class _Block(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w1, b1, w2, b2, act, residual):
+        y, s = forward(x, w1, b1, w2, b2, act=act, residual=residual, save=True)
+        ctx.save_for_backward(s.x.codes, s.x.scales, s.z.codes, s.z.scales, w1, w2)
+        ctx.how = (x.dtype, act, residual, b1 is not None, b2 is not None)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        xc, xs, zc, zs, w1, w2 = ctx.saved_tensors
+        dt, act, residual, has1, has2 = ctx.how
+        s = Saved(ckpt8.Ckpt8(xc, xs, dt), ckpt8.Ckpt8(zc, zs, dt), act, residual)
+        dx, dw1, db1, dw2, db2 = backward(dy.contiguous(), s, w1, w2, need_dx=ctx.needs_input_grad[0],
+                                          need_db=has1 or has2)
+        return dx, dw1, db1 if has1 else None, dw2, db2 if has2 else None, None, None
+
+
+def block(x, w1, b1, w2, b2, act: str = "gelu", residual: bool = False):
+    """The block as a function that torch's autograd differentiates through."""
+    return _Block.apply(x, w1, b1, w2, b2, act, residual)

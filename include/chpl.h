@@ -349,6 +349,119 @@ int chpl_hpl_run_host(const chpl_hpl_config *cfg, const double *Ab, size_t ldab,
                       chpl_hpl_result *res, double *x_out);
 
 /* ------------------------------------------------------------------------ */
+/* Linear layers of a model: 16-bit products with their epilogue, their      */
+/* gradients, and 8-bit activation checkpoints                               */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Matrices here are ROW-major (a row is a token, or an output feature of a
+ * weight), ld* is the distance between rows in elements, and any alignment
+ * down to the element's size is served (rows that TMA cannot read, i.e. a base
+ * or row distance that is no multiple of 16 bytes, are copied into `work`
+ * first).  The calls allocate nothing, synchronize nothing and can be captured
+ * in a CUDA graph.  Results do not vary from run to run.  Sums are FP32;
+ * products run on the tensor cores from 16-bit operands.  A device-side wait
+ * that runs out of time leaves the outputs undefined while the call itself has
+ * returned CHPL_OK: check chpl_device_status after synchronizing.
+ * The reference has no counterpart to any of these.
+ */
+
+/* element types */
+#define CHPL_TYPE_BF16 0
+#define CHPL_TYPE_F16 1
+#define CHPL_TYPE_F32 2
+/* activations */
+#define CHPL_ACT_NONE 0
+#define CHPL_ACT_RELU 1
+#define CHPL_ACT_GELU 2      /* z Phi(z), by erf */
+#define CHPL_ACT_GELU_TANH 3 /* its tanh form, z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+#define CHPL_ACT_SILU 4      /* z / (1 + exp(-z)) */
+
+/*
+ * An 8-bit checkpoint of a row-major matrix (rows x cols).  The 32 consecutive
+ * features 32g..32g+31 of row t share the power-of-two step 2^(s - 133) with
+ * s = scales[t * lds + g], and feature j is codes[t * ldc + j] * step.  s is
+ * the exponent field (FP32, biased by 127) of the group's largest magnitude,
+ * at least 7; code = x / step rounded to nearest, ties to even, clamped to
+ * +-127 (a largest magnitude in the topmost 1/256 of its binade is clamped by
+ * at most one step).  These are the elements (INT8 with 2^-6) and scales
+ * (E8M0) of the OCP Microscaling MXINT8 format, block size 32.  A group that
+ * holds an infinity or a NaN has s = 255 and codes 0, and reads back as NaN.
+ * Codes have 7 bits, so a code times its step is exact in bf16 and (inside
+ * FP16's normal range) in f16.  ldc >= cols, lds >= ceil(cols / 32); codes ==
+ * NULL: no checkpoint.
+ */
+typedef struct chpl_ckpt8 {
+    int8_t *codes;
+    uint8_t *scales;
+    int64_t ldc, lds;
+} chpl_ckpt8;
+
+/* x (rows x cols, `type` BF16, F16 or F32) -> checkpoint */
+int chpl_ckpt8_pack(void *stream, int type, int64_t rows, int64_t cols, const void *x, int64_t ldx,
+                    const chpl_ckpt8 *c);
+/* checkpoint -> x of any of the three types (rounded once, to nearest) */
+int chpl_ckpt8_unpack(void *stream, int type, int64_t rows, int64_t cols, const chpl_ckpt8 *c, void *x,
+                      int64_t ldx);
+
+/*
+ * Y = act(Z) + R,  Z = X W^T + b.  X is tokens x k, W n x k, Y, R and Z
+ * tokens x n, b n; all of `type` (BF16 or F16).  b and R may be NULL.  Z is
+ * kept for the backward pass where z (16 bits) or z8.codes (8 bits, coded from
+ * the FP32 value) is given.  Y may be R (same pointer and ld); no other output
+ * may overlap an input.  k = 0 gives act(b) + R.
+ */
+typedef struct chpl_linear_fwd {
+    int type, act;
+    int64_t tokens, n, k;
+    const void *x; int64_t ldx;
+    const void *w; int64_t ldw;
+    const void *bias;
+    const void *residual; int64_t ldr;
+    void *y; int64_t ldy;
+    void *z; int64_t ldz;
+    chpl_ckpt8 z8;
+} chpl_linear_fwd;
+
+/* bytes of `work` that chpl_linear_forward needs with these arguments (pointers and lds count by their
+ * alignment only); 0 when every row is 16-byte aligned */
+int chpl_linear_forward_worksize(const chpl_linear_fwd *a, size_t *work_bytes);
+/* `work`: 256-byte aligned device memory of work_bytes bytes, or NULL when none is needed */
+int chpl_linear_forward(void *stream, const chpl_linear_fwd *a, void *work, size_t work_bytes);
+
+/*
+ * Gradients of that layer.  With G = dY * act'(Z) (G = dY for CHPL_ACT_NONE):
+ *   dX = G W [* in_act'(Xz)] [+ add],   dW = G^T Xv,   db = sum over tokens of G.
+ * Z comes in 16 bits (z) or as a checkpoint (z8); X likewise (x or x8).
+ * in_act == CHPL_ACT_NONE: Xv is X.  Otherwise X is the pre-activation Xz that
+ * the layer's input came from, Xv = in_act(Xz) is recomputed, and dX is the
+ * gradient of Xz: the activation between two layers costs no pass of its own.
+ * dx, dw and db may each be NULL (not computed; X is needed for dW and, with
+ * in_act, for dX).  dX, G and Xv are of `type` (G and Xv are rounded to it to
+ * feed the tensor cores; db is summed from the unrounded G).  dW (n x k) and
+ * db (n) are of grad_type: `type`, or CHPL_TYPE_F32; accumulate != 0 adds
+ * to what they hold.  dX may be add (same pointer and ld); no other output may
+ * overlap an input.  tokens = 0 gives dW = 0, db = 0 (unchanged if accumulating).
+ */
+typedef struct chpl_linear_bwd {
+    int type, act, in_act, grad_type, accumulate;
+    int64_t tokens, n, k;
+    const void *dy; int64_t lddy;
+    const void *w; int64_t ldw;
+    const void *x; int64_t ldx;
+    chpl_ckpt8 x8;
+    const void *z; int64_t ldz;
+    chpl_ckpt8 z8;
+    const void *add; int64_t ldadd;
+    void *dx; int64_t lddx;
+    void *dw; int64_t lddw;
+    void *db;
+} chpl_linear_bwd;
+
+int chpl_linear_backward_worksize(const chpl_linear_bwd *a, size_t *work_bytes);
+int chpl_linear_backward(void *stream, const chpl_linear_bwd *a, void *work, size_t work_bytes);
+
+/* ------------------------------------------------------------------------ */
 /* P x Q process grid (one process per GPU, NCCL over NVLink)                */
 /* ------------------------------------------------------------------------ */
 
