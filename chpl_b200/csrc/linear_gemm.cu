@@ -1,8 +1,28 @@
-// The linear-layer products: D[f][t] = sum_c A(f, c) B(t, c) with the
-// epilogue of linear_epilogue.cuh.
+// The linear-layer products on the tensor cores: D[f][t] = sum_c A(f, c) B(t, c)
+// with the epilogue of linear_epilogue.cuh.
 //
-// Every product is oriented so that the output's contiguous dimension is f,
-// the dimension that a warp's lanes run along when they store.
+// Every product is oriented so that the output's contiguous dimension f (the
+// features) lies along the 128 TMEM lanes: a warp's lanes hold consecutive
+// features of one row t, so its stores and the reads of a residual or a
+// pre-activation are coalesced row by row, a checkpoint group is one warp, and
+// a few tokens fill a narrow tile (t is the MMA's N dimension, 16 to 256)
+// instead of a fraction of a 128-row one.
+//
+//   forward      A = W (c contiguous)      B = X (c contiguous)
+//   grad input   A = W^T (f contiguous)    B = G (c contiguous)
+//   grad weight  A = Xv^T (f contiguous)   B = G^T (t contiguous)
+//
+// Operands whose contiguous dimension is c are K-major for tcgen05.mma, the
+// others MN-major; both come by TMA as 128-byte swizzled boxes 64 elements
+// wide, zero beyond the matrix, so no size needs padding.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+#include <type_traits>
+
 #include "linear_epilogue.cuh"
 
 namespace chpl {
@@ -10,53 +30,335 @@ namespace linear {
 
 __device__ int g_status;  // sticky device-side error of this module
 
-constexpr int TF = 128, TT = 32, TC = 32;
+constexpr int BM = 128;               // features of a tile (TMEM lanes)
+constexpr int BK = 64;                // contraction elements of a stage: 128 bytes
+constexpr int UK = 16;                // contraction elements of one MMA
+constexpr int A_BYTES = BM * BK * 2;  // one stage of A
+constexpr int BOX_BYTES = 64 * BK * 2;  // a 64-wide MN-major box
+constexpr int MAX_STAGES = 12;
+constexpr int SMEM_LIMIT = 227 * 1024;
 
-// FP32 multiply-adds from shared memory: a thread per feature, 32 rows each
-template <typename T, Kind KIND>
-__global__ void __launch_bounds__(TF) simple_kernel(const T* __restrict__ A, int64_t lda, bool akm,
-                                                    const T* __restrict__ B, int64_t ldb, bool bkm, int k, Epilogue e)
+// ----------------------------------------------------------------------------
+// tcgen05 kind::f16 (bf16 / f16 operands, FP32 accumulators)
+// ----------------------------------------------------------------------------
+// Shared-memory matrix descriptor, 128-byte swizzle.  K-major: rows of 128
+// bytes, 8-row groups 1024 bytes apart (stride offset; the leading offset is
+// not used).  MN-major: 64 elements of M or N per 128-byte row, c down the
+// rows in groups of 8 that are 1024 bytes apart (stride offset), the next 64
+// of M or N one box further (leading offset).
+__device__ __forceinline__ uint64_t umma_desc(uint32_t addr, bool k_major)
 {
-    __shared__ float sa[TC][TF + 1];
-    __shared__ float sb[TC][TT + 4];
-    const int f0 = blockIdx.x * TF, t0 = blockIdx.y * TT, tid = threadIdx.x;
-    float acc[TT];
+    uint64_t d = 0;
+    d |= (uint64_t)((addr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(k_major ? 1u : BOX_BYTES >> 4) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
+}
+
+// bytes from one MMA's 16 contraction elements to the next inside a stage
+__device__ __forceinline__ uint32_t umma_step(bool k_major) { return k_major ? UK * 2 : UK * 128; }
+
+__host__ __device__ constexpr uint32_t idesc_f16(bool bf16, bool a_k_major, bool b_k_major, int M, int N)
+{
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_k_major ? 0u : 1u) << 15) |
+           ((b_k_major ? 0u : 1u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, float (&v)[16])
+{
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    tmem_wait_ld();
 #pragma unroll
-    for (int j = 0; j < TT; ++j) acc[j] = 0.0f;
-    for (int c0 = 0; c0 < k; c0 += TC) {
-        for (int i = tid; i < TF * TC; i += TF) {
-            const int c = akm ? i % TC : i / TF, f = akm ? i / TC : i % TF;
-            const bool in = f0 + f < e.m && c0 + c < k;
-            sa[c][f] = in ? to_f32(akm ? A[(int64_t)(f0 + f) * lda + c0 + c] : A[(int64_t)(c0 + c) * lda + f0 + f]) : 0.0f;
-        }
-        for (int i = tid; i < TT * TC; i += TF) {
-            const int c = bkm ? i % TC : i / TT, t = bkm ? i / TC : i % TT;
-            const bool in = t0 + t < e.n && c0 + c < k;
-            sb[c][t] = in ? to_f32(bkm ? B[(int64_t)(t0 + t) * ldb + c0 + c] : B[(int64_t)(c0 + c) * ldb + t0 + t]) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll 4
-        for (int c = 0; c < TC; ++c) {
-            const float a = sa[c][tid];
-#pragma unroll
-            for (int j = 0; j < TT; ++j) acc[j] = fmaf(a, sb[c][j], acc[j]);
-        }
-        __syncthreads();
+    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+template <Kind KIND>
+struct Major {
+    static constexpr bool a = KIND == kForward;      // A is K-major
+    static constexpr bool b = KIND != kGradWeight;   // B is K-major
+};
+
+// one stage of an operand tile, `width` of its M or N dimension from i0
+template <bool K_MAJOR>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* tm, uint64_t* bar, int i0, int c0, int width)
+{
+    if (K_MAJOR) {
+        tma_load_2d(dst, tm, bar, c0, i0);
+    } else {
+        for (int i = 0; i < width; i += 64) tma_load_2d(dst + (i / 64) * BOX_BYTES, tm, bar, i0 + i, c0);
     }
-    epilogue<T, KIND, TT>(e, f0 + tid, t0, acc, bias_of<T>(e, f0 + tid));
+}
+
+// ----------------------------------------------------------------------------
+// Split kernel: a cluster of S CTAs computes one tile of 128 features x BN rows,
+// each over its share of the contraction, and joins the S partial sums through
+// distributed shared memory in rank order: no atomics and no second pass over
+// memory, and results do not depend on timing.
+//
+//   warp 0     TMA producer (ring of `stages` boxes of A and B)
+//   warp 1     TMEM allocation, tcgen05.mma issue
+//   warps 0-7  epilogue, once the accumulator is complete
+// ----------------------------------------------------------------------------
+constexpr int SPLIT_THREADS = 256;
+constexpr int JOIN = 4;  // rows that a thread joins at a time
+
+struct SplitShape {
+    int bn;      // rows t of a tile: 16, 32, 64, 128 or 256
+    int split;   // CTAs per tile
+    int stages;
+};
+
+__host__ __device__ constexpr int stage_bytes(int bn) { return A_BYTES + bn * BK * 2; }
+
+template <typename T, Kind KIND>
+__global__ void __launch_bounds__(SPLIT_THREADS, 2)
+    split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const int kblocks,
+                 const SplitShape sh, const __grid_constant__ Epilogue e)
+{
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int sbytes = stage_bytes(sh.bn);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + sh.stages * sbytes);
+    uint64_t* empty = full + MAX_STAGES;
+    uint64_t* done = empty + MAX_STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = warp_id(), lane = lane_id();
+    const int rank = sh.split > 1 ? (int)cluster_ctarank() : 0;
+    const int tile = (int)(blockIdx.x / sh.split), mtiles = (e.m + BM - 1) / BM;
+    const int f0 = tile % mtiles * BM, t0 = tile / mtiles * sh.bn;
+    const int kb0 = (int)((int64_t)kblocks * rank / sh.split), kb1 = (int)((int64_t)kblocks * (rank + 1) / sh.split);
+    const uint32_t cols = sh.bn < 32 ? 32u : (uint32_t)sh.bn;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < sh.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+    }
+    if (warp == 1) { tmem_alloc(tmem_slot, cols); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            int stage = 0, started = 0;
+            uint32_t ph = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(&empty[stage], ph ^ 1u, abort_flag)) {
+                    // let the copies already in flight land before the CTA exits
+                    int never = 0;
+                    for (int s = 0; s < min(started, sh.stages); ++s) {
+                        const int i = started - 1 - s;
+                        mbar_wait(&full[i % sh.stages], (uint32_t)(i / sh.stages) & 1u, &never, 20000000ull);
+                    }
+                    break;
+                }
+                uint8_t* sa = smem + stage * sbytes;
+                mbar_arrive_expect_tx(&full[stage], sbytes);
+                load_tile<Major<KIND>::a>(sa, &tmA, &full[stage], f0, kb * BK, BM);
+                load_tile<Major<KIND>::b>(sa + A_BYTES, &tmB, &full[stage], t0, kb * BK, sh.bn);
+                ++started;
+                if (++stage == sh.stages) { stage = 0; ph ^= 1u; }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (kb1 > kb0 && elect_one()) {
+            const uint32_t idesc = idesc_f16(std::is_same<T, __nv_bfloat16>::value, Major<KIND>::a,
+                                             Major<KIND>::b, BM, sh.bn);
+            int stage = 0;
+            uint32_t ph = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(&full[stage], ph, abort_flag)) break;
+                tc_fence_after();
+                const uint32_t a0 = smem_u32(smem + stage * sbytes), b0 = a0 + A_BYTES;
+#pragma unroll
+                for (int kk = 0; kk < BK / UK; ++kk)
+                    mma_f16(tmem, umma_desc(a0 + kk * umma_step(Major<KIND>::a), Major<KIND>::a),
+                            umma_desc(b0 + kk * umma_step(Major<KIND>::b), Major<KIND>::b), idesc, kb > kb0 || kk ? 1u : 0u);
+                mma_commit(&empty[stage]);
+                if (++stage == sh.stages) { stage = 0; ph ^= 1u; }
+            }
+            mma_commit(done);
+        }
+        __syncwarp();
+    }
+    // every MMA of this CTA has completed (so every copy has landed and been read)
+    bool ok = true;
+    if (kb1 > kb0) ok = mbar_wait(done, 0, abort_flag);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+
+    const int quarter = warp & 3, half = warp >> 2;
+    const int f = f0 + quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int rows = min(sh.bn, e.n - t0);  // rows of this tile that exist
+    const float bias = bias_of<T>(e, f);
+    if (sh.split == 1) {
+        for (int c = half * 16; c < rows; c += 32) {
+            float v[16];
+            if (kb1 > kb0) {
+                __syncwarp();
+                tmem_ld_x16(tmem + lanes + c, v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+            }
+            if (ok) epilogue<T, KIND, 16>(e, f, t0 + c, v, bias);
+        }
+    } else {
+        // partial sums as [row][128 features] into the ring's shared memory
+        float* part = reinterpret_cast<float*>(smem);
+        for (int c = half * 16; c < rows; c += 32) {
+            float v[16];
+            __syncwarp();
+            tmem_ld_x16(tmem + lanes + c, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) part[(c + j) * BM + quarter * 32 + lane] = v[j];
+        }
+        cluster_sync();
+        const uint32_t mine = smem_u32(part + quarter * 32 + lane);
+        for (int c = (rank * 2 + half) * JOIN; c < rows; c += sh.split * 2 * JOIN) {
+            float v[JOIN] = {};
+            for (int r = 0; r < sh.split; ++r) {
+                const uint32_t peer = map_to_rank(mine + c * BM * 4, (uint32_t)r);
+#pragma unroll
+                for (int j = 0; j < JOIN; ++j) v[j] += ld_cluster_f32(peer + j * BM * 4);
+            }
+            if (ok) epilogue<T, KIND, JOIN>(e, f, t0 + c, v, bias);
+        }
+        cluster_sync();  // no CTA leaves while another still reads its sums
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, cols);
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_status, CHPL_ERR_TIMEOUT);
+}
+
+// ----------------------------------------------------------------------------
+// host side
+// ----------------------------------------------------------------------------
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
+{
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    });
+    return fn;
+}
+
+// Map of an operand with i (M or N dimension) < extent and c < k; box: 64
+// contiguous elements by `box` of i (K-major) or by 64 of c (MN-major).
+static int make_tmap(CUtensorMap* tm, const Operand& o, int64_t extent, int64_t k, int box)
+{
+    auto fn = encode_fn();
+    if (!fn) { set_error("cuTensorMapEncodeTiled unavailable"); return CHPL_ERR_CUDA; }
+    const int64_t inner = o.k_major ? k : extent, outer = o.k_major ? extent : k;
+    cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+    cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
+    cuuint32_t boxes[2] = {64u, (cuuint32_t)(o.k_major ? box : BK)};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(o.p), dims, strides, boxes, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed (%d)", (int)r); return CHPL_ERR_CUDA; }
+    return CHPL_OK;
+}
+
+static int num_sms()
+{
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    return n;
+}
+
+// Narrowest tile that holds all rows (256 at most; 64 at least where B comes
+// in 64-wide boxes); then as many CTAs per tile, up to a portable cluster, as
+// fill two per SM, each with at least two stages of work.
+static SplitShape shape_for(Kind kind, int m, int n, int kblocks)
+{
+    SplitShape s;
+    s.bn = kind == kGradWeight ? 64 : 16;
+    while (s.bn < n && s.bn < 256) s.bn *= 2;
+    const int64_t tiles = (int64_t)((m + BM - 1) / BM) * ((n + s.bn - 1) / s.bn);
+    const int sms = num_sms();
+    s.split = 1;
+    while (s.split < 8 && tiles * s.split * 2 <= 2 * sms && kblocks >= s.split * 2 * 2) s.split *= 2;
+    const int room = (s.bn <= 64 ? SMEM_LIMIT / 2 : SMEM_LIMIT) - 1024 - 1024;
+    s.stages = std::min(MAX_STAGES, room / stage_bytes(s.bn));
+    return s;
 }
 
 template <typename T, Kind KIND>
 static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
 {
-    for (int64_t t = 0; t < e.n; t += (int64_t)65535 * TT) {  // the grid's second dimension ends at 65535
-        const int64_t nt = e.n - t < (int64_t)65535 * TT ? e.n - t : (int64_t)65535 * TT;
-        if (t != 0) { set_error("linear: more than %d rows", 65535 * TT); return CHPL_ERR_UNSUPPORTED; }
-        const dim3 grid((unsigned)((e.m + TF - 1) / TF), (unsigned)((nt + TT - 1) / TT));
-        simple_kernel<T, KIND><<<grid, TF, 0, st>>>(static_cast<const T*>(a.p), a.ld, a.k_major,
-                                                    static_cast<const T*>(b.p), b.ld, b.k_major, (int)k, e);
-        CHPL_CUDA(cudaGetLastError());
+    const int kblocks = (int)((k + BK - 1) / BK);
+    const SplitShape s = shape_for(KIND, e.m, e.n, kblocks);
+    const int64_t ctas = (int64_t)((e.m + BM - 1) / BM) * ((e.n + s.bn - 1) / s.bn) * s.split;
+    if (ctas > 0x7fffffff) { set_error("linear: an output of %d x %d is more than one launch serves", e.n, e.m); return CHPL_ERR_UNSUPPORTED; }
+    CUtensorMap tmA, tmB;
+    std::memset(&tmA, 0, sizeof(tmA));
+    std::memset(&tmB, 0, sizeof(tmB));
+    if (kblocks > 0) {
+        CHPL_TRY(make_tmap(&tmA, a, e.m, k, BM));
+        CHPL_TRY(make_tmap(&tmB, b, e.n, k, s.bn));
     }
+    const int smem = 1024 + s.stages * stage_bytes(s.bn) + 512;
+    CHPL_CUDA(cudaFuncSetAttribute(split_kernel<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)s.split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(SPLIT_THREADS);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CHPL_CUDA(cudaLaunchKernelEx(&cfg, split_kernel<T, KIND>, tmA, tmB, kblocks, s, e));
     return CHPL_OK;
 }
 
