@@ -76,6 +76,19 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64
         : "memory");
 }
 
+// a CTA pair's MMA, issued by its even CTA: A's 256 rows and B's N rows lie half
+// in each CTA's shared memory, D's rows 0..127 in the even CTA's TMEM
+__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, float (&v)[16])
 {
     uint32_t r[16];
@@ -102,6 +115,12 @@ struct Major {
     static constexpr bool a = KIND == kForward;      // A is K-major
     static constexpr bool b = KIND != kGradWeight;   // B is K-major
 };
+
+template <typename T, Kind KIND>
+__host__ __device__ constexpr uint32_t idesc_of(int M, int N)
+{
+    return idesc_f16(std::is_same<T, __nv_bfloat16>::value, Major<KIND>::a, Major<KIND>::b, M, N);
+}
 
 // one stage of an operand tile, `width` of its M or N dimension from i0
 template <bool K_MAJOR>
@@ -194,8 +213,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
         __syncwarp();
     } else if (warp == 1) {
         if (kb1 > kb0 && elect_one()) {
-            const uint32_t idesc = idesc_f16(std::is_same<T, __nv_bfloat16>::value, Major<KIND>::a,
-                                             Major<KIND>::b, BM, sh.bn);
+            const uint32_t idesc = idesc_of<T, KIND>(BM, sh.bn);
             int stage = 0;
             uint32_t ph = 0;
             for (int kb = kb0; kb < kb1; ++kb) {
@@ -270,6 +288,194 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
 }
 
 // ----------------------------------------------------------------------------
+// Pair kernel: persistent pairs of CTAs (tcgen05 cta_group::2), one tile of 256
+// features x bn rows after another.  Each CTA stages 128 features of A and half
+// of B's rows, so a stage feeds twice the multiply-adds per byte of shared
+// memory that a lone CTA's would; the accumulator is double buffered in TMEM
+// (2 x bn <= 512 columns), so the epilogue of one tile runs under the products
+// of the next.
+//
+//   warp 0      TMA producer (both CTAs)
+//   warp 1      TMEM allocation; tcgen05.mma issue (even CTA)
+//   warps 2-9   epilogue (both CTAs)
+// ----------------------------------------------------------------------------
+constexpr int PAIR_THREADS = 320;
+constexpr int PAIR_STAGES = 6;
+constexpr int PAIR_STAGE_BYTES = A_BYTES + 128 * BK * 2;
+constexpr int PAIR_SMEM = 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + 256;
+constexpr int PAIR_EPI_WARPS = 8;
+
+struct PairShape {
+    int bn;              // rows t of a tile, a multiple of 32 (128 where B is MN-major), <= 256
+    int mtiles, ntiles;
+    int group;           // feature tiles walked before the next row tile: what L2 holds of A meanwhile
+};
+
+__device__ __forceinline__ void pair_tile(const PairShape& sh, int tile, int& mt, int& nt)
+{
+    const int per_group = sh.group * sh.ntiles;
+    const int g = tile / per_group, first = g * sh.group;
+    const int size = min(sh.group, sh.mtiles - first), local = tile - g * per_group;
+    mt = first + local % size;
+    nt = local / size;
+}
+
+template <bool K_MAJOR>
+__device__ __forceinline__ void load_tile_pair(uint8_t* dst, const CUtensorMap* tm, uint32_t bar, int i0, int c0, int width)
+{
+    if (K_MAJOR) {
+        tma_load_2d_pair(dst, tm, bar, c0, i0);
+    } else {
+        for (int i = 0; i < width; i += 64) tma_load_2d_pair(dst + (i / 64) * BOX_BYTES, tm, bar, i0 + i, c0);
+    }
+}
+
+template <typename T, Kind KIND>
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const int kblocks,
+                const PairShape sh, const __grid_constant__ Epilogue e)
+{
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + PAIR_STAGES * PAIR_STAGE_BYTES);
+    uint64_t* empty = full + PAIR_STAGES;
+    uint64_t* acc_full = empty + PAIR_STAGES;
+    uint64_t* acc_empty = acc_full + 2;
+    uint64_t* drain = acc_empty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = warp_id(), lane = lane_id();
+    const uint32_t rank = cluster_ctarank();
+    const int unit = (int)(blockIdx.x >> 1), nunits = (int)(gridDim.x >> 1);
+    const int total = sh.mtiles * sh.ntiles;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < PAIR_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * PAIR_EPI_WARPS); }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+    }
+    if (warp == 1) { tmem_alloc_pair(tmem_slot, 512); tmem_relinquish_pair(); }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    // barriers of the even CTA, where the MMAs are issued, as shared::cluster addresses
+    const uint32_t lead_full = map_to_rank(smem_u32(full), 0), lead_acc_empty = map_to_rank(smem_u32(acc_empty), 0);
+    const int half_rows = sh.bn / 2;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            const uint32_t bytes = 2u * (A_BYTES + (uint32_t)half_rows * BK * 2);  // both CTAs' copies
+            int stage = 0, started = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int tile = unit; tile < total && ok; tile += nunits) {
+                int mt, nt;
+                pair_tile(sh, tile, mt, nt);
+                const int f0 = mt * 2 * BM + (int)rank * BM, t0 = nt * sh.bn + (int)rank * half_rows;
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!mbar_wait(&empty[stage], ph ^ 1u, abort_flag)) { ok = false; break; }
+                    uint8_t* sa = smem + stage * PAIR_STAGE_BYTES;
+                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
+                    load_tile_pair<Major<KIND>::a>(sa, &tmA, lead_full + stage * 8, f0, kb * BK, BM);
+                    load_tile_pair<Major<KIND>::b>(sa + A_BYTES, &tmB, lead_full + stage * 8, t0, kb * BK, half_rows);
+                    ++started;
+                    if (++stage == PAIR_STAGES) { stage = 0; ph ^= 1u; }
+                }
+            }
+            if (!ok) {  // let the copies already in flight land before the CTA exits
+                const uint64_t t0 = globaltimer();
+                while (globaltimer() - t0 < 1000000ull) {
+                }
+            } else {
+                // every stage's last release (a commit of the even CTA's MMA thread) has landed here
+                for (int s = 0; s < PAIR_STAGES; ++s) {
+                    if (s >= PAIR_STAGES - started && !mbar_wait(&empty[stage], ph ^ 1u, abort_flag)) break;
+                    if (++stage == PAIR_STAGES) { stage = 0; ph ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            const uint32_t idesc = idesc_of<T, KIND>(2 * BM, sh.bn);
+            const uint32_t peer_empty = map_to_rank(smem_u32(empty), 1), peer_acc_full = map_to_rank(smem_u32(acc_full), 1);
+            int stage = 0;
+            uint32_t ph = 0, acc = 0;
+            bool ok = true;
+            for (int tile = unit; tile < total && ok; tile += nunits) {
+                const uint32_t buf = acc & 1u, aph = (acc >> 1) & 1u;
+                if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t d = tmem + buf * 256;
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!mbar_wait(&full[stage], ph, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t a0 = smem_u32(smem + stage * PAIR_STAGE_BYTES), b0 = a0 + A_BYTES;
+#pragma unroll
+                    for (int kk = 0; kk < BK / UK; ++kk)
+                        mma_f16_pair(d, umma_desc(a0 + kk * umma_step(Major<KIND>::a), Major<KIND>::a),
+                                     umma_desc(b0 + kk * umma_step(Major<KIND>::b), Major<KIND>::b), idesc, kb || kk ? 1u : 0u);
+                    mma_commit_pair(smem_u32(&empty[stage]));
+                    mma_commit_pair(peer_empty + stage * 8);
+                    if (++stage == PAIR_STAGES) { stage = 0; ph ^= 1u; }
+                }
+                if (!ok) break;
+                mma_commit_pair(smem_u32(&acc_full[buf]));
+                mma_commit_pair(peer_acc_full + buf * 8);
+                ++acc;
+            }
+            if (!ok) {  // the MMAs already issued complete before TMEM is released
+                int never = 0;
+                mma_commit_pair(smem_u32(drain));
+                mbar_wait(drain, 0, &never, 20000000ull);
+            } else {
+                // both CTAs' epilogues have released both buffers (their arrivals have landed here)
+                for (int b = 0; b < 2; ++b, ++acc)
+                    if (!mbar_wait(&acc_empty[acc & 1u], ((acc >> 1) & 1u) ^ 1u, abort_flag)) break;
+            }
+        }
+        __syncwarp();
+    } else {
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        uint32_t acc = 0;
+        for (int tile = unit; tile < total; tile += nunits, ++acc) {
+            int mt, nt;
+            pair_tile(sh, tile, mt, nt);
+            const int f = mt * 2 * BM + (int)rank * BM + quarter * 32 + lane, t0 = nt * sh.bn;
+            const uint32_t buf = acc & 1u, aph = (acc >> 1) & 1u;
+            const float bias = bias_of<T>(e, f);
+            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aph, abort_flag))) break;
+            tc_fence_after();
+            for (int c = half * 16; c < sh.bn; c += 32) {
+                float v[16];
+                tmem_ld_x16(tmem + lanes + buf * 256 + c, v);
+                if (c + 32 >= sh.bn) {  // this warp's last columns are in registers
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(lead_acc_empty + buf * 8);
+                }
+                if (t0 + c < e.n) epilogue<T, KIND, 16>(e, f, t0 + c, v, bias);
+                __syncwarp();
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_status, CHPL_ERR_TIMEOUT);
+}
+
+// ----------------------------------------------------------------------------
 // host side
 // ----------------------------------------------------------------------------
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
@@ -329,10 +535,25 @@ static SplitShape shape_for(Kind kind, int m, int n, int kblocks)
     return s;
 }
 
-template <typename T, Kind KIND>
-static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
+static void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, cudaStream_t st, int64_t ctas, int threads,
+                           int smem, int cluster)
 {
-    const int kblocks = (int)((k + BK - 1) / BK);
+    std::memset(&cfg, 0, sizeof(cfg));
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+}
+
+template <typename T, Kind KIND>
+static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, int kblocks, const Epilogue& e)
+{
     const SplitShape s = shape_for(KIND, e.m, e.n, kblocks);
     const int64_t ctas = (int64_t)((e.m + BM - 1) / BM) * ((e.n + s.bn - 1) / s.bn) * s.split;
     if (ctas > 0x7fffffff) { set_error("linear: an output of %d x %d is more than one launch serves", e.n, e.m); return CHPL_ERR_UNSUPPORTED; }
@@ -343,23 +564,45 @@ static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k
         CHPL_TRY(make_tmap(&tmA, a, e.m, k, BM));
         CHPL_TRY(make_tmap(&tmB, b, e.n, k, s.bn));
     }
-    const int smem = 1024 + s.stages * stage_bytes(s.bn) + 512;
     CHPL_CUDA(cudaFuncSetAttribute(split_kernel<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
     cudaLaunchConfig_t cfg;
-    std::memset(&cfg, 0, sizeof(cfg));
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)s.split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(SPLIT_THREADS);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr;
+    cluster_config(cfg, attr, st, ctas, SPLIT_THREADS, 1024 + s.stages * stage_bytes(s.bn) + 512, s.split);
     CHPL_CUDA(cudaLaunchKernelEx(&cfg, split_kernel<T, KIND>, tmA, tmB, kblocks, s, e));
     return CHPL_OK;
+}
+
+template <typename T, Kind KIND>
+static int launch_pair(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, int kblocks, const Epilogue& e,
+                       PairShape s)
+{
+    CUtensorMap tmA, tmB;
+    CHPL_TRY(make_tmap(&tmA, a, e.m, k, BM));
+    CHPL_TRY(make_tmap(&tmB, b, e.n, k, s.bn / 2));
+    CHPL_CUDA(cudaFuncSetAttribute(pair_kernel<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM));
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    const int units = std::min(s.mtiles * s.ntiles, num_sms() / 2);
+    cluster_config(cfg, attr, st, 2 * units, PAIR_THREADS, PAIR_SMEM, 2);
+    CHPL_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<T, KIND>, tmA, tmB, kblocks, s, e));
+    return CHPL_OK;
+}
+
+// Pairs where their tiles fill most of the GPU and more than half of each, clusters of lone CTAs elsewhere.
+template <typename T, Kind KIND>
+static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
+{
+    const int kblocks = (int)((k + BK - 1) / BK);
+    const int64_t mt = (e.m + 2 * BM - 1) / (2 * BM), nt = (e.n + 255) / 256;
+    if (kblocks > 0 && e.n > 128 && mt * nt >= num_sms() * 2 / 5 && mt * nt < 0x7fffffff) {
+        PairShape s;
+        s.bn = 256;
+        s.mtiles = (int)mt;
+        s.ntiles = (int)nt;
+        s.group = 8;
+        return launch_pair<T, KIND>(st, a, b, k, kblocks, e, s);
+    }
+    return launch_split<T, KIND>(st, a, b, k, kblocks, e);
 }
 
 template <typename T>

@@ -29,7 +29,7 @@ def out_like(T, width, dt, pad):
 
 SIZES = [(1, 1, 1), (1, 64, 32), (1, 1024, 1024), (2, 31, 33), (5, 4096, 40), (17, 129, 255), (24, 2048, 520), (64, 256, 128),
          (100, 8, 1000), (128, 128, 256), (130, 1000, 514), (257, 515, 1029), (300, 1024, 4096), (1000, 777, 300),
-         (1024, 192, 2050), (2048, 264, 1160)]
+         (1024, 192, 2050), (2048, 264, 1160), (1500, 200, 3100), (4096, 1000, 1100)]
 
 
 @pytest.mark.parametrize("T,k,n", SIZES)
@@ -67,7 +67,7 @@ def test_forward(cuda, T, k, n, dt, pad):
 
 
 GRADS = [(1, 1, 1), (1, 1024, 512), (3, 65, 31), (16, 128, 64), (40, 4096, 24), (77, 40, 1000), (128, 256, 128),
-         (200, 520, 264), (257, 1031, 519), (512, 1024, 2048), (1000, 300, 777), (2100, 520, 392)]
+         (200, 520, 264), (257, 1031, 519), (512, 1024, 2048), (1000, 300, 777), (2100, 520, 392), (2050, 1800, 2100)]
 
 
 @pytest.mark.parametrize("T,k,n", GRADS)
