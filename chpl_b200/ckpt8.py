@@ -8,7 +8,6 @@ Everything runs in libchpl.so on the GPU; there is no host implementation here.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple
 
 import torch
@@ -37,15 +36,23 @@ def invalid(where: str, msg: str) -> _lib.ChplError:
     return _lib.ChplError(_lib.CHPL_ERR_INVALID, where, msg)
 
 
-def matrix(where: str, name: str, t, dtype=None, shape=None, device=None) -> int:
-    """Checks a CUDA matrix with unit column stride; returns the distance between its rows."""
+def matrix(where: str, name: str, t, dtype, device: int, shape) -> int:
+    """The distance between the rows of a CUDA matrix with unit column stride, of this type, device and shape; any may
+    be None.  Raises ChplError for another."""
+    try:
+        if t.shape == shape and t.dtype is dtype and t.get_device() == device:  # what nearly every call passes
+            ld, unit = t.stride()
+            if unit == 1 and ld >= shape[1]:
+                return ld
+    except (AttributeError, TypeError, ValueError):
+        pass
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise invalid(where, f"{name} is not a matrix")
-    if not t.is_cuda or (device is not None and t.device != device):
-        raise invalid(where, f"{name} is on {t.device}, not on {device or 'a GPU'}")
+    if not t.is_cuda or (device is not None and t.get_device() != device):
+        raise invalid(where, f"{name} is on {t.device}, not on {'a GPU' if device is None else f'cuda:{device}'}")
     if dtype is not None and t.dtype != dtype:
         raise invalid(where, f"{name} is {t.dtype}, not {dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise invalid(where, f"{name} is {tuple(t.shape)}, not {tuple(shape)}")
     rows, cols = t.shape
     ld, unit = t.stride()
@@ -56,11 +63,12 @@ def matrix(where: str, name: str, t, dtype=None, shape=None, device=None) -> int
     return ld if rows > 1 else cols
 
 
-def struct_of(where: str, name: str, c: Ckpt8, shape=None, device=None) -> _lib.Ckpt8:
-    ldc = matrix(where, f"{name}.codes", c.codes, torch.int8, shape, device)
+def pointers(where: str, name: str, c: Ckpt8, device, shape) -> tuple[int, int, int, int]:
+    """(codes, scales, ldc, lds) of a checkpoint, as chpl_ckpt8 has them."""
+    ldc = matrix(where, name + ".codes", c.codes, torch.int8, device, shape)
     rows, cols = c.codes.shape
-    lds = matrix(where, f"{name}.scales", c.scales, torch.uint8, (rows, -(-cols // GROUP)), c.codes.device)
-    return _lib.Ckpt8(c.codes.data_ptr(), c.scales.data_ptr(), ldc, lds)
+    lds = matrix(where, name + ".scales", c.scales, torch.uint8, c.codes.get_device(), (rows, -(-cols // GROUP)))
+    return c.codes.data_ptr(), c.scales.data_ptr(), ldc, lds
 
 
 def empty(rows: int, cols: int, dtype: torch.dtype, device) -> Ckpt8:
@@ -68,60 +76,75 @@ def empty(rows: int, cols: int, dtype: torch.dtype, device) -> Ckpt8:
                  torch.empty(rows, -(-cols // GROUP), dtype=torch.uint8, device=device), dtype)
 
 
+def elsewhere(device: int, stream) -> bool:
+    """Whether a call has to change torch's current device or stream first."""
+    return stream is not None or device != torch.cuda.current_device()
+
+
 class on_stream:
-    """The device of `device` and, where one is given, `stream`: outputs and workspaces come from that stream's
-    memory.  `self.handle` is the stream's handle."""
+    """Makes `device` and `stream` (a torch stream, a raw handle, or None for that device's current one) torch's
+    current ones, so that outputs and workspaces come from that stream's memory."""
 
     def __init__(self, device: torch.device, stream):
-        self.handle = None
-        self._stack = []
-        if device.index != torch.cuda.current_device():
-            self._stack.append(torch.cuda.device(device))
+        self._stack = [torch.cuda.device(device)]
         if stream is not None:
             if isinstance(stream, int):
                 stream = torch.cuda.ExternalStream(stream, device=device)
             self._stack.append(torch.cuda.stream(stream))
-        self._device = device
 
     def __enter__(self):
         for c in self._stack:
             c.__enter__()
-        self.handle = torch.cuda.current_stream(self._device).cuda_stream
-        return self
 
     def __exit__(self, *exc):
         for c in reversed(self._stack):
             c.__exit__(*exc)
 
 
+#: handle of a device's current stream (torch.cuda.current_stream(i).cuda_stream without the two objects around it)
+current_handle = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def pack(x: torch.Tensor, out: Ckpt8 | None = None, stream=None) -> Ckpt8:
     """The checkpoint of x (rows x cols), on torch's current stream or on `stream`."""
     where = "ckpt8.pack"
-    ldx = matrix(where, "x", x)
-    if x.dtype not in _TYPES:
+    ldx = matrix(where, "x", x, None, None, None)
+    code = _TYPES.get(x.dtype)
+    if code is None:
         raise invalid(where, f"x is {x.dtype}: bfloat16, float16 or float32 is wanted")
+    dev = x.get_device()
+    if elsewhere(dev, stream):
+        with on_stream(x.device, stream):
+            return pack(x, out)
     rows, cols = x.shape
-    with on_stream(x.device, stream) as on:
-        if out is None:
-            out = empty(rows, cols, x.dtype, x.device)
-        c = struct_of(where, "out", out, x.shape, x.device)
-        _lib.check(_lib.load().chpl_ckpt8_pack(on.handle, _TYPES[x.dtype], rows, cols, x.data_ptr(), ldx,
-                                               ctypes.byref(c)), "chpl_ckpt8_pack")
+    if out is None:
+        out = empty(rows, cols, x.dtype, x.device)
+        c = (out.codes.data_ptr(), out.scales.data_ptr(), cols, -(-cols // GROUP))
+    else:
+        c = pointers(where, "out", out, dev, x.shape)
+    _lib.check(_lib.load().chpl_ckpt8_pack(current_handle(dev), code, rows, cols, x.data_ptr(), ldx,
+                                           _lib.CKPT8.pack(*c)), "chpl_ckpt8_pack")
     return out
 
 
 def unpack(c: Ckpt8, dtype: torch.dtype | None = None, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """The values that a checkpoint stands for, in `dtype` (default: the type of what was coded)."""
     where = "ckpt8.unpack"
-    s = struct_of(where, "c", c)
+    s = pointers(where, "c", c, None, None)
     dtype = out.dtype if out is not None else dtype or c.dtype
-    if dtype not in _TYPES:
+    code = _TYPES.get(dtype)
+    if code is None:
         raise invalid(where, f"{dtype}: bfloat16, float16 or float32 is wanted")
+    dev = c.codes.get_device()
+    if elsewhere(dev, stream):
+        with on_stream(c.codes.device, stream):
+            return unpack(c, dtype, out)
     rows, cols = c.codes.shape
-    with on_stream(c.codes.device, stream) as on:
-        if out is None:
-            out = torch.empty(rows, cols, dtype=dtype, device=c.codes.device)
-        ldx = matrix(where, "out", out, dtype, c.codes.shape, c.codes.device)
-        _lib.check(_lib.load().chpl_ckpt8_unpack(on.handle, _TYPES[dtype], rows, cols, ctypes.byref(s),
-                                                 out.data_ptr(), ldx), "chpl_ckpt8_unpack")
+    if out is None:
+        out, ldx = torch.empty(rows, cols, dtype=dtype, device=c.codes.device), cols
+    else:
+        ldx = matrix(where, "out", out, dtype, dev, c.codes.shape)
+    _lib.check(_lib.load().chpl_ckpt8_unpack(current_handle(dev), code, rows, cols, _lib.CKPT8.pack(*s),
+                                             out.data_ptr(), ldx), "chpl_ckpt8_unpack")
     return out

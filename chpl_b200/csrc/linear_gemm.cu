@@ -599,7 +599,7 @@ static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k
         s.bn = 256;
         s.mtiles = (int)mt;
         s.ntiles = (int)nt;
-        s.group = 8;
+        s.group = 16;
         return launch_pair<T, KIND>(st, a, b, k, kblocks, e, s);
     }
     return launch_split<T, KIND>(st, a, b, k, kblocks, e);

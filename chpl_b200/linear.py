@@ -16,12 +16,12 @@ import ctypes
 import torch
 
 from . import _lib
-from .ckpt8 import Ckpt8, empty, invalid, matrix, on_stream, struct_of
+from .ckpt8 import GROUP, Ckpt8, current_handle, elsewhere, empty, invalid, matrix, on_stream, pointers
 
 ACTS = {"none": _lib.CHPL_ACT_NONE, "relu": _lib.CHPL_ACT_RELU, "gelu": _lib.CHPL_ACT_GELU,
         "gelu_tanh": _lib.CHPL_ACT_GELU_TANH, "silu": _lib.CHPL_ACT_SILU}
 _TYPES = {torch.bfloat16: _lib.CHPL_TYPE_BF16, torch.float16: _lib.CHPL_TYPE_F16}
-_NONE = _lib.Ckpt8()
+_NO_CKPT = (0, 0, 0, 0)
 
 
 def _type(where: str, t) -> int:
@@ -38,21 +38,18 @@ def _act(where: str, name: str) -> int:
     return code
 
 
-def _vector(where: str, name: str, t, n: int, dtype, device) -> None:
-    if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+def _vector(where: str, name: str, t, n: int, dtype, device: int) -> int:
+    if not isinstance(t, torch.Tensor) or t.shape != (n,) or not t.is_contiguous():
         raise invalid(where, f"{name} is not a contiguous vector of {n}")
-    if t.dtype != dtype or t.device != device:
-        raise invalid(where, f"{name} is {t.dtype} on {t.device}, not {dtype} on {device}")
+    if t.dtype is not dtype or t.get_device() != device:
+        raise invalid(where, f"{name} is {t.dtype} on {t.device}, not {dtype} on cuda:{device}")
+    return t.data_ptr()
 
 
-def _run(entry: str, args, device, on, work) -> None:
-    L = _lib.load()
+def _workspace(worksize, entry: str, args: bytes, device):
     need = ctypes.c_size_t()
-    _lib.check(getattr(L, entry + "_worksize")(args, need), entry + "_worksize")
-    if work is None:
-        work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-    ptr, size = (work.data_ptr(), work.numel() * work.element_size()) if work is not None else (None, 0)
-    _lib.check(getattr(L, entry)(on.handle, args, ptr, size), entry)
+    _lib.check(worksize(args, need), entry)
+    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
 
 
 def forward(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, *, residual: torch.Tensor | None = None,
@@ -65,34 +62,41 @@ def forward(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, 
     """
     where = "linear.forward"
     code, act_code = _type(where, x), _act(where, act)
-    dt, dev = x.dtype, x.device
-    ldx = matrix(where, "x", x)
-    ldw = matrix(where, "w", w, dt, None, dev)
+    dt = x.dtype
+    ldx = matrix(where, "x", x, None, None, None)
+    dev = x.get_device()
+    if elsewhere(dev, stream):
+        with on_stream(x.device, stream):
+            return forward(x, w, bias, residual=residual, act=act, save=save, out=out, z=z, work=work)
     tokens, k = x.shape
-    n = w.shape[0]
-    if w.shape[1] != k:
-        raise invalid(where, f"x has {k} features and w {w.shape[1]}")
-    if save not in ("none", "z", "z8"):
+    n = len(w)
+    ldw = matrix(where, "w", w, dt, dev, (n, k))
+    bp = _vector(where, "bias", bias, n, dt, dev) if bias is not None else 0
+    rp, ldr = (residual.data_ptr(), matrix(where, "residual", residual, dt, dev, (tokens, n))) if residual is not None else (0, 0)
+    if out is None:
+        out, ldy = x.new_empty(tokens, n), n
+    else:
+        ldy = matrix(where, "out", out, dt, dev, (tokens, n))
+    zp, ldz, z8 = 0, 0, _NO_CKPT
+    if save == "z":
+        z = x.new_empty(tokens, n) if z is None else z
+        zp, ldz = z.data_ptr(), matrix(where, "z", z, dt, dev, (tokens, n))
+    elif save == "z8":
+        if z is None:
+            z = empty(tokens, n, dt, x.device)
+            z8 = (z.codes.data_ptr(), z.scales.data_ptr(), n, -(-n // GROUP))
+        else:
+            z8 = pointers(where, "z", z, dev, (tokens, n))
+    elif save != "none":
         raise invalid(where, f"save {save!r} is none of none, z, z8")
-    if bias is not None:
-        _vector(where, "bias", bias, n, dt, dev)
-    ldr = matrix(where, "residual", residual, dt, (tokens, n), dev) if residual is not None else 0
-    with on_stream(dev, stream) as on:
-        if out is None:
-            out = torch.empty(tokens, n, dtype=dt, device=dev)
-        ldy = matrix(where, "out", out, dt, (tokens, n), dev)
-        ldz, z8 = 0, _NONE
-        if save == "z":
-            z = torch.empty(tokens, n, dtype=dt, device=dev) if z is None else z
-            ldz = matrix(where, "z", z, dt, (tokens, n), dev)
-        elif save == "z8":
-            z = empty(tokens, n, dt, dev) if z is None else z
-            z8 = struct_of(where, "z", z, (tokens, n), dev)
-        a = _lib.LinearFwd(code, act_code, tokens, n, k, x.data_ptr(), ldx, w.data_ptr(), ldw,
-                           bias.data_ptr() if bias is not None else None,
-                           residual.data_ptr() if residual is not None else None, ldr, out.data_ptr(), ldy,
-                           z.data_ptr() if save == "z" else None, ldz, z8)
-        _run("chpl_linear_forward", a, dev, on, work)
+    a = _lib.LINEAR_FWD.pack(code, act_code, tokens, n, k, x.data_ptr(), ldx, w.data_ptr(), ldw, bp, rp, ldr,
+                             out.data_ptr(), ldy, zp, ldz, *z8)
+    L = _lib.load()
+    # rows that TMA can read (a base and a row distance of whole 16 bytes) need no workspace
+    if work is None and ((ldx | ldw) & 7 or (x.data_ptr() | w.data_ptr()) & 15):
+        work = _workspace(L.chpl_linear_forward_worksize, "chpl_linear_forward_worksize", a, x.device)
+    ptr, size = (work.data_ptr(), work.numel() * work.element_size()) if work is not None else (None, 0)
+    _lib.check(L.chpl_linear_forward(current_handle(dev), a, ptr, size), "chpl_linear_forward")
     return out if save == "none" else (out, z)
 
 
@@ -109,13 +113,16 @@ def backward(dy: torch.Tensor, x, w: torch.Tensor, *, act: str = "none", z=None,
     """
     where = "linear.backward"
     code, act_code, in_code = _type(where, dy), _act(where, act), _act(where, in_act)
-    dt, dev = dy.dtype, dy.device
-    lddy = matrix(where, "dy", dy)
-    ldw = matrix(where, "w", w, dt, None, dev)
+    dt = dy.dtype
+    lddy = matrix(where, "dy", dy, None, None, None)
+    dev = dy.get_device()
+    if elsewhere(dev, stream):
+        with on_stream(dy.device, stream):
+            return backward(dy, x, w, act=act, z=z, in_act=in_act, add=add, need_dx=need_dx, need_dw=need_dw, need_db=need_db,
+                            dx=dx, dw=dw, db=db, grad_dtype=grad_dtype, accumulate=accumulate, work=work)
     tokens, n = dy.shape
+    ldw = matrix(where, "w", w, dt, dev, (n, w.shape[-1]))
     k = w.shape[1]
-    if w.shape[0] != n:
-        raise invalid(where, f"dy has {n} features and w {w.shape[0]} rows")
     gt = grad_dtype or (dw.dtype if dw is not None else db.dtype if db is not None else dt)
     if gt != dt and gt != torch.float32:
         raise invalid(where, f"gradients in {gt}: {dt} or float32 is wanted")
@@ -124,28 +131,39 @@ def backward(dy: torch.Tensor, x, w: torch.Tensor, *, act: str = "none", z=None,
 
     def saved(name, v, width):
         if v is None:
-            return None, 0, _NONE
+            return (0, 0, *_NO_CKPT)
         if isinstance(v, Ckpt8):
-            return None, 0, struct_of(where, name, v, (tokens, width), dev)
-        return v.data_ptr(), matrix(where, name, v, dt, (tokens, width), dev), _NONE
+            return (0, 0, *pointers(where, name, v, dev, (tokens, width)))
+        return (v.data_ptr(), matrix(where, name, v, dt, dev, (tokens, width)), *_NO_CKPT)
 
-    xp, ldx, x8 = saved("x", x, k)
-    zp, ldz, z8 = saved("z", z, n) if act != "none" else (None, 0, _NONE)
-    ldadd = matrix(where, "add", add, dt, (tokens, k), dev) if add is not None else 0
-    with on_stream(dev, stream) as on:
-        lddx = lddw = 0
-        if need_dx:
-            dx = torch.empty(tokens, k, dtype=dt, device=dev) if dx is None else dx
-            lddx = matrix(where, "dx", dx, dt, (tokens, k), dev)
-        if need_dw:
-            dw = torch.empty(n, k, dtype=gt, device=dev) if dw is None else dw
-            lddw = matrix(where, "dw", dw, gt, (n, k), dev)
-        if need_db:
-            db = torch.empty(n, dtype=gt, device=dev) if db is None else db
-            _vector(where, "db", db, n, gt, dev)
-        a = _lib.LinearBwd(code, act_code, in_code, _lib.CHPL_TYPE_F32 if gt == torch.float32 else code, int(accumulate),
-                           tokens, n, k, dy.data_ptr(), lddy, w.data_ptr(), ldw, xp, ldx, x8, zp, ldz, z8,
-                           add.data_ptr() if add is not None else None, ldadd, dx.data_ptr() if need_dx else None,
-                           lddx, dw.data_ptr() if need_dw else None, lddw, db.data_ptr() if need_db else None)
-        _run("chpl_linear_backward", a, dev, on, work)
-    return dx if need_dx else None, dw if need_dw else None, db if need_db else None
+    xs = saved("x", x, k)
+    zs = saved("z", z, n) if act != "none" else (0, 0, *_NO_CKPT)
+    ap, ldadd = (add.data_ptr(), matrix(where, "add", add, dt, dev, (tokens, k))) if add is not None else (0, 0)
+    lddx = lddw = 0
+    if not need_dx:
+        dx = None
+    elif dx is None:
+        dx, lddx = dy.new_empty(tokens, k), k
+    else:
+        lddx = matrix(where, "dx", dx, dt, dev, (tokens, k))
+    if not need_dw:
+        dw = None
+    elif dw is None:
+        dw, lddw = dy.new_empty(n, k, dtype=gt), k
+    else:
+        lddw = matrix(where, "dw", dw, gt, dev, (n, k))
+    if not need_db:
+        db = None
+    elif db is None:
+        db = dy.new_empty(n, dtype=gt)
+    else:
+        _vector(where, "db", db, n, gt, dev)
+    xp, wp, bp = (v.data_ptr() if v is not None else 0 for v in (dx, dw, db))
+    a = _lib.LINEAR_BWD.pack(code, act_code, in_code, _lib.CHPL_TYPE_F32 if gt == torch.float32 else code, bool(accumulate),
+                             tokens, n, k, dy.data_ptr(), lddy, w.data_ptr(), ldw, *xs, *zs, ap, ldadd, xp, lddx, wp, lddw, bp)
+    L = _lib.load()
+    if work is None:
+        work = _workspace(L.chpl_linear_backward_worksize, "chpl_linear_backward_worksize", a, dy.device)
+    ptr, size = (work.data_ptr(), work.numel() * work.element_size()) if work is not None else (None, 0)
+    _lib.check(L.chpl_linear_backward(current_handle(dev), a, ptr, size), "chpl_linear_backward")
+    return dx, dw, db
