@@ -9,39 +9,6 @@
 namespace chpl {
 namespace linear {
 
-constexpr int kPackThreads = 256;
-
-// one warp per group of 32 features, a lane per feature
-template <typename T>
-__global__ void __launch_bounds__(kPackThreads) ckpt8_pack_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
-                                                                  int cols, int groups, chpl_ckpt8 c)
-{
-    const int lane = lane_id();
-    const int64_t total = rows * groups, step = (int64_t)gridDim.x * (kPackThreads / 32);
-    for (int64_t w = (int64_t)blockIdx.x * (kPackThreads / 32) + warp_id(); w < total; w += step) {
-        const int64_t t = w / groups;
-        const int g = (int)(w - t * groups), j = g * kCkptGroup + lane;
-        const float v = j < cols ? to_f32(x[t * ldx + j]) : 0.0f;
-        const uint32_t s = ckpt_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
-        const int code = ckpt_code(v, ckpt_inv_step(s));
-        if (j < cols) c.codes[t * c.ldc + j] = (int8_t)code;
-        if (lane == 0) c.scales[t * c.lds + g] = (uint8_t)s;
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kPackThreads) ckpt8_unpack_kernel(T* __restrict__ x, int64_t ldx, int64_t rows,
-                                                                    int cols, int groups, chpl_ckpt8 c)
-{
-    const int lane = lane_id();
-    const int64_t total = rows * groups, step = (int64_t)gridDim.x * (kPackThreads / 32);
-    for (int64_t w = (int64_t)blockIdx.x * (kPackThreads / 32) + warp_id(); w < total; w += step) {
-        const int64_t t = w / groups;
-        const int g = (int)(w - t * groups), j = g * kCkptGroup + lane;
-        if (j < cols) x[t * ldx + j] = from_f32<T>((float)c.codes[t * c.ldc + j] * ckpt_step(c.scales[t * c.lds + g]));
-    }
-}
-
 static int check_matrix(const char* who, int type, int64_t rows, int64_t cols, const void* x, int64_t ldx,
                         const chpl_ckpt8* c)
 {
@@ -60,21 +27,13 @@ static int check_matrix(const char* who, int type, int64_t rows, int64_t cols, c
 template <typename T>
 static int pack(cudaStream_t st, int64_t rows, int64_t cols, const void* x, int64_t ldx, const chpl_ckpt8& c)
 {
-    const int groups = (int)((cols + kCkptGroup - 1) / kCkptGroup);
-    ckpt8_pack_kernel<T><<<grid_for(rows * groups, kPackThreads / 32), kPackThreads, 0, st>>>(
-        static_cast<const T*>(x), ldx, rows, (int)cols, groups, c);
-    CHPL_CUDA(cudaGetLastError());
-    return CHPL_OK;
+    return run_rows(st, rows_in<T>(x, ldx), ckpt_out(c), Keep(), rows, cols);
 }
 
 template <typename T>
 static int unpack(cudaStream_t st, int64_t rows, int64_t cols, void* x, int64_t ldx, const chpl_ckpt8& c)
 {
-    const int groups = (int)((cols + kCkptGroup - 1) / kCkptGroup);
-    ckpt8_unpack_kernel<T><<<grid_for(rows * groups, kPackThreads / 32), kPackThreads, 0, st>>>(
-        static_cast<T*>(x), ldx, rows, (int)cols, groups, c);
-    CHPL_CUDA(cudaGetLastError());
-    return CHPL_OK;
+    return run_rows(st, ckpt_in(c), rows_out<T>(x, ldx), Keep(), rows, cols);
 }
 
 }  // namespace linear

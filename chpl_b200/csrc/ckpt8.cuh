@@ -39,13 +39,22 @@ __device__ __forceinline__ float ckpt_step(uint32_t s)
     return s == kCkptBadScale ? __uint_as_float(0x7fffffffu) : __uint_as_float((s - 6u) << 23);
 }
 
-// Code of x: x * inv is exact (a power of two, no underflow to speak of: what
-// it could lose is below half a code), rounded half to even.  In a poisoned
-// group inv is 0, and x * 0 of an infinity or a NaN converts to 0.
-__device__ __forceinline__ int ckpt_code(float x, float inv)
+// Code of x in the low byte: x * inv is exact (a power of two; what could
+// underflow is far below half a code), the clamp keeps it within +-127, and
+// adding 3 * 2^22 rounds it half to even into the sum's low mantissa bits (no
+// conversion instruction, which runs at an eighth of an addition's rate).  A
+// poisoned group's codes are not numbers' and have to be replaced by 0.
+__device__ __forceinline__ uint32_t ckpt_code(float x, float inv)
 {
-    const int c = __float2int_rn(x * inv);
-    return max(-127, min(127, c));
+    return __float_as_uint(fminf(fmaxf(x * inv, -127.0f), 127.0f) + 12582912.0f);
+}
+
+// Value of the code in byte `b` of w (w's bytes biased by 128, i.e. xor 0x80):
+// as the low byte of 2^23's mantissa, less 2^23 + 128, times the step; exact.
+__device__ __forceinline__ float ckpt_value(uint32_t w_biased, int b, float step)
+{
+    const float f = __uint_as_float(__byte_perm(w_biased, 0x4B000000u, 0x7440 | b));
+    return (f - 8388736.0f) * step;
 }
 
 template <typename T>
@@ -65,5 +74,183 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// ----------------------------------------------------------------------------
+// Eight consecutive elements of a row, as one lane of rows_kernel holds them:
+// raw() issues the loads, value() converts.  `vec`: base and row distance allow
+// one 16-byte (8-byte for codes) access per lane; other rows, and a row's end,
+// are read and written element by element.
+// ----------------------------------------------------------------------------
+template <typename T>
+struct RowsIn {
+    const T* p;
+    int64_t ld;
+    bool vec;
+    struct Raw {
+        uint4 w[sizeof(T) / 2];
+    };
+    __device__ __forceinline__ Raw raw(int64_t t, int j, int cols) const
+    {
+        Raw r;
+        const T* at = p + t * ld + j;
+        if (vec && j + 8 <= cols) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
+        } else {
+            T* e = reinterpret_cast<T*>(r.w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = j + i < cols ? at[i] : from_f32<T>(0.0f);
+        }
+        return r;
+    }
+    __device__ __forceinline__ void value(const Raw& r, float (&v)[8]) const
+    {
+        const T* e = reinterpret_cast<const T*>(r.w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+    }
+};
+
+struct CkptIn {
+    chpl_ckpt8 c;
+    bool vec;
+    struct Raw {
+        uint2 w;
+        uint32_t s;
+    };
+    __device__ __forceinline__ Raw raw(int64_t t, int j, int cols) const
+    {
+        Raw r = {make_uint2(0, 0), kCkptMinScale};
+        if (j >= cols) return r;
+        const int8_t* at = c.codes + t * c.ldc + j;
+        r.s = c.scales[t * c.lds + j / kCkptGroup];
+        if (vec && j + 8 <= cols) {
+            r.w = __ldg(reinterpret_cast<const uint2*>(at));
+        } else {
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i >> 2] |= (j + i < cols ? (uint32_t)(uint8_t)at[i] : 0u) << (8 * (i & 3));
+            r.w = make_uint2(w[0], w[1]);
+        }
+        return r;
+    }
+    __device__ __forceinline__ void value(const Raw& r, float (&v)[8]) const
+    {
+        const float step = ckpt_step(r.s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = ckpt_value((i < 4 ? r.w.x : r.w.y) ^ 0x80808080u, i & 3, step);
+    }
+};
+
+template <typename T>
+struct RowsOut {
+    T* p;
+    int64_t ld;
+    bool vec;
+    __device__ __forceinline__ void put(int64_t t, int j, int cols, const float (&v)[8]) const
+    {
+        T* at = p + t * ld + j;
+        if (vec && j + 8 <= cols) {
+            uint4 w[sizeof(T) / 2];
+            T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(at)[i] = w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (j + i < cols) at[i] = from_f32<T>(v[i]);
+        }
+    }
+};
+
+struct CkptOut {
+    chpl_ckpt8 c;
+    bool vec;
+    // every lane of a group's four calls it; elements past the row's end are 0
+    __device__ __forceinline__ void put(int64_t t, int j, int cols, const float (&v)[8]) const
+    {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t s = ckpt_scale(top);
+        const float inv = ckpt_inv_step(s);
+        uint32_t q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = ckpt_code(v[i], inv);
+        uint2 w;
+        w.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+        w.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+        if (s == kCkptBadScale) w = make_uint2(0, 0);
+        if (j >= cols) return;
+        int8_t* at = c.codes + t * c.ldc + j;
+        if (vec && j + 8 <= cols) {
+            *reinterpret_cast<uint2*>(at) = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (j + i < cols) at[i] = (int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+        }
+        if (j % kCkptGroup == 0) c.scales[t * c.lds + j / kCkptGroup] = (uint8_t)s;
+    }
+};
+
+inline bool aligned(const void* p, int64_t ld_bytes, int to)
+{
+    return reinterpret_cast<uintptr_t>(p) % to == 0 && ld_bytes % to == 0;
+}
+template <typename T>
+RowsIn<T> rows_in(const void* p, int64_t ld) { return {static_cast<const T*>(p), ld, aligned(p, ld * (int64_t)sizeof(T), 16)}; }
+template <typename T>
+RowsOut<T> rows_out(void* p, int64_t ld) { return {static_cast<T*>(p), ld, aligned(p, ld * (int64_t)sizeof(T), 16)}; }
+inline CkptIn ckpt_in(const chpl_ckpt8& c) { return {c, aligned(c.codes, c.ldc, 8)}; }
+inline CkptOut ckpt_out(const chpl_ckpt8& c) { return {c, aligned(c.codes, c.ldc, 8)}; }
+
+// out = f(in), row by row: a warp takes UNITS x 256 columns of a row at a time,
+// a lane 8 consecutive ones of each, every load before any arithmetic.
+constexpr int kRowsThreads = 256;
+
+template <int UNITS, typename In, typename Out, typename F>
+__global__ void __launch_bounds__(kRowsThreads) rows_kernel(In in, Out out, F f, int64_t items, uint32_t segs, int cols)
+{
+    const int lane = lane_id();
+    const int64_t step = (int64_t)gridDim.x * (kRowsThreads / 32);
+    for (int64_t i = (int64_t)blockIdx.x * (kRowsThreads / 32) + warp_id(); i < items; i += step) {
+        const int64_t t = items < 0xffffffffll ? (int64_t)((uint32_t)i / segs) : i / segs;
+        const int j0 = (int)(i - t * segs) * (UNITS * 256) + lane * 8;
+        typename In::Raw raw[UNITS];
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) raw[u] = in.raw(t, j0 + u * 256, cols);
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            float v[8];
+            in.value(raw[u], v);
+            f(v);
+            out.put(t, j0 + u * 256, cols, v);
+        }
+    }
+}
+
+struct Keep {
+    __device__ __forceinline__ void operator()(float (&)[8]) const {}
+};
+
+template <typename In, typename Out, typename F>
+int run_rows(cudaStream_t st, const In& in, const Out& out, const F& f, int64_t rows, int64_t cols)
+{
+    constexpr int64_t kBlocks = 148 * 8, kWarps = kRowsThreads / 32;  // eight resident blocks per SM, then a grid stride
+    // long rows in pieces of four units, as long as that leaves every warp a piece
+    const int64_t segs4 = (cols + 1023) / 1024, segs1 = (cols + 255) / 256;
+    const bool wide = cols > 256 && rows * segs4 >= kBlocks * kWarps;
+    const int64_t segs = wide ? segs4 : segs1, items = rows * segs, blocks = (items + kWarps - 1) / kWarps;
+    const unsigned grid = (unsigned)(blocks < kBlocks ? blocks : kBlocks);
+    if (wide) rows_kernel<4><<<grid, kRowsThreads, 0, st>>>(in, out, f, items, (uint32_t)segs, (int)cols);
+    else rows_kernel<1><<<grid, kRowsThreads, 0, st>>>(in, out, f, items, (uint32_t)segs, (int)cols);
+    CHPL_CUDA(cudaGetLastError());
+    return CHPL_OK;
+}
 
 }  // namespace chpl

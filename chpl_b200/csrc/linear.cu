@@ -7,7 +7,7 @@
 // products dX = G W and dW = G^T Xv.
 #include "linear.h"
 
-#include <algorithm>
+#include <type_traits>
 
 #include "linear_epilogue.cuh"
 
@@ -60,81 +60,120 @@ static int check_work(const char* who, const void* work, size_t have, size_t nee
     return CHPL_OK;
 }
 
-unsigned grid_for(int64_t items, int64_t per_block)
-{
-    const int64_t want = (items + per_block - 1) / per_block;
-    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(want, 148 * 16));
-}
-
 // ----------------------------------------------------------------------------
 // elementwise kernels
 // ----------------------------------------------------------------------------
-constexpr int kEltThreads = 256;
+struct Activate {
+    int act;
+    __device__ __forceinline__ void operator()(float (&v)[8]) const
+    {
+        with_act(act, [&](auto tag) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = activate<decltype(tag)::value>(v[i]);
+        });
+    }
+};
 
-// rows x cols, out = act(in), in 16-bit or a checkpoint: rows that TMA can read
-template <typename T, bool CKPT>
-__global__ void __launch_bounds__(kEltThreads) expand_kernel(const T* __restrict__ x, int64_t ldx, chpl_ckpt8 c, int act,
-                                                             int64_t rows, int cols, T* __restrict__ out, int64_t ldo)
+// A layer's incoming gradient: G = dY * act'(Z) into g (where given), and the
+// sums of its columns over kSumRows rows at a time into part[chunk][n] (or,
+// when there is one chunk, into db itself).  One pass over dY and Z: HBM-bound.
+//
+// A block takes 256 columns (a lane 8 consecutive ones) of one chunk, its warps
+// every eighth row of it; their sums meet in shared memory, always in the same
+// order.
+constexpr int kSumRows = 128;
+constexpr int kSumThreads = 256;
+constexpr int kSumWarps = kSumThreads / 32;
+
+// db, of the operands' type T or FP32
+struct Sums {
+    void* db;
+    int f32, accumulate;
+};
+
+template <typename T>
+__device__ __forceinline__ void put_sum(const Sums& s, int j, float v)
 {
-    const int64_t total = rows * cols, step = (int64_t)gridDim.x * kEltThreads;
-    for (int64_t i = (int64_t)blockIdx.x * kEltThreads + threadIdx.x; i < total; i += step) {
-        const int64_t t = i / cols;
-        const int j = (int)(i - t * cols);
-        if (!CKPT && act == CHPL_ACT_NONE) {  // a plain copy keeps every bit
-            out[t * ldo + j] = x[t * ldx + j];
-            continue;
-        }
-        float v = CKPT ? (float)c.codes[t * c.ldc + j] * ckpt_step(c.scales[t * c.lds + j / kCkptGroup])
-                       : to_f32(x[t * ldx + j]);
-        with_act(act, [&](auto tag) { v = activate<decltype(tag)::value>(v); });
-        out[t * ldo + j] = from_f32<T>(v);
+    if (s.f32) {
+        float* o = static_cast<float*>(s.db) + j;
+        *o = s.accumulate ? *o + v : v;
+    } else {
+        T* o = static_cast<T*>(s.db) + j;
+        *o = from_f32<T>(s.accumulate ? to_f32(*o) + v : v);
     }
 }
 
-// G = dY * act'(Z) into g (where given), and the sums of its columns over each
-// chunk of kSumRows rows into part[chunk][n]
-constexpr int kSumRows = 64;
+struct NoZ {
+    struct Raw {};
+    __device__ __forceinline__ Raw raw(int64_t, int, int) const { return {}; }
+    __device__ __forceinline__ void value(const Raw&, float (&)[8]) const {}
+};
 
-template <typename T, bool CKPT>
-__global__ void __launch_bounds__(kEltThreads) grad_act_kernel(const T* __restrict__ dy, int64_t lddy,
-                                                               const T* __restrict__ z, int64_t ldz, chpl_ckpt8 z8,
-                                                               int act, int rows, int n, T* __restrict__ g, int64_t ldg,
-                                                               float* __restrict__ part)
+template <typename T, typename Z>
+__global__ void __launch_bounds__(kSumThreads) grad_act_kernel(RowsIn<T> dy, Z z, int act, int rows, int n, RowsOut<T> g,
+                                                               float* __restrict__ part, Sums out)
 {
-    const int j = blockIdx.x * kEltThreads + threadIdx.x;
-    if (j >= n) return;
-    const int chunks = (rows + kSumRows - 1) / kSumRows;
-    for (int ch = blockIdx.y; ch < chunks; ch += gridDim.y) {
-        float sum = 0.0f;
-        const int end = min(rows, (ch + 1) * kSumRows);
-        for (int t = ch * kSumRows; t < end; ++t) {
-            float v = to_f32(dy[t * lddy + j]);
-            if (act != CHPL_ACT_NONE) {
-                const float zv = CKPT ? (float)z8.codes[t * z8.ldc + j] * ckpt_step(z8.scales[t * z8.lds + j / kCkptGroup])
-                                      : to_f32(z[t * ldz + j]);
-                with_act(act, [&](auto tag) {
-                    float slope, value;
-                    slope_and_value<decltype(tag)::value>(zv, slope, value);
-                    v *= slope;
-                });
+    constexpr int kAhead = 2;  // rows whose loads are under way at once
+    __shared__ float sums[kSumWarps][256 + 8];
+    const int blocks = (n + 255) / 256, chunk = blockIdx.x / blocks, j0 = (blockIdx.x - chunk * blocks) * 256;
+    const int lane = lane_id(), warp = warp_id(), j = j0 + lane * 8;
+    const int64_t first = (int64_t)chunk * kSumRows;
+    const int count = (int)min((int64_t)kSumRows, rows - first);
+    float sum[8] = {};
+    for (int r = warp; r < count; r += kAhead * kSumWarps) {
+        typename RowsIn<T>::Raw a[kAhead];
+        typename Z::Raw b[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (r + u * kSumWarps < count) {
+                a[u] = dy.raw(first + r + u * kSumWarps, j, n);
+                b[u] = z.raw(first + r + u * kSumWarps, j, n);
             }
-            if (g) g[t * ldg + j] = from_f32<T>(v);
-            sum += v;
-        }
-        if (part) part[(int64_t)ch * n + j] = sum;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (r + u * kSumWarps < count) {
+                float v[8];
+                dy.value(a[u], v);
+                if (!std::is_same<Z, NoZ>::value) {
+                    float zv[8];
+                    z.value(b[u], zv);
+                    with_act(act, [&](auto tag) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float slope, value;
+                            slope_and_value<decltype(tag)::value>(zv[i], slope, value);
+                            v[i] *= slope;
+                        }
+                    });
+                }
+                if (g.p) g.put(first + r + u * kSumWarps, j, n, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[i] += v[i];
+            }
     }
+    if (!out.db) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sums[warp][lane * 8 + i] = sum[i];
+    __syncthreads();
+    const int c = threadIdx.x, col = j0 + c;
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kSumWarps; ++w) total += sums[w][c];
+    if (col >= n) return;
+    if (part) part[(int64_t)chunk * n + col] = total;
+    else put_sum<T>(out, col, total);
 }
 
 // db[j] (+)= sum of part[0..chunks)[j], in order
 template <typename T>
-__global__ void __launch_bounds__(kEltThreads) sum_chunks_kernel(const float* __restrict__ part, int chunks, int n,
-                                                                 T* __restrict__ db, int accumulate)
+__global__ void __launch_bounds__(kSumThreads) sum_chunks_kernel(const float* __restrict__ part, int chunks, int n, Sums out)
 {
-    const int j = blockIdx.x * kEltThreads + threadIdx.x;
+    const int j = blockIdx.x * kSumThreads + threadIdx.x;
     if (j >= n) return;
     float sum = 0.0f;
+#pragma unroll 8
     for (int ch = 0; ch < chunks; ++ch) sum += part[(int64_t)ch * n + j];
-    db[j] = from_f32<T>(accumulate ? to_f32(db[j]) + sum : sum);
+    put_sum<T>(out, j, sum);
 }
 
 // ----------------------------------------------------------------------------
@@ -200,7 +239,7 @@ struct BackwardPlan {
     Staged g, w, x;
     bool need_xv;   // Xv is not X as it stands
     size_t part;
-    int chunks;
+    int chunks;  // of kSumRows tokens: partial sums of db
     size_t bytes;
 };
 
@@ -214,8 +253,8 @@ static BackwardPlan plan(const chpl_linear_bwd& a)
     p.w = stage(m, products && a.dx && !tma_rows(a.w, a.ldw, a.n), a.ldw, a.n, a.k);
     p.need_xv = a.x8.codes || a.in_act != CHPL_ACT_NONE || !tma_rows(a.x, a.ldx, a.tokens);
     p.x = stage(m, products && a.dw && p.need_xv, a.ldx, a.tokens, a.k);
-    p.chunks = (int)((a.tokens + kSumRows - 1) / kSumRows);
-    p.part = a.db && a.n > 0 ? m.take((size_t)p.chunks * a.n * 4) : 0;
+    p.chunks = (int)((a.tokens + kSumRows - 1) / kSumRows);  // <= 2^23
+    p.part = a.db && a.n > 0 && p.chunks != 1 ? m.take((size_t)p.chunks * a.n * 4) : 0;
     p.bytes = m.used;
     return p;
 }
@@ -283,18 +322,15 @@ static int check(const char* who, const chpl_linear_bwd* a, bool pointers)
 // ----------------------------------------------------------------------------
 // the two passes
 // ----------------------------------------------------------------------------
+// the operand of a product as TMA can read it: values of a checkpoint, an
+// activation of either, or a copy
 template <typename T>
 static int expand(cudaStream_t st, const void* x, int64_t ldx, const chpl_ckpt8& c, int act, int64_t rows, int64_t cols,
                   void* out, int64_t ldo)
 {
-    const unsigned grid = grid_for(rows * cols, kEltThreads);
-    if (c.codes)
-        expand_kernel<T, true><<<grid, kEltThreads, 0, st>>>(nullptr, 0, c, act, rows, (int)cols, static_cast<T*>(out), ldo);
-    else
-        expand_kernel<T, false><<<grid, kEltThreads, 0, st>>>(static_cast<const T*>(x), ldx, c, act, rows, (int)cols,
-                                                              static_cast<T*>(out), ldo);
-    CHPL_CUDA(cudaGetLastError());
-    return CHPL_OK;
+    const Activate f = {act};
+    if (c.codes) return run_rows(st, ckpt_in(c), rows_out<T>(out, ldo), f, rows, cols);
+    return run_rows(st, rows_in<T>(x, ldx), rows_out<T>(out, ldo), f, rows, cols);
 }
 
 static const chpl_ckpt8 kNoCkpt = {nullptr, nullptr, 0, 0};
@@ -326,25 +362,27 @@ static int backward(cudaStream_t st, const chpl_linear_bwd& a, void* work)
     const BackwardPlan p = plan(a);
     char* wk = static_cast<char*>(work);
     if (a.n > 0 && (p.g.copy || a.db)) {
-        float* part = a.db ? reinterpret_cast<float*>(wk + p.part) : nullptr;
-        T* g = p.g.copy ? reinterpret_cast<T*>(wk + p.g.at) : nullptr;
+        const Sums sums = {a.db, a.grad_type == CHPL_TYPE_F32, a.accumulate};
+        // one chunk's sums go straight to db, several (or none: zeros) by way of the workspace
+        const bool join = a.db && p.chunks != 1;
+        float* part = join ? reinterpret_cast<float*>(wk + p.part) : nullptr;
         if (a.tokens > 0) {
-            const dim3 grid((unsigned)((a.n + kEltThreads - 1) / kEltThreads), (unsigned)std::min(p.chunks, 65535));
-            if (a.z8.codes)
-                grad_act_kernel<T, true><<<grid, kEltThreads, 0, st>>>(static_cast<const T*>(a.dy), a.lddy, nullptr, 0, a.z8,
-                                                                       a.act, (int)a.tokens, (int)a.n, g, p.g.ld, part);
+            const int64_t blocks = (a.n + 255) / 256 * p.chunks;
+            if (blocks > 0x7fffffff) { set_error("linear_backward: dy of %lld x %lld is more than one launch serves", (long long)a.tokens, (long long)a.n); return CHPL_ERR_UNSUPPORTED; }
+            const unsigned grid = (unsigned)blocks;
+            const RowsIn<T> dy = rows_in<T>(a.dy, a.lddy);
+            const RowsOut<T> go = rows_out<T>(p.g.copy ? wk + p.g.at : nullptr, p.g.ld);
+            const int rows = (int)a.tokens, n = (int)a.n;
+            if (a.act == CHPL_ACT_NONE)
+                grad_act_kernel<T><<<grid, kSumThreads, 0, st>>>(dy, NoZ(), a.act, rows, n, go, part, sums);
+            else if (a.z8.codes)
+                grad_act_kernel<T><<<grid, kSumThreads, 0, st>>>(dy, ckpt_in(a.z8), a.act, rows, n, go, part, sums);
             else
-                grad_act_kernel<T, false><<<grid, kEltThreads, 0, st>>>(static_cast<const T*>(a.dy), a.lddy,
-                                                                        static_cast<const T*>(a.z), a.ldz, a.z8, a.act,
-                                                                        (int)a.tokens, (int)a.n, g, p.g.ld, part);
+                grad_act_kernel<T><<<grid, kSumThreads, 0, st>>>(dy, rows_in<T>(a.z, a.ldz), a.act, rows, n, go, part, sums);
             CHPL_CUDA(cudaGetLastError());
         }
-        if (a.db) {
-            const unsigned blocks = (unsigned)((a.n + kEltThreads - 1) / kEltThreads);
-            if (a.grad_type == CHPL_TYPE_F32)
-                sum_chunks_kernel<float><<<blocks, kEltThreads, 0, st>>>(part, p.chunks, (int)a.n, static_cast<float*>(a.db), a.accumulate);
-            else
-                sum_chunks_kernel<T><<<blocks, kEltThreads, 0, st>>>(part, p.chunks, (int)a.n, static_cast<T*>(a.db), a.accumulate);
+        if (join) {
+            sum_chunks_kernel<T><<<(unsigned)((a.n + kSumThreads - 1) / kSumThreads), kSumThreads, 0, st>>>(part, p.chunks, (int)a.n, sums);
             CHPL_CUDA(cudaGetLastError());
         }
     }

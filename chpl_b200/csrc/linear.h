@@ -55,9 +55,6 @@ int check_size(const char* who, const char* what, int64_t v);
 int check_operand(const char* who, const char* what, const void* p, int64_t ld, int64_t width, int elt);
 int check_ckpt(const char* who, const char* what, const chpl_ckpt8& c, int64_t width);
 
-// blocks for `items` units of work at `per_block` each: enough to fill the GPU several times over
-unsigned grid_for(int64_t items, int64_t per_block);
-
 int read_clear_status(int* st);
 
 }  // namespace linear

@@ -121,7 +121,7 @@ __device__ __forceinline__ void epilogue(const Epilogue& e, int f, int t0, float
             for (int j = 0; j < NB; ++j) {
                 const uint32_t bits = ok ? __float_as_uint(v[j]) & 0x7fffffffu : 0u;
                 const uint32_t s = ckpt_scale(__reduce_max_sync(0xffffffffu, bits));
-                const int code = ckpt_code(v[j], ckpt_inv_step(s));
+                const uint32_t code = s == kCkptBadScale ? 0u : ckpt_code(v[j], ckpt_inv_step(s));
                 if (ok && j < nt) {
                     o[j * e.z8.ldc] = (int8_t)code;
                     if ((f & (kCkptGroup - 1)) == 0) os[j * e.z8.lds] = (uint8_t)s;
