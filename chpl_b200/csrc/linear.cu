@@ -388,7 +388,9 @@ static int backward(cudaStream_t st, const chpl_linear_bwd& a, void* work)
     }
     if (a.k == 0) return CHPL_OK;
     const Operand g_rows = {at(p.g, a.dy, work), p.g.ld, true}, g_cols = {g_rows.p, p.g.ld, false};
-    if (p.x.copy) CHPL_TRY(expand<T>(st, a.x, a.ldx, a.x8, a.in_act, a.tokens, a.k, wk + p.x.at, p.x.ld));
+    // an activation's value comes with its slope out of dX's epilogue
+    const bool xv_from_dx = p.x.copy && a.dx && a.in_act != CHPL_ACT_NONE;
+    if (p.x.copy && !xv_from_dx) CHPL_TRY(expand<T>(st, a.x, a.ldx, a.x8, a.in_act, a.tokens, a.k, wk + p.x.at, p.x.ld));
     if (a.dx) {
         if (p.w.copy) CHPL_TRY(expand<T>(st, a.w, a.ldw, kNoCkpt, CHPL_ACT_NONE, a.n, a.k, wk + p.w.at, p.w.ld));
         Epilogue e = {};
@@ -402,6 +404,8 @@ static int backward(cudaStream_t st, const chpl_linear_bwd& a, void* work)
         e.z = const_cast<void*>(a.x);
         e.ldz = a.ldx;
         e.z8 = a.x8;
+        e.xv = xv_from_dx ? wk + p.x.at : nullptr;
+        e.ldxv = p.x.ld;
         CHPL_TRY(gemm(st, a.type, kGradInput, {at(p.w, a.w, work), p.w.ld, false}, g_rows, a.n, e));
     }
     if (a.dw && (a.tokens > 0 || !a.accumulate)) {
@@ -409,9 +413,10 @@ static int backward(cudaStream_t st, const chpl_linear_bwd& a, void* work)
         e.m = (int)a.k;
         e.n = (int)a.n;
         e.out_f32 = a.grad_type == CHPL_TYPE_F32;
-        e.accumulate = a.accumulate;
         e.out = a.dw;
         e.ldo = a.lddw;
+        e.add = a.accumulate ? a.dw : nullptr;
+        e.ldadd = a.lddw;
         CHPL_TRY(gemm(st, a.type, kGradWeight, {at(p.x, a.x, work), p.x.ld, false}, g_cols, a.tokens, e));
     }
     return CHPL_OK;

@@ -20,14 +20,13 @@ constexpr int64_t kMaxLd = (int64_t)1 << 32;
 enum Kind {
     kForward = 0,     // Y[t][f] = act(D + bias[f]) + add[t][f]; z / z8 keep D + bias
     kGradInput = 1,   // dX[t][f] = D * act'(z[t][f]) + add[t][f]; z comes in 16 bits or as z8; xv keeps act(z)
-    kGradWeight = 2,  // dW[t][f] (+)= D
+    kGradWeight = 2,  // dW[t][f] = D + add[t][f] (add: dW itself, of its type)
 };
 
 struct Epilogue {
     int m, n;        // f < m, t < n
     int act;
     int out_f32;     // out is FP32 (kGradWeight), else of the operands' type
-    int accumulate;  // out += (kGradWeight)
     void* out;
     int64_t ldo;
     const void* bias;

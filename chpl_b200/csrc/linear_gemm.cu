@@ -231,28 +231,37 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
         }
         __syncwarp();
     }
-    // every MMA of this CTA has completed (so every copy has landed and been read)
-    bool ok = true;
-    if (kb1 > kb0) ok = mbar_wait(done, 0, abort_flag);
-    ok = __all_sync(0xffffffffu, ok);
-    tc_fence_after();
-
     const int quarter = warp & 3, half = warp >> 2;
     const int f = f0 + quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int rows = min(sh.bn, e.n - t0);  // rows of this tile that exist
     const float bias = bias_of<T>(e, f);
+    Fetched<16> ahead;
+    Fetched<JOIN> ahead_join;
+    const int c_join = (rank * 2 + half) * JOIN;
+    if (sh.split == 1) {
+        if (half * 16 < rows) fetch<T, KIND, 16>(e, f, t0 + half * 16, ahead);
+    } else if (c_join < rows) {
+        fetch<T, KIND, JOIN>(e, f, t0 + c_join, ahead_join);
+    }
+
+    // every MMA of this CTA has completed (so every copy has landed and been read)
+    bool ok = true;
+    if (kb1 > kb0) ok = mbar_wait(done, 0, abort_flag);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
     if (sh.split == 1) {
         for (int c = half * 16; c < rows; c += 32) {
             float v[16];
-            if (kb1 > kb0) {
+            if (kblocks > 0) {
                 __syncwarp();
                 tmem_ld_x16(tmem + lanes + c, v);
             } else {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = 0.0f;
             }
-            if (ok) epilogue<T, KIND, 16>(e, f, t0 + c, v, bias);
+            if (ok) finish<T, KIND, 16>(e, f, t0 + c, v, bias, ahead);
+            if (c + 32 < rows) fetch<T, KIND, 16>(e, f, t0 + c + 32, ahead);
         }
     } else {
         // partial sums as [row][128 features] into the ring's shared memory
@@ -266,14 +275,16 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
         }
         cluster_sync();
         const uint32_t mine = smem_u32(part + quarter * 32 + lane);
-        for (int c = (rank * 2 + half) * JOIN; c < rows; c += sh.split * 2 * JOIN) {
+        const int step = sh.split * 2 * JOIN;
+        for (int c = c_join; c < rows; c += step) {
             float v[JOIN] = {};
             for (int r = 0; r < sh.split; ++r) {
                 const uint32_t peer = map_to_rank(mine + c * BM * 4, (uint32_t)r);
 #pragma unroll
                 for (int j = 0; j < JOIN; ++j) v[j] += ld_cluster_f32(peer + j * BM * 4);
             }
-            if (ok) epilogue<T, KIND, JOIN>(e, f, t0 + c, v, bias);
+            if (ok) finish<T, KIND, JOIN>(e, f, t0 + c, v, bias, ahead_join);
+            if (c + step < rows) fetch<T, KIND, JOIN>(e, f, t0 + c + step, ahead_join);
         }
         cluster_sync();  // no CTA leaves while another still reads its sums
     }
@@ -442,12 +453,15 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         __syncwarp();
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const int f_in = (int)rank * BM + quarter * 32 + lane;  // feature within a tile
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         uint32_t acc = 0;
+        int mt, nt;
+        pair_tile(sh, unit, mt, nt);
+        Fetched<16> ahead;  // what the next 16 rows need
+        if (nt * sh.bn + half * 16 < e.n) fetch<T, KIND, 16>(e, mt * 2 * BM + f_in, nt * sh.bn + half * 16, ahead);
         for (int tile = unit; tile < total; tile += nunits, ++acc) {
-            int mt, nt;
-            pair_tile(sh, tile, mt, nt);
-            const int f = mt * 2 * BM + (int)rank * BM + quarter * 32 + lane, t0 = nt * sh.bn;
+            const int f = mt * 2 * BM + f_in, t0 = nt * sh.bn;
             const uint32_t buf = acc & 1u, aph = (acc >> 1) & 1u;
             const float bias = bias_of<T>(e, f);
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aph, abort_flag))) break;
@@ -455,12 +469,17 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
             for (int c = half * 16; c < sh.bn; c += 32) {
                 float v[16];
                 tmem_ld_x16(tmem + lanes + buf * 256 + c, v);
-                if (c + 32 >= sh.bn) {  // this warp's last columns are in registers
+                const bool last = c + 32 >= sh.bn;
+                if (last) {  // this warp's last columns are in registers
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(lead_acc_empty + buf * 8);
+                    if (tile + nunits < total) pair_tile(sh, tile + nunits, mt, nt);
                 }
-                if (t0 + c < e.n) epilogue<T, KIND, 16>(e, f, t0 + c, v, bias);
+                const Fetched<16> now = ahead;
+                const int fn = mt * 2 * BM + f_in, tn = last ? nt * sh.bn + half * 16 : t0 + c + 32;
+                if ((!last || tile + nunits < total) && tn < e.n) fetch<T, KIND, 16>(e, fn, tn, ahead);
+                if (t0 + c < e.n) finish<T, KIND, 16>(e, f, t0 + c, v, bias, now);
                 __syncwarp();
             }
         }
