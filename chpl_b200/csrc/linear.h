@@ -27,6 +27,7 @@ struct Epilogue {
     int m, n;        // f < m, t < n
     int act;
     int out_f32;     // out is FP32 (kGradWeight), else of the operands' type
+    bool vec_out, vec_add, vec_z, vec_codes;  // 16-byte (8 for codes) accesses fit; set by gemm()
     void* out;
     int64_t ldo;
     const void* bias;

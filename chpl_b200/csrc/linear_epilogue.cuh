@@ -90,137 +90,363 @@ __device__ __forceinline__ void with_act(int act, F&& f)
     }
 }
 
-// The epilogue of one thread: its feature f (lane l of a warp holds f0 + l, f0
-// a multiple of 32, so a warp holds one checkpoint group) and NB consecutive
-// rows t0 .. t0 + NB - 1 (NB <= 32).  Every lane of the warp calls both halves.  Each store or
-// load of a row is one coalesced access of the warp (64 bytes in 16 bits).
+// ----------------------------------------------------------------------------
+// The epilogue of one warp: 32 features from f0 (a multiple of 32, so a warp
+// holds whole checkpoint groups) by NCB blocks of 8 rows from t0.
 //
-// What it reads (an addend, a pre-activation) is fetched in a call of its own,
-// ahead of the accumulators, so that the loads run under the products or under
-// the arithmetic of the previous rows: one round trip to memory per 16 rows,
-// taken one after another, is longer than a tile's products.
-template <int NB>
+// The accumulators come as tcgen05.ld's 16x256b fragments, laid out like an
+// mma accumulator: element (h, cb, rr, p) of lane l is feature 16 h + 8 rr + l/4
+// and row 8 cb + 2 (l % 4) + p.  A pair of rows packs into one register, so
+// stmatrix / ldmatrix with .trans turn 8 x 8 blocks between fragments and rows
+// of 8 consecutive features in shared memory, and global memory is read and
+// written 16 bytes a lane: row l / 4 of a block, features 8 (l % 4) to + 7
+// ("line" order).  Per 32 outputs that is about two instructions beyond the
+// arithmetic; a store of 2 bytes per lane and row took over twenty and bounded
+// every product with a short contraction.
+//
+// What the epilogue reads (an addend, a pre-activation) is fetched ahead of the
+// accumulators: for a warp's first rows before it waits for them, for the others
+// as soon as the rows before have taken theirs out of the registers.  READS is
+// false where there is nothing to read.
+// ----------------------------------------------------------------------------
+constexpr int kStageBytes = 2048;  // a warp's shared memory: 32 rows of 64 bytes
+
+template <int NCB>
 struct Fetched {
-    uint32_t add[NB];  // raw bits: 16-bit, or FP32
-    uint32_t z[NB];    // raw bits: 16-bit, or a code
-    uint32_t scale;    // lane j: the scale of row j's group
+    uint4 add[NCB];          // line order, 16-bit
+    float add32[8 * NCB];    // fragment order (FP32 gradients)
+    uint4 z[NCB];            // line order: 16-bit, or codes in x and y
+    uint32_t scale[NCB];     // of row l / 4 of each block
 };
 
-template <typename T>
-__device__ __forceinline__ float from_bits(uint32_t b)
+template <int NCB>
+__device__ __forceinline__ constexpr int frag(int h, int cb, int rr, int p) { return (h * NCB + cb) * 4 + rr * 2 + p; }
+
+// eight 16-bit elements of row t from feature f, zero where there are none
+__device__ __forceinline__ uint4 line16(const void* base, int64_t ld, int64_t t, int f, int n, int m, bool vec)
 {
-    const unsigned short h = (unsigned short)b;
-    return to_f32(reinterpret_cast<const T&>(h));
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (t >= n || f >= m) return w;
+    const unsigned short* at = static_cast<const unsigned short*>(base) + t * ld + f;
+    if (vec && f + 8 <= m) return *reinterpret_cast<const uint4*>(at);
+    uint32_t* u = &w.x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (f + i < m) u[i >> 1] |= (uint32_t)at[i] << (16 * (i & 1));
+    return w;
 }
 
-template <typename T, Kind KIND, int NB>
-__device__ __forceinline__ void fetch(const Epilogue& e, int f, int t0, Fetched<NB>& x)
+// where a warp goes after these rows; f0 < 0: nowhere
+struct Next {
+    int f0, t0;
+};
+
+template <typename T, Kind KIND, int NCB>
+__device__ __forceinline__ void fetch(const Epilogue& e, int f0, int t0, Fetched<NCB>& x)
 {
-    const bool ok = f < e.m;
-    const int nt = min(NB, e.n - t0);
+    const int lane = lane_id(), f = f0 + 8 * (lane & 3);
     if (e.add) {
         if (KIND == kGradWeight && e.out_f32) {
-            const uint32_t* a = static_cast<const uint32_t*>(e.add) + (int64_t)t0 * e.ldadd + f;
 #pragma unroll
-            for (int j = 0; j < NB; ++j) x.add[j] = ok && j < nt ? a[j * e.ldadd] : 0u;
+            for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const int t = t0 + 8 * cb + 2 * (lane & 3) + p;
+                    const float* a = static_cast<const float*>(e.add) + (int64_t)t * e.ldadd + f0 + (lane >> 2);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        x.add32[frag<NCB>(g >> 1, cb, g & 1, p)] = t < e.n && f0 + (lane >> 2) + 8 * g < e.m ? a[8 * g] : 0.0f;
+                }
         } else {
-            const unsigned short* a = static_cast<const unsigned short*>(e.add) + (int64_t)t0 * e.ldadd + f;
 #pragma unroll
-            for (int j = 0; j < NB; ++j) x.add[j] = ok && j < nt ? a[j * e.ldadd] : 0u;
+            for (int cb = 0; cb < NCB; ++cb) x.add[cb] = line16(e.add, e.ldadd, t0 + 8 * cb + (lane >> 2), f, e.n, e.m, e.vec_add);
         }
     }
     if (KIND == kGradInput && e.act != CHPL_ACT_NONE) {
-        if (e.z8.codes) {
-            const uint8_t* c = reinterpret_cast<const uint8_t*>(e.z8.codes) + (int64_t)t0 * e.z8.ldc + f;
 #pragma unroll
-            for (int j = 0; j < NB; ++j) x.z[j] = ok && j < nt ? c[j * e.z8.ldc] : 0u;
-            const int lane = lane_id(), g = f - lane;
-            x.scale = g < e.m && lane < nt ? e.z8.scales[(int64_t)(t0 + lane) * e.z8.lds + g / kCkptGroup] : kCkptMinScale;
-        } else {
-            const unsigned short* z = static_cast<const unsigned short*>(e.z) + (int64_t)t0 * e.ldz + f;
-#pragma unroll
-            for (int j = 0; j < NB; ++j) x.z[j] = ok && j < nt ? z[j * e.ldz] : 0u;
+        for (int cb = 0; cb < NCB; ++cb) {
+            const int64_t t = t0 + 8 * cb + (lane >> 2);
+            if (!e.z8.codes) {
+                x.z[cb] = line16(e.z, e.ldz, t, f, e.n, e.m, e.vec_z);
+                continue;
+            }
+            const CkptIn::Raw r = CkptIn{e.z8, e.vec_codes}.raw(t < e.n ? t : 0, t < e.n ? f : e.m, e.m);
+            x.z[cb] = make_uint4(r.w.x, r.w.y, 0, 0);
+            x.scale[cb] = r.s;
         }
     }
 }
 
-template <typename T, int NB>
-__device__ __forceinline__ void put_rows(void* out, int64_t ld, int f, int t0, int nt, const float (&v)[NB])
-{
-    T* o = static_cast<T*>(out) + (int64_t)t0 * ld + f;
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-        if (j < nt) o[j * ld] = from_f32<T>(v[j]);
-}
+// byte offset of row t's features 8 c .. 8 c + 7 (16-bit) in a staged matrix of
+// 64-byte rows: the 16-byte pieces of every other row are swapped about, so
+// that eight rows' pieces fall into different banks
+__device__ __forceinline__ uint32_t staged(int t, int c) { return (uint32_t)(t * 64 + ((c ^ ((t >> 1) & 3)) << 4)); }
 
-template <typename T, Kind KIND, int NB>
-__device__ __forceinline__ void finish(const Epilogue& e, int f, int t0, float (&v)[NB], float bias, const Fetched<NB>& x)
+// line order -> fragments of two rows each, through `at` (shared)
+template <int NCB>
+__device__ __forceinline__ void to_fragments(uint32_t at, const uint4 (&line)[NCB], uint32_t (&r)[4 * NCB])
 {
-    const bool ok = f < e.m;
-    const int nt = ok ? min(NB, e.n - t0) : 0;  // rows this lane stores
-    if (KIND == kGradWeight) {
-        if (e.out_f32) {
-            if (e.add) {
+    const int lane = lane_id();
+    __syncwarp();  // the warp's reads of what was staged before are over
 #pragma unroll
-                for (int j = 0; j < NB; ++j) v[j] += __uint_as_float(x.add[j]);
-            }
-            put_rows<float, NB>(e.out, e.ldo, f, t0, nt, v);
-            return;
-        }
-    } else if (KIND == kForward) {
+    for (int cb = 0; cb < NCB; ++cb)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + staged(8 * cb + (lane >> 2), lane & 3)),
+                     "r"(line[cb].x), "r"(line[cb].y), "r"(line[cb].z), "r"(line[cb].w)
+                     : "memory");
+    __syncwarp();
 #pragma unroll
-        for (int j = 0; j < NB; ++j) v[j] += bias;
-        if (e.z) put_rows<T, NB>(e.z, e.ldz, f, t0, nt, v);
-        if (e.z8.codes) {
-            const int lane = lane_id(), g = f - lane;
-            int8_t* o = e.z8.codes + (int64_t)t0 * e.z8.ldc + f;
-            uint32_t mine = 0;  // lane j: the scale of row j
-#pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                const uint32_t bits = ok ? __float_as_uint(v[j]) & 0x7fffffffu : 0u;
-                const uint32_t s = ckpt_scale(__reduce_max_sync(0xffffffffu, bits));
-                const uint32_t code = s == kCkptBadScale ? 0u : ckpt_code(v[j], ckpt_inv_step(s));
-                mine = lane == j ? s : mine;
-                if (j < nt) o[j * e.z8.ldc] = (int8_t)code;
-            }
-            if (g < e.m && lane < min(NB, e.n - t0))
-                e.z8.scales[(int64_t)(t0 + lane) * e.z8.lds + g / kCkptGroup] = (uint8_t)mine;
-        }
-        with_act(e.act, [&](auto tag) {
-#pragma unroll
-            for (int j = 0; j < NB; ++j) v[j] = activate<decltype(tag)::value>(v[j]);
-        });
-    } else if (e.act != CHPL_ACT_NONE) {
-        float z[NB];
-        if (e.z8.codes) {
-            const float step = ckpt_step(x.scale);
-#pragma unroll
-            for (int j = 0; j < NB; ++j) z[j] = ckpt_value(x.z[j] ^ 0x80u, 0, __shfl_sync(0xffffffffu, step, j));
-        } else {
-#pragma unroll
-            for (int j = 0; j < NB; ++j) z[j] = from_bits<T>(x.z[j]);
-        }
-        with_act(e.act, [&](auto tag) {
-#pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                float slope;
-                slope_and_value<decltype(tag)::value>(z[j], slope, z[j]);
-                v[j] *= slope;
-            }
-        });
-        if (e.xv) put_rows<T, NB>(e.xv, e.ldxv, f, t0, nt, z);
-    }
-    if (e.add) {
-#pragma unroll
-        for (int j = 0; j < NB; ++j) v[j] += from_bits<T>(x.add[j]);
-    }
-    put_rows<T, NB>(e.out, e.ldo, f, t0, nt, v);
+    for (int cb = 0; cb < NCB; ++cb)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[4 * cb]), "=r"(r[4 * cb + 1]), "=r"(r[4 * cb + 2]), "=r"(r[4 * cb + 3])
+                     : "r"(at + staged(8 * cb + (lane & 7), lane >> 3))
+                     : "memory");
 }
 
 template <typename T>
-__device__ __forceinline__ float bias_of(const Epilogue& e, int f)
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w)
 {
-    return e.bias && f < e.m ? to_f32(static_cast<const T*>(e.bias)[f]) : 0.0f;
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w)
+{
+    return __half22float2(reinterpret_cast<const __half2&>(w));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
+{
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return reinterpret_cast<const uint32_t&>(v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
+{
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return reinterpret_cast<const uint32_t&>(v);
+}
+
+// v (fragments) as 16-bit rows of `out`, through `at` (shared)
+template <typename T, int NCB>
+__device__ __forceinline__ void put16(const Epilogue& e, void* out, int64_t ld, bool vec, int f0, int t0, uint32_t at,
+                                      const float (&v)[8 * NCB])
+{
+    const int lane = lane_id();
+    __syncwarp();
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+        uint32_t w[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) w[g] = pack2<T>(v[frag<NCB>(g >> 1, cb, g & 1, 0)], v[frag<NCB>(g >> 1, cb, g & 1, 1)]);
+        asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                         at + staged(8 * cb + (lane & 7), lane >> 3)),
+                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                     : "memory");
+    }
+    __syncwarp();
+    unsigned short* o = static_cast<unsigned short*>(out) + (int64_t)t0 * ld + f0;
+    if (vec && f0 + 32 <= e.m) {
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
+            const int t = 8 * cb + (lane >> 2);
+            uint4 w;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                         : "r"(at + staged(t, lane & 3))
+                         : "memory");
+            if (t0 + t < e.n) *reinterpret_cast<uint4*>(o + t * ld + 8 * (lane & 3)) = w;
+        }
+    } else {  // rows that 16-byte stores cannot start on, and the last features: a lane per feature
+        const int rows = min(8 * NCB, e.n - t0);
+        if (f0 + lane < e.m) {
+#pragma unroll 4
+            for (int t = 0; t < rows; ++t) {
+                unsigned short w;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(at + staged(t, lane >> 3) + 2 * (lane & 7)) : "memory");
+                o[t * ld + lane] = w;
+            }
+        }
+    }
+}
+
+// codes and scales of v, through `at` (shared, 32-byte rows)
+template <int NCB>
+__device__ __forceinline__ void put_ckpt(const Epilogue& e, int f0, int t0, uint32_t at, const float (&v)[8 * NCB])
+{
+    const int lane = lane_id();
+    const bool whole = f0 + 32 <= e.m;
+    uint32_t scale[2 * NCB], worst = 0;
+    __syncwarp();
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            // the row's group: four features in this lane, the others in the lanes of the same l % 4
+            uint32_t top = 0;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const uint32_t bits = __float_as_uint(v[frag<NCB>(g >> 1, cb, g & 1, p)]) & 0x7fffffffu;
+                top = max(top, whole || f0 + (lane >> 2) + 8 * g < e.m ? bits : 0u);
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const uint32_t s = ckpt_scale(top);
+            scale[2 * cb + p] = s;
+            worst = max(worst, s);
+            const float inv = ckpt_inv_step(s);
+            const uint32_t row = at + (8 * cb + 2 * (lane & 3) + p) * 32 + (lane >> 2);
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                asm volatile("st.shared.u8 [%0], %1;" ::"r"(row + 8 * g), "r"(ckpt_code(v[frag<NCB>(g >> 1, cb, g & 1, p)], inv))
+                             : "memory");
+        }
+    if (__any_sync(0xffffffffu, worst == kCkptBadScale)) {  // rows with an infinity or a NaN in the group: codes 0
+#pragma unroll
+        for (int i = 0; i < 2 * NCB; ++i)
+            if (scale[i] == kCkptBadScale) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(at + (8 * (i >> 1) + 2 * (lane & 3) + (i & 1)) * 32 + (lane >> 2) + 8 * g),
+                                 "r"(0u)
+                                 : "memory");
+            }
+    }
+    if (lane < 4) {
+        uint8_t* o = e.z8.scales + (int64_t)(t0 + 2 * lane) * e.z8.lds + f0 / kCkptGroup;
+#pragma unroll
+        for (int i = 0; i < 2 * NCB; ++i) {
+            const int t = 8 * (i >> 1) + (i & 1);
+            if (t0 + 2 * lane + t < e.n) o[t * e.z8.lds] = (uint8_t)scale[i];
+        }
+    }
+    __syncwarp();
+    int8_t* o = e.z8.codes + (int64_t)t0 * e.z8.ldc + f0;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+        const int t = 8 * cb + (lane >> 2), f = 8 * (lane & 3);
+        uint2 w;
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "r"(at + t * 32 + f) : "memory");
+        if (t0 + t >= e.n) continue;
+        if (e.vec_codes && whole) {
+            *reinterpret_cast<uint2*>(o + t * e.z8.ldc + f) = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (f0 + f + i < e.m) o[t * e.z8.ldc + f + i] = (int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+        }
+    }
+}
+
+// Every lane of the warp calls it.  bias[2 h + rr]; `stage`: kStageBytes of
+// shared memory of the warp's own (shared-space address, 128-byte aligned).
+// READS: x holds what these rows read, and what the rows `next` do on return.
+template <typename T, Kind KIND, bool READS, int NCB>
+__device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float (&v)[8 * NCB], const float (&bias)[4],
+                                       Fetched<NCB>& x, Next next, uint32_t stage)
+{
+    static_assert(NCB * 8 * 64 <= kStageBytes, "stage");
+    const int lane = lane_id();
+    const bool here = f0 < e.m && t0 < e.n;
+    uint32_t add[4 * NCB], zf[4 * NCB];
+    if (READS && here) {
+        if (KIND == kGradWeight && e.out_f32) {
+            if (e.add) {
+#pragma unroll
+                for (int i = 0; i < 8 * NCB; ++i) v[i] += x.add32[i];
+            }
+        } else if (e.add) {
+            to_fragments<NCB>(stage, x.add, add);
+        }
+        if (KIND == kGradInput && e.act != CHPL_ACT_NONE) {
+            if (e.z8.codes) {
+                // a code times its step is exact in bf16, whatever T is
+#pragma unroll
+                for (int cb = 0; cb < NCB; ++cb) {
+                    const CkptIn::Raw r = {make_uint2(x.z[cb].x, x.z[cb].y), x.scale[cb]};
+                    float z[8];
+                    CkptIn{e.z8, e.vec_codes}.value(r, z);
+                    x.z[cb] = make_uint4(pack2<__nv_bfloat16>(z[0], z[1]), pack2<__nv_bfloat16>(z[2], z[3]),
+                                         pack2<__nv_bfloat16>(z[4], z[5]), pack2<__nv_bfloat16>(z[6], z[7]));
+                }
+            }
+            to_fragments<NCB>(stage, x.z, zf);
+        }
+    }
+    if (READS && next.f0 >= 0) fetch<T, KIND, NCB>(e, next.f0, next.t0, x);
+    if (!here) return;
+    if (KIND == kGradWeight && e.out_f32) {
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int t = t0 + 8 * cb + 2 * (lane & 3) + p;
+                float* o = static_cast<float*>(e.out) + (int64_t)t * e.ldo + f0 + (lane >> 2);
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    if (t < e.n && f0 + (lane >> 2) + 8 * g < e.m) o[8 * g] = v[frag<NCB>(g >> 1, cb, g & 1, p)];
+            }
+        return;
+    }
+    if (KIND == kForward) {
+#pragma unroll
+        for (int i = 0; i < 8 * NCB; ++i) v[i] += bias[(i / (4 * NCB)) * 2 + ((i >> 1) & 1)];
+        if (e.z) put16<T, NCB>(e, e.z, e.ldz, e.vec_z, f0, t0, stage, v);
+        if (e.z8.codes) put_ckpt<NCB>(e, f0, t0, stage, v);
+        with_act(e.act, [&](auto tag) {
+#pragma unroll
+            for (int i = 0; i < 8 * NCB; ++i) v[i] = activate<decltype(tag)::value>(v[i]);
+        });
+    }
+    if (KIND == kGradInput && READS && e.act != CHPL_ACT_NONE) {
+        float z[8 * NCB];
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float2 two = e.z8.codes ? unpack2<__nv_bfloat16>(zf[4 * cb + g]) : unpack2<T>(zf[4 * cb + g]);
+                z[frag<NCB>(g >> 1, cb, g & 1, 0)] = two.x;
+                z[frag<NCB>(g >> 1, cb, g & 1, 1)] = two.y;
+            }
+        with_act(e.act, [&](auto tag) {
+#pragma unroll
+            for (int i = 0; i < 8 * NCB; ++i) {
+                float slope;
+                slope_and_value<decltype(tag)::value>(z[i], slope, z[i]);
+                v[i] *= slope;
+            }
+        });
+        if (e.xv) put16<T, NCB>(e, e.xv, e.ldxv, true, f0, t0, stage, z);
+    }
+    if (READS && e.add) {
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float2 two = unpack2<T>(add[4 * cb + g]);
+                v[frag<NCB>(g >> 1, cb, g & 1, 0)] += two.x;
+                v[frag<NCB>(g >> 1, cb, g & 1, 1)] += two.y;
+            }
+    }
+    put16<T, NCB>(e, e.out, e.ldo, e.vec_out, f0, t0, stage, v);
+}
+
+// whether an epilogue reads anything but the accumulators and the bias
+inline bool reads(Kind kind, const Epilogue& e) { return e.add || (kind == kGradInput && e.act != CHPL_ACT_NONE); }
+
+// the biases of a lane's four features of f0 .. f0 + 31
+template <typename T>
+__device__ __forceinline__ void bias_of(const Epilogue& e, int f0, float (&b)[4])
+{
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int f = f0 + 8 * g + (lane_id() >> 2);
+        b[g] = e.bias && f < e.m ? to_f32(static_cast<const T*>(e.bias)[f]) : 0.0f;
+    }
 }
 
 }  // namespace linear

@@ -2,11 +2,10 @@
 // with the epilogue of linear_epilogue.cuh.
 //
 // Every product is oriented so that the output's contiguous dimension f (the
-// features) lies along the 128 TMEM lanes: a warp's lanes hold consecutive
-// features of one row t, so its stores and the reads of a residual or a
-// pre-activation are coalesced row by row, a checkpoint group is one warp, and
-// a few tokens fill a narrow tile (t is the MMA's N dimension, 16 to 256)
-// instead of a fraction of a 128-row one.
+// features) lies along the 128 TMEM lanes and its rows t along the columns: a
+// checkpoint group of 32 features is one warp's lanes, and a few tokens fill a
+// narrow tile (t is the MMA's N dimension, 16 to 256) instead of a fraction of
+// a 128-row one.
 //
 //   forward      A = W (c contiguous)      B = X (c contiguous)
 //   grad input   A = W^T (f contiguous)    B = G (c contiguous)
@@ -89,24 +88,41 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a_desc, u
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, float (&v)[16])
+// accumulators of 32 lanes (features) and NCB x 8 columns (rows t), as the
+// fragments that the epilogue takes
+template <int NCB>
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&v)[8 * NCB])
 {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
+    uint32_t r[8 * NCB];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < NCB / 2; ++c) {
+            uint32_t* q = r + (h * NCB + 2 * c) * 4;
+            asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                         : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7])
+                         : "r"(taddr + ((uint32_t)(16 * h) << 16) + 16 * c));
+        }
     tmem_wait_ld();
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+    for (int j = 0; j < 8 * NCB; ++j) v[j] = __uint_as_float(r[j]);
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
+// Arrival on the even CTA's barrier that this warp has read its accumulators
+// (ordered by tcgen05.fence, not by the memory model: the default CTA-scope
+// release does not wait for the stores under way, as a cluster-scope one would).
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr)
 {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
     return v;
 }
 
@@ -144,7 +160,7 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* tm, u
 //   warps 0-7  epilogue, once the accumulator is complete
 // ----------------------------------------------------------------------------
 constexpr int SPLIT_THREADS = 256;
-constexpr int JOIN = 4;  // rows that a thread joins at a time
+constexpr int JOIN_LD = BM + 4;  // row distance of the partial sums: a lane quad's rows in different banks
 
 struct SplitShape {
     int bn;      // rows t of a tile: 16, 32, 64, 128 or 256
@@ -154,7 +170,7 @@ struct SplitShape {
 
 __host__ __device__ constexpr int stage_bytes(int bn) { return A_BYTES + bn * BK * 2; }
 
-template <typename T, Kind KIND>
+template <typename T, Kind KIND, bool READS>
 __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const int kblocks,
                  const SplitShape sh, const __grid_constant__ Epilogue e)
@@ -231,18 +247,20 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
         }
         __syncwarp();
     }
-    const int quarter = warp & 3, half = warp >> 2;
-    const int f = f0 + quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    // One CTA per tile: a warp takes its TMEM quarter's features and every other
+    // 16 rows.  Several: CTA r takes the 8-row blocks r, r + S, ... of the tile.
     const int rows = min(sh.bn, e.n - t0);  // rows of this tile that exist
-    const float bias = bias_of<T>(e, f);
-    Fetched<16> ahead;
-    Fetched<JOIN> ahead_join;
-    const int c_join = (rank * 2 + half) * JOIN;
-    if (sh.split == 1) {
-        if (half * 16 < rows) fetch<T, KIND, 16>(e, f, t0 + half * 16, ahead);
-    } else if (c_join < rows) {
-        fetch<T, KIND, JOIN>(e, f, t0 + c_join, ahead_join);
+    const bool joined = sh.split > 1;
+    const int quarter = warp & 3, half = warp >> 2, fq = f0 + quarter * 32;
+    const int mine = rows > rank * 8 ? ((rows + 7) / 8 - rank + sh.split - 1) / sh.split : 0;  // blocks of this CTA
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    Fetched<2> ahead;
+    Fetched<1> ahead1;
+    float bias[4];
+    bias_of<T>(e, fq, bias);
+    if (READS) {
+        if (!joined) fetch<T, KIND, 2>(e, fq, t0 + half * 16, ahead);
+        else if (half < mine) fetch<T, KIND, 1>(e, fq, t0 + (rank + half * sh.split) * 8, ahead1);
     }
 
     // every MMA of this CTA has completed (so every copy has landed and been read)
@@ -250,41 +268,51 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     if (kb1 > kb0) ok = mbar_wait(done, 0, abort_flag);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
-    if (sh.split == 1) {
-        for (int c = half * 16; c < rows; c += 32) {
-            float v[16];
-            if (kblocks > 0) {
-                __syncwarp();
-                tmem_ld_x16(tmem + lanes + c, v);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = 0.0f;
-            }
-            if (ok) finish<T, KIND, 16>(e, f, t0 + c, v, bias, ahead);
-            if (c + 32 < rows) fetch<T, KIND, 16>(e, f, t0 + c + 32, ahead);
+
+    if (!joined) {
+        const uint32_t stage = smem_u32(smem) + warp * kStageBytes;
+        for (int c = half * 16; ok && c < rows; c += 32) {
+            float v[16] = {};
+            if (kblocks > 0) tmem_ld_frag<2>(tmem + lanes + c, v);
+            finish<T, KIND, READS, 2>(e, fq, t0 + c, v, bias, ahead, {c + 32 < rows ? fq : -1, t0 + c + 32}, stage);
         }
     } else {
         // partial sums as [row][128 features] into the ring's shared memory
         float* part = reinterpret_cast<float*>(smem);
+        const uint32_t stage = smem_u32(part + sh.bn * JOIN_LD) + warp * kStageBytes;
+        const int at = (lane & 3) * 2 * JOIN_LD + (lane >> 2);  // of fragment 0
         for (int c = half * 16; c < rows; c += 32) {
             float v[16];
-            __syncwarp();
-            tmem_ld_x16(tmem + lanes + c, v);
+            tmem_ld_frag<2>(tmem + lanes + c, v);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) part[(c + j) * BM + quarter * 32 + lane] = v[j];
+            for (int i = 0; i < 16; ++i)
+                part[(c + (i >> 2 & 1) * 8 + (i & 1)) * JOIN_LD + quarter * 32 + (i >> 3) * 16 + (i >> 1 & 1) * 8 + at] = v[i];
         }
         cluster_sync();
-        const uint32_t mine = smem_u32(part + quarter * 32 + lane);
-        const int step = sh.split * 2 * JOIN;
-        for (int c = c_join; c < rows; c += step) {
-            float v[JOIN] = {};
+        // a warp sums one row of each block over the CTAs, 16 bytes a lane, in
+        // rank order; nobody else reads that row of this CTA's, so it stays there
+        for (int b = 0; b < mine; ++b) {
+            const int row = (rank + b * sh.split) * 8 + warp;
+            if (row >= rows) break;
+            float* here = part + row * JOIN_LD + lane * 4;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
             for (int r = 0; r < sh.split; ++r) {
-                const uint32_t peer = map_to_rank(mine + c * BM * 4, (uint32_t)r);
-#pragma unroll
-                for (int j = 0; j < JOIN; ++j) v[j] += ld_cluster_f32(peer + j * BM * 4);
+                const float4 w = ld_cluster_f32x4(map_to_rank(smem_u32(here), (uint32_t)r));
+                sum.x += w.x;
+                sum.y += w.y;
+                sum.z += w.z;
+                sum.w += w.w;
             }
-            if (ok) finish<T, KIND, JOIN>(e, f, t0 + c, v, bias, ahead_join);
-            if (c + step < rows) fetch<T, KIND, JOIN>(e, f, t0 + c + step, ahead_join);
+            *reinterpret_cast<float4*>(here) = sum;
+        }
+        __syncthreads();
+        for (int b = half; ok && b < mine; b += 2) {
+            const int c = (rank + b * sh.split) * 8;
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = part[(c + (i & 1)) * JOIN_LD + quarter * 32 + (i >> 1) * 8 + at];
+            finish<T, KIND, READS, 1>(e, fq, t0 + c, v, bias, ahead1, {b + 2 < mine ? fq : -1, t0 + c + 16 * sh.split}, stage);
         }
         cluster_sync();  // no CTA leaves while another still reads its sums
     }
@@ -313,11 +341,13 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
 constexpr int PAIR_THREADS = 320;
 constexpr int PAIR_STAGES = 6;
 constexpr int PAIR_STAGE_BYTES = A_BYTES + 128 * BK * 2;
-constexpr int PAIR_SMEM = 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + 256;
 constexpr int PAIR_EPI_WARPS = 8;
+constexpr int PAIR_NCB = 4;         // row blocks that an epilogue warp takes at a time
+constexpr int ROWS = 8 * PAIR_NCB;
+constexpr int PAIR_SMEM = 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + PAIR_EPI_WARPS * kStageBytes + 256;
 
 struct PairShape {
-    int bn;              // rows t of a tile, a multiple of 32 (128 where B is MN-major), <= 256
+    int bn;              // rows t of a tile, a multiple of 64 (128 where B is MN-major), <= 256
     int mtiles, ntiles;
     int group;           // feature tiles walked before the next row tile: what L2 holds of A meanwhile
 };
@@ -341,14 +371,15 @@ __device__ __forceinline__ void load_tile_pair(uint8_t* dst, const CUtensorMap* 
     }
 }
 
-template <typename T, Kind KIND>
+template <typename T, Kind KIND, bool READS>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const int kblocks,
                 const PairShape sh, const __grid_constant__ Epilogue e)
 {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + PAIR_STAGES * PAIR_STAGE_BYTES);
+    uint8_t* stages = smem + PAIR_STAGES * PAIR_STAGE_BYTES;  // of the epilogue
+    uint64_t* full = reinterpret_cast<uint64_t*>(stages + PAIR_EPI_WARPS * kStageBytes);
     uint64_t* empty = full + PAIR_STAGES;
     uint64_t* acc_full = empty + PAIR_STAGES;
     uint64_t* acc_empty = acc_full + 2;
@@ -453,34 +484,36 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         __syncwarp();
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
-        const int f_in = (int)rank * BM + quarter * 32 + lane;  // feature within a tile
+        const int f_in = (int)rank * BM + quarter * 32;  // the warp's features within a tile
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t stage = smem_u32(stages) + (warp - 2) * kStageBytes;
         uint32_t acc = 0;
         int mt, nt;
         pair_tile(sh, unit, mt, nt);
-        Fetched<16> ahead;  // what the next 16 rows need
-        if (nt * sh.bn + half * 16 < e.n) fetch<T, KIND, 16>(e, mt * 2 * BM + f_in, nt * sh.bn + half * 16, ahead);
+        Fetched<PAIR_NCB> ahead;
+        if (READS) fetch<T, KIND, PAIR_NCB>(e, mt * 2 * BM + f_in, nt * sh.bn + half * ROWS, ahead);
         for (int tile = unit; tile < total; tile += nunits, ++acc) {
             const int f = mt * 2 * BM + f_in, t0 = nt * sh.bn;
             const uint32_t buf = acc & 1u, aph = (acc >> 1) & 1u;
-            const float bias = bias_of<T>(e, f);
+            float bias[4];
+            bias_of<T>(e, f, bias);
+            Next after = {-1, 0};  // the first rows of the next tile
+            if (tile + nunits < total) {
+                pair_tile(sh, tile + nunits, mt, nt);
+                after = {mt * 2 * BM + f_in, nt * sh.bn + half * ROWS};
+            }
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aph, abort_flag))) break;
             tc_fence_after();
-            for (int c = half * 16; c < sh.bn; c += 32) {
-                float v[16];
-                tmem_ld_x16(tmem + lanes + buf * 256 + c, v);
-                const bool last = c + 32 >= sh.bn;
+            for (int c = half * ROWS; c < sh.bn; c += 2 * ROWS) {
+                float v[ROWS];
+                tmem_ld_frag<PAIR_NCB>(tmem + lanes + buf * 256 + c, v);
+                const bool last = c + 2 * ROWS >= sh.bn;
                 if (last) {  // this warp's last columns are in registers
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(lead_acc_empty + buf * 8);
-                    if (tile + nunits < total) pair_tile(sh, tile + nunits, mt, nt);
+                    if (lane == 0) mbar_arrive_peer(lead_acc_empty + buf * 8);
                 }
-                const Fetched<16> now = ahead;
-                const int fn = mt * 2 * BM + f_in, tn = last ? nt * sh.bn + half * 16 : t0 + c + 32;
-                if ((!last || tile + nunits < total) && tn < e.n) fetch<T, KIND, 16>(e, fn, tn, ahead);
-                if (t0 + c < e.n) finish<T, KIND, 16>(e, f, t0 + c, v, bias, now);
-                __syncwarp();
+                finish<T, KIND, READS, PAIR_NCB>(e, f, t0 + c, v, bias, ahead, last ? after : Next{f, t0 + c + 2 * ROWS}, stage);
             }
         }
     }
@@ -570,7 +603,7 @@ static void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, c
     cfg.numAttrs = 1;
 }
 
-template <typename T, Kind KIND>
+template <typename T, Kind KIND, bool READS>
 static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, int kblocks, const Epilogue& e)
 {
     const SplitShape s = shape_for(KIND, e.m, e.n, kblocks);
@@ -583,32 +616,32 @@ static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int
         CHPL_TRY(make_tmap(&tmA, a, e.m, k, BM));
         CHPL_TRY(make_tmap(&tmB, b, e.n, k, s.bn));
     }
-    CHPL_CUDA(cudaFuncSetAttribute(split_kernel<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
+    CHPL_CUDA(cudaFuncSetAttribute(split_kernel<T, KIND, READS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr;
     cluster_config(cfg, attr, st, ctas, SPLIT_THREADS, 1024 + s.stages * stage_bytes(s.bn) + 512, s.split);
-    CHPL_CUDA(cudaLaunchKernelEx(&cfg, split_kernel<T, KIND>, tmA, tmB, kblocks, s, e));
+    CHPL_CUDA(cudaLaunchKernelEx(&cfg, split_kernel<T, KIND, READS>, tmA, tmB, kblocks, s, e));
     return CHPL_OK;
 }
 
-template <typename T, Kind KIND>
+template <typename T, Kind KIND, bool READS>
 static int launch_pair(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, int kblocks, const Epilogue& e,
                        PairShape s)
 {
     CUtensorMap tmA, tmB;
     CHPL_TRY(make_tmap(&tmA, a, e.m, k, BM));
     CHPL_TRY(make_tmap(&tmB, b, e.n, k, s.bn / 2));
-    CHPL_CUDA(cudaFuncSetAttribute(pair_kernel<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM));
+    CHPL_CUDA(cudaFuncSetAttribute(pair_kernel<T, KIND, READS>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM));
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr;
     const int units = std::min(s.mtiles * s.ntiles, num_sms() / 2);
     cluster_config(cfg, attr, st, 2 * units, PAIR_THREADS, PAIR_SMEM, 2);
-    CHPL_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<T, KIND>, tmA, tmB, kblocks, s, e));
+    CHPL_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<T, KIND, READS>, tmA, tmB, kblocks, s, e));
     return CHPL_OK;
 }
 
 // Pairs where their tiles fill most of the GPU and more than half of each, clusters of lone CTAs elsewhere.
-template <typename T, Kind KIND>
+template <typename T, Kind KIND, bool READS>
 static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
 {
     const int kblocks = (int)((k + BK - 1) / BK);
@@ -619,24 +652,36 @@ static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k
         s.mtiles = (int)mt;
         s.ntiles = (int)nt;
         s.group = 16;
-        return launch_pair<T, KIND>(st, a, b, k, kblocks, e, s);
+        return launch_pair<T, KIND, READS>(st, a, b, k, kblocks, e, s);
     }
-    return launch_split<T, KIND>(st, a, b, k, kblocks, e);
+    return launch_split<T, KIND, READS>(st, a, b, k, kblocks, e);
+}
+
+template <typename T, Kind KIND>
+static int launch_kind(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
+{
+    return reads(KIND, e) ? launch<T, KIND, true>(st, a, b, k, e) : launch<T, KIND, false>(st, a, b, k, e);
 }
 
 template <typename T>
-static int launch_kind(cudaStream_t st, Kind kind, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
+static int launch_type(cudaStream_t st, Kind kind, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
 {
-    if (kind == kForward) return launch<T, kForward>(st, a, b, k, e);
-    if (kind == kGradInput) return launch<T, kGradInput>(st, a, b, k, e);
-    return launch<T, kGradWeight>(st, a, b, k, e);
+    if (kind == kForward) return launch_kind<T, kForward>(st, a, b, k, e);
+    if (kind == kGradInput) return launch_kind<T, kGradInput>(st, a, b, k, e);
+    return launch_kind<T, kGradWeight>(st, a, b, k, e);
 }
 
-int gemm(cudaStream_t st, int type, Kind kind, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
+int gemm(cudaStream_t st, int type, Kind kind, const Operand& a, const Operand& b, int64_t k, const Epilogue& e0)
 {
-    if (e.m == 0 || e.n == 0) return CHPL_OK;
-    return type == CHPL_TYPE_BF16 ? launch_kind<__nv_bfloat16>(st, kind, a, b, k, e)
-                                  : launch_kind<__half>(st, kind, a, b, k, e);
+    if (e0.m == 0 || e0.n == 0) return CHPL_OK;
+    Epilogue e = e0;
+    const int elt = e.out_f32 ? 4 : 2;
+    e.vec_out = aligned(e.out, e.ldo * elt, 16);
+    e.vec_add = aligned(e.add, e.ldadd * elt, 16);
+    e.vec_z = aligned(e.z, e.ldz * 2, 16);
+    e.vec_codes = aligned(e.z8.codes, e.z8.ldc, 8);
+    return type == CHPL_TYPE_BF16 ? launch_type<__nv_bfloat16>(st, kind, a, b, k, e)
+                                  : launch_type<__half>(st, kind, a, b, k, e);
 }
 
 int read_clear_status(int* st)
