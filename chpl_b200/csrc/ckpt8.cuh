@@ -11,9 +11,46 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cstring>
+#include <utility>
+
 #include "common.cuh"
 
 namespace chpl {
+
+// Kernels of these modules are launched with programmatic stream serialization:
+// a kernel's blocks may start, and set themselves up, while the last ones of the
+// kernel before it finish.  start_of_inputs() stands before a kernel's first
+// access to global memory and waits until that kernel has completed; every
+// thread calls it.  It first lets the next kernel in the same way.
+__device__ __forceinline__ void start_of_inputs()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <typename... P, typename... A>
+int launch_kernel(void (*kernel)(P...), int64_t grid, int threads, int smem, int cluster, cudaStream_t st, A&&... args)
+{
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    std::memset(&cfg, 0, sizeof(cfg));
+    std::memset(attr, 0, sizeof(attr));
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    CHPL_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
+    return CHPL_OK;
+}
 
 constexpr int kCkptGroup = 32;
 constexpr uint32_t kCkptMinScale = 7;
@@ -218,6 +255,7 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(In in, Out out, F f,
 {
     const int lane = lane_id();
     const int64_t step = (int64_t)gridDim.x * (kRowsThreads / 32);
+    start_of_inputs();
     for (int64_t i = (int64_t)blockIdx.x * (kRowsThreads / 32) + warp_id(); i < items; i += step) {
         const int64_t t = items < 0xffffffffll ? (int64_t)((uint32_t)i / segs) : i / segs;
         const int j0 = (int)(i - t * segs) * (UNITS * 256) + lane * 8;
@@ -247,10 +285,8 @@ int run_rows(cudaStream_t st, const In& in, const Out& out, const F& f, int64_t 
     const bool wide = cols > 256 && rows * segs4 >= kBlocks * kWarps;
     const int64_t segs = wide ? segs4 : segs1, items = rows * segs, blocks = (items + kWarps - 1) / kWarps;
     const unsigned grid = (unsigned)(blocks < kBlocks ? blocks : kBlocks);
-    if (wide) rows_kernel<4><<<grid, kRowsThreads, 0, st>>>(in, out, f, items, (uint32_t)segs, (int)cols);
-    else rows_kernel<1><<<grid, kRowsThreads, 0, st>>>(in, out, f, items, (uint32_t)segs, (int)cols);
-    CHPL_CUDA(cudaGetLastError());
-    return CHPL_OK;
+    return launch_kernel(wide ? rows_kernel<4, In, Out, F> : rows_kernel<1, In, Out, F>, grid, kRowsThreads, 0, 1, st, in, out,
+                         f, items, (uint32_t)segs, (int)cols);
 }
 
 }  // namespace chpl

@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_act_kernel(RowsIn<T> dy, Z z
     const int64_t first = (int64_t)chunk * kSumRows;
     const int count = (int)min((int64_t)kSumRows, rows - first);
     float sum[8] = {};
+    start_of_inputs();
     for (int r = warp; r < count; r += kAhead * kSumWarps) {
         typename RowsIn<T>::Raw a[kAhead];
         typename Z::Raw b[kAhead];
@@ -169,6 +170,7 @@ template <typename T>
 __global__ void __launch_bounds__(kSumThreads) sum_chunks_kernel(const float* __restrict__ part, int chunks, int n, Sums out)
 {
     const int j = blockIdx.x * kSumThreads + threadIdx.x;
+    start_of_inputs();
     if (j >= n) return;
     float sum = 0.0f;
 #pragma unroll 8
@@ -369,22 +371,21 @@ static int backward(cudaStream_t st, const chpl_linear_bwd& a, void* work)
         if (a.tokens > 0) {
             const int64_t blocks = (a.n + 255) / 256 * p.chunks;
             if (blocks > 0x7fffffff) { set_error("linear_backward: dy of %lld x %lld is more than one launch serves", (long long)a.tokens, (long long)a.n); return CHPL_ERR_UNSUPPORTED; }
-            const unsigned grid = (unsigned)blocks;
             const RowsIn<T> dy = rows_in<T>(a.dy, a.lddy);
             const RowsOut<T> go = rows_out<T>(p.g.copy ? wk + p.g.at : nullptr, p.g.ld);
             const int rows = (int)a.tokens, n = (int)a.n;
             if (a.act == CHPL_ACT_NONE)
-                grad_act_kernel<T><<<grid, kSumThreads, 0, st>>>(dy, NoZ(), a.act, rows, n, go, part, sums);
+                CHPL_TRY(launch_kernel(grad_act_kernel<T, NoZ>, blocks, kSumThreads, 0, 1, st, dy, NoZ(), a.act, rows, n, go, part, sums));
             else if (a.z8.codes)
-                grad_act_kernel<T><<<grid, kSumThreads, 0, st>>>(dy, ckpt_in(a.z8), a.act, rows, n, go, part, sums);
+                CHPL_TRY(launch_kernel(grad_act_kernel<T, CkptIn>, blocks, kSumThreads, 0, 1, st, dy, ckpt_in(a.z8), a.act, rows, n, go,
+                                       part, sums));
             else
-                grad_act_kernel<T><<<grid, kSumThreads, 0, st>>>(dy, rows_in<T>(a.z, a.ldz), a.act, rows, n, go, part, sums);
-            CHPL_CUDA(cudaGetLastError());
+                CHPL_TRY(launch_kernel(grad_act_kernel<T, RowsIn<T>>, blocks, kSumThreads, 0, 1, st, dy, rows_in<T>(a.z, a.ldz), a.act,
+                                       rows, n, go, part, sums));
         }
-        if (join) {
-            sum_chunks_kernel<T><<<(unsigned)((a.n + kSumThreads - 1) / kSumThreads), kSumThreads, 0, st>>>(part, p.chunks, (int)a.n, sums);
-            CHPL_CUDA(cudaGetLastError());
-        }
+        if (join)
+            CHPL_TRY(launch_kernel(sum_chunks_kernel<T>, (a.n + kSumThreads - 1) / kSumThreads, kSumThreads, 0, 1, st, part, p.chunks,
+                                   (int)a.n, sums));
     }
     if (a.k == 0) return CHPL_OK;
     const Operand g_rows = {at(p.g, a.dy, work), p.g.ld, true}, g_cols = {g_rows.p, p.g.ld, false};

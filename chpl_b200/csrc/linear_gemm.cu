@@ -18,6 +18,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <mutex>
 #include <type_traits>
@@ -203,6 +204,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    start_of_inputs();
 
     if (warp == 0) {
         if (elect_one()) {
@@ -408,6 +410,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     // barriers of the even CTA, where the MMAs are issued, as shared::cluster addresses
     const uint32_t lead_full = map_to_rank(smem_u32(full), 0), lead_acc_empty = map_to_rank(smem_u32(acc_empty), 0);
     const int half_rows = sh.bn / 2;
+    start_of_inputs();
 
     if (warp == 0) {
         if (elect_one()) {
@@ -587,20 +590,17 @@ static SplitShape shape_for(Kind kind, int m, int n, int kblocks)
     return s;
 }
 
-static void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, cudaStream_t st, int64_t ctas, int threads,
-                           int smem, int cluster)
+// lets a kernel use `bytes` of shared memory, once per device (bit d of ready: done on device d < 64)
+template <typename K>
+static int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& ready)
 {
-    std::memset(&cfg, 0, sizeof(cfg));
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)cluster;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    int dev = 0;
+    CHPL_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (bit & ready.load(std::memory_order_relaxed)) return CHPL_OK;
+    CHPL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    ready.fetch_or(bit, std::memory_order_relaxed);
+    return CHPL_OK;
 }
 
 template <typename T, Kind KIND, bool READS>
@@ -616,12 +616,10 @@ static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int
         CHPL_TRY(make_tmap(&tmA, a, e.m, k, BM));
         CHPL_TRY(make_tmap(&tmB, b, e.n, k, s.bn));
     }
-    CHPL_CUDA(cudaFuncSetAttribute(split_kernel<T, KIND, READS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
-    cudaLaunchConfig_t cfg;
-    cudaLaunchAttribute attr;
-    cluster_config(cfg, attr, st, ctas, SPLIT_THREADS, 1024 + s.stages * stage_bytes(s.bn) + 512, s.split);
-    CHPL_CUDA(cudaLaunchKernelEx(&cfg, split_kernel<T, KIND, READS>, tmA, tmB, kblocks, s, e));
-    return CHPL_OK;
+    static std::atomic<uint64_t> ready{0};
+    CHPL_TRY(allow_smem(split_kernel<T, KIND, READS>, SMEM_LIMIT, ready));
+    return launch_kernel(split_kernel<T, KIND, READS>, ctas, SPLIT_THREADS, 1024 + s.stages * stage_bytes(s.bn) + 512, s.split, st,
+                         tmA, tmB, kblocks, s, e);
 }
 
 template <typename T, Kind KIND, bool READS>
@@ -631,13 +629,10 @@ static int launch_pair(cudaStream_t st, const Operand& a, const Operand& b, int6
     CUtensorMap tmA, tmB;
     CHPL_TRY(make_tmap(&tmA, a, e.m, k, BM));
     CHPL_TRY(make_tmap(&tmB, b, e.n, k, s.bn / 2));
-    CHPL_CUDA(cudaFuncSetAttribute(pair_kernel<T, KIND, READS>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM));
-    cudaLaunchConfig_t cfg;
-    cudaLaunchAttribute attr;
+    static std::atomic<uint64_t> ready{0};
+    CHPL_TRY(allow_smem(pair_kernel<T, KIND, READS>, PAIR_SMEM, ready));
     const int units = std::min(s.mtiles * s.ntiles, num_sms() / 2);
-    cluster_config(cfg, attr, st, 2 * units, PAIR_THREADS, PAIR_SMEM, 2);
-    CHPL_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<T, KIND, READS>, tmA, tmB, kblocks, s, e));
-    return CHPL_OK;
+    return launch_kernel(pair_kernel<T, KIND, READS>, 2 * units, PAIR_THREADS, PAIR_SMEM, 2, st, tmA, tmB, kblocks, s, e);
 }
 
 // Pairs where their tiles fill most of the GPU and more than half of each, clusters of lone CTAs elsewhere.
