@@ -75,15 +75,21 @@ struct Activate {
 };
 
 // A layer's incoming gradient: G = dY * act'(Z) into g (where given), and the
-// sums of its columns over kSumRows rows at a time into part[chunk][n] (or,
+// sums of its columns over sum_rows rows at a time into part[chunk][n] (or,
 // when there is one chunk, into db itself).  One pass over dY and Z: HBM-bound.
 //
 // A block takes 256 columns (a lane 8 consecutive ones) of one chunk, its warps
 // every eighth row of it; their sums meet in shared memory, always in the same
 // order.
-constexpr int kSumRows = 128;
 constexpr int kSumThreads = 256;
 constexpr int kSumWarps = kSumThreads / 32;
+
+// Rows of a chunk: 128 where that makes four blocks per SM, else 32, which a
+// warp has under way all at once (257 x 519: 18 us by 128, 6 by 32).
+static int sum_rows(int64_t tokens, int64_t n)
+{
+    return (tokens + 127) / 128 * ((n + 255) / 256) >= 4 * 148 ? 128 : 32;
+}
 
 // db, of the operands' type T or FP32
 struct Sums {
@@ -110,15 +116,15 @@ struct NoZ {
 };
 
 template <typename T, typename Z>
-__global__ void __launch_bounds__(kSumThreads) grad_act_kernel(RowsIn<T> dy, Z z, int act, int rows, int n, RowsOut<T> g,
-                                                               float* __restrict__ part, Sums out)
+__global__ void __launch_bounds__(kSumThreads) grad_act_kernel(RowsIn<T> dy, Z z, int act, int rows, int n, int chunk_rows,
+                                                               RowsOut<T> g, float* __restrict__ part, Sums out)
 {
-    constexpr int kAhead = 2;  // rows whose loads are under way at once
+    constexpr int kAhead = 4;  // rows whose loads are under way at once
     __shared__ float sums[kSumWarps][256 + 8];
     const int blocks = (n + 255) / 256, chunk = blockIdx.x / blocks, j0 = (blockIdx.x - chunk * blocks) * 256;
     const int lane = lane_id(), warp = warp_id(), j = j0 + lane * 8;
-    const int64_t first = (int64_t)chunk * kSumRows;
-    const int count = (int)min((int64_t)kSumRows, rows - first);
+    const int64_t first = (int64_t)chunk * chunk_rows;
+    const int count = (int)min((int64_t)chunk_rows, rows - first);
     float sum[8] = {};
     start_of_inputs();
     for (int r = warp; r < count; r += kAhead * kSumWarps) {
@@ -241,7 +247,7 @@ struct BackwardPlan {
     Staged g, w, x;
     bool need_xv;   // Xv is not X as it stands
     size_t part;
-    int chunks;  // of kSumRows tokens: partial sums of db
+    int rows, chunks;  // tokens of a chunk, chunks: partial sums of db
     size_t bytes;
 };
 
@@ -255,7 +261,8 @@ static BackwardPlan plan(const chpl_linear_bwd& a)
     p.w = stage(m, products && a.dx && !tma_rows(a.w, a.ldw, a.n), a.ldw, a.n, a.k);
     p.need_xv = a.x8.codes || a.in_act != CHPL_ACT_NONE || !tma_rows(a.x, a.ldx, a.tokens);
     p.x = stage(m, products && a.dw && p.need_xv, a.ldx, a.tokens, a.k);
-    p.chunks = (int)((a.tokens + kSumRows - 1) / kSumRows);  // <= 2^23
+    p.rows = sum_rows(a.tokens, a.n);
+    p.chunks = (int)((a.tokens + p.rows - 1) / p.rows);
     p.part = a.db && a.n > 0 && p.chunks != 1 ? m.take((size_t)p.chunks * a.n * 4) : 0;
     p.bytes = m.used;
     return p;
@@ -375,13 +382,13 @@ static int backward(cudaStream_t st, const chpl_linear_bwd& a, void* work)
             const RowsOut<T> go = rows_out<T>(p.g.copy ? wk + p.g.at : nullptr, p.g.ld);
             const int rows = (int)a.tokens, n = (int)a.n;
             if (a.act == CHPL_ACT_NONE)
-                CHPL_TRY(launch_kernel(grad_act_kernel<T, NoZ>, blocks, kSumThreads, 0, 1, st, dy, NoZ(), a.act, rows, n, go, part, sums));
+                CHPL_TRY(launch_kernel(grad_act_kernel<T, NoZ>, blocks, kSumThreads, 0, 1, st, dy, NoZ(), a.act, rows, n, p.rows, go, part, sums));
             else if (a.z8.codes)
-                CHPL_TRY(launch_kernel(grad_act_kernel<T, CkptIn>, blocks, kSumThreads, 0, 1, st, dy, ckpt_in(a.z8), a.act, rows, n, go,
-                                       part, sums));
+                CHPL_TRY(launch_kernel(grad_act_kernel<T, CkptIn>, blocks, kSumThreads, 0, 1, st, dy, ckpt_in(a.z8), a.act, rows, n,
+                                       p.rows, go, part, sums));
             else
                 CHPL_TRY(launch_kernel(grad_act_kernel<T, RowsIn<T>>, blocks, kSumThreads, 0, 1, st, dy, rows_in<T>(a.z, a.ldz), a.act,
-                                       rows, n, go, part, sums));
+                                       rows, n, p.rows, go, part, sums));
         }
         if (join)
             CHPL_TRY(launch_kernel(sum_chunks_kernel<T>, (a.n + kSumThreads - 1) / kSumThreads, kSumThreads, 0, 1, st, part, p.chunks,

@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <mutex>
 #include <type_traits>
@@ -573,21 +574,61 @@ static int num_sms()
     return n;
 }
 
-// Narrowest tile that holds all rows (256 at most; 64 at least where B comes
-// in 64-wide boxes); then as many CTAs per tile, up to a portable cluster, as
-// fill two per SM, each with at least two stages of work.
-static SplitShape shape_for(Kind kind, int m, int n, int kblocks)
+// Which kernel, tile and split: the candidate of least estimated time.  The
+// estimate, in us, is a start-up time, the waves of tiles that the SMs run, the
+// staging of A and B per k-block (what a stage of 128 features and bn rows
+// weighs, 16 + bn / 8 KB, at the rate each kernel was seen to stage it), the
+// epilogue, and the join of a split.  Its constants are fitted to 2400 timings
+// of 120 products (each kind, 1 to 7000 tokens, 64 to 16384 features): the
+// choice is 3 % slower than the best candidate in the mean, 26 % at worst; one
+// fixed tile was up to 5 times slower.  E.g. 512 x 4096 x 4096: a lone CTA's 128
+// rows 17 us, a pair's 128 rows 19, 256 rows 26, split in two 25.
+struct Plan {
+    bool pair;
+    SplitShape split;
+    PairShape tiles;
+};
+
+static Plan plan_for(Kind kind, int m, int n, int kblocks)
 {
-    SplitShape s;
-    s.bn = kind == kGradWeight ? 64 : 16;
-    while (s.bn < n && s.bn < 256) s.bn *= 2;
-    const int64_t tiles = (int64_t)((m + BM - 1) / BM) * ((n + s.bn - 1) / s.bn);
+    const bool boxes = kind == kGradWeight;  // B comes in 64-wide boxes: no narrower tile, no other multiple
     const int sms = num_sms();
-    s.split = 1;
-    while (s.split < 8 && tiles * s.split * 2 <= 2 * sms && kblocks >= s.split * 2 * 2) s.split *= 2;
-    const int room = (s.bn <= 64 ? SMEM_LIMIT / 2 : SMEM_LIMIT) - 1024 - 1024;
-    s.stages = std::min(MAX_STAGES, room / stage_bytes(s.bn));
-    return s;
+    Plan best;
+    std::memset(&best, 0, sizeof(best));
+    double least = 1e300;
+    for (int bn = boxes ? 64 : 16; bn <= 256 && (bn < 2 * n || bn <= 64); bn *= 2) {
+        const int64_t tiles = (int64_t)((m + BM - 1) / BM) * ((n + bn - 1) / bn);
+        const int resident = bn <= 64 ? 2 : 1;  // CTAs per SM that the ring leaves room for
+        for (int split = 1; split <= 8 && split <= std::max(1, kblocks); split *= 2) {
+            const double ctas = (double)tiles * split, waves = std::ceil(ctas / (sms * resident));
+            const double share = std::max(1.0, std::min((double)resident, waves > 1 ? resident : ctas / sms));
+            const double t = waves * share * ((kblocks + split - 1) / split * 0.0098 * (16 + bn / 8) + 0.0028 * bn) +
+                             (split > 1 ? 1.7 + 0.023 * bn : 0.0);
+            if (t < least) {
+                least = t;
+                best.pair = false;
+                best.split.bn = bn;
+                best.split.split = split;
+            }
+        }
+    }
+    for (int bn = boxes ? 128 : 64; bn <= 256 && kblocks > 0 && n > bn / 2; bn += boxes ? 128 : 64) {
+        const int64_t mt = (m + 2 * BM - 1) / (2 * BM), nt = (n + bn - 1) / bn;
+        const double waves = std::ceil((double)mt * nt / (sms / 2));
+        const double products = kblocks * 0.0066 * (16 + bn / 8), rest = 0.0037 * bn;  // one runs under the other
+        const double t = waves * std::max(products, rest) + std::min(products, rest);
+        if (t < least && mt * nt < 0x7fffffff) {
+            least = t;
+            best.pair = true;
+            best.tiles.bn = bn;
+            best.tiles.mtiles = (int)mt;
+            best.tiles.ntiles = (int)nt;
+            best.tiles.group = 16;
+        }
+    }
+    const int room = (best.split.bn <= 64 ? SMEM_LIMIT / 2 : SMEM_LIMIT) - 2048;
+    best.split.stages = std::min(MAX_STAGES, room / stage_bytes(best.split.bn));
+    return best;
 }
 
 // lets a kernel use `bytes` of shared memory, once per device (bit d of ready: done on device d < 64)
@@ -604,9 +645,9 @@ static int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& ready)
 }
 
 template <typename T, Kind KIND, bool READS>
-static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, int kblocks, const Epilogue& e)
+static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, int kblocks, const Epilogue& e,
+                        const SplitShape& s)
 {
-    const SplitShape s = shape_for(KIND, e.m, e.n, kblocks);
     const int64_t ctas = (int64_t)((e.m + BM - 1) / BM) * ((e.n + s.bn - 1) / s.bn) * s.split;
     if (ctas > 0x7fffffff) { set_error("linear: an output of %d x %d is more than one launch serves", e.n, e.m); return CHPL_ERR_UNSUPPORTED; }
     CUtensorMap tmA, tmB;
@@ -624,7 +665,7 @@ static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int
 
 template <typename T, Kind KIND, bool READS>
 static int launch_pair(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, int kblocks, const Epilogue& e,
-                       PairShape s)
+                       const PairShape& s)
 {
     CUtensorMap tmA, tmB;
     CHPL_TRY(make_tmap(&tmA, a, e.m, k, BM));
@@ -635,21 +676,13 @@ static int launch_pair(cudaStream_t st, const Operand& a, const Operand& b, int6
     return launch_kernel(pair_kernel<T, KIND, READS>, 2 * units, PAIR_THREADS, PAIR_SMEM, 2, st, tmA, tmB, kblocks, s, e);
 }
 
-// Pairs where their tiles fill most of the GPU and more than half of each, clusters of lone CTAs elsewhere.
 template <typename T, Kind KIND, bool READS>
 static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
 {
     const int kblocks = (int)((k + BK - 1) / BK);
-    const int64_t mt = (e.m + 2 * BM - 1) / (2 * BM), nt = (e.n + 255) / 256;
-    if (kblocks > 0 && e.n > 128 && mt * nt >= num_sms() * 2 / 5 && mt * nt < 0x7fffffff) {
-        PairShape s;
-        s.bn = 256;
-        s.mtiles = (int)mt;
-        s.ntiles = (int)nt;
-        s.group = 16;
-        return launch_pair<T, KIND, READS>(st, a, b, k, kblocks, e, s);
-    }
-    return launch_split<T, KIND, READS>(st, a, b, k, kblocks, e);
+    const Plan p = plan_for(KIND, e.m, e.n, kblocks);
+    return p.pair ? launch_pair<T, KIND, READS>(st, a, b, k, kblocks, e, p.tiles)
+                  : launch_split<T, KIND, READS>(st, a, b, k, kblocks, e, p.split);
 }
 
 template <typename T, Kind KIND>
