@@ -78,7 +78,7 @@ def empty(rows: int, cols: int, dtype: torch.dtype, device) -> Ckpt8:
 
 def elsewhere(device: int, stream) -> bool:
     """Whether a call has to change torch's current device or stream first."""
-    return stream is not None or device != torch.cuda.current_device()
+    return stream is not None or device != _current_device()
 
 
 class on_stream:
@@ -101,9 +101,10 @@ class on_stream:
             c.__exit__(*exc)
 
 
-#: handle of a device's current stream (torch.cuda.current_stream(i).cuda_stream without the two objects around it)
-current_handle = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
-    lambda i: torch.cuda.current_stream(i).cuda_stream)
+# torch's current device, and the handle of a device's current stream, without the checks and objects that the public
+# calls put around them (2.5 us a call, a quarter of a one-token product's)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+current_handle = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def pack(x: torch.Tensor, out: Ckpt8 | None = None, stream=None) -> Ckpt8:

@@ -52,6 +52,45 @@ int launch_kernel(void (*kernel)(P...), int64_t grid, int threads, int smem, int
     return CHPL_OK;
 }
 
+// Two FP32 values in one register pair: Blackwell's packed add, multiply and
+// fused multiply-add take one issue slot for both.  Each half rounds as the
+// scalar instruction does.
+struct Two {
+    uint64_t v;
+};
+
+__device__ __forceinline__ Two two(float lo, float hi)
+{
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ Two both(float a) { return two(a, a); }
+__device__ __forceinline__ float2 apart(Two a)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+    return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b)
+{
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b)
+{
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c)
+{
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
 constexpr int kCkptGroup = 32;
 constexpr uint32_t kCkptMinScale = 7;
 constexpr uint32_t kCkptBadScale = 255;  // the group held an infinity or a NaN
@@ -86,12 +125,19 @@ __device__ __forceinline__ uint32_t ckpt_code(float x, float inv)
     return __float_as_uint(fminf(fmaxf(x * inv, -127.0f), 127.0f) + 12582912.0f);
 }
 
-// Value of the code in byte `b` of w (w's bytes biased by 128, i.e. xor 0x80):
-// as the low byte of 2^23's mantissa, less 2^23 + 128, times the step; exact.
-__device__ __forceinline__ float ckpt_value(uint32_t w_biased, int b, float step)
+// Values of the codes in bytes 0..3 of w: each, biased by 128, as the low byte of
+// 2^23's mantissa, less 2^23 + 128, times the step; exact.
+__device__ __forceinline__ void ckpt_values(uint32_t w, float step, float* v)
 {
-    const float f = __uint_as_float(__byte_perm(w_biased, 0x4B000000u, 0x7440 | b));
-    return (f - 8388736.0f) * step;
+    w ^= 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const Two f = two(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 | i)),
+                          __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 | (i + 1))));
+        const float2 r = apart((f + both(-8388736.0f)) * both(step));
+        v[i] = r.x;
+        v[i + 1] = r.y;
+    }
 }
 
 template <typename T>
@@ -174,8 +220,8 @@ struct CkptIn {
     __device__ __forceinline__ void value(const Raw& r, float (&v)[8]) const
     {
         const float step = ckpt_step(r.s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = ckpt_value((i < 4 ? r.w.x : r.w.y) ^ 0x80808080u, i & 3, step);
+        ckpt_values(r.w.x, step, v);
+        ckpt_values(r.w.y, step, v + 4);
     }
 };
 

@@ -69,26 +69,29 @@ struct Activate {
     {
         with_act(act, [&](auto tag) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = activate<decltype(tag)::value>(v[i]);
+            for (int i = 0; i < 8; i += 2) activate<decltype(tag)::value>(v[i], v[i + 1]);
         });
     }
 };
 
 // A layer's incoming gradient: G = dY * act'(Z) into g (where given), and the
-// sums of its columns over sum_rows rows at a time into part[chunk][n] (or,
-// when there is one chunk, into db itself).  One pass over dY and Z: HBM-bound.
+// sums of its columns.  One pass over dY and Z: HBM-bound.
 //
-// A block takes 256 columns (a lane 8 consecutive ones) of one chunk, its warps
-// every eighth row of it; their sums meet in shared memory, always in the same
-// order.
+// A block takes 256 columns (a lane 8 consecutive ones) of one chunk of rows,
+// its warps every eighth row of it; a cluster takes kSumCluster chunks and joins
+// their sums in shared memory.  One cluster's sums are db, several clusters' go
+// to part[cluster][n] and sum_chunks_kernel adds them.  Every order is fixed.
 constexpr int kSumThreads = 256;
 constexpr int kSumWarps = kSumThreads / 32;
+constexpr int kSumCluster = 8;
 
-// Rows of a chunk: 128 where that makes four blocks per SM, else 32, which a
-// warp has under way all at once (257 x 519: 18 us by 128, 6 by 32).
+// Rows of a chunk: an eighth of up to 1024 tokens, so that one launch does it
+// (257 x 519: 18 us by chunks of 128 and a second launch, 6 by chunks of 32);
+// then 64, or 128 where that still makes four blocks per SM.
 static int sum_rows(int64_t tokens, int64_t n)
 {
-    return (tokens + 127) / 128 * ((n + 255) / 256) >= 4 * 148 ? 128 : 32;
+    if (tokens <= 128 * kSumCluster) return (int)round_up((size_t)(tokens + kSumCluster - 1) / kSumCluster, kSumWarps);
+    return (tokens + 127) / 128 * ((n + 255) / 256) >= 4 * 148 ? 128 : 64;
 }
 
 // db, of the operands' type T or FP32
@@ -121,10 +124,11 @@ __global__ void __launch_bounds__(kSumThreads) grad_act_kernel(RowsIn<T> dy, Z z
 {
     constexpr int kAhead = 4;  // rows whose loads are under way at once
     __shared__ float sums[kSumWarps][256 + 8];
-    const int blocks = (n + 255) / 256, chunk = blockIdx.x / blocks, j0 = (blockIdx.x - chunk * blocks) * 256;
+    const int blocks = (n + 255) / 256, cl = blockIdx.x / kSumCluster, rank = blockIdx.x % kSumCluster;
+    const int group = cl / blocks, j0 = (cl - group * blocks) * 256;
     const int lane = lane_id(), warp = warp_id(), j = j0 + lane * 8;
-    const int64_t first = (int64_t)chunk * chunk_rows;
-    const int count = (int)min((int64_t)chunk_rows, rows - first);
+    const int64_t first = ((int64_t)group * kSumCluster + rank) * chunk_rows;
+    const int count = (int)max((int64_t)0, min((int64_t)chunk_rows, rows - first));
     float sum[8] = {};
     start_of_inputs();
     for (int r = warp; r < count; r += kAhead * kSumWarps) {
@@ -146,10 +150,11 @@ __global__ void __launch_bounds__(kSumThreads) grad_act_kernel(RowsIn<T> dy, Z z
                     z.value(b[u], zv);
                     with_act(act, [&](auto tag) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float slope, value;
-                            slope_and_value<decltype(tag)::value>(zv[i], slope, value);
-                            v[i] *= slope;
+                        for (int i = 0; i < 8; i += 2) {
+                            float sa, sb;
+                            slope_and_value<decltype(tag)::value>(zv[i], zv[i + 1], sa, sb);
+                            v[i] *= sa;
+                            v[i + 1] *= sb;
                         }
                     });
                 }
@@ -162,13 +167,28 @@ __global__ void __launch_bounds__(kSumThreads) grad_act_kernel(RowsIn<T> dy, Z z
 #pragma unroll
     for (int i = 0; i < 8; ++i) sums[warp][lane * 8 + i] = sum[i];
     __syncthreads();
-    const int c = threadIdx.x, col = j0 + c;
+    const int c = threadIdx.x;
     float total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kSumWarps; ++w) total += sums[w][c];
-    if (col >= n) return;
-    if (part) part[(int64_t)chunk * n + col] = total;
-    else put_sum<T>(out, col, total);
+    __syncthreads();
+    sums[0][c] = total;
+    cluster_sync();
+    if (c < 256 / kSumCluster) {  // CTA r adds up the columns r 32 .. r 32 + 31
+        const int at = rank * (256 / kSumCluster) + c, col = j0 + at;
+        total = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kSumCluster; ++r) {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(smem_u32(&sums[0][at]), (uint32_t)r)) : "memory");
+            total += v;
+        }
+        if (col < n) {
+            if (part) part[(int64_t)group * n + col] = total;
+            else put_sum<T>(out, col, total);
+        }
+    }
+    cluster_sync();  // no CTA leaves while another still reads its sums
 }
 
 // db[j] (+)= sum of part[0..chunks)[j], in order
@@ -247,7 +267,7 @@ struct BackwardPlan {
     Staged g, w, x;
     bool need_xv;   // Xv is not X as it stands
     size_t part;
-    int rows, chunks;  // tokens of a chunk, chunks: partial sums of db
+    int rows, chunks;  // tokens of a chunk, clusters of chunks: partial sums of db
     size_t bytes;
 };
 
@@ -262,7 +282,7 @@ static BackwardPlan plan(const chpl_linear_bwd& a)
     p.need_xv = a.x8.codes || a.in_act != CHPL_ACT_NONE || !tma_rows(a.x, a.ldx, a.tokens);
     p.x = stage(m, products && a.dw && p.need_xv, a.ldx, a.tokens, a.k);
     p.rows = sum_rows(a.tokens, a.n);
-    p.chunks = (int)((a.tokens + p.rows - 1) / p.rows);
+    p.chunks = a.tokens > 0 ? (int)((a.tokens + (int64_t)p.rows * kSumCluster - 1) / ((int64_t)p.rows * kSumCluster)) : 0;
     p.part = a.db && a.n > 0 && p.chunks != 1 ? m.take((size_t)p.chunks * a.n * 4) : 0;
     p.bytes = m.used;
     return p;
@@ -376,18 +396,18 @@ static int backward(cudaStream_t st, const chpl_linear_bwd& a, void* work)
         const bool join = a.db && p.chunks != 1;
         float* part = join ? reinterpret_cast<float*>(wk + p.part) : nullptr;
         if (a.tokens > 0) {
-            const int64_t blocks = (a.n + 255) / 256 * p.chunks;
+            const int64_t blocks = (a.n + 255) / 256 * p.chunks * kSumCluster;
             if (blocks > 0x7fffffff) { set_error("linear_backward: dy of %lld x %lld is more than one launch serves", (long long)a.tokens, (long long)a.n); return CHPL_ERR_UNSUPPORTED; }
             const RowsIn<T> dy = rows_in<T>(a.dy, a.lddy);
             const RowsOut<T> go = rows_out<T>(p.g.copy ? wk + p.g.at : nullptr, p.g.ld);
             const int rows = (int)a.tokens, n = (int)a.n;
             if (a.act == CHPL_ACT_NONE)
-                CHPL_TRY(launch_kernel(grad_act_kernel<T, NoZ>, blocks, kSumThreads, 0, 1, st, dy, NoZ(), a.act, rows, n, p.rows, go, part, sums));
+                CHPL_TRY(launch_kernel(grad_act_kernel<T, NoZ>, blocks, kSumThreads, 0, kSumCluster, st, dy, NoZ(), a.act, rows, n, p.rows, go, part, sums));
             else if (a.z8.codes)
-                CHPL_TRY(launch_kernel(grad_act_kernel<T, CkptIn>, blocks, kSumThreads, 0, 1, st, dy, ckpt_in(a.z8), a.act, rows, n,
+                CHPL_TRY(launch_kernel(grad_act_kernel<T, CkptIn>, blocks, kSumThreads, 0, kSumCluster, st, dy, ckpt_in(a.z8), a.act, rows, n,
                                        p.rows, go, part, sums));
             else
-                CHPL_TRY(launch_kernel(grad_act_kernel<T, RowsIn<T>>, blocks, kSumThreads, 0, 1, st, dy, rows_in<T>(a.z, a.ldz), a.act,
+                CHPL_TRY(launch_kernel(grad_act_kernel<T, RowsIn<T>>, blocks, kSumThreads, 0, kSumCluster, st, dy, rows_in<T>(a.z, a.ldz), a.act,
                                        rows, n, p.rows, go, part, sums));
         }
         if (join)

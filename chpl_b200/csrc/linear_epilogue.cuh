@@ -7,9 +7,35 @@
 namespace chpl {
 namespace linear {
 
-// 1 / (1 + exp(-v)); exp and the reciprocal by the hardware's approximations
-// (relative error below 2^-20 where the result matters to 16 bits)
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+__device__ __forceinline__ float ex2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ Two ex2(Two a)
+{
+    const float2 x = apart(a);
+    return two(ex2(x.x), ex2(x.y));
+}
+__device__ __forceinline__ Two rcp(Two a)
+{
+    const float2 x = apart(a);
+    return two(rcp(x.x), rcp(x.y));
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 1 / (1 + 2^-w), i.e. the logistic function of w / log2(e); 2^x and the
+// reciprocal by the hardware's approximations (relative error below 2^-20
+// where the result matters to 16 bits)
+__device__ __forceinline__ Two logistic2(Two w) { return rcp(both(1.0f) + ex2(w * both(-1.0f))); }
 
 constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluA = 0.044715f;
@@ -18,58 +44,84 @@ constexpr float kGeluA = 0.044715f;
 // Abramowitz and Stegun 7.1.26 (Hastings), erfc(x) = t (a1 + ... + a5 t^4) E
 // with t = 1 / (1 + p x), x = |z| / sqrt(2), absolute error below 1.5e-7.  One
 // exponential and one reciprocal, and the slope's density is E again.
-__device__ __forceinline__ float normal_cdf(float z, float& E)
+__device__ __forceinline__ Two normal_cdf(Two z, Two& E)
 {
-    E = __expf(-0.5f * z * z);
-    const float t = __fdividef(1.0f, 1.0f + 0.3275911f * 0.70710678f * fabsf(z));
-    const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-    const float tail = 0.5f * poly * E;
-    return z < 0.0f ? tail : 1.0f - tail;
+    const float2 s = apart(z);
+    E = ex2(z * (z * both(-0.5f * kLog2e)));
+    const Two t = rcp(fma2(both(0.3275911f * 0.70710678f), two(fabsf(s.x), fabsf(s.y)), both(1.0f)));
+    Two q = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
+    q = fma2(q, t, both(0.5f * 1.421413741f));
+    q = fma2(q, t, both(0.5f * -0.284496736f));
+    q = fma2(q, t, both(0.5f * 0.254829592f));
+    const Two tail = (q * t) * E, head = fma2(tail, both(-1.0f), both(1.0f));
+    const float2 a = apart(tail), b = apart(head);
+    return two(s.x < 0.0f ? a.x : b.x, s.y < 0.0f ? a.y : b.y);
 }
 
-// act(z).  The tanh form uses 1/2 (1 + tanh u) = sigmoid(2u), which keeps the
+// act(z).  The tanh form uses 1/2 (1 + tanh u) = logistic(2u), which keeps the
 // relative accuracy of the left tail.  ReLU passes a NaN on.
 template <int ACT>
-__device__ __forceinline__ float activate(float z)
+__device__ __forceinline__ void activate(float& a, float& b)
 {
-    if (ACT == CHPL_ACT_RELU) return z < 0.0f ? 0.0f : z;
-    if (ACT == CHPL_ACT_GELU) {
-        float E;
-        return z * normal_cdf(z, E);
+    if (ACT == CHPL_ACT_NONE) return;
+    if (ACT == CHPL_ACT_RELU) {
+        a = a < 0.0f ? 0.0f : a;
+        b = b < 0.0f ? 0.0f : b;
+        return;
     }
-    if (ACT == CHPL_ACT_GELU_TANH) return z * sigmoid(2.0f * kGeluC * z * (1.0f + kGeluA * z * z));
-    if (ACT == CHPL_ACT_SILU) return z * sigmoid(z);
-    return z;
+    const Two z = two(a, b);
+    Two g, E;
+    if (ACT == CHPL_ACT_GELU) g = normal_cdf(z, E);
+    else if (ACT == CHPL_ACT_GELU_TANH)
+        g = logistic2(z * fma2(z * z, both(2.0f * kLog2e * kGeluC * kGeluA), both(2.0f * kLog2e * kGeluC)));
+    else g = logistic2(z * both(kLog2e));
+    const float2 r = apart(z * g);
+    a = r.x;
+    b = r.y;
 }
 
-// act'(z), and act(z) from the same transcendental.  Where the slope has
-// settled, |z| above 20, its polynomial factors are held at 20 so that they
-// cannot overflow against a zero.
+// act'(z) into s and act(z) into z, from the same transcendental.  Where the
+// slope has settled, |z| above 20, its polynomial factors are held at 20 so that
+// they cannot overflow against a zero.
+__device__ __forceinline__ float hold20(float z) { return fminf(fmaxf(z, -20.0f), 20.0f); }
+
 template <int ACT>
-__device__ __forceinline__ void slope_and_value(float z, float& slope, float& value)
+__device__ __forceinline__ void slope_and_value(float& za, float& zb, float& sa, float& sb)
 {
-    if (ACT == CHPL_ACT_RELU) {
-        slope = z > 0.0f ? 1.0f : 0.0f;
-        value = z < 0.0f ? 0.0f : z;
-    } else if (ACT == CHPL_ACT_GELU) {
-        float E;
-        const float cdf = normal_cdf(z, E);
-        slope = cdf + z * (0.3989422804014327f * E);
-        value = z * cdf;
-    } else if (ACT == CHPL_ACT_GELU_TANH) {
-        const float s = sigmoid(2.0f * kGeluC * z * (1.0f + kGeluA * z * z));
-        const float zc = fminf(fmaxf(z, -20.0f), 20.0f);
-        slope = s + zc * (s * (1.0f - s)) * (2.0f * kGeluC * (1.0f + 3.0f * kGeluA * zc * zc));
-        value = z * s;
-    } else if (ACT == CHPL_ACT_SILU) {
-        const float s = sigmoid(z);
-        const float zc = fminf(fmaxf(z, -20.0f), 20.0f);
-        slope = s * (1.0f + zc * (1.0f - s));
-        value = z * s;
-    } else {
-        slope = 1.0f;
-        value = z;
+    if (ACT == CHPL_ACT_NONE) {
+        sa = sb = 1.0f;
+        return;
     }
+    if (ACT == CHPL_ACT_RELU) {
+        sa = za > 0.0f ? 1.0f : 0.0f;
+        sb = zb > 0.0f ? 1.0f : 0.0f;
+        za = za < 0.0f ? 0.0f : za;
+        zb = zb < 0.0f ? 0.0f : zb;
+        return;
+    }
+    const Two z = two(za, zb);
+    Two g, slope;
+    if (ACT == CHPL_ACT_GELU) {
+        Two E;
+        g = normal_cdf(z, E);
+        slope = fma2(z, E * both(0.3989422804014327f), g);
+    } else {
+        const Two zc = two(hold20(za), hold20(zb));
+        if (ACT == CHPL_ACT_GELU_TANH) {
+            g = logistic2(z * fma2(z * z, both(2.0f * kLog2e * kGeluC * kGeluA), both(2.0f * kLog2e * kGeluC)));
+            const Two d = fma2(zc * zc, both(6.0f * kGeluC * kGeluA), both(2.0f * kGeluC));  // of 2u
+            slope = fma2((zc * d) * g, fma2(g, both(-1.0f), both(1.0f)), g);
+        } else {
+            g = logistic2(z * both(kLog2e));
+            slope = fma2(zc * g, fma2(g, both(-1.0f), both(1.0f)), g);
+        }
+    }
+    float2 r = apart(slope);
+    sa = r.x;
+    sb = r.y;
+    r = apart(z * g);
+    za = r.x;
+    zb = r.y;
 }
 
 // f(std::integral_constant-like tag) with the activation as a compile-time value
@@ -122,18 +174,66 @@ struct Fetched {
 template <int NCB>
 __device__ __forceinline__ constexpr int frag(int h, int cb, int rr, int p) { return (h * NCB + cb) * 4 + rr * 2 + p; }
 
-// eight 16-bit elements of row t from feature f, zero where there are none
-__device__ __forceinline__ uint4 line16(const void* base, int64_t ld, int64_t t, int f, int n, int m, bool vec)
+// Lines of 16-bit rows t0 + 8 cb + l / 4, features f0 + 8 (l % 4) to + 7; zero
+// where there are none.  Whole lines come without a branch among the loads.
+template <int NCB>
+__device__ __forceinline__ void lines16(const void* base, int64_t ld, int t0, int f0, int n, int m, bool vec, uint4 (&w)[NCB])
 {
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (t >= n || f >= m) return w;
-    const unsigned short* at = static_cast<const unsigned short*>(base) + t * ld + f;
-    if (vec && f + 8 <= m) return *reinterpret_cast<const uint4*>(at);
-    uint32_t* u = &w.x;
+    const int lane = lane_id(), f = f0 + 8 * (lane & 3);
+    const unsigned short* at = static_cast<const unsigned short*>(base) + (int64_t)(t0 + (lane >> 2)) * ld + f;
+    if (vec && f0 + 32 <= m) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (f + i < m) u[i >> 1] |= (uint32_t)at[i] << (16 * (i & 1));
-    return w;
+        for (int cb = 0; cb < NCB; ++cb) {
+            w[cb] = make_uint4(0, 0, 0, 0);
+            if (t0 + 8 * cb + (lane >> 2) < n) w[cb] = *reinterpret_cast<const uint4*>(at + 8 * cb * ld);
+        }
+        return;
+    }
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+        w[cb] = make_uint4(0, 0, 0, 0);
+        uint32_t* u = &w[cb].x;
+        if (t0 + 8 * cb + (lane >> 2) < n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (f + i < m) u[i >> 1] |= (uint32_t)at[8 * cb * ld + i] << (16 * (i & 1));
+        }
+    }
+}
+
+// the same of a checkpoint: codes into x and y, the lines' scales
+template <int NCB>
+__device__ __forceinline__ void lines_ckpt(const chpl_ckpt8& c, int t0, int f0, int n, int m, bool vec, uint4 (&w)[NCB],
+                                           uint32_t (&scale)[NCB])
+{
+    const int lane = lane_id(), f = f0 + 8 * (lane & 3);
+    const int64_t t = t0 + (lane >> 2);
+    const int8_t* at = c.codes + t * c.ldc + f;
+    const uint8_t* sc = c.scales + t * c.lds + f0 / kCkptGroup;
+    const bool whole = vec && f0 + 32 <= m;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+        w[cb] = make_uint4(0, 0, 0, 0);
+        scale[cb] = kCkptMinScale;
+        if (t0 + 8 * cb + (lane >> 2) < n && f0 < m) {
+            scale[cb] = sc[8 * cb * c.lds];
+            if (whole) {
+                const uint2 two = *reinterpret_cast<const uint2*>(at + 8 * cb * c.ldc);
+                w[cb].x = two.x;
+                w[cb].y = two.y;
+            }
+        }
+    }
+    if (whole) return;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+        uint32_t* u = &w[cb].x;
+        if (t0 + 8 * cb + (lane >> 2) < n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (f + i < m) u[i >> 2] |= (uint32_t)(uint8_t)at[8 * cb * c.ldc + i] << (8 * (i & 3));
+        }
+    }
 }
 
 // where a warp goes after these rows; f0 < 0: nowhere
@@ -144,7 +244,7 @@ struct Next {
 template <typename T, Kind KIND, int NCB>
 __device__ __forceinline__ void fetch(const Epilogue& e, int f0, int t0, Fetched<NCB>& x)
 {
-    const int lane = lane_id(), f = f0 + 8 * (lane & 3);
+    const int lane = lane_id();
     if (e.add) {
         if (KIND == kGradWeight && e.out_f32) {
 #pragma unroll
@@ -158,22 +258,12 @@ __device__ __forceinline__ void fetch(const Epilogue& e, int f0, int t0, Fetched
                         x.add32[frag<NCB>(g >> 1, cb, g & 1, p)] = t < e.n && f0 + (lane >> 2) + 8 * g < e.m ? a[8 * g] : 0.0f;
                 }
         } else {
-#pragma unroll
-            for (int cb = 0; cb < NCB; ++cb) x.add[cb] = line16(e.add, e.ldadd, t0 + 8 * cb + (lane >> 2), f, e.n, e.m, e.vec_add);
+            lines16<NCB>(e.add, e.ldadd, t0, f0, e.n, e.m, e.vec_add, x.add);
         }
     }
     if (KIND == kGradInput && e.act != CHPL_ACT_NONE) {
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb) {
-            const int64_t t = t0 + 8 * cb + (lane >> 2);
-            if (!e.z8.codes) {
-                x.z[cb] = line16(e.z, e.ldz, t, f, e.n, e.m, e.vec_z);
-                continue;
-            }
-            const CkptIn::Raw r = CkptIn{e.z8, e.vec_codes}.raw(t < e.n ? t : 0, t < e.n ? f : e.m, e.m);
-            x.z[cb] = make_uint4(r.w.x, r.w.y, 0, 0);
-            x.scale[cb] = r.s;
-        }
+        if (e.z8.codes) lines_ckpt<NCB>(e.z8, t0, f0, e.n, e.m, e.vec_codes, x.z, x.scale);
+        else lines16<NCB>(e.z, e.ldz, t0, f0, e.n, e.m, e.vec_z, x.z);
     }
 }
 
@@ -279,32 +369,50 @@ __device__ __forceinline__ void put_ckpt(const Epilogue& e, int f0, int t0, uint
 {
     const int lane = lane_id();
     const bool whole = f0 + 32 <= e.m;
+    // row r = 2 cb + p: its group is four features in this lane and those of the
+    // lanes of the same l % 4.  Step by step over all rows, so that the
+    // shuffles' latencies overlap.
     uint32_t scale[2 * NCB], worst = 0;
+#pragma unroll
+    for (int r = 0; r < 2 * NCB; ++r) {
+        scale[r] = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const uint32_t bits = __float_as_uint(v[frag<NCB>(g >> 1, r >> 1, g & 1, r & 1)]) & 0x7fffffffu;
+            scale[r] = max(scale[r], whole || f0 + (lane >> 2) + 8 * g < e.m ? bits : 0u);
+        }
+    }
+#pragma unroll
+    for (int x = 4; x <= 16; x *= 2)
+#pragma unroll
+        for (int r = 0; r < 2 * NCB; ++r) scale[r] = max(scale[r], __shfl_xor_sync(0xffffffffu, scale[r], x));
+#pragma unroll
+    for (int r = 0; r < 2 * NCB; ++r) {
+        scale[r] = ckpt_scale(scale[r]);
+        worst = max(worst, scale[r]);
+    }
+    // ckpt_code() of two rows at a time
+    constexpr int kZero = 0x4B400000;  // 3 * 2^22
+    int code[8 * NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+        const Two inv = two(ckpt_inv_step(scale[2 * cb]), ckpt_inv_step(scale[2 * cb + 1]));
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int i = frag<NCB>(g >> 1, cb, g & 1, 0);
+            const float2 q = apart(fma2(two(v[i], v[i + 1]), inv, both(12582912.0f)));
+            code[8 * cb + g] = min(max(__float_as_int(q.x), kZero - 127), kZero + 127);
+            code[8 * cb + 4 + g] = min(max(__float_as_int(q.y), kZero - 127), kZero + 127);
+        }
+    }
     __syncwarp();
 #pragma unroll
-    for (int cb = 0; cb < NCB; ++cb)
+    for (int r = 0; r < 2 * NCB; ++r)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            // the row's group: four features in this lane, the others in the lanes of the same l % 4
-            uint32_t top = 0;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const uint32_t bits = __float_as_uint(v[frag<NCB>(g >> 1, cb, g & 1, p)]) & 0x7fffffffu;
-                top = max(top, whole || f0 + (lane >> 2) + 8 * g < e.m ? bits : 0u);
-            }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const uint32_t s = ckpt_scale(top);
-            scale[2 * cb + p] = s;
-            worst = max(worst, s);
-            const float inv = ckpt_inv_step(s);
-            const uint32_t row = at + (8 * cb + 2 * (lane & 3) + p) * 32 + (lane >> 2);
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                asm volatile("st.shared.u8 [%0], %1;" ::"r"(row + 8 * g), "r"(ckpt_code(v[frag<NCB>(g >> 1, cb, g & 1, p)], inv))
-                             : "memory");
-        }
+        for (int g = 0; g < 4; ++g)
+            asm volatile("st.shared.u8 [%0], %1;" ::"r"(at + (8 * (r >> 1) + 2 * (lane & 3) + (r & 1)) * 32 + (lane >> 2) + 8 * g),
+                         "r"(code[4 * r + g])
+                         : "memory");
     if (__any_sync(0xffffffffu, worst == kCkptBadScale)) {  // rows with an infinity or a NaN in the group: codes 0
 #pragma unroll
         for (int i = 0; i < 2 * NCB; ++i)
@@ -399,7 +507,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float 
         if (e.z8.codes) put_ckpt<NCB>(e, f0, t0, stage, v);
         with_act(e.act, [&](auto tag) {
 #pragma unroll
-            for (int i = 0; i < 8 * NCB; ++i) v[i] = activate<decltype(tag)::value>(v[i]);
+            for (int i = 0; i < 8 * NCB; i += 2) activate<decltype(tag)::value>(v[i], v[i + 1]);
         });
     }
     if (KIND == kGradInput && READS && e.act != CHPL_ACT_NONE) {
@@ -414,10 +522,11 @@ __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float 
             }
         with_act(e.act, [&](auto tag) {
 #pragma unroll
-            for (int i = 0; i < 8 * NCB; ++i) {
-                float slope;
-                slope_and_value<decltype(tag)::value>(z[i], slope, z[i]);
-                v[i] *= slope;
+            for (int i = 0; i < 8 * NCB; i += 2) {
+                float sa, sb;
+                slope_and_value<decltype(tag)::value>(z[i], z[i + 1], sa, sb);
+                v[i] *= sa;
+                v[i + 1] *= sb;
             }
         });
         if (e.xv) put16<T, NCB>(e, e.xv, e.ldxv, true, f0, t0, stage, z);

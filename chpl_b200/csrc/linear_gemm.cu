@@ -339,14 +339,19 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
 //
 //   warp 0      TMA producer (both CTAs)
 //   warp 1      TMEM allocation; tcgen05.mma issue (even CTA)
-//   warps 2-9   epilogue (both CTAs)
+//   the others  epilogue (both CTAs)
 // ----------------------------------------------------------------------------
-constexpr int PAIR_THREADS = 320;
 constexpr int PAIR_STAGES = 6;
 constexpr int PAIR_STAGE_BYTES = A_BYTES + 128 * BK * 2;
-constexpr int PAIR_EPI_WARPS = 8;
-constexpr int PAIR_NCB = 4;         // row blocks that an epilogue warp takes at a time
-constexpr int ROWS = 8 * PAIR_NCB;
+// Sixteen epilogue warps with 16 rows each at a time: with a short contraction
+// the epilogue's latencies bound the kernel, and four warps per scheduler hide
+// them best (1024 x 1024 x 16384 with GELU and codes written 42 us; eight warps
+// with 32 rows 47, with 16 rows 51; without either all three 28).
+constexpr int PAIR_EPI_WARPS = 16;
+constexpr int PAIR_NCB = 2;
+constexpr int PAIR_THREADS = 64 + 32 * PAIR_EPI_WARPS;
+constexpr int ROWS = 8 * PAIR_NCB;               // rows that an epilogue warp takes at a time
+constexpr int ROUND = PAIR_EPI_WARPS / 4 * ROWS;  // rows that all of them do: a tile's bn is a multiple
 constexpr int PAIR_SMEM = 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + PAIR_EPI_WARPS * kStageBytes + 256;
 
 struct PairShape {
@@ -487,7 +492,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         }
         __syncwarp();
     } else {
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const int quarter = warp & 3, part = (warp - 2) >> 2;
         const int f_in = (int)rank * BM + quarter * 32;  // the warp's features within a tile
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t stage = smem_u32(stages) + (warp - 2) * kStageBytes;
@@ -495,7 +500,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         int mt, nt;
         pair_tile(sh, unit, mt, nt);
         Fetched<PAIR_NCB> ahead;
-        if (READS) fetch<T, KIND, PAIR_NCB>(e, mt * 2 * BM + f_in, nt * sh.bn + half * ROWS, ahead);
+        if (READS) fetch<T, KIND, PAIR_NCB>(e, mt * 2 * BM + f_in, nt * sh.bn + part * ROWS, ahead);
         for (int tile = unit; tile < total; tile += nunits, ++acc) {
             const int f = mt * 2 * BM + f_in, t0 = nt * sh.bn;
             const uint32_t buf = acc & 1u, aph = (acc >> 1) & 1u;
@@ -504,20 +509,20 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
             Next after = {-1, 0};  // the first rows of the next tile
             if (tile + nunits < total) {
                 pair_tile(sh, tile + nunits, mt, nt);
-                after = {mt * 2 * BM + f_in, nt * sh.bn + half * ROWS};
+                after = {mt * 2 * BM + f_in, nt * sh.bn + part * ROWS};
             }
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aph, abort_flag))) break;
             tc_fence_after();
-            for (int c = half * ROWS; c < sh.bn; c += 2 * ROWS) {
+            for (int c = part * ROWS; c < sh.bn; c += ROUND) {
                 float v[ROWS];
                 tmem_ld_frag<PAIR_NCB>(tmem + lanes + buf * 256 + c, v);
-                const bool last = c + 2 * ROWS >= sh.bn;
+                const bool last = c + ROUND >= sh.bn;
                 if (last) {  // this warp's last columns are in registers
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_peer(lead_acc_empty + buf * 8);
                 }
-                finish<T, KIND, READS, PAIR_NCB>(e, f, t0 + c, v, bias, ahead, last ? after : Next{f, t0 + c + 2 * ROWS}, stage);
+                finish<T, KIND, READS, PAIR_NCB>(e, f, t0 + c, v, bias, ahead, last ? after : Next{f, t0 + c + ROUND}, stage);
             }
         }
     }
@@ -596,10 +601,11 @@ static Plan plan_for(Kind kind, int m, int n, int kblocks)
     Plan best;
     std::memset(&best, 0, sizeof(best));
     double least = 1e300;
-    for (int bn = boxes ? 64 : 16; bn <= 256 && (bn < 2 * n || bn <= 64); bn *= 2) {
+    for (int bn = boxes ? 64 : 16; bn <= 256; bn *= 2) {
+        if (bn >= 2 * n && bn > (boxes ? 64 : 16)) break;  // half the size holds every row
         const int64_t tiles = (int64_t)((m + BM - 1) / BM) * ((n + bn - 1) / bn);
         const int resident = bn <= 64 ? 2 : 1;  // CTAs per SM that the ring leaves room for
-        for (int split = 1; split <= 8 && split <= std::max(1, kblocks); split *= 2) {
+        for (int split = 1; split <= 8 && (split == 1 || split <= kblocks); split *= 2) {
             const double ctas = (double)tiles * split, waves = std::ceil(ctas / (sms * resident));
             const double share = std::max(1.0, std::min((double)resident, waves > 1 ? resident : ctas / sms));
             const double t = waves * share * ((kblocks + split - 1) / split * 0.0098 * (16 + bn / 8) + 0.0028 * bn) +

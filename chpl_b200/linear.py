@@ -24,11 +24,18 @@ _TYPES = {torch.bfloat16: _lib.CHPL_TYPE_BF16, torch.float16: _lib.CHPL_TYPE_F16
 _NO_CKPT = (0, 0, 0, 0)
 
 
-def _type(where: str, t) -> int:
-    code = _TYPES.get(getattr(t, "dtype", None))
-    if code is None:
-        raise invalid(where, f"{getattr(t, 'dtype', type(t).__name__)}: bfloat16 or float16 is wanted")
-    return code
+def _lead(where: str, name: str, t) -> tuple[int, int, int, int, int]:
+    """(type, rows, columns, row distance, device) of the matrix that sets a call's type and device."""
+    try:
+        code, (rows, cols), (ld, unit), device = _TYPES[t.dtype], t.shape, t.stride(), t.get_device()
+        if unit == 1 and ld >= cols and device >= 0:
+            return code, rows, cols, ld, device
+    except (AttributeError, KeyError, TypeError, ValueError):
+        pass
+    ld = matrix(where, name, t, None, None, None)
+    if t.dtype not in _TYPES:
+        raise invalid(where, f"{name} is {t.dtype}: bfloat16 or float16 is wanted")
+    return _TYPES[t.dtype], *t.shape, ld, t.get_device()
 
 
 def _act(where: str, name: str) -> int:
@@ -39,7 +46,7 @@ def _act(where: str, name: str) -> int:
 
 
 def _vector(where: str, name: str, t, n: int, dtype, device: int) -> int:
-    if not isinstance(t, torch.Tensor) or t.shape != (n,) or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.shape != (n,) or t.stride() != (1,) and n > 1:
         raise invalid(where, f"{name} is not a contiguous vector of {n}")
     if t.dtype is not dtype or t.get_device() != device:
         raise invalid(where, f"{name} is {t.dtype} on {t.device}, not {dtype} on cuda:{device}")
@@ -61,15 +68,12 @@ def forward(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, 
     workspace instead of allocating one.
     """
     where = "linear.forward"
-    code, act_code = _type(where, x), _act(where, act)
-    dt = x.dtype
-    ldx = matrix(where, "x", x, None, None, None)
-    dev = x.get_device()
+    code, tokens, k, ldx, dev = _lead(where, "x", x)
+    act_code, dt = _act(where, act), x.dtype
     if elsewhere(dev, stream):
         with on_stream(x.device, stream):
             return forward(x, w, bias, residual=residual, act=act, save=save, out=out, z=z, work=work)
-    tokens, k = x.shape
-    n = len(w)
+    n = w.shape[0]
     ldw = matrix(where, "w", w, dt, dev, (n, k))
     bp = _vector(where, "bias", bias, n, dt, dev) if bias is not None else 0
     rp, ldr = (residual.data_ptr(), matrix(where, "residual", residual, dt, dev, (tokens, n))) if residual is not None else (0, 0)
@@ -112,17 +116,14 @@ def backward(dy: torch.Tensor, x, w: torch.Tensor, *, act: str = "none", z=None,
     out (None).  dW and db are of grad_dtype: dY's type, or torch.float32; accumulate adds them to the dw and db given.
     """
     where = "linear.backward"
-    code, act_code, in_code = _type(where, dy), _act(where, act), _act(where, in_act)
-    dt = dy.dtype
-    lddy = matrix(where, "dy", dy, None, None, None)
-    dev = dy.get_device()
+    code, tokens, n, lddy, dev = _lead(where, "dy", dy)
+    act_code, in_code, dt = _act(where, act), _act(where, in_act), dy.dtype
     if elsewhere(dev, stream):
         with on_stream(dy.device, stream):
             return backward(dy, x, w, act=act, z=z, in_act=in_act, add=add, need_dx=need_dx, need_dw=need_dw, need_db=need_db,
                             dx=dx, dw=dw, db=db, grad_dtype=grad_dtype, accumulate=accumulate, work=work)
-    tokens, n = dy.shape
-    ldw = matrix(where, "w", w, dt, dev, (n, w.shape[-1]))
-    k = w.shape[1]
+    k = w.shape[-1]
+    ldw = matrix(where, "w", w, dt, dev, (n, k))
     gt = grad_dtype or (dw.dtype if dw is not None else db.dtype if db is not None else dt)
     if gt != dt and gt != torch.float32:
         raise invalid(where, f"gradients in {gt}: {dt} or float32 is wanted")

@@ -51,7 +51,7 @@ def test_forward_refuses(kw, code):
     (dict(dy=None), INVALID), (dict(lddy=7), INVALID), (dict(w=None), INVALID), (dict(x=None), INVALID), (dict(lddx=8), INVALID),
     (dict(lddw=8), INVALID), (dict(db=131073), INVALID), (dict(act=_lib.CHPL_ACT_SILU), INVALID), (dict(add=4096, ldadd=8), INVALID),
     (dict(add=32768, ldadd=24), INVALID), (dict(grad_type=2, dw=65538), INVALID), (dict(x8=_lib.Ckpt8(4096, 4096, 8, 1)), INVALID),
-    (dict(dw=None, in_act=2, x=None), INVALID), (dict(), WORKSPACE)])
+    (dict(dw=None, in_act=2, x=None), INVALID), (dict(tokens=4000), WORKSPACE)])
 def test_backward_refuses(kw, code):
     L = _lib.load()
     assert L.chpl_linear_backward(None, ctypes.byref(bwd(**kw)), None, 0) == code
