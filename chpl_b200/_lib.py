@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libchpl.so")
@@ -77,14 +76,6 @@ class LinearBwd(ctypes.Structure):
                 ("ldadd", _i64), ("dx", _vp), ("lddx", _i64), ("dw", _vp), ("lddw", _i64), ("db", _vp)]
 
 
-# The same three structures as `struct` formats (native alignment): packing the arguments of a call into bytes takes a
-# third of the time that filling a ctypes structure does, and a one-token product is about as long as that.
-CKPT8 = struct.Struct("@PPqq")
-LINEAR_FWD = struct.Struct("@2i3qPqPqPPqPqPqPPqq")
-LINEAR_BWD = struct.Struct("@5i3qPqPqPqPPqqPqPPqqPqPqPqP")
-assert (CKPT8.size, LINEAR_FWD.size, LINEAR_BWD.size) == tuple(map(ctypes.sizeof, (Ckpt8, LinearFwd, LinearBwd)))
-
-
 # name -> (restype, argtypes); every function declared in include/chpl.h
 SIGNATURES = {
     "chpl_last_error_string": (ctypes.c_char_p, []),
@@ -124,12 +115,12 @@ SIGNATURES = {
     "chpl_hpl_default_config": (None, [ctypes.POINTER(HplConfig)]),
     "chpl_hpl_run": (_int, [ctypes.POINTER(HplConfig), ctypes.POINTER(HplResult), _vp]),
     "chpl_hpl_run_host": (_int, [ctypes.POINTER(HplConfig), _vp, _sz, _int, ctypes.POINTER(HplResult), _vp]),
-    "chpl_ckpt8_pack": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp]),
-    "chpl_ckpt8_unpack": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _i64]),
-    "chpl_linear_forward_worksize": (_int, [_vp, ctypes.POINTER(_sz)]),
-    "chpl_linear_forward": (_int, [_vp, _vp, _vp, _sz]),
-    "chpl_linear_backward_worksize": (_int, [_vp, ctypes.POINTER(_sz)]),
-    "chpl_linear_backward": (_int, [_vp, _vp, _vp, _sz]),
+    "chpl_ckpt8_pack": (_int, [_vp, _int, _i64, _i64, _vp, _i64, ctypes.POINTER(Ckpt8)]),
+    "chpl_ckpt8_unpack": (_int, [_vp, _int, _i64, _i64, ctypes.POINTER(Ckpt8), _vp, _i64]),
+    "chpl_linear_forward_worksize": (_int, [ctypes.POINTER(LinearFwd), ctypes.POINTER(_sz)]),
+    "chpl_linear_forward": (_int, [_vp, ctypes.POINTER(LinearFwd), _vp, _sz]),
+    "chpl_linear_backward_worksize": (_int, [ctypes.POINTER(LinearBwd), ctypes.POINTER(_sz)]),
+    "chpl_linear_backward": (_int, [_vp, ctypes.POINTER(LinearBwd), _vp, _sz]),
     "chpl_grid_unique_id": (_int, [_vp, _sz]),
     "chpl_grid_create": (_int, [_int, _int, _int, _vp, _sz, _dbl, ctypes.POINTER(_vp)]),
     "chpl_grid_run": (_int, [_vp, ctypes.POINTER(HplConfig), ctypes.POINTER(HplResult), _vp]),
@@ -160,6 +151,17 @@ def load() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+def torch_ops():
+    """The module chpl_b200._torch: the linear-layer entry points for torch tensors (raises if it is missing)."""
+    try:
+        import torch  # noqa: F401  (its libraries first)
+
+        from . import _torch
+    except ImportError as e:
+        raise ImportError(f"chpl_b200/_torch.so does not load: run `python -m chpl_b200.build` (no CPU fallback exists): {e}") from e
+    return _torch
 
 
 def check(code: int, where: str) -> None:

@@ -48,6 +48,8 @@ NCCL_INC = ["-I", os.path.join(NCCL_DIR, "include")] if NCCL_DIR else []
 NCCL_LINK = (["-L", os.path.join(NCCL_DIR, "lib"), "-l:libnccl.so.2", "-Xlinker", "-rpath," + os.path.join(NCCL_DIR, "lib")]
              if NCCL_DIR else ["-lnccl"])
 LINK = ["-cudart", "shared"] + NCCL_LINK + ["-Xlinker", "-rpath," + os.path.join(CUDA, "lib64")]
+# the Python module chpl_b200._torch (CPython's and torch's C++ API): tensors in, libchpl's C ABI out
+TORCH_EXT = os.path.join(HERE, "_torch.so")
 EXES = {"chpl_single": "chpl_single_main.cpp", "chpl_p2": "chpl_p2_main.cpp"}
 
 
@@ -75,6 +77,19 @@ def _run(cmd: list[str], verbose: bool) -> None:
         sys.stderr.write(r.stdout + r.stderr)
 
 
+def _torch_ext_command(src: str) -> list[str]:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ce
+    inc = [a for d in ce.include_paths() + [os.path.join(CUDA, "include"), sysconfig.get_paths()["include"]] for a in ("-isystem", d)]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE] + inc + [
+            src, "-o", TORCH_EXT, "-L", HERE, "-lchpl", "-Wl,-rpath,$ORIGIN", "-L", libs, "-ltorch_python", "-ltorch", "-ltorch_cpu",
+            "-lc10", "-lc10_cuda", "-Wl,-rpath," + libs]
+
+
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None) -> str:
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(BIN, exist_ok=True)
@@ -93,6 +108,9 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
             list(ex.map(lambda c: _run(c, verbose), jobs))
     if force or _newer(LIB, objs):
         _run([NVCC] + ARCH + ["-shared", "-o", LIB] + objs + LINK, verbose)
+    s = os.path.join(CSRC, "bindings.cpp")
+    if force or _newer(TORCH_EXT, [s, LIB] + hdrs):
+        _run(_torch_ext_command(s), verbose)
     for exe, src in EXES.items():
         s = os.path.join(CSRC, src)
         out = os.path.join(BIN, exe)
