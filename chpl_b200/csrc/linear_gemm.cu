@@ -165,12 +165,20 @@ constexpr int SPLIT_THREADS = 256;
 constexpr int JOIN_LD = BM + 4;  // row distance of the partial sums: a lane quad's rows in different banks
 
 struct SplitShape {
-    int bn;      // rows t of a tile: 16, 32, 64, 128 or 256
+    int bn;      // rows t of a tile, a multiple of 16, <= 256
     int split;   // CTAs per tile
     int stages;
 };
 
-__host__ __device__ constexpr int stage_bytes(int bn) { return A_BYTES + bn * BK * 2; }
+// bytes of a stage's `rows` rows of B; MN-major ones come in whole boxes of 64
+template <Kind KIND>
+__host__ __device__ constexpr int b_bytes(int rows)
+{
+    return Major<KIND>::b ? rows * BK * 2 : (rows + 63) / 64 * BOX_BYTES;
+}
+template <Kind KIND>
+__host__ __device__ constexpr int stage_bytes(int bn) { return A_BYTES + b_bytes<KIND>(bn); }
+__host__ __device__ constexpr uint32_t tmem_cols(int bn) { return bn <= 32 ? 32u : bn <= 64 ? 64u : bn <= 128 ? 128u : 256u; }
 
 template <typename T, Kind KIND, bool READS>
 __global__ void __launch_bounds__(SPLIT_THREADS, 2)
@@ -179,7 +187,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
 {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int sbytes = stage_bytes(sh.bn);
+    const int sbytes = stage_bytes<KIND>(sh.bn);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + sh.stages * sbytes);
     uint64_t* empty = full + MAX_STAGES;
     uint64_t* done = empty + MAX_STAGES;
@@ -191,7 +199,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     const int tile = (int)(blockIdx.x / sh.split), mtiles = (e.m + BM - 1) / BM;
     const int f0 = tile % mtiles * BM, t0 = tile / mtiles * sh.bn;
     const int kb0 = (int)((int64_t)kblocks * rank / sh.split), kb1 = (int)((int64_t)kblocks * (rank + 1) / sh.split);
-    const uint32_t cols = sh.bn < 32 ? 32u : (uint32_t)sh.bn;
+    const uint32_t cols = tmem_cols(sh.bn);
     if (threadIdx.x == 0) {
         for (int s = 0; s < sh.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_init(done, 1);
@@ -351,11 +359,11 @@ constexpr int PAIR_EPI_WARPS = 16;
 constexpr int PAIR_NCB = 2;
 constexpr int PAIR_THREADS = 64 + 32 * PAIR_EPI_WARPS;
 constexpr int ROWS = 8 * PAIR_NCB;               // rows that an epilogue warp takes at a time
-constexpr int ROUND = PAIR_EPI_WARPS / 4 * ROWS;  // rows that all of them do: a tile's bn is a multiple
+constexpr int ROUND = PAIR_EPI_WARPS / 4 * ROWS;  // rows that all of them do: a tile has as many at least
 constexpr int PAIR_SMEM = 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + PAIR_EPI_WARPS * kStageBytes + 256;
 
 struct PairShape {
-    int bn;              // rows t of a tile, a multiple of 64 (128 where B is MN-major), <= 256
+    int bn;              // rows t of a tile, a multiple of 32, 64 to 256
     int mtiles, ntiles;
     int group;           // feature tiles walked before the next row tile: what L2 holds of A meanwhile
 };
@@ -420,7 +428,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 
     if (warp == 0) {
         if (elect_one()) {
-            const uint32_t bytes = 2u * (A_BYTES + (uint32_t)half_rows * BK * 2);  // both CTAs' copies
+            const uint32_t bytes = 2u * (A_BYTES + (uint32_t)b_bytes<KIND>(half_rows));  // both CTAs' copies
             int stage = 0, started = 0;
             uint32_t ph = 0;
             bool ok = true;
@@ -580,36 +588,46 @@ static int num_sms()
 }
 
 // Which kernel, tile and split: the candidate of least estimated time.  The
-// estimate, in us, is a start-up time, the waves of tiles that the SMs run, the
-// staging of A and B per k-block (what a stage of 128 features and bn rows
-// weighs, 16 + bn / 8 KB, at the rate each kernel was seen to stage it), the
-// epilogue, and the join of a split.  Its constants are fitted to 2400 timings
-// of 120 products (each kind, 1 to 7000 tokens, 64 to 16384 features): the
-// choice is 3 % slower than the best candidate in the mean, 26 % at worst; one
-// fixed tile was up to 5 times slower.  E.g. 512 x 4096 x 4096: a lone CTA's 128
-// rows 17 us, a pair's 128 rows 19, 256 rows 26, split in two 25.
+// estimate, in us, is a start-up time and, for each wave of tiles that the SMs
+// run, the staging of A and B per k-block (what a stage of 128 features and bn
+// rows weighs, 16 + bn / 8 KB, at the rate each kernel was seen to stage it),
+// which also covers the multiply-adds; a lone CTA's epilogue and the join of a
+// split come on top.  The constants are fitted to 3000 timings of 150 products
+// (each kind, 1 to 8000 tokens, 64 to 16384 features): the choice is 2.5 % slower
+// than the best candidate in the mean, 23 % at worst; one fixed tile was up to 5
+// times slower.  E.g. 512 x 4096 x 4096: a lone CTA's 128 rows 17 us, a pair's 128
+// rows 19, 256 rows 26, split in two 25.
 struct Plan {
     bool pair;
     SplitShape split;
     PairShape tiles;
 };
 
-static Plan plan_for(Kind kind, int m, int n, int kblocks)
+// the narrowest multiple of `step` rows that makes no more tiles of n rows than bn does
+static int fit_rows(int n, int bn, int step)
 {
-    const bool boxes = kind == kGradWeight;  // B comes in 64-wide boxes: no narrower tile, no other multiple
+    const int tiles = (n + bn - 1) / bn;
+    return (int)round_up((size_t)((n + tiles - 1) / tiles), (size_t)step);
+}
+
+template <Kind KIND>
+static Plan plan_for(int m, int n, int kblocks)
+{
     const int sms = num_sms();
     Plan best;
     std::memset(&best, 0, sizeof(best));
     double least = 1e300;
-    for (int bn = boxes ? 64 : 16; bn <= 256; bn *= 2) {
-        if (bn >= 2 * n && bn > (boxes ? 64 : 16)) break;  // half the size holds every row
+    for (int size = Major<KIND>::b ? 16 : 64; size <= 256; size *= 2) {
+        if (size >= 2 * n && least < 1e300) break;  // half the size holds every row
+        const int bn = fit_rows(n, size, Major<KIND>::b ? 16 : 64);
         const int64_t tiles = (int64_t)((m + BM - 1) / BM) * ((n + bn - 1) / bn);
         const int resident = bn <= 64 ? 2 : 1;  // CTAs per SM that the ring leaves room for
+        const double stage = 0.0096 / 1024 * stage_bytes<KIND>(bn);
         for (int split = 1; split <= 8 && (split == 1 || split <= kblocks); split *= 2) {
             const double ctas = (double)tiles * split, waves = std::ceil(ctas / (sms * resident));
             const double share = std::max(1.0, std::min((double)resident, waves > 1 ? resident : ctas / sms));
-            const double t = waves * share * ((kblocks + split - 1) / split * 0.0098 * (16 + bn / 8) + 0.0028 * bn) +
-                             (split > 1 ? 1.7 + 0.023 * bn : 0.0);
+            const double t = 2.0 + waves * (share * stage * ((kblocks + split - 1) / split) + 0.41) +
+                             (split > 1 ? 1.0 + 0.0215 * bn : 0.0);
             if (t < least) {
                 least = t;
                 best.pair = false;
@@ -618,11 +636,13 @@ static Plan plan_for(Kind kind, int m, int n, int kblocks)
             }
         }
     }
-    for (int bn = boxes ? 128 : 64; bn <= 256 && kblocks > 0 && n > bn / 2; bn += boxes ? 128 : 64) {
+    // B's halves in whole boxes where it is MN-major
+    const int step = Major<KIND>::b ? 32 : 128;
+    for (int size = Major<KIND>::b ? ROUND : 128; size <= 256 && kblocks > 0 && n > size / 2; size += step) {
+        const int bn = std::max(ROUND, fit_rows(n, size, step));
         const int64_t mt = (m + 2 * BM - 1) / (2 * BM), nt = (n + bn - 1) / bn;
-        const double waves = std::ceil((double)mt * nt / (sms / 2));
-        const double products = kblocks * 0.0066 * (16 + bn / 8), rest = 0.0037 * bn;  // one runs under the other
-        const double t = waves * std::max(products, rest) + std::min(products, rest);
+        const double stage = 0.0064 / 1024 * (A_BYTES + 2 * b_bytes<KIND>(bn / 2));
+        const double t = 3.1 + std::ceil((double)mt * nt / (sms / 2)) * stage * kblocks;
         if (t < least && mt * nt < 0x7fffffff) {
             least = t;
             best.pair = true;
@@ -633,7 +653,7 @@ static Plan plan_for(Kind kind, int m, int n, int kblocks)
         }
     }
     const int room = (best.split.bn <= 64 ? SMEM_LIMIT / 2 : SMEM_LIMIT) - 2048;
-    best.split.stages = std::min(MAX_STAGES, room / stage_bytes(best.split.bn));
+    best.split.stages = std::min(MAX_STAGES, room / stage_bytes<KIND>(best.split.bn));
     return best;
 }
 
@@ -665,7 +685,7 @@ static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int
     }
     static std::atomic<uint64_t> ready{0};
     CHPL_TRY(allow_smem(split_kernel<T, KIND, READS>, SMEM_LIMIT, ready));
-    return launch_kernel(split_kernel<T, KIND, READS>, ctas, SPLIT_THREADS, 1024 + s.stages * stage_bytes(s.bn) + 512, s.split, st,
+    return launch_kernel(split_kernel<T, KIND, READS>, ctas, SPLIT_THREADS, 1024 + s.stages * stage_bytes<KIND>(s.bn) + 512, s.split, st,
                          tmA, tmB, kblocks, s, e);
 }
 
@@ -686,7 +706,7 @@ template <typename T, Kind KIND, bool READS>
 static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
 {
     const int kblocks = (int)((k + BK - 1) / BK);
-    const Plan p = plan_for(KIND, e.m, e.n, kblocks);
+    const Plan p = plan_for<KIND>(e.m, e.n, kblocks);
     return p.pair ? launch_pair<T, KIND, READS>(st, a, b, k, kblocks, e, p.tiles)
                   : launch_split<T, KIND, READS>(st, a, b, k, kblocks, e, p.split);
 }
