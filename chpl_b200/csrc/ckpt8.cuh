@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 
 #include <cstring>
+#include <type_traits>
 #include <utility>
 
 #include "common.cuh"
@@ -115,15 +116,12 @@ __device__ __forceinline__ float ckpt_step(uint32_t s)
     return s == kCkptBadScale ? __uint_as_float(0x7fffffffu) : __uint_as_float((s - 6u) << 23);
 }
 
-// Code of x in the low byte: x * inv is exact (a power of two; what could
-// underflow is far below half a code), the clamp keeps it within +-127, and
-// adding 3 * 2^22 rounds it half to even into the sum's low mantissa bits (no
-// conversion instruction, which runs at an eighth of an addition's rate).  A
-// poisoned group's codes are not numbers' and have to be replaced by 0.
-__device__ __forceinline__ uint32_t ckpt_code(float x, float inv)
-{
-    return __float_as_uint(fminf(fmaxf(x * inv, -127.0f), 127.0f) + 12582912.0f);
-}
+// Codes: x * inv is exact (a power of two; what could underflow is far below
+// half a code), and adding 3 * 2^22 in the same instruction rounds it half to
+// even into the sum's low mantissa bits, a 16-bit integer there (no conversion
+// instruction, which runs at an eighth of an addition's rate); a clamp keeps it
+// within +-127.  A poisoned group's codes are not numbers' and have to be
+// replaced by 0.
 
 // Values of the codes in bytes 0..3 of w: each, biased by 128, as the low byte of
 // 2^23's mantissa, less 2^23 + 128, times the step; exact.
@@ -192,6 +190,22 @@ struct RowsIn {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
     }
+    // the largest magnitude's FP32 bits; 16-bit patterns (sign cleared) order as
+    // their values do, NaN on top, so two at a time compare as integers
+    __device__ __forceinline__ uint32_t top(const Raw& r) const
+    {
+        if (sizeof(T) == 4) {
+            uint32_t t = 0;
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t = max(t, w[i] & 0x7fffffffu);
+            return t;
+        }
+        const uint32_t t = __vmaxu2(__vmaxu2(r.w[0].x & 0x7fff7fffu, r.w[0].y & 0x7fff7fffu),
+                                    __vmaxu2(r.w[0].z & 0x7fff7fffu, r.w[0].w & 0x7fff7fffu));
+        const unsigned short h = (unsigned short)max(t & 0xffffu, t >> 16);
+        return __float_as_uint(to_f32(reinterpret_cast<const T&>(h)));
+    }
 };
 
 struct CkptIn {
@@ -251,22 +265,21 @@ struct RowsOut {
 struct CkptOut {
     chpl_ckpt8 c;
     bool vec;
-    // every lane of a group's four calls it; elements past the row's end are 0
-    __device__ __forceinline__ void put(int64_t t, int j, int cols, const float (&v)[8]) const
+    // v and the largest magnitude's bits among them; every lane of a group's four
+    // calls it; elements past the row's end are 0
+    __device__ __forceinline__ void put(int64_t t, int j, int cols, const float (&v)[8], uint32_t top) const
     {
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const uint32_t s = ckpt_scale(top);
-        const float inv = ckpt_inv_step(s);
-        uint32_t q[8];
+        const Two inv = both(ckpt_inv_step(s));
+        uint32_t h[4];  // the codes as pairs of 16-bit integers: two at a time
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = ckpt_code(v[i], inv);
-        uint2 w;
-        w.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-        w.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+        for (int i = 0; i < 4; ++i) {
+            const float2 q = apart(fma2(two(v[2 * i], v[2 * i + 1]), inv, both(12582912.0f)));
+            h[i] = __vmins2(__vmaxs2(__byte_perm(__float_as_uint(q.x), __float_as_uint(q.y), 0x5410), 0xff81ff81u), 0x007f007fu);
+        }
+        uint2 w = make_uint2(__byte_perm(h[0], h[1], 0x6420), __byte_perm(h[2], h[3], 0x6420));
         if (s == kCkptBadScale) w = make_uint2(0, 0);
         if (j >= cols) return;
         int8_t* at = c.codes + t * c.ldc + j;
@@ -292,7 +305,7 @@ RowsOut<T> rows_out(void* p, int64_t ld) { return {static_cast<T*>(p), ld, align
 inline CkptIn ckpt_in(const chpl_ckpt8& c) { return {c, aligned(c.codes, c.ldc, 8)}; }
 inline CkptOut ckpt_out(const chpl_ckpt8& c) { return {c, aligned(c.codes, c.ldc, 8)}; }
 
-// out = f(in), row by row: a warp takes UNITS x 256 columns of a row at a time,
+// out = f(in), row by row (a checkpoint takes in as it is): a warp takes UNITS x 256 columns of a row at a time,
 // a lane 8 consecutive ones of each, every load before any arithmetic.
 constexpr int kRowsThreads = 256;
 
@@ -313,7 +326,8 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(In in, Out out, F f,
             float v[8];
             in.value(raw[u], v);
             f(v);
-            out.put(t, j0 + u * 256, cols, v);
+            if constexpr (std::is_same<Out, CkptOut>::value) out.put(t, j0 + u * 256, cols, v, in.top(raw[u]));
+            else out.put(t, j0 + u * 256, cols, v);
         }
     }
 }

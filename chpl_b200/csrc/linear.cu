@@ -78,20 +78,28 @@ struct Activate {
 // sums of its columns.  One pass over dY and Z: HBM-bound.
 //
 // A block takes 256 columns (a lane 8 consecutive ones) of one chunk of rows,
-// its warps every eighth row of it; a cluster takes kSumCluster chunks and joins
-// their sums in shared memory.  One cluster's sums are db, several clusters' go
-// to part[cluster][n] and sum_chunks_kernel adds them.  Every order is fixed.
+// its warps every eighth row of it.  Up to 1024 tokens are eight chunks, the
+// blocks of a cluster, which joins their sums in shared memory: one launch does
+// it (257 x 519: 6 us; two launches with chunks of 128 rows 18).  More tokens
+// leave each chunk's sums in part[chunk][n], which sum_chunks_kernel adds
+// (8192 x 16384: 50 us, 5.3 TB/s; in clusters 104).  Every order is fixed.
 constexpr int kSumThreads = 256;
 constexpr int kSumWarps = kSumThreads / 32;
 constexpr int kSumCluster = 8;
 
-// Rows of a chunk: an eighth of up to 1024 tokens, so that one launch does it
-// (257 x 519: 18 us by chunks of 128 and a second launch, 6 by chunks of 32);
-// then 64, or 128 where that still makes four blocks per SM.
-static int sum_rows(int64_t tokens, int64_t n)
+struct SumShape {
+    int rows;     // of a chunk
+    int chunks;
+    int cluster;  // blocks that join their sums: 1 or kSumCluster
+};
+
+// chunks of 128 rows where that makes four blocks per SM, else of 64
+static SumShape sum_shape(int64_t tokens, int64_t n)
 {
-    if (tokens <= 128 * kSumCluster) return (int)round_up((size_t)(tokens + kSumCluster - 1) / kSumCluster, kSumWarps);
-    return (tokens + 127) / 128 * ((n + 255) / 256) >= 4 * 148 ? 128 : 64;
+    if (tokens <= 128 * kSumCluster)
+        return {(int)round_up((size_t)(tokens + kSumCluster - 1) / kSumCluster, kSumWarps), tokens > 0 ? 1 : 0, kSumCluster};
+    const int rows = (tokens + 127) / 128 * ((n + 255) / 256) >= 4 * 148 ? 128 : 64;
+    return {rows, (int)((tokens + rows - 1) / rows), 1};
 }
 
 // db, of the operands' type T or FP32
@@ -120,14 +128,14 @@ struct NoZ {
 
 template <typename T, typename Z>
 __global__ void __launch_bounds__(kSumThreads) grad_act_kernel(RowsIn<T> dy, Z z, int act, int rows, int n, int chunk_rows,
-                                                               RowsOut<T> g, float* __restrict__ part, Sums out)
+                                                               int cluster, RowsOut<T> g, float* __restrict__ part, Sums out)
 {
     constexpr int kAhead = 4;  // rows whose loads are under way at once
     __shared__ float sums[kSumWarps][256 + 8];
-    const int blocks = (n + 255) / 256, cl = blockIdx.x / kSumCluster, rank = blockIdx.x % kSumCluster;
+    const int blocks = (n + 255) / 256, cl = blockIdx.x / cluster, rank = blockIdx.x - cl * cluster;
     const int group = cl / blocks, j0 = (cl - group * blocks) * 256;
     const int lane = lane_id(), warp = warp_id(), j = j0 + lane * 8;
-    const int64_t first = ((int64_t)group * kSumCluster + rank) * chunk_rows;
+    const int64_t first = ((int64_t)group * cluster + rank) * chunk_rows;
     const int count = (int)max((int64_t)0, min((int64_t)chunk_rows, rows - first));
     float sum[8] = {};
     start_of_inputs();
@@ -171,11 +179,15 @@ __global__ void __launch_bounds__(kSumThreads) grad_act_kernel(RowsIn<T> dy, Z z
     float total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kSumWarps; ++w) total += sums[w][c];
+    if (cluster == 1) {
+        if (j0 + c < n) part[(int64_t)group * n + j0 + c] = total;
+        return;
+    }
     __syncthreads();
     sums[0][c] = total;
     cluster_sync();
-    if (c < 256 / kSumCluster) {  // CTA r adds up the columns r 32 .. r 32 + 31
-        const int at = rank * (256 / kSumCluster) + c, col = j0 + at;
+    if (c < 256 / kSumCluster) {  // block r adds up the columns r 32 .. r 32 + 31
+        const int at = rank * (256 / kSumCluster) + c;
         total = 0.0f;
 #pragma unroll
         for (int r = 0; r < kSumCluster; ++r) {
@@ -183,12 +195,9 @@ __global__ void __launch_bounds__(kSumThreads) grad_act_kernel(RowsIn<T> dy, Z z
             asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(smem_u32(&sums[0][at]), (uint32_t)r)) : "memory");
             total += v;
         }
-        if (col < n) {
-            if (part) part[(int64_t)group * n + col] = total;
-            else put_sum<T>(out, col, total);
-        }
+        if (j0 + at < n) put_sum<T>(out, j0 + at, total);
     }
-    cluster_sync();  // no CTA leaves while another still reads its sums
+    cluster_sync();  // no block leaves while another still reads its sums
 }
 
 // db[j] (+)= sum of part[0..chunks)[j], in order
@@ -267,7 +276,7 @@ struct BackwardPlan {
     Staged g, w, x;
     bool need_xv;   // Xv is not X as it stands
     size_t part;
-    int rows, chunks;  // tokens of a chunk, clusters of chunks: partial sums of db
+    SumShape sum;   // of db
     size_t bytes;
 };
 
@@ -281,9 +290,8 @@ static BackwardPlan plan(const chpl_linear_bwd& a)
     p.w = stage(m, products && a.dx && !tma_rows(a.w, a.ldw, a.n), a.ldw, a.n, a.k);
     p.need_xv = a.x8.codes || a.in_act != CHPL_ACT_NONE || !tma_rows(a.x, a.ldx, a.tokens);
     p.x = stage(m, products && a.dw && p.need_xv, a.ldx, a.tokens, a.k);
-    p.rows = sum_rows(a.tokens, a.n);
-    p.chunks = a.tokens > 0 ? (int)((a.tokens + (int64_t)p.rows * kSumCluster - 1) / ((int64_t)p.rows * kSumCluster)) : 0;
-    p.part = a.db && a.n > 0 && p.chunks != 1 ? m.take((size_t)p.chunks * a.n * 4) : 0;
+    p.sum = sum_shape(a.tokens, a.n);
+    p.part = a.db && a.n > 0 && p.sum.cluster == 1 ? m.take((size_t)p.sum.chunks * a.n * 4) : 0;
     p.bytes = m.used;
     return p;
 }
@@ -392,26 +400,29 @@ static int backward(cudaStream_t st, const chpl_linear_bwd& a, void* work)
     char* wk = static_cast<char*>(work);
     if (a.n > 0 && (p.g.copy || a.db)) {
         const Sums sums = {a.db, a.grad_type == CHPL_TYPE_F32, a.accumulate};
-        // one chunk's sums go straight to db, several (or none: zeros) by way of the workspace
-        const bool join = a.db && p.chunks != 1;
+        // one cluster's sums go straight to db, chunks' (or none: zeros) by way of the workspace
+        const bool join = a.db && (p.sum.cluster == 1 || a.tokens == 0);
         float* part = join ? reinterpret_cast<float*>(wk + p.part) : nullptr;
         if (a.tokens > 0) {
-            const int64_t blocks = (a.n + 255) / 256 * p.chunks * kSumCluster;
+            const int64_t blocks = (a.n + 255) / 256 * (int64_t)p.sum.chunks * p.sum.cluster;
             if (blocks > 0x7fffffff) { set_error("linear_backward: dy of %lld x %lld is more than one launch serves", (long long)a.tokens, (long long)a.n); return CHPL_ERR_UNSUPPORTED; }
             const RowsIn<T> dy = rows_in<T>(a.dy, a.lddy);
             const RowsOut<T> go = rows_out<T>(p.g.copy ? wk + p.g.at : nullptr, p.g.ld);
             const int rows = (int)a.tokens, n = (int)a.n;
             if (a.act == CHPL_ACT_NONE)
-                CHPL_TRY(launch_kernel(grad_act_kernel<T, NoZ>, blocks, kSumThreads, 0, kSumCluster, st, dy, NoZ(), a.act, rows, n, p.rows, go, part, sums));
+                CHPL_TRY(launch_kernel(grad_act_kernel<T, NoZ>, blocks, kSumThreads, 0, p.sum.cluster, st, dy, NoZ(), a.act, rows, n, p.sum.rows,
+                                       p.sum.cluster, go, part, sums));
             else if (a.z8.codes)
-                CHPL_TRY(launch_kernel(grad_act_kernel<T, CkptIn>, blocks, kSumThreads, 0, kSumCluster, st, dy, ckpt_in(a.z8), a.act, rows, n,
-                                       p.rows, go, part, sums));
+                CHPL_TRY(launch_kernel(grad_act_kernel<T, CkptIn>, blocks, kSumThreads, 0, p.sum.cluster, st, dy, ckpt_in(a.z8), a.act, rows, n,
+                                       p.sum.rows,
+                                       p.sum.cluster, go, part, sums));
             else
-                CHPL_TRY(launch_kernel(grad_act_kernel<T, RowsIn<T>>, blocks, kSumThreads, 0, kSumCluster, st, dy, rows_in<T>(a.z, a.ldz), a.act,
-                                       rows, n, p.rows, go, part, sums));
+                CHPL_TRY(launch_kernel(grad_act_kernel<T, RowsIn<T>>, blocks, kSumThreads, 0, p.sum.cluster, st, dy, rows_in<T>(a.z, a.ldz), a.act,
+                                       rows, n, p.sum.rows,
+                                       p.sum.cluster, go, part, sums));
         }
         if (join)
-            CHPL_TRY(launch_kernel(sum_chunks_kernel<T>, (a.n + kSumThreads - 1) / kSumThreads, kSumThreads, 0, 1, st, part, p.chunks,
+            CHPL_TRY(launch_kernel(sum_chunks_kernel<T>, (a.n + kSumThreads - 1) / kSumThreads, kSumThreads, 0, 1, st, part, p.sum.chunks,
                                    (int)a.n, sums));
     }
     if (a.k == 0) return CHPL_OK;

@@ -391,7 +391,7 @@ __device__ __forceinline__ void put_ckpt(const Epilogue& e, int f0, int t0, uint
         scale[r] = ckpt_scale(scale[r]);
         worst = max(worst, scale[r]);
     }
-    // ckpt_code() of two rows at a time
+    // two rows at a time
     constexpr int kZero = 0x4B400000;  // 3 * 2^22
     int code[8 * NCB];
 #pragma unroll
