@@ -340,12 +340,13 @@ template <typename In, typename Out, typename F>
 int run_rows(cudaStream_t st, const In& in, const Out& out, const F& f, int64_t rows, int64_t cols)
 {
     constexpr int64_t kBlocks = 148 * 8, kWarps = kRowsThreads / 32;  // eight resident blocks per SM, then a grid stride
-    // long rows in pieces of four units, as long as that leaves every warp a piece
-    const int64_t segs4 = (cols + 1023) / 1024, segs1 = (cols + 255) / 256;
+    // long rows in pieces of several units, as long as that leaves every warp a piece
+    constexpr int kUnits = std::is_same<In, CkptIn>::value ? 8 : 4;  // 64 bytes a lane under way
+    const int64_t segs4 = (cols + kUnits * 256 - 1) / (kUnits * 256), segs1 = (cols + 255) / 256;
     const bool wide = cols > 256 && rows * segs4 >= kBlocks * kWarps;
     const int64_t segs = wide ? segs4 : segs1, items = rows * segs, blocks = (items + kWarps - 1) / kWarps;
     const unsigned grid = (unsigned)(blocks < kBlocks ? blocks : kBlocks);
-    return launch_kernel(wide ? rows_kernel<4, In, Out, F> : rows_kernel<1, In, Out, F>, grid, kRowsThreads, 0, 1, st, in, out,
+    return launch_kernel(wide ? rows_kernel<kUnits, In, Out, F> : rows_kernel<1, In, Out, F>, grid, kRowsThreads, 0, 1, st, in, out,
                          f, items, (uint32_t)segs, (int)cols);
 }
 
