@@ -349,8 +349,6 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
 //   warp 1      TMEM allocation; tcgen05.mma issue (even CTA)
 //   the others  epilogue (both CTAs)
 // ----------------------------------------------------------------------------
-constexpr int PAIR_STAGES = 6;
-constexpr int PAIR_STAGE_BYTES = A_BYTES + 128 * BK * 2;
 // Sixteen epilogue warps with 16 rows each at a time: with a short contraction
 // the epilogue's latencies bound the kernel, and four warps per scheduler hide
 // them best (1024 x 1024 x 16384 with GELU and codes written 42 us; eight warps
@@ -360,12 +358,14 @@ constexpr int PAIR_NCB = 2;
 constexpr int PAIR_THREADS = 64 + 32 * PAIR_EPI_WARPS;
 constexpr int ROWS = 8 * PAIR_NCB;               // rows that an epilogue warp takes at a time
 constexpr int ROUND = PAIR_EPI_WARPS / 4 * ROWS;  // rows that all of them do: a tile has as many at least
-constexpr int PAIR_SMEM = 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + PAIR_EPI_WARPS * kStageBytes + 256;
+constexpr int PAIR_RING = 6 * (A_BYTES + 128 * BK * 2);  // bytes of the ring: six stages at 256 rows, more at fewer
+constexpr int PAIR_SMEM = 1024 + PAIR_RING + PAIR_EPI_WARPS * kStageBytes + 512;
 
 struct PairShape {
     int bn;              // rows t of a tile, a multiple of 32, 64 to 256
     int mtiles, ntiles;
     int group;           // feature tiles walked before the next row tile: what L2 holds of A meanwhile
+    int stages;          // of the ring
 };
 
 __device__ __forceinline__ void pair_tile(const PairShape& sh, int tile, int& mt, int& nt)
@@ -394,10 +394,11 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* stages = smem + PAIR_STAGES * PAIR_STAGE_BYTES;  // of the epilogue
+    const int nstages = sh.stages, sbytes = A_BYTES + b_bytes<KIND>(sh.bn / 2);
+    uint8_t* stages = smem + PAIR_RING;  // of the epilogue
     uint64_t* full = reinterpret_cast<uint64_t*>(stages + PAIR_EPI_WARPS * kStageBytes);
-    uint64_t* empty = full + PAIR_STAGES;
-    uint64_t* acc_full = empty + PAIR_STAGES;
+    uint64_t* empty = full + MAX_STAGES;
+    uint64_t* acc_full = empty + MAX_STAGES;
     uint64_t* acc_empty = acc_full + 2;
     uint64_t* drain = acc_empty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -408,7 +409,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     const int unit = (int)(blockIdx.x >> 1), nunits = (int)(gridDim.x >> 1);
     const int total = sh.mtiles * sh.ntiles;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < PAIR_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < nstages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * PAIR_EPI_WARPS); }
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 
     if (warp == 0) {
         if (elect_one()) {
-            const uint32_t bytes = 2u * (A_BYTES + (uint32_t)b_bytes<KIND>(half_rows));  // both CTAs' copies
+            const uint32_t bytes = 2u * (uint32_t)sbytes;  // both CTAs' copies
             int stage = 0, started = 0;
             uint32_t ph = 0;
             bool ok = true;
@@ -438,12 +439,12 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                 const int f0 = mt * 2 * BM + (int)rank * BM, t0 = nt * sh.bn + (int)rank * half_rows;
                 for (int kb = 0; kb < kblocks; ++kb) {
                     if (!mbar_wait(&empty[stage], ph ^ 1u, abort_flag)) { ok = false; break; }
-                    uint8_t* sa = smem + stage * PAIR_STAGE_BYTES;
+                    uint8_t* sa = smem + stage * sbytes;
                     if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
                     load_tile_pair<Major<KIND>::a>(sa, &tmA, lead_full + stage * 8, f0, kb * BK, BM);
                     load_tile_pair<Major<KIND>::b>(sa + A_BYTES, &tmB, lead_full + stage * 8, t0, kb * BK, half_rows);
                     ++started;
-                    if (++stage == PAIR_STAGES) { stage = 0; ph ^= 1u; }
+                    if (++stage == nstages) { stage = 0; ph ^= 1u; }
                 }
             }
             if (!ok) {  // let the copies already in flight land before the CTA exits
@@ -452,9 +453,9 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                 }
             } else {
                 // every stage's last release (a commit of the even CTA's MMA thread) has landed here
-                for (int s = 0; s < PAIR_STAGES; ++s) {
-                    if (s >= PAIR_STAGES - started && !mbar_wait(&empty[stage], ph ^ 1u, abort_flag)) break;
-                    if (++stage == PAIR_STAGES) { stage = 0; ph ^= 1u; }
+                for (int s = 0; s < nstages; ++s) {
+                    if (s >= nstages - started && !mbar_wait(&empty[stage], ph ^ 1u, abort_flag)) break;
+                    if (++stage == nstages) { stage = 0; ph ^= 1u; }
                 }
             }
         }
@@ -474,14 +475,14 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                 for (int kb = 0; kb < kblocks; ++kb) {
                     if (!mbar_wait(&full[stage], ph, abort_flag)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t a0 = smem_u32(smem + stage * PAIR_STAGE_BYTES), b0 = a0 + A_BYTES;
+                    const uint32_t a0 = smem_u32(smem + stage * sbytes), b0 = a0 + A_BYTES;
 #pragma unroll
                     for (int kk = 0; kk < BK / UK; ++kk)
                         mma_f16_pair(d, umma_desc(a0 + kk * umma_step(Major<KIND>::a), Major<KIND>::a),
                                      umma_desc(b0 + kk * umma_step(Major<KIND>::b), Major<KIND>::b), idesc, kb || kk ? 1u : 0u);
                     mma_commit_pair(smem_u32(&empty[stage]));
                     mma_commit_pair(peer_empty + stage * 8);
-                    if (++stage == PAIR_STAGES) { stage = 0; ph ^= 1u; }
+                    if (++stage == nstages) { stage = 0; ph ^= 1u; }
                 }
                 if (!ok) break;
                 mma_commit_pair(smem_u32(&acc_full[buf]));
@@ -590,18 +591,28 @@ static int num_sms()
 // Which kernel, tile and split: the candidate of least estimated time.  The
 // estimate, in us, is a start-up time and, for each wave of tiles that the SMs
 // run, the staging of A and B per k-block (what a stage of 128 features and bn
-// rows weighs, 16 + bn / 8 KB, at the rate each kernel was seen to stage it),
-// which also covers the multiply-adds; a lone CTA's epilogue and the join of a
-// split come on top.  The constants are fitted to 3000 timings of 150 products
-// (each kind, 1 to 8000 tokens, 64 to 16384 features): the choice is 2.5 % slower
-// than the best candidate in the mean, 23 % at worst; one fixed tile was up to 5
-// times slower.  E.g. 512 x 4096 x 4096: a lone CTA's 128 rows 17 us, a pair's 128
-// rows 19, 256 rows 26, split in two 25.
+// rows weighs, 16 + bn / 8 KB, at the rate each kernel was seen to stage it; for
+// a lone CTA no less than four MMAs of 128 features take, which do not get
+// shorter below 128 rows) and the epilogue, which a pair runs under the next
+// tile; the join of a split comes on top.  The constants are fitted to 3000
+// timings of 150 products (each kind, 1 to 8000 tokens, 64 to 16384 features): the
+// choice is 2.5 % slower than the best candidate in the mean, a third at worst; one
+// fixed tile was up to 5 times slower.  E.g. 512 x 4096 x 4096: a lone CTA's 128
+// rows 17 us, a pair's 128 rows 19, 256 rows 26, split in two 25.
 struct Plan {
     bool pair;
     SplitShape split;
     PairShape tiles;
 };
+
+// CTAs of the split kernel that run at once, one or two to an SM: clusters of 4
+// and 8 do not fill the GPU's processor clusters (132 and 120 of 148 SMs, 284 and
+// 264 of 296 places, by the occupancy calculation for this GPU)
+static int slots(int split, int resident, int sms)
+{
+    const int lost = split <= 2 ? 0 : resident == 1 ? (split == 4 ? 16 : 28) : (split == 4 ? 12 : 32);
+    return std::max(1, sms * resident - lost);
+}
 
 // the narrowest multiple of `step` rows that makes no more tiles of n rows than bn does
 static int fit_rows(int n, int bn, int step)
@@ -621,18 +632,21 @@ static Plan plan_for(int m, int n, int kblocks)
         if (size >= 2 * n && least < 1e300) break;  // half the size holds every row
         const int bn = fit_rows(n, size, Major<KIND>::b ? 16 : 64);
         const int64_t tiles = (int64_t)((m + BM - 1) / BM) * ((n + bn - 1) / bn);
-        const int resident = bn <= 64 ? 2 : 1;  // CTAs per SM that the ring leaves room for
-        const double stage = 0.0096 / 1024 * stage_bytes<KIND>(bn);
+        const double stage = std::max(0.18, 0.0090 / 1024 * stage_bytes<KIND>(bn)), rest = 0.0068 * bn;
         for (int split = 1; split <= 8 && (split == 1 || split <= kblocks); split *= 2) {
-            const double ctas = (double)tiles * split, waves = std::ceil(ctas / (sms * resident));
-            const double share = std::max(1.0, std::min((double)resident, waves > 1 ? resident : ctas / sms));
-            const double t = 2.0 + waves * (share * stage * ((kblocks + split - 1) / split) + 0.41) +
-                             (split > 1 ? 1.0 + 0.0215 * bn : 0.0);
+            const double ctas = (double)tiles * split;
+            // CTAs on an SM, which share its memory: two where one each does not hold them all
+            const int resident = bn <= 64 && ctas > slots(split, 1, sms) ? 2 : 1;
+            const double waves = std::ceil(ctas / slots(split, resident, sms));
+            const double share = waves > 1 ? resident : std::max(1.0, std::min((double)resident, ctas / sms));
+            const double t = 2.2 + waves * (share * ((kblocks + split - 1) / split * stage + rest) + 0.48) +
+                             (split > 1 ? 1.3 + 0.0174 * bn : 0.0);
             if (t < least) {
                 least = t;
                 best.pair = false;
                 best.split.bn = bn;
                 best.split.split = split;
+                best.split.stages = std::min(MAX_STAGES, (SMEM_LIMIT / resident - 2048) / stage_bytes<KIND>(bn));
             }
         }
     }
@@ -641,8 +655,8 @@ static Plan plan_for(int m, int n, int kblocks)
     for (int size = Major<KIND>::b ? ROUND : 128; size <= 256 && kblocks > 0 && n > size / 2; size += step) {
         const int bn = std::max(ROUND, fit_rows(n, size, step));
         const int64_t mt = (m + 2 * BM - 1) / (2 * BM), nt = (n + bn - 1) / bn;
-        const double stage = 0.0064 / 1024 * (A_BYTES + 2 * b_bytes<KIND>(bn / 2));
-        const double t = 3.1 + std::ceil((double)mt * nt / (sms / 2)) * stage * kblocks;
+        const double products = kblocks * 0.0078 / 1024 * (A_BYTES + 2 * b_bytes<KIND>(bn / 2)), rest = 0.006 * bn;
+        const double t = 2.95 + std::ceil((double)mt * nt / (sms / 2)) * (std::max(products, rest) + 0.47) + std::min(products, rest);
         if (t < least && mt * nt < 0x7fffffff) {
             least = t;
             best.pair = true;
@@ -650,10 +664,9 @@ static Plan plan_for(int m, int n, int kblocks)
             best.tiles.mtiles = (int)mt;
             best.tiles.ntiles = (int)nt;
             best.tiles.group = 16;
+            best.tiles.stages = std::min(MAX_STAGES, PAIR_RING / (A_BYTES + b_bytes<KIND>(bn / 2)));
         }
     }
-    const int room = (best.split.bn <= 64 ? SMEM_LIMIT / 2 : SMEM_LIMIT) - 2048;
-    best.split.stages = std::min(MAX_STAGES, room / stage_bytes<KIND>(best.split.bn));
     return best;
 }
 
