@@ -6,6 +6,7 @@
     python -m chpl_b200.cases panel --m 139264 --n 1024
     python -m chpl_b200.cases dgemm --m 8192 --n 8192 --k 8192   (FP64 DGEMM, beside cuBLAS's)
     python -m chpl_b200.cases trsm --m 139264 --n 1024           (m right-hand sides)
+    python -m chpl_b200.cases ffn --tokens 4096 --d 4096 --hidden 16384   (a feed-forward block trained from 8-bit checkpoints)
     torchrun --nproc-per-node 8 --master-addr 127.0.0.1 -m chpl_b200.cases grid --N 131072 --NB 2048 --moduli 11 12
 
 Prints one JSON line per case.  Inputs are uniform [-0.5, 0.5) (the
@@ -99,6 +100,49 @@ def fp64_case(what: str, m: int, n: int, k: int, reps: int) -> dict:
     Bt = Bm.t().contiguous()
     tc = timed(lambda: torch.linalg.solve_triangular(Lt, Bt, upper=False, unitriangular=True))
     return {"case": "trsm", "n": n, "nrhs": m, "ms": t * 1e3, "tflops": n * n * m / t / 1e12, "cublas_ms": tc * 1e3}
+
+
+def ffn_case(tokens: int, d: int, hidden: int, act: str, steps: int) -> dict:
+    """A few steps of gradient descent on Y = act(X W1^T + b1) W2^T + b2 + X (BF16, X in hand, a target made by another
+    random block), holding 8-bit checkpoints between the passes; then one token through it."""
+    from . import ffn
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+
+    def mk(*shape, scale=1.0):
+        return torch.empty(*shape, dtype=torch.bfloat16, device="cuda").normal_(0.0, scale, generator=g)
+
+    def weights():
+        return [mk(hidden, d, scale=d ** -0.5), mk(hidden, scale=0.1), mk(d, hidden, scale=hidden ** -0.5), mk(d, scale=0.1)]
+
+    x, w = mk(tokens, d), weights()
+    target = ffn.forward(x, *weights(), act=act, residual=True)
+    loss, ms = [], []
+    for _ in range(steps):
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+        y, saved = ffn.forward(x, *w, act=act, residual=True, save=True)
+        dy = y - target
+        dx, *grads = ffn.backward(dy, saved, w[0], w[2])
+        e1.record()
+        for p, gr in zip(w, grads):
+            p.add_(gr, alpha=-0.5 / (tokens * hidden))
+        loss.append(float(dy.float().square().mean()))
+        ms.append(e0.elapsed_time(e1))
+    flops = 12.0 * tokens * d * hidden
+    one = x[:1]
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    for _ in range(3):
+        ffn.forward(one, *w, act=act, residual=True)
+    e0.record()
+    for _ in range(20):
+        ffn.forward(one, *w, act=act, residual=True)
+    e1.record()
+    torch.cuda.synchronize()
+    return {"case": "ffn", "tokens": tokens, "d": d, "hidden": hidden, "act": act, "loss": loss, "step_ms": min(ms),
+            "tflops": flops / min(ms) / 1e9, "held_bytes": saved.x.nbytes() + saved.z.nbytes(),
+            "held_bytes_16bit": 2 * tokens * (d + 2 * hidden), "one_token_us": e0.elapsed_time(e1) / 20 * 1e3,
+            "one_token_gbs": 4.0 * d * hidden / (e0.elapsed_time(e1) / 20 * 1e-3) / 1e9}
 
 
 def panel_case(m: int, n: int, reps: int) -> dict:
@@ -247,6 +291,12 @@ def main() -> None:
     lw.add_argument("--cols", type=int, default=65536)
     lw.add_argument("--swaps", type=int, default=1024)
     lw.add_argument("--reps", type=int, default=5)
+    ff = sub.add_parser("ffn", help="a feed-forward block trained from 8-bit checkpoints")
+    ff.add_argument("--tokens", type=int, default=4096)
+    ff.add_argument("--d", type=int, default=4096)
+    ff.add_argument("--hidden", type=int, default=16384)
+    ff.add_argument("--act", default="gelu")
+    ff.add_argument("--steps", type=int, default=6)
     gr = sub.add_parser("grid")
     gr.add_argument("--N", type=int, default=131072)
     gr.add_argument("--NB", type=int, default=2048)
@@ -274,6 +324,8 @@ def main() -> None:
         print(json.dumps(gemm_case(a.m, a.n, a.k, a.moduli, a.reps, a.scaled, a.sustain)), flush=True)
     elif a.what in ("dgemm", "trsm"):
         print(json.dumps(fp64_case(a.what, a.m, a.n, a.k, a.reps)), flush=True)
+    elif a.what == "ffn":
+        print(json.dumps(ffn_case(a.tokens, a.d, a.hidden, a.act, a.steps)), flush=True)
     elif a.what == "panel":
         print(json.dumps(panel_case(a.m, a.n, a.reps)), flush=True)
     elif a.what == "ingest":

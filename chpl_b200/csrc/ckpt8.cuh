@@ -123,6 +123,18 @@ __device__ __forceinline__ float ckpt_step(uint32_t s)
 // within +-127.  A poisoned group's codes are not numbers' and have to be
 // replaced by 0.
 
+// codes of v[0..3] in bytes 0..3
+__device__ __forceinline__ uint32_t ckpt_codes4(const float* v, float inv)
+{
+    uint32_t h[2];  // as pairs of 16-bit integers
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 q = apart(fma2(two(v[2 * i], v[2 * i + 1]), both(inv), both(12582912.0f)));
+        h[i] = __vmins2(__vmaxs2(__byte_perm(__float_as_uint(q.x), __float_as_uint(q.y), 0x5410), 0xff81ff81u), 0x007f007fu);
+    }
+    return __byte_perm(h[0], h[1], 0x6420);
+}
+
 // Values of the codes in bytes 0..3 of w: each, biased by 128, as the low byte of
 // 2^23's mantissa, less 2^23 + 128, times the step; exact.
 __device__ __forceinline__ void ckpt_values(uint32_t w, float step, float* v)
@@ -272,14 +284,8 @@ struct CkptOut {
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const uint32_t s = ckpt_scale(top);
-        const Two inv = both(ckpt_inv_step(s));
-        uint32_t h[4];  // the codes as pairs of 16-bit integers: two at a time
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 q = apart(fma2(two(v[2 * i], v[2 * i + 1]), inv, both(12582912.0f)));
-            h[i] = __vmins2(__vmaxs2(__byte_perm(__float_as_uint(q.x), __float_as_uint(q.y), 0x5410), 0xff81ff81u), 0x007f007fu);
-        }
-        uint2 w = make_uint2(__byte_perm(h[0], h[1], 0x6420), __byte_perm(h[2], h[3], 0x6420));
+        const float inv = ckpt_inv_step(s);
+        uint2 w = make_uint2(ckpt_codes4(v, inv), ckpt_codes4(v + 4, inv));
         if (s == kCkptBadScale) w = make_uint2(0, 0);
         if (j >= cols) return;
         int8_t* at = c.codes + t * c.ldc + j;

@@ -544,6 +544,154 @@ __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float 
     put16<T, NCB>(e, e.out, e.ldo, e.vec_out, f0, t0, stage, v);
 }
 
+// ----------------------------------------------------------------------------
+// The same epilogue where a warp holds one row, a lane four consecutive
+// features (the joined sums of a split): memory is read and written 8 bytes a
+// lane, a checkpoint group is eight lanes.
+// ----------------------------------------------------------------------------
+struct RowFetched {
+    uint2 add;        // four 16-bit elements
+    float4 add32;     // FP32 gradients
+    uint2 z;          // four 16-bit elements, or codes in x
+    uint32_t scale;
+};
+
+__device__ __forceinline__ uint2 row16(const void* base, int64_t ld, int t, int f, int n, int m, bool vec)
+{
+    uint2 w = make_uint2(0, 0);
+    if (t >= n || f >= m) return w;
+    const unsigned short* at = static_cast<const unsigned short*>(base) + (int64_t)t * ld + f;
+    if (vec && f + 4 <= m) return *reinterpret_cast<const uint2*>(at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (f + i < m) (i < 2 ? w.x : w.y) |= (uint32_t)at[i] << (16 * (i & 1));
+    return w;
+}
+
+template <Kind KIND>
+__device__ __forceinline__ void fetch_row(const Epilogue& e, int f, int t, RowFetched& x)
+{
+    if (e.add) {
+        if (KIND == kGradWeight && e.out_f32) {
+            float* v = &x.add32.x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = t < e.n && f + i < e.m ? static_cast<const float*>(e.add)[(int64_t)t * e.ldadd + f + i] : 0.0f;
+        } else {
+            x.add = row16(e.add, e.ldadd, t, f, e.n, e.m, e.vec_add);
+        }
+    }
+    if (KIND == kGradInput && e.act != CHPL_ACT_NONE) {
+        if (!e.z8.codes) {
+            x.z = row16(e.z, e.ldz, t, f, e.n, e.m, e.vec_z);
+        } else {
+            x.z = make_uint2(0, 0);
+            x.scale = kCkptMinScale;
+            if (t < e.n && f < e.m) {
+                const int8_t* c = e.z8.codes + (int64_t)t * e.z8.ldc + f;
+                x.scale = e.z8.scales[(int64_t)t * e.z8.lds + f / kCkptGroup];
+                if (e.vec_codes && f + 4 <= e.m) {
+                    x.z.x = *reinterpret_cast<const uint32_t*>(c);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (f + i < e.m) x.z.x |= (uint32_t)(uint8_t)c[i] << (8 * i);
+                }
+            }
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void put_row16(void* out, int64_t ld, bool vec, int f, int t, int m, const float (&v)[4])
+{
+    T* o = static_cast<T*>(out) + (int64_t)t * ld + f;
+    if (vec && f + 4 <= m) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (f + i < m) o[i] = from_f32<T>(v[i]);
+    }
+}
+
+// Every lane of the warp calls it; t < e.n; bias of the four features.
+template <typename T, Kind KIND, bool READS>
+__device__ __forceinline__ void finish_row(const Epilogue& e, int f, int t, float (&v)[4], const float (&bias)[4], const RowFetched& x)
+{
+    if (KIND == kGradWeight && e.out_f32) {
+        float* o = static_cast<float*>(e.out) + (int64_t)t * e.ldo + f;
+        if (READS && e.add) {
+            v[0] += x.add32.x;
+            v[1] += x.add32.y;
+            v[2] += x.add32.z;
+            v[3] += x.add32.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (f + i < e.m) o[i] = v[i];
+        return;
+    }
+    if (KIND == kForward) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += bias[i];
+        if (e.z) put_row16<T>(e.z, e.ldz, e.vec_z, f, t, e.m, v);
+        if (e.z8.codes) {
+            uint32_t s = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s = max(s, f + i < e.m ? __float_as_uint(v[i]) & 0x7fffffffu : 0u);
+#pragma unroll
+            for (int d = 1; d <= 4; d *= 2) s = max(s, __shfl_xor_sync(0xffffffffu, s, d));
+            s = ckpt_scale(s);
+            uint32_t w = ckpt_codes4(v, ckpt_inv_step(s));
+            if (s == kCkptBadScale) w = 0;
+            int8_t* c = e.z8.codes + (int64_t)t * e.z8.ldc + f;
+            if (e.vec_codes && f + 4 <= e.m) {
+                *reinterpret_cast<uint32_t*>(c) = w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (f + i < e.m) c[i] = (int8_t)(w >> (8 * i));
+            }
+            if (f % kCkptGroup == 0 && f < e.m) e.z8.scales[(int64_t)t * e.z8.lds + f / kCkptGroup] = (uint8_t)s;
+        }
+        with_act(e.act, [&](auto tag) {
+            activate<decltype(tag)::value>(v[0], v[1]);
+            activate<decltype(tag)::value>(v[2], v[3]);
+        });
+    }
+    if (KIND == kGradInput && READS && e.act != CHPL_ACT_NONE) {
+        float z[4];
+        if (e.z8.codes) {
+            ckpt_values(x.z.x, ckpt_step(x.scale), z);
+        } else {
+            const float2 a = unpack2<T>(x.z.x), b = unpack2<T>(x.z.y);
+            z[0] = a.x;
+            z[1] = a.y;
+            z[2] = b.x;
+            z[3] = b.y;
+        }
+        with_act(e.act, [&](auto tag) {
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                float sa, sb;
+                slope_and_value<decltype(tag)::value>(z[i], z[i + 1], sa, sb);
+                v[i] *= sa;
+                v[i + 1] *= sb;
+            }
+        });
+        if (e.xv) put_row16<T>(e.xv, e.ldxv, true, f, t, e.m, z);
+    }
+    if (READS && e.add) {
+        const float2 a = unpack2<T>(x.add.x), b = unpack2<T>(x.add.y);
+        v[0] += a.x;
+        v[1] += a.y;
+        v[2] += b.x;
+        v[3] += b.y;
+    }
+    put_row16<T>(e.out, e.ldo, e.vec_out, f, t, e.m, v);
+}
+
 // whether an epilogue reads anything but the accumulators and the bias
 inline bool reads(Kind kind, const Epilogue& e) { return e.add || (kind == kGradInput && e.act != CHPL_ACT_NONE); }
 

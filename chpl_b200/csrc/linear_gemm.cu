@@ -162,6 +162,7 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* tm, u
 //   warps 0-7  epilogue, once the accumulator is complete
 // ----------------------------------------------------------------------------
 constexpr int SPLIT_THREADS = 256;
+constexpr int JOIN = 4;          // rows that a warp joins at a time
 constexpr int JOIN_LD = BM + 4;  // row distance of the partial sums: a lane quad's rows in different banks
 
 struct SplitShape {
@@ -259,19 +260,26 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
         __syncwarp();
     }
     // One CTA per tile: a warp takes its TMEM quarter's features and every other
-    // 16 rows.  Several: CTA r takes the 8-row blocks r, r + S, ... of the tile.
+    // 16 rows.  Several: the rows are dealt out to the warps of the cluster.
     const int rows = min(sh.bn, e.n - t0);  // rows of this tile that exist
     const bool joined = sh.split > 1;
     const int quarter = warp & 3, half = warp >> 2, fq = f0 + quarter * 32;
-    const int mine = rows > rank * 8 ? ((rows + 7) / 8 - rank + sh.split - 1) / sh.split : 0;  // blocks of this CTA
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int f4 = f0 + lane * 4, mine = warp * sh.split + rank, deal = 8 * sh.split;
     Fetched<2> ahead;
-    Fetched<1> ahead1;
+    RowFetched ahead_rows[JOIN];
     float bias[4];
-    bias_of<T>(e, fq, bias);
-    if (READS) {
-        if (!joined) fetch<T, KIND, 2>(e, fq, t0 + half * 16, ahead);
-        else if (half < mine) fetch<T, KIND, 1>(e, fq, t0 + (rank + half * sh.split) * 8, ahead1);
+    if (!joined) {
+        bias_of<T>(e, fq, bias);
+        if (READS) fetch<T, KIND, 2>(e, fq, t0 + half * 16, ahead);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bias[i] = e.bias && f4 + i < e.m ? to_f32(static_cast<const T*>(e.bias)[f4 + i]) : 0.0f;
+        if (READS) {
+#pragma unroll
+            for (int u = 0; u < JOIN; ++u)
+                if (mine + u * deal < rows) fetch_row<KIND>(e, f4, t0 + mine + u * deal, ahead_rows[u]);
+        }
     }
 
     // every MMA of this CTA has completed (so every copy has landed and been read)
@@ -290,7 +298,6 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     } else {
         // partial sums as [row][128 features] into the ring's shared memory
         float* part = reinterpret_cast<float*>(smem);
-        const uint32_t stage = smem_u32(part + sh.bn * JOIN_LD) + warp * kStageBytes;
         const int at = (lane & 3) * 2 * JOIN_LD + (lane >> 2);  // of fragment 0
         for (int c = half * 16; c < rows; c += 32) {
             float v[16];
@@ -300,30 +307,30 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
                 part[(c + (i >> 2 & 1) * 8 + (i & 1)) * JOIN_LD + quarter * 32 + (i >> 3) * 16 + (i >> 1 & 1) * 8 + at] = v[i];
         }
         cluster_sync();
-        // a warp sums one row of each block over the CTAs, 16 bytes a lane, in
-        // rank order; nobody else reads that row of this CTA's, so it stays there
-        for (int b = 0; b < mine; ++b) {
-            const int row = (rank + b * sh.split) * 8 + warp;
-            if (row >= rows) break;
-            float* here = part + row * JOIN_LD + lane * 4;
-            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
+        // a warp sums whole rows over the CTAs, 16 bytes a lane, in rank order
+        const uint32_t here = smem_u32(part + lane * 4);
+        for (int row = mine; row < rows; row += JOIN * deal) {
+            float v[JOIN][4] = {};
             for (int r = 0; r < sh.split; ++r) {
-                const float4 w = ld_cluster_f32x4(map_to_rank(smem_u32(here), (uint32_t)r));
-                sum.x += w.x;
-                sum.y += w.y;
-                sum.z += w.z;
-                sum.w += w.w;
-            }
-            *reinterpret_cast<float4*>(here) = sum;
-        }
-        __syncthreads();
-        for (int b = half; ok && b < mine; b += 2) {
-            const int c = (rank + b * sh.split) * 8;
-            float v[8];
+                const uint32_t peer = map_to_rank(here, (uint32_t)r);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = part[(c + (i & 1)) * JOIN_LD + quarter * 32 + (i >> 1) * 8 + at];
-            finish<T, KIND, READS, 1>(e, fq, t0 + c, v, bias, ahead1, {b + 2 < mine ? fq : -1, t0 + c + 16 * sh.split}, stage);
+                for (int u = 0; u < JOIN; ++u)
+                    if (row + u * deal < rows) {
+                        const float4 w = ld_cluster_f32x4(peer + (uint32_t)((row + u * deal) * JOIN_LD * 4));
+                        v[u][0] += w.x;
+                        v[u][1] += w.y;
+                        v[u][2] += w.z;
+                        v[u][3] += w.w;
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < JOIN; ++u)
+                if (ok && row + u * deal < rows) finish_row<T, KIND, READS>(e, f4, t0 + row + u * deal, v[u], bias, ahead_rows[u]);
+            if (READS) {
+#pragma unroll
+                for (int u = 0; u < JOIN; ++u)
+                    if (row + (JOIN + u) * deal < rows) fetch_row<KIND>(e, f4, t0 + row + (JOIN + u) * deal, ahead_rows[u]);
+            }
         }
         cluster_sync();  // no CTA leaves while another still reads its sums
     }
