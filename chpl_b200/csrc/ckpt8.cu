@@ -27,13 +27,13 @@ static int check_matrix(const char* who, int type, int64_t rows, int64_t cols, c
 template <typename T>
 static int pack(cudaStream_t st, int64_t rows, int64_t cols, const void* x, int64_t ldx, const chpl_ckpt8& c)
 {
-    return run_rows(st, rows_in<T>(x, ldx), ckpt_out(c), Keep(), rows, cols);
+    return run_rows(st, RowsJob<RowsIn<T>, CkptOut, Keep>(rows_in<T>(x, ldx), ckpt_out(c), Keep(), rows, cols));
 }
 
 template <typename T>
 static int unpack(cudaStream_t st, int64_t rows, int64_t cols, void* x, int64_t ldx, const chpl_ckpt8& c)
 {
-    return run_rows(st, ckpt_in(c), rows_out<T>(x, ldx), Keep(), rows, cols);
+    return run_rows(st, RowsJob<CkptIn, RowsOut<T>, Keep>(ckpt_in(c), rows_out<T>(x, ldx), Keep(), rows, cols));
 }
 
 }  // namespace linear

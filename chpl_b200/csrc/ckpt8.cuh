@@ -311,49 +311,96 @@ RowsOut<T> rows_out(void* p, int64_t ld) { return {static_cast<T*>(p), ld, align
 inline CkptIn ckpt_in(const chpl_ckpt8& c) { return {c, aligned(c.codes, c.ldc, 8)}; }
 inline CkptOut ckpt_out(const chpl_ckpt8& c) { return {c, aligned(c.codes, c.ldc, 8)}; }
 
-// out = f(in), row by row (a checkpoint takes in as it is): a warp takes UNITS x 256 columns of a row at a time,
-// a lane 8 consecutive ones of each, every load before any arithmetic.
+// out = f(in), row by row (a checkpoint takes in as it is): a warp takes UNITS x
+// 256 columns of a row at a time, a lane 8 consecutive ones of each, every load
+// before any arithmetic.
 constexpr int kRowsThreads = 256;
-
-template <int UNITS, typename In, typename Out, typename F>
-__global__ void __launch_bounds__(kRowsThreads) rows_kernel(In in, Out out, F f, int64_t items, uint32_t segs, int cols)
-{
-    const int lane = lane_id();
-    const int64_t step = (int64_t)gridDim.x * (kRowsThreads / 32);
-    start_of_inputs();
-    for (int64_t i = (int64_t)blockIdx.x * (kRowsThreads / 32) + warp_id(); i < items; i += step) {
-        const int64_t t = items < 0xffffffffll ? (int64_t)((uint32_t)i / segs) : i / segs;
-        const int j0 = (int)(i - t * segs) * (UNITS * 256) + lane * 8;
-        typename In::Raw raw[UNITS];
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u) raw[u] = in.raw(t, j0 + u * 256, cols);
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            float v[8];
-            in.value(raw[u], v);
-            f(v);
-            if constexpr (std::is_same<Out, CkptOut>::value) out.put(t, j0 + u * 256, cols, v, in.top(raw[u]));
-            else out.put(t, j0 + u * 256, cols, v);
-        }
-    }
-}
 
 struct Keep {
     __device__ __forceinline__ void operator()(float (&)[8]) const {}
 };
 
-template <typename In, typename Out, typename F>
-int run_rows(cudaStream_t st, const In& in, const Out& out, const F& f, int64_t rows, int64_t cols)
+template <typename In_, typename Out_, typename F_>
+struct RowsJob {
+    using In = In_;
+    using Out = Out_;
+    In in;
+    Out out;
+    F_ f;
+    int64_t items;   // pieces of rows
+    uint32_t segs;   // pieces of a row
+    int cols;
+    unsigned blocks;
+    bool wide;       // pieces of UNITS units, else of one
+
+    // units of a long row's piece: 64 bytes a lane under way
+    static constexpr int kUnits = std::is_same<In, CkptIn>::value ? 8 : 4;
+
+    RowsJob(const In& i, const Out& o, const F_& fn, int64_t rows, int64_t ncols) : in(i), out(o), f(fn), cols((int)ncols)
+    {
+        constexpr int64_t kBlocks = 148 * 8, kWarps = kRowsThreads / 32;  // eight resident blocks per SM, then a grid stride
+        // long rows in pieces of several units, as long as that leaves every warp a piece
+        const int64_t segs_wide = (ncols + kUnits * 256 - 1) / (kUnits * 256);
+        wide = ncols > 256 && rows * segs_wide >= kBlocks * kWarps;
+        segs = (uint32_t)(wide ? segs_wide : (ncols + 255) / 256);
+        items = rows * segs;
+        const int64_t want = (items + kWarps - 1) / kWarps;
+        blocks = (unsigned)(want < kBlocks ? want : kBlocks);
+    }
+
+    template <int UNITS>
+    __device__ __forceinline__ void run(unsigned block) const
+    {
+        const int lane = lane_id();
+        const int64_t step = (int64_t)blocks * (kRowsThreads / 32);
+        for (int64_t i = (int64_t)block * (kRowsThreads / 32) + warp_id(); i < items; i += step) {
+            const int64_t t = items < 0xffffffffll ? (int64_t)((uint32_t)i / segs) : i / segs;
+            const int j0 = (int)(i - t * segs) * (UNITS * 256) + lane * 8;
+            typename In::Raw raw[UNITS];
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) raw[u] = in.raw(t, j0 + u * 256, cols);
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+                float v[8];
+                in.value(raw[u], v);
+                f(v);
+                if constexpr (std::is_same<Out, CkptOut>::value) out.put(t, j0 + u * 256, cols, v, in.top(raw[u]));
+                else out.put(t, j0 + u * 256, cols, v);
+            }
+        }
+    }
+};
+
+template <int UNITS, typename Job>
+__global__ void __launch_bounds__(kRowsThreads) rows_kernel(const Job job)
 {
-    constexpr int64_t kBlocks = 148 * 8, kWarps = kRowsThreads / 32;  // eight resident blocks per SM, then a grid stride
-    // long rows in pieces of several units, as long as that leaves every warp a piece
-    constexpr int kUnits = std::is_same<In, CkptIn>::value ? 8 : 4;  // 64 bytes a lane under way
-    const int64_t segs4 = (cols + kUnits * 256 - 1) / (kUnits * 256), segs1 = (cols + 255) / 256;
-    const bool wide = cols > 256 && rows * segs4 >= kBlocks * kWarps;
-    const int64_t segs = wide ? segs4 : segs1, items = rows * segs, blocks = (items + kWarps - 1) / kWarps;
-    const unsigned grid = (unsigned)(blocks < kBlocks ? blocks : kBlocks);
-    return launch_kernel(wide ? rows_kernel<kUnits, In, Out, F> : rows_kernel<1, In, Out, F>, grid, kRowsThreads, 0, 1, st, in, out,
-                         f, items, (uint32_t)segs, (int)cols);
+    start_of_inputs();
+    job.template run<UNITS>(blockIdx.x);
+}
+
+// two jobs side by side
+template <typename A, typename B>
+__global__ void __launch_bounds__(kRowsThreads) rows_pair_kernel(const A a, const B b)
+{
+    start_of_inputs();
+    if (blockIdx.x < a.blocks) a.template run<1>(blockIdx.x);
+    else b.template run<1>(blockIdx.x - a.blocks);
+}
+
+template <typename Job>
+int run_rows(cudaStream_t st, const Job& job)
+{
+    return launch_kernel(job.wide ? rows_kernel<Job::kUnits, Job> : rows_kernel<1, Job>, job.blocks, kRowsThreads, 0, 1, st, job);
+}
+
+// small ones in one launch
+template <typename A, typename B>
+int run_rows(cudaStream_t st, const A& a, const B& b)
+{
+    if (!a.wide && !b.wide)
+        return launch_kernel(rows_pair_kernel<A, B>, (int64_t)a.blocks + b.blocks, kRowsThreads, 0, 1, st, a, b);
+    CHPL_TRY(run_rows(st, a));
+    return run_rows(st, b);
 }
 
 }  // namespace chpl

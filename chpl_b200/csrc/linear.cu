@@ -130,7 +130,7 @@ template <typename T, typename Z>
 __global__ void __launch_bounds__(kSumThreads) grad_act_kernel(RowsIn<T> dy, Z z, int act, int rows, int n, int chunk_rows,
                                                                int cluster, RowsOut<T> g, float* __restrict__ part, Sums out)
 {
-    constexpr int kAhead = 4;  // rows whose loads are under way at once
+    constexpr int kAhead = std::is_same<Z, NoZ>::value ? 4 : 2;  // rows whose loads are under way at once
     __shared__ float sums[kSumWarps][256 + 8];
     const int blocks = (n + 255) / 256, cl = blockIdx.x / cluster, rank = blockIdx.x - cl * cluster;
     const int group = cl / blocks, j0 = (cl - group * blocks) * 256;
@@ -359,25 +359,35 @@ static int check(const char* who, const chpl_linear_bwd* a, bool pointers)
 // ----------------------------------------------------------------------------
 // the two passes
 // ----------------------------------------------------------------------------
-// the operand of a product as TMA can read it: values of a checkpoint, an
-// activation of either, or a copy
+// An operand of a product as TMA can read it: the values of a checkpoint, an
+// activation of either, or a copy.
 template <typename T>
-static int expand(cudaStream_t st, const void* x, int64_t ldx, const chpl_ckpt8& c, int act, int64_t rows, int64_t cols,
-                  void* out, int64_t ldo)
+using CkptJob = RowsJob<CkptIn, RowsOut<T>, Activate>;
+template <typename T>
+using CopyJob = RowsJob<RowsIn<T>, RowsOut<T>, Activate>;
+
+template <typename T>
+static CopyJob<T> copy_job(const void* x, int64_t ldx, int act, int64_t rows, int64_t cols, void* out, int64_t ldo)
 {
-    const Activate f = {act};
-    if (c.codes) return run_rows(st, ckpt_in(c), rows_out<T>(out, ldo), f, rows, cols);
-    return run_rows(st, rows_in<T>(x, ldx), rows_out<T>(out, ldo), f, rows, cols);
+    return CopyJob<T>(rows_in<T>(x, ldx), rows_out<T>(out, ldo), Activate{act}, rows, cols);
 }
 
-static const chpl_ckpt8 kNoCkpt = {nullptr, nullptr, 0, 0};
+template <typename T>
+static CkptJob<T> ckpt_job(const chpl_ckpt8& c, int act, int64_t rows, int64_t cols, void* out, int64_t ldo)
+{
+    return CkptJob<T>(ckpt_in(c), rows_out<T>(out, ldo), Activate{act}, rows, cols);
+}
 
 template <typename T>
 static int forward(cudaStream_t st, const chpl_linear_fwd& a, void* work)
 {
     const ForwardPlan p = plan(a);
-    if (p.x.copy) CHPL_TRY(expand<T>(st, a.x, a.ldx, kNoCkpt, CHPL_ACT_NONE, a.tokens, a.k, static_cast<char*>(work) + p.x.at, p.x.ld));
-    if (p.w.copy) CHPL_TRY(expand<T>(st, a.w, a.ldw, kNoCkpt, CHPL_ACT_NONE, a.n, a.k, static_cast<char*>(work) + p.w.at, p.w.ld));
+    char* wk = static_cast<char*>(work);
+    const auto xj = [&] { return copy_job<T>(a.x, a.ldx, CHPL_ACT_NONE, a.tokens, a.k, wk + p.x.at, p.x.ld); };
+    const auto wj = [&] { return copy_job<T>(a.w, a.ldw, CHPL_ACT_NONE, a.n, a.k, wk + p.w.at, p.w.ld); };
+    if (p.x.copy && p.w.copy) CHPL_TRY(run_rows(st, xj(), wj()));
+    else if (p.x.copy) CHPL_TRY(run_rows(st, xj()));
+    else if (p.w.copy) CHPL_TRY(run_rows(st, wj()));
     Epilogue e = {};
     e.m = (int)a.n;
     e.n = (int)a.tokens;
@@ -429,9 +439,18 @@ static int backward(cudaStream_t st, const chpl_linear_bwd& a, void* work)
     const Operand g_rows = {at(p.g, a.dy, work), p.g.ld, true}, g_cols = {g_rows.p, p.g.ld, false};
     // an activation's value comes with its slope out of dX's epilogue
     const bool xv_from_dx = p.x.copy && a.dx && a.in_act != CHPL_ACT_NONE;
-    if (p.x.copy && !xv_from_dx) CHPL_TRY(expand<T>(st, a.x, a.ldx, a.x8, a.in_act, a.tokens, a.k, wk + p.x.at, p.x.ld));
+    const bool expand = p.x.copy && !xv_from_dx;
+    const auto wj = [&] { return copy_job<T>(a.w, a.ldw, CHPL_ACT_NONE, a.n, a.k, wk + p.w.at, p.w.ld); };
+    if (expand && a.x8.codes) {
+        const CkptJob<T> xj = ckpt_job<T>(a.x8, a.in_act, a.tokens, a.k, wk + p.x.at, p.x.ld);
+        CHPL_TRY(p.w.copy ? run_rows(st, xj, wj()) : run_rows(st, xj));
+    } else if (expand) {
+        const CopyJob<T> xj = copy_job<T>(a.x, a.ldx, a.in_act, a.tokens, a.k, wk + p.x.at, p.x.ld);
+        CHPL_TRY(p.w.copy ? run_rows(st, xj, wj()) : run_rows(st, xj));
+    } else if (p.w.copy) {
+        CHPL_TRY(run_rows(st, wj()));
+    }
     if (a.dx) {
-        if (p.w.copy) CHPL_TRY(expand<T>(st, a.w, a.ldw, kNoCkpt, CHPL_ACT_NONE, a.n, a.k, wk + p.w.at, p.w.ld));
         Epilogue e = {};
         e.m = (int)a.k;
         e.n = (int)a.tokens;

@@ -371,7 +371,7 @@ constexpr int PAIR_SMEM = 1024 + PAIR_RING + PAIR_EPI_WARPS * kStageBytes + 512;
 struct PairShape {
     int bn;              // rows t of a tile, a multiple of 32, 64 to 256
     int mtiles, ntiles;
-    int group;           // feature tiles walked before the next row tile: what L2 holds of A meanwhile
+    int group;           // feature tiles walked before the next row tile: see plan_for()
     int stages;          // of the ring
 };
 
@@ -606,6 +606,12 @@ static int num_sms()
 // choice is 2.5 % slower than the best candidate in the mean, a third at worst; one
 // fixed tile was up to 5 times slower.  E.g. 512 x 4096 x 4096: a lone CTA's 128
 // rows 17 us, a pair's 128 rows 19, 256 rows 26, split in two 25.
+//
+// Large products run at the board's power limit, where traffic costs clock: a
+// pair's tiles are walked in groups of features whose A, 32 MB of it, stays in
+// L2 from one row tile to the next, 8 to 16 tiles.  Products of 1.1 TFLOP each,
+// one after another: contraction 4096 in groups of 16 811 us, of 8 835, of 4 849;
+// contraction 8192 876, 835, 861 (cuBLAS 780 to 815 for either).
 struct Plan {
     bool pair;
     SplitShape split;
@@ -670,7 +676,7 @@ static Plan plan_for(int m, int n, int kblocks)
             best.tiles.bn = bn;
             best.tiles.mtiles = (int)mt;
             best.tiles.ntiles = (int)nt;
-            best.tiles.group = 16;
+            best.tiles.group = std::max(8, std::min(16, 1024 / kblocks));
             best.tiles.stages = std::min(MAX_STAGES, PAIR_RING / (A_BYTES + b_bytes<KIND>(bn / 2)));
         }
     }
