@@ -27,6 +27,11 @@ struct Epilogue {
     int m, n;        // f < m, t < n
     int act;
     int out_f32;     // out is FP32 (kGradWeight), else of the operands' type
+    // the product's operands, and how near to 1/2 a quotient has to be taken from them (SETTLE); set by gemm()
+    const void *w, *x;
+    int64_t ldw, ldx;
+    int k;
+    float tie;
     bool vec_out, vec_add, vec_z, vec_codes;  // 16-byte (8 for codes) accesses fit; set by gemm()
     void* out;
     int64_t ldo;

@@ -363,9 +363,91 @@ __device__ __forceinline__ void put16(const Epilogue& e, void* out, int64_t ld, 
     }
 }
 
-// codes and scales of v, through `at` (shared, 32-byte rows)
-template <int NCB>
-__device__ __forceinline__ void put_ckpt(const Epilogue& e, int f0, int t0, uint32_t at, const float (&v)[8 * NCB])
+// ReLU's slope at a checkpoint hangs on whether a code is 0 or 1.  tcgen05 adds
+// into FP32 accumulators by cutting, so its sums are off by some 2^-24 for each
+// 16 elements of the contraction, several times an FP32 sum's rounding, and a
+// quotient that near to a half would let the tiling decide over a gradient (777
+// x 1024 x 4096: 28 slopes in 40 calls, an FP32 product 7).  With ReLU those few
+// quotients, one in 100000, are formed again from the operands (SETTLE): products
+// exact in FP32, eight added there, the eights in FP64, by the whole warp, about
+// 2 us each; at most kSettled of a warp's rows at a time, so that data made of
+// ties costs no more than a few times the product.
+constexpr int kSettled = 8;
+
+template <typename T>
+__device__ __noinline__ double exact_z(const T* __restrict__ a, const T* __restrict__ b, int k, double bias)
+{
+    constexpr int kAhead = 4;
+    double sum = 0.0;
+    for (int c0 = lane_id() * 8; c0 < k; c0 += kAhead * 256) {
+        uint4 u[kAhead], v[kAhead];  // rows lie on 16-byte boundaries, as TMA wants them
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (c0 + i * 256 + 8 <= k) {
+                u[i] = *reinterpret_cast<const uint4*>(a + c0 + i * 256);
+                v[i] = *reinterpret_cast<const uint4*>(b + c0 + i * 256);
+            }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int c = c0 + i * 256;
+            float part = 0.0f;
+            if (c + 8 <= k) {
+                const T *p = reinterpret_cast<const T*>(&u[i]), *q = reinterpret_cast<const T*>(&v[i]);
+#pragma unroll
+                for (int h = 0; h < 8; ++h) part = fmaf(to_f32(p[h]), to_f32(q[h]), part);
+            } else {
+                for (int h = c; h < k; ++h) part = fmaf(to_f32(a[h]), to_f32(b[h]), part);
+            }
+            sum += (double)part;
+        }
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return sum + bias;
+}
+
+template <typename T>
+__device__ __forceinline__ double exact_z(const Epilogue& e, int f, int t)
+{
+    return exact_z<T>(static_cast<const T*>(e.w) + (int64_t)f * e.ldw, static_cast<const T*>(e.x) + (int64_t)t * e.ldx, e.k,
+                      e.bias ? (double)to_f32(static_cast<const T*>(e.bias)[f]) : 0.0);
+}
+
+// Settles the codes of a warp's near quotients (bit i of `near`: element i of
+// the lane, in the order of put_ckpt, or four features of one row with ROW) in
+// global memory, after the codes and scales have been written there.
+template <typename T, bool ROW>
+__device__ __noinline__ void settle(const Epilogue& e, int f0, int t0, uint32_t near)
+{
+    __syncwarp();  // orders the warp's stores before these
+    int settled = 0;
+    for (uint32_t lanes = __ballot_sync(0xffffffffu, near != 0); lanes; lanes &= lanes - 1) {
+        const int src = __ffs(lanes) - 1;
+        for (uint32_t bits = __shfl_sync(0xffffffffu, near, src); bits && settled < kSettled; bits &= bits - 1) {
+            const int i = __ffs(bits) - 1, r = i >> 2;
+            const int f = ROW ? f0 + 4 * src + i : f0 + 8 * (i & 3) + (src >> 2);
+            const int t = ROW ? t0 : t0 + 8 * (r >> 1) + 2 * (src & 3) + (r & 1);
+            if (f >= e.m || t >= e.n) continue;
+            ++settled;
+            const double z = exact_z<T>(e, f, t);
+            const uint32_t s = *const_cast<volatile uint8_t*>(e.z8.scales + (int64_t)t * e.z8.lds + f / kCkptGroup);
+            if (lane_id() == src)
+                e.z8.codes[(int64_t)t * e.z8.ldc + f] = (int8_t)max(-127, min(127, __double2int_rn(z * (double)ckpt_inv_step(s))));
+        }
+    }
+}
+
+// bit 0, 1: whether a quotient of the two lies within e.tie of +-1/2
+__device__ __forceinline__ uint32_t near_half(Two v, Two inv, float tie)
+{
+    const float2 q = apart(v * inv);
+    return (fabsf(fabsf(q.x) - 0.5f) < tie ? 1u : 0u) | (fabsf(fabsf(q.y) - 0.5f) < tie ? 2u : 0u);
+}
+
+// Codes and scales of v, through `at` (shared, 32-byte rows).  Returns, with
+// SETTLE, which of the lane's quotients are near +-1/2: bit 8 cb + 4 p + g.
+template <bool SETTLE, int NCB>
+__device__ __forceinline__ uint32_t put_ckpt(const Epilogue& e, int f0, int t0, uint32_t at, const float (&v)[8 * NCB])
 {
     const int lane = lane_id();
     const bool whole = f0 + 32 <= e.m;
@@ -394,12 +476,17 @@ __device__ __forceinline__ void put_ckpt(const Epilogue& e, int f0, int t0, uint
     // two rows at a time
     constexpr int kZero = 0x4B400000;  // 3 * 2^22
     int code[8 * NCB];
+    uint32_t near = 0;
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
         const Two inv = two(ckpt_inv_step(scale[2 * cb]), ckpt_inv_step(scale[2 * cb + 1]));
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int i = frag<NCB>(g >> 1, cb, g & 1, 0);
+            if (SETTLE) {
+                const uint32_t n2 = near_half(two(v[i], v[i + 1]), inv, e.tie);
+                near |= (n2 & 1u) << (8 * cb + g) | (n2 >> 1) << (8 * cb + 4 + g);
+            }
             const float2 q = apart(fma2(two(v[i], v[i + 1]), inv, both(12582912.0f)));
             code[8 * cb + g] = min(max(__float_as_int(q.x), kZero - 127), kZero + 127);
             code[8 * cb + 4 + g] = min(max(__float_as_int(q.y), kZero - 127), kZero + 127);
@@ -448,18 +535,20 @@ __device__ __forceinline__ void put_ckpt(const Epilogue& e, int f0, int t0, uint
                 if (f0 + f + i < e.m) o[t * e.z8.ldc + f + i] = (int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
         }
     }
+    return near;
 }
 
 // Every lane of the warp calls it.  bias[2 h + rr]; `stage`: kStageBytes of
 // shared memory of the warp's own (shared-space address, 128-byte aligned).
 // READS: x holds what these rows read, and what the rows `next` do on return.
-template <typename T, Kind KIND, bool READS, int NCB>
+template <typename T, Kind KIND, bool READS, bool SETTLE, int NCB>
 __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float (&v)[8 * NCB], const float (&bias)[4],
                                        Fetched<NCB>& x, Next next, uint32_t stage)
 {
     static_assert(NCB * 8 * 64 <= kStageBytes, "stage");
     const int lane = lane_id();
     const bool here = f0 < e.m && t0 < e.n;
+    uint32_t near = 0;
     uint32_t add[4 * NCB], zf[4 * NCB];
     if (READS && here) {
         if (KIND == kGradWeight && e.out_f32) {
@@ -504,7 +593,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float 
 #pragma unroll
         for (int i = 0; i < 8 * NCB; ++i) v[i] += bias[(i / (4 * NCB)) * 2 + ((i >> 1) & 1)];
         if (e.z) put16<T, NCB>(e, e.z, e.ldz, e.vec_z, f0, t0, stage, v);
-        if (e.z8.codes) put_ckpt<NCB>(e, f0, t0, stage, v);
+        if (e.z8.codes) near = put_ckpt<SETTLE, NCB>(e, f0, t0, stage, v);
         with_act(e.act, [&](auto tag) {
 #pragma unroll
             for (int i = 0; i < 8 * NCB; i += 2) activate<decltype(tag)::value>(v[i], v[i + 1]);
@@ -542,6 +631,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float 
             }
     }
     put16<T, NCB>(e, e.out, e.ldo, e.vec_out, f0, t0, stage, v);
+    if (SETTLE && __any_sync(0xffffffffu, near != 0)) settle<T, false>(e, f0, t0, near);
 }
 
 // ----------------------------------------------------------------------------
@@ -616,9 +706,10 @@ __device__ __forceinline__ void put_row16(void* out, int64_t ld, bool vec, int f
 }
 
 // Every lane of the warp calls it; t < e.n; bias of the four features.
-template <typename T, Kind KIND, bool READS>
+template <typename T, Kind KIND, bool READS, bool SETTLE>
 __device__ __forceinline__ void finish_row(const Epilogue& e, int f, int t, float (&v)[4], const float (&bias)[4], const RowFetched& x)
 {
+    uint32_t near = 0;
     if (KIND == kGradWeight && e.out_f32) {
         float* o = static_cast<float*>(e.out) + (int64_t)t * e.ldo + f;
         if (READS && e.add) {
@@ -643,7 +734,9 @@ __device__ __forceinline__ void finish_row(const Epilogue& e, int f, int t, floa
 #pragma unroll
             for (int d = 1; d <= 4; d *= 2) s = max(s, __shfl_xor_sync(0xffffffffu, s, d));
             s = ckpt_scale(s);
-            uint32_t w = ckpt_codes4(v, ckpt_inv_step(s));
+            const float inv = ckpt_inv_step(s);
+            uint32_t w = ckpt_codes4(v, inv);
+            if (SETTLE) near = near_half(two(v[0], v[1]), both(inv), e.tie) | near_half(two(v[2], v[3]), both(inv), e.tie) << 2;
             if (s == kCkptBadScale) w = 0;
             int8_t* c = e.z8.codes + (int64_t)t * e.z8.ldc + f;
             if (e.vec_codes && f + 4 <= e.m) {
@@ -690,9 +783,12 @@ __device__ __forceinline__ void finish_row(const Epilogue& e, int f, int t, floa
         v[3] += b.y;
     }
     put_row16<T>(e.out, e.ldo, e.vec_out, f, t, e.m, v);
+    if (SETTLE && __any_sync(0xffffffffu, near != 0)) settle<T, true>(e, f - 4 * lane_id(), t, near);
 }
 
-// whether an epilogue reads anything but the accumulators and the bias
+// whether an epilogue settles codes from the operands, and whether it reads
+// anything else but the accumulators and the bias
+inline bool settles(Kind kind, const Epilogue& e) { return kind == kForward && e.z8.codes && e.act == CHPL_ACT_RELU; }
 inline bool reads(Kind kind, const Epilogue& e) { return e.add || (kind == kGradInput && e.act != CHPL_ACT_NONE); }
 
 // the biases of a lane's four features of f0 .. f0 + 31

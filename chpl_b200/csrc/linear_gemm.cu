@@ -181,7 +181,7 @@ template <Kind KIND>
 __host__ __device__ constexpr int stage_bytes(int bn) { return A_BYTES + b_bytes<KIND>(bn); }
 __host__ __device__ constexpr uint32_t tmem_cols(int bn) { return bn <= 32 ? 32u : bn <= 64 ? 64u : bn <= 128 ? 128u : 256u; }
 
-template <typename T, Kind KIND, bool READS>
+template <typename T, Kind KIND, bool READS, bool SETTLE>
 __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const int kblocks,
                  const SplitShape sh, const __grid_constant__ Epilogue e)
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
         for (int c = half * 16; ok && c < rows; c += 32) {
             float v[16] = {};
             if (kblocks > 0) tmem_ld_frag<2>(tmem + lanes + c, v);
-            finish<T, KIND, READS, 2>(e, fq, t0 + c, v, bias, ahead, {c + 32 < rows ? fq : -1, t0 + c + 32}, stage);
+            finish<T, KIND, READS, SETTLE, 2>(e, fq, t0 + c, v, bias, ahead, {c + 32 < rows ? fq : -1, t0 + c + 32}, stage);
         }
     } else {
         // partial sums as [row][128 features] into the ring's shared memory
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
             }
 #pragma unroll
             for (int u = 0; u < JOIN; ++u)
-                if (ok && row + u * deal < rows) finish_row<T, KIND, READS>(e, f4, t0 + row + u * deal, v[u], bias, ahead_rows[u]);
+                if (ok && row + u * deal < rows) finish_row<T, KIND, READS, SETTLE>(e, f4, t0 + row + u * deal, v[u], bias, ahead_rows[u]);
             if (READS) {
 #pragma unroll
                 for (int u = 0; u < JOIN; ++u)
@@ -394,7 +394,7 @@ __device__ __forceinline__ void load_tile_pair(uint8_t* dst, const CUtensorMap* 
     }
 }
 
-template <typename T, Kind KIND, bool READS>
+template <typename T, Kind KIND, bool READS, bool SETTLE>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const int kblocks,
                 const PairShape sh, const __grid_constant__ Epilogue e)
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive_peer(lead_acc_empty + buf * 8);
                 }
-                finish<T, KIND, READS, PAIR_NCB>(e, f, t0 + c, v, bias, ahead, last ? after : Next{f, t0 + c + ROUND}, stage);
+                finish<T, KIND, READS, SETTLE, PAIR_NCB>(e, f, t0 + c, v, bias, ahead, last ? after : Next{f, t0 + c + ROUND}, stage);
             }
         }
     }
@@ -696,7 +696,7 @@ static int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& ready)
     return CHPL_OK;
 }
 
-template <typename T, Kind KIND, bool READS>
+template <typename T, Kind KIND, bool READS, bool SETTLE>
 static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, int kblocks, const Epilogue& e,
                         const SplitShape& s)
 {
@@ -710,12 +710,12 @@ static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int
         CHPL_TRY(make_tmap(&tmB, b, e.n, k, s.bn));
     }
     static std::atomic<uint64_t> ready{0};
-    CHPL_TRY(allow_smem(split_kernel<T, KIND, READS>, SMEM_LIMIT, ready));
-    return launch_kernel(split_kernel<T, KIND, READS>, ctas, SPLIT_THREADS, 1024 + s.stages * stage_bytes<KIND>(s.bn) + 512, s.split, st,
+    CHPL_TRY(allow_smem(split_kernel<T, KIND, READS, SETTLE>, SMEM_LIMIT, ready));
+    return launch_kernel(split_kernel<T, KIND, READS, SETTLE>, ctas, SPLIT_THREADS, 1024 + s.stages * stage_bytes<KIND>(s.bn) + 512, s.split, st,
                          tmA, tmB, kblocks, s, e);
 }
 
-template <typename T, Kind KIND, bool READS>
+template <typename T, Kind KIND, bool READS, bool SETTLE>
 static int launch_pair(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, int kblocks, const Epilogue& e,
                        const PairShape& s)
 {
@@ -723,24 +723,27 @@ static int launch_pair(cudaStream_t st, const Operand& a, const Operand& b, int6
     CHPL_TRY(make_tmap(&tmA, a, e.m, k, BM));
     CHPL_TRY(make_tmap(&tmB, b, e.n, k, s.bn / 2));
     static std::atomic<uint64_t> ready{0};
-    CHPL_TRY(allow_smem(pair_kernel<T, KIND, READS>, PAIR_SMEM, ready));
+    CHPL_TRY(allow_smem(pair_kernel<T, KIND, READS, SETTLE>, PAIR_SMEM, ready));
     const int units = std::min(s.mtiles * s.ntiles, num_sms() / 2);
-    return launch_kernel(pair_kernel<T, KIND, READS>, 2 * units, PAIR_THREADS, PAIR_SMEM, 2, st, tmA, tmB, kblocks, s, e);
+    return launch_kernel(pair_kernel<T, KIND, READS, SETTLE>, 2 * units, PAIR_THREADS, PAIR_SMEM, 2, st, tmA, tmB, kblocks, s, e);
 }
 
-template <typename T, Kind KIND, bool READS>
+template <typename T, Kind KIND, bool READS, bool SETTLE>
 static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
 {
     const int kblocks = (int)((k + BK - 1) / BK);
     const Plan p = plan_for<KIND>(e.m, e.n, kblocks);
-    return p.pair ? launch_pair<T, KIND, READS>(st, a, b, k, kblocks, e, p.tiles)
-                  : launch_split<T, KIND, READS>(st, a, b, k, kblocks, e, p.split);
+    return p.pair ? launch_pair<T, KIND, READS, SETTLE>(st, a, b, k, kblocks, e, p.tiles)
+                  : launch_split<T, KIND, READS, SETTLE>(st, a, b, k, kblocks, e, p.split);
 }
 
 template <typename T, Kind KIND>
 static int launch_kind(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
 {
-    return reads(KIND, e) ? launch<T, KIND, true>(st, a, b, k, e) : launch<T, KIND, false>(st, a, b, k, e);
+    if constexpr (KIND == kForward)
+        if (settles(KIND, e))
+            return reads(KIND, e) ? launch<T, KIND, true, true>(st, a, b, k, e) : launch<T, KIND, false, true>(st, a, b, k, e);
+    return reads(KIND, e) ? launch<T, KIND, true, false>(st, a, b, k, e) : launch<T, KIND, false, false>(st, a, b, k, e);
 }
 
 template <typename T>
@@ -760,6 +763,12 @@ int gemm(cudaStream_t st, int type, Kind kind, const Operand& a, const Operand& 
     e.vec_add = aligned(e.add, e.ldadd * elt, 16);
     e.vec_z = aligned(e.z, e.ldz * 2, 16);
     e.vec_codes = aligned(e.z8.codes, e.z8.ldc, 8);
+    e.w = a.p;
+    e.ldw = a.ld;
+    e.x = b.p;
+    e.ldx = b.ld;
+    e.k = (int)k;
+    e.tie = 5e-6f * (float)((k + BK - 1) / BK);  // some 10 times the error seen, of quotients up to 128
     return type == CHPL_TYPE_BF16 ? launch_type<__nv_bfloat16>(st, kind, a, b, k, e)
                                   : launch_type<__half>(st, kind, a, b, k, e);
 }

@@ -299,3 +299,25 @@ def test_refusals(cuda):
             f()
         assert err.value.code == _lib.CHPL_ERR_INVALID, i
     assert linear.backward(dy, None, w, need_dw=False)[0].shape == (4, 16)
+
+
+@pytest.mark.parametrize("T,k,n", [(777, 1024, 1024), (400, 2048, 1040), (1024, 1023, 2100)])
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_relu_codes_settle_at_the_slope(cuda, T, k, n, dt):
+    """Whether a code is 0, and with it ReLU's slope at the checkpoint, follows the exact Z and not the tiling: of some
+    thousand quotients within 1e-3 of 1/2, those further than 1e-6 from it (FP32's rounding of partial sums of eight,
+    2^-24 of a few steps) have the code that Z has."""
+    g = gen(31)
+    x, w = rows(g, T, k, dt), rows(g, n, k, dt, 0, k ** -0.5)
+    z = x.double() @ w.double().t()
+    b = torch.zeros(n, dtype=dt, device="cuda")
+    codes, scales = ref.pack(z)
+    step = torch.ldexp(torch.ones_like(scales, dtype=torch.float64), scales.int() - 133).repeat_interleave(32, 1)[:, :n]
+    q = z / step
+    near = (q.abs() - 0.5).abs()
+    assert bool((near < 1e-3).any())                      # there are some to settle
+    _, c = linear.forward(x, w, b, act="relu", save="z8")
+    want = q.abs() > 0.5
+    sure = near > 1e-6                                     # beyond FP64's own doubt and the exact sum's FP32 eights
+    same = c.scales.repeat_interleave(32, 1)[:, :n] == scales.repeat_interleave(32, 1)[:, :n]
+    assert torch.equal(((c.codes != 0) == want) | ~sure | ~same, torch.ones_like(want))
