@@ -73,7 +73,7 @@ class LinearBwd(ctypes.Structure):
     _fields_ = [("type", _int), ("act", _int), ("in_act", _int), ("grad_type", _int), ("accumulate", _int),
                 ("tokens", _i64), ("n", _i64), ("k", _i64), ("dy", _vp), ("lddy", _i64), ("w", _vp), ("ldw", _i64),
                 ("x", _vp), ("ldx", _i64), ("x8", Ckpt8), ("z", _vp), ("ldz", _i64), ("z8", Ckpt8), ("add", _vp),
-                ("ldadd", _i64), ("dx", _vp), ("lddx", _i64), ("dw", _vp), ("lddw", _i64), ("db", _vp)]
+                ("ldadd", _i64), ("dx", _vp), ("lddx", _i64), ("dw", _vp), ("lddw", _i64), ("db", _vp), ("dx_sum", _vp)]
 
 
 # name -> (restype, argtypes); every function declared in include/chpl.h

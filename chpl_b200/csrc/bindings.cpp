@@ -270,12 +270,12 @@ PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n)
 }
 
 // linear_backward(dy, w, x, x.codes, x.scales, z, z.codes, z.scales, add, act, in_act, float32 gradients, accumulate,
-//                 need dx, need dw, need db, dx, dw, db, work) -> (dx, dw, db)
+//                 need dx, need dw, need db, need dx_sum, dx, dw, db, dx_sum, work) -> (dx, dw, db, dx_sum)
 PyObject* linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
     CHPL_PY_BEGIN
     const char* where = "linear.backward";
-    arguments(where, n, 20);
+    arguments(where, n, 22);
     const at::Tensor &dy = tensor(where, "dy", a[0], 2), &w = tensor(where, "w", a[1], 2);
     chpl_linear_bwd b = {};
     b.type = type_code(dy.scalar_type());
@@ -283,7 +283,7 @@ PyObject* linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
     b.in_act = (int)PyLong_AsLong(a[10]);
     if (PyErr_Occurred()) return nullptr;
     const bool f32 = PyObject_IsTrue(a[11]), dx_wanted = PyObject_IsTrue(a[13]), dw_wanted = PyObject_IsTrue(a[14]),
-               db_wanted = PyObject_IsTrue(a[15]);
+               db_wanted = PyObject_IsTrue(a[15]), sum_wanted = PyObject_IsTrue(a[16]);
     b.accumulate = PyObject_IsTrue(a[12]);
     b.grad_type = f32 ? CHPL_TYPE_F32 : b.type;
     const at::ScalarType gt = f32 ? at::kFloat : dy.scalar_type();
@@ -305,28 +305,33 @@ PyObject* linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
     }
     if (given(a[8])) b.add = call.matrix("add", a[8], call.type, b.tokens, b.k, &b.ldadd).data_ptr();
     b.lddx = b.lddw = b.k;
-    at::Tensor dx, dw, db;
+    at::Tensor dx, dw, db, sum;
     if (dx_wanted) {
-        dx = given(a[16]) ? call.matrix("dx", a[16], call.type, b.tokens, b.k, &b.lddx) : call.empty(b.tokens, b.k, call.type);
+        dx = given(a[17]) ? call.matrix("dx", a[17], call.type, b.tokens, b.k, &b.lddx) : call.empty(b.tokens, b.k, call.type);
         b.dx = dx.data_ptr();
     }
     if (dw_wanted) {
-        dw = given(a[17]) ? call.matrix("dw", a[17], gt, b.n, b.k, &b.lddw) : call.empty(b.n, b.k, gt);
+        dw = given(a[18]) ? call.matrix("dw", a[18], gt, b.n, b.k, &b.lddw) : call.empty(b.n, b.k, gt);
         b.dw = dw.data_ptr();
     }
     if (db_wanted) {
-        db = given(a[18]) ? call.vector("db", a[18], gt, b.n) : call.empty(b.n, gt);
+        db = given(a[19]) ? call.vector("db", a[19], gt, b.n) : call.empty(b.n, gt);
         b.db = db.data_ptr();
+    }
+    if (sum_wanted) {
+        sum = given(a[20]) ? call.vector("dx_sum", a[20], gt, b.k) : call.empty(b.k, gt);
+        b.dx_sum = sum.data_ptr();
     }
     size_t need = 0;
     check(chpl_linear_backward_worksize(&b, &need), "chpl_linear_backward_worksize");
-    const Workspace work(call, a[19], need);
+    const Workspace work(call, a[21], need);
     check(chpl_linear_backward(call.stream(), &b, work.at, work.bytes), "chpl_linear_backward");
     const auto result = [&](bool wanted, PyObject* mine, at::Tensor& t) {
         return !wanted ? same_object(Py_None) : given(mine) ? same_object(mine) : wrap(std::move(t));
     };
-    PyObject *px = result(dx_wanted, a[16], dx), *pw = result(dw_wanted, a[17], dw), *pb = result(db_wanted, a[18], db);
-    return Py_BuildValue("NNN", px, pw, pb);
+    PyObject *px = result(dx_wanted, a[17], dx), *pw = result(dw_wanted, a[18], dw), *pb = result(db_wanted, a[19], db),
+             *ps = result(sum_wanted, a[20], sum);
+    return Py_BuildValue("NNNN", px, pw, pb, ps);
     CHPL_PY_END
 }
 

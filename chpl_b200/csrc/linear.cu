@@ -276,6 +276,7 @@ struct BackwardPlan {
     Staged g, w, x;
     bool need_xv;   // Xv is not X as it stands
     size_t part;
+    size_t sums;    // of dX's columns
     SumShape sum;   // of db
     size_t bytes;
 };
@@ -292,6 +293,7 @@ static BackwardPlan plan(const chpl_linear_bwd& a)
     p.x = stage(m, products && a.dw && p.need_xv, a.ldx, a.tokens, a.k);
     p.sum = sum_shape(a.tokens, a.n);
     p.part = a.db && a.n > 0 && p.sum.cluster == 1 ? m.take((size_t)p.sum.chunks * a.n * 4) : 0;
+    p.sums = a.dx_sum && a.k > 0 ? m.take((size_t)sum_parts(a.k, a.tokens, a.n) * a.k * 4) : 0;
     p.bytes = m.used;
     return p;
 }
@@ -341,6 +343,8 @@ static int check(const char* who, const chpl_linear_bwd* a, bool pointers)
     }
     if (a->dw && a->n > 0 && a->k > 0) CHPL_TRY(check_operand(who, "dw", a->dw, a->lddw, a->k, ge));
     if (a->db && a->n > 0) CHPL_TRY(check_operand(who, "db", a->db, a->n, a->n, ge));
+    if (a->dx_sum && a->k > 0) CHPL_TRY(check_operand(who, "dx_sum", a->dx_sum, a->k, a->k, ge));
+    if (a->dx_sum && !a->dx && a->tokens > 0 && a->k > 0) { set_error("%s: dx_sum without dx", who); return CHPL_ERR_INVALID; }
     const bool any = a->tokens > 0 && a->n > 0 && (a->dx || a->dw || a->db);
     if (any) {
         CHPL_TRY(check_operand(who, "dy", a->dy, a->lddy, a->n, 2));
@@ -464,8 +468,13 @@ static int backward(cudaStream_t st, const chpl_linear_bwd& a, void* work)
         e.z8 = a.x8;
         e.xv = xv_from_dx ? wk + p.x.at : nullptr;
         e.ldxv = p.x.ld;
+        e.sums = a.dx_sum ? reinterpret_cast<float*>(wk + p.sums) : nullptr;
         CHPL_TRY(gemm(st, a.type, kGradInput, {at(p.w, a.w, work), p.w.ld, false}, g_rows, a.n, e));
     }
+    if (a.dx_sum)
+        CHPL_TRY(launch_kernel(sum_chunks_kernel<T>, (a.k + kSumThreads - 1) / kSumThreads, kSumThreads, 0, 1, st,
+                               reinterpret_cast<const float*>(wk + p.sums), (int)sum_parts(a.k, a.tokens, a.n), (int)a.k,
+                               Sums{a.dx_sum, a.grad_type == CHPL_TYPE_F32, a.accumulate}));
     if (a.dw && (a.tokens > 0 || !a.accumulate)) {
         Epilogue e = {};
         e.m = (int)a.k;

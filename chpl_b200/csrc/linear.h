@@ -27,6 +27,7 @@ struct Epilogue {
     int m, n;        // f < m, t < n
     int act;
     int out_f32;     // out is FP32 (kGradWeight), else of the operands' type
+    float* sums;     // kGradInput: sums of out's columns over parts of its rows, [sum_parts()][m]
     // the product's operands, and how near to 1/2 a quotient has to be taken from them (SETTLE); set by gemm()
     const void *w, *x;
     int64_t ldw, ldx;
@@ -55,6 +56,9 @@ struct Operand {
 
 // D[f][t] = sum_{c < k} A(f, c) B(t, c), handed to the epilogue; type BF16 or F16
 int gemm(cudaStream_t st, int type, Kind kind, const Operand& a, const Operand& b, int64_t k, const Epilogue& e);
+
+// parts that a product's column sums come in
+int64_t sum_parts(int64_t m, int64_t n, int64_t k);
 
 int check_size(const char* who, const char* what, int64_t v);
 int check_operand(const char* who, const char* what, const void* p, int64_t ld, int64_t width, int elt);

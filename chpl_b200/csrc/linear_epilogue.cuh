@@ -541,9 +541,11 @@ __device__ __forceinline__ uint32_t put_ckpt(const Epilogue& e, int f0, int t0, 
 // Every lane of the warp calls it.  bias[2 h + rr]; `stage`: kStageBytes of
 // shared memory of the warp's own (shared-space address, 128-byte aligned).
 // READS: x holds what these rows read, and what the rows `next` do on return.
-template <typename T, Kind KIND, bool READS, bool SETTLE, int NCB>
+// EXTRA: kForward settles codes, kGradInput adds the rows into sums (features
+// f0 + 8 g + l / 4).
+template <typename T, Kind KIND, bool READS, bool EXTRA, int NCB>
 __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float (&v)[8 * NCB], const float (&bias)[4],
-                                       Fetched<NCB>& x, Next next, uint32_t stage)
+                                       Fetched<NCB>& x, Next next, uint32_t stage, float (&sums)[4])
 {
     static_assert(NCB * 8 * 64 <= kStageBytes, "stage");
     const int lane = lane_id();
@@ -593,7 +595,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float 
 #pragma unroll
         for (int i = 0; i < 8 * NCB; ++i) v[i] += bias[(i / (4 * NCB)) * 2 + ((i >> 1) & 1)];
         if (e.z) put16<T, NCB>(e, e.z, e.ldz, e.vec_z, f0, t0, stage, v);
-        if (e.z8.codes) near = put_ckpt<SETTLE, NCB>(e, f0, t0, stage, v);
+        if (e.z8.codes) near = put_ckpt<EXTRA, NCB>(e, f0, t0, stage, v);
         with_act(e.act, [&](auto tag) {
 #pragma unroll
             for (int i = 0; i < 8 * NCB; i += 2) activate<decltype(tag)::value>(v[i], v[i + 1]);
@@ -630,8 +632,14 @@ __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float 
                 v[frag<NCB>(g >> 1, cb, g & 1, 1)] += two.y;
             }
     }
+    if (KIND == kGradInput && EXTRA) {  // rows past the end are zero
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int i = 0; i < 2 * NCB; ++i) sums[g] += v[frag<NCB>(g >> 1, i >> 1, g & 1, i & 1)];
+    }
     put16<T, NCB>(e, e.out, e.ldo, e.vec_out, f0, t0, stage, v);
-    if (SETTLE && __any_sync(0xffffffffu, near != 0)) settle<T, false>(e, f0, t0, near);
+    if (KIND == kForward && EXTRA && __any_sync(0xffffffffu, near != 0)) settle<T, false>(e, f0, t0, near);
 }
 
 // ----------------------------------------------------------------------------
@@ -706,8 +714,9 @@ __device__ __forceinline__ void put_row16(void* out, int64_t ld, bool vec, int f
 }
 
 // Every lane of the warp calls it; t < e.n; bias of the four features.
-template <typename T, Kind KIND, bool READS, bool SETTLE>
-__device__ __forceinline__ void finish_row(const Epilogue& e, int f, int t, float (&v)[4], const float (&bias)[4], const RowFetched& x)
+template <typename T, Kind KIND, bool READS, bool EXTRA>
+__device__ __forceinline__ void finish_row(const Epilogue& e, int f, int t, float (&v)[4], const float (&bias)[4], const RowFetched& x,
+                                           float (&sums)[4])
 {
     uint32_t near = 0;
     if (KIND == kGradWeight && e.out_f32) {
@@ -736,7 +745,7 @@ __device__ __forceinline__ void finish_row(const Epilogue& e, int f, int t, floa
             s = ckpt_scale(s);
             const float inv = ckpt_inv_step(s);
             uint32_t w = ckpt_codes4(v, inv);
-            if (SETTLE) near = near_half(two(v[0], v[1]), both(inv), e.tie) | near_half(two(v[2], v[3]), both(inv), e.tie) << 2;
+            if (EXTRA) near = near_half(two(v[0], v[1]), both(inv), e.tie) | near_half(two(v[2], v[3]), both(inv), e.tie) << 2;
             if (s == kCkptBadScale) w = 0;
             int8_t* c = e.z8.codes + (int64_t)t * e.z8.ldc + f;
             if (e.vec_codes && f + 4 <= e.m) {
@@ -782,13 +791,34 @@ __device__ __forceinline__ void finish_row(const Epilogue& e, int f, int t, floa
         v[2] += b.x;
         v[3] += b.y;
     }
+    if (KIND == kGradInput && EXTRA) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[i] += v[i];
+    }
     put_row16<T>(e.out, e.ldo, e.vec_out, f, t, e.m, v);
-    if (SETTLE && __any_sync(0xffffffffu, near != 0)) settle<T, true>(e, f - 4 * lane_id(), t, near);
+    if (KIND == kForward && EXTRA && __any_sync(0xffffffffu, near != 0)) settle<T, true>(e, f - 4 * lane_id(), t, near);
 }
 
-// whether an epilogue settles codes from the operands, and whether it reads
-// anything else but the accumulators and the bias
-inline bool settles(Kind kind, const Epilogue& e) { return kind == kForward && e.z8.codes && e.act == CHPL_ACT_RELU; }
+// sums of a warp's rows into part `part` of e.sums
+__device__ __forceinline__ void put_sums(const Epilogue& e, int part, int f0, float (&sums)[4])
+{
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+        const int f = f0 + 8 * g + (lane_id() >> 2);
+        if ((lane_id() & 3) == 0 && f < e.m) e.sums[(int64_t)part * e.m + f] = sums[g];
+        sums[g] = 0.0f;
+    }
+}
+
+// whether an epilogue does EXTRA, and whether it reads anything but the
+// accumulators and the bias
+inline bool extra(Kind kind, const Epilogue& e)
+{
+    if (kind == kGradInput) return e.sums != nullptr;
+    return kind == kForward && e.z8.codes && e.act == CHPL_ACT_RELU;
+}
 inline bool reads(Kind kind, const Epilogue& e) { return e.add || (kind == kGradInput && e.act != CHPL_ACT_NONE); }
 
 // the biases of a lane's four features of f0 .. f0 + 31

@@ -181,7 +181,7 @@ template <Kind KIND>
 __host__ __device__ constexpr int stage_bytes(int bn) { return A_BYTES + b_bytes<KIND>(bn); }
 __host__ __device__ constexpr uint32_t tmem_cols(int bn) { return bn <= 32 ? 32u : bn <= 64 ? 64u : bn <= 128 ? 128u : 256u; }
 
-template <typename T, Kind KIND, bool READS, bool SETTLE>
+template <typename T, Kind KIND, bool READS, bool EXTRA>
 __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const int kblocks,
                  const SplitShape sh, const __grid_constant__ Epilogue e)
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     const int f4 = f0 + lane * 4, mine = warp * sh.split + rank, deal = 8 * sh.split;
     Fetched<2> ahead;
     RowFetched ahead_rows[JOIN];
-    float bias[4];
+    float bias[4], sums[4] = {};
     if (!joined) {
         bias_of<T>(e, fq, bias);
         if (READS) fetch<T, KIND, 2>(e, fq, t0 + half * 16, ahead);
@@ -293,8 +293,9 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
         for (int c = half * 16; ok && c < rows; c += 32) {
             float v[16] = {};
             if (kblocks > 0) tmem_ld_frag<2>(tmem + lanes + c, v);
-            finish<T, KIND, READS, SETTLE, 2>(e, fq, t0 + c, v, bias, ahead, {c + 32 < rows ? fq : -1, t0 + c + 32}, stage);
+            finish<T, KIND, READS, EXTRA, 2>(e, fq, t0 + c, v, bias, ahead, {c + 32 < rows ? fq : -1, t0 + c + 32}, stage, sums);
         }
+        if (KIND == kGradInput && EXTRA) put_sums(e, tile / mtiles * 2 + half, fq, sums);
     } else {
         // partial sums as [row][128 features] into the ring's shared memory
         float* part = reinterpret_cast<float*>(smem);
@@ -325,12 +326,18 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
             }
 #pragma unroll
             for (int u = 0; u < JOIN; ++u)
-                if (ok && row + u * deal < rows) finish_row<T, KIND, READS, SETTLE>(e, f4, t0 + row + u * deal, v[u], bias, ahead_rows[u]);
+                if (ok && row + u * deal < rows) finish_row<T, KIND, READS, EXTRA>(e, f4, t0 + row + u * deal, v[u], bias, ahead_rows[u], sums);
             if (READS) {
 #pragma unroll
                 for (int u = 0; u < JOIN; ++u)
                     if (row + (JOIN + u) * deal < rows) fetch_row<KIND>(e, f4, t0 + row + (JOIN + u) * deal, ahead_rows[u]);
             }
+        }
+        if (KIND == kGradInput && EXTRA) {
+            float* o = e.sums + ((int64_t)(tile / mtiles) * deal + mine) * e.m + f4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (f4 + i < e.m) o[i] = sums[i];
         }
         cluster_sync();  // no CTA leaves while another still reads its sums
     }
@@ -394,7 +401,7 @@ __device__ __forceinline__ void load_tile_pair(uint8_t* dst, const CUtensorMap* 
     }
 }
 
-template <typename T, Kind KIND, bool READS, bool SETTLE>
+template <typename T, Kind KIND, bool READS, bool EXTRA>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const int kblocks,
                 const PairShape sh, const __grid_constant__ Epilogue e)
@@ -513,6 +520,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t stage = smem_u32(stages) + (warp - 2) * kStageBytes;
         uint32_t acc = 0;
+        float sums[4] = {};
         int mt, nt;
         pair_tile(sh, unit, mt, nt);
         Fetched<PAIR_NCB> ahead;
@@ -538,8 +546,9 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive_peer(lead_acc_empty + buf * 8);
                 }
-                finish<T, KIND, READS, SETTLE, PAIR_NCB>(e, f, t0 + c, v, bias, ahead, last ? after : Next{f, t0 + c + ROUND}, stage);
+                finish<T, KIND, READS, EXTRA, PAIR_NCB>(e, f, t0 + c, v, bias, ahead, last ? after : Next{f, t0 + c + ROUND}, stage, sums);
             }
+            if (KIND == kGradInput && EXTRA) put_sums(e, t0 / sh.bn * (PAIR_EPI_WARPS / 4) + part, f, sums);
         }
     }
     __syncwarp();
@@ -696,7 +705,7 @@ static int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& ready)
     return CHPL_OK;
 }
 
-template <typename T, Kind KIND, bool READS, bool SETTLE>
+template <typename T, Kind KIND, bool READS, bool EXTRA>
 static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, int kblocks, const Epilogue& e,
                         const SplitShape& s)
 {
@@ -710,12 +719,12 @@ static int launch_split(cudaStream_t st, const Operand& a, const Operand& b, int
         CHPL_TRY(make_tmap(&tmB, b, e.n, k, s.bn));
     }
     static std::atomic<uint64_t> ready{0};
-    CHPL_TRY(allow_smem(split_kernel<T, KIND, READS, SETTLE>, SMEM_LIMIT, ready));
-    return launch_kernel(split_kernel<T, KIND, READS, SETTLE>, ctas, SPLIT_THREADS, 1024 + s.stages * stage_bytes<KIND>(s.bn) + 512, s.split, st,
+    CHPL_TRY(allow_smem(split_kernel<T, KIND, READS, EXTRA>, SMEM_LIMIT, ready));
+    return launch_kernel(split_kernel<T, KIND, READS, EXTRA>, ctas, SPLIT_THREADS, 1024 + s.stages * stage_bytes<KIND>(s.bn) + 512, s.split, st,
                          tmA, tmB, kblocks, s, e);
 }
 
-template <typename T, Kind KIND, bool READS, bool SETTLE>
+template <typename T, Kind KIND, bool READS, bool EXTRA>
 static int launch_pair(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, int kblocks, const Epilogue& e,
                        const PairShape& s)
 {
@@ -723,25 +732,25 @@ static int launch_pair(cudaStream_t st, const Operand& a, const Operand& b, int6
     CHPL_TRY(make_tmap(&tmA, a, e.m, k, BM));
     CHPL_TRY(make_tmap(&tmB, b, e.n, k, s.bn / 2));
     static std::atomic<uint64_t> ready{0};
-    CHPL_TRY(allow_smem(pair_kernel<T, KIND, READS, SETTLE>, PAIR_SMEM, ready));
+    CHPL_TRY(allow_smem(pair_kernel<T, KIND, READS, EXTRA>, PAIR_SMEM, ready));
     const int units = std::min(s.mtiles * s.ntiles, num_sms() / 2);
-    return launch_kernel(pair_kernel<T, KIND, READS, SETTLE>, 2 * units, PAIR_THREADS, PAIR_SMEM, 2, st, tmA, tmB, kblocks, s, e);
+    return launch_kernel(pair_kernel<T, KIND, READS, EXTRA>, 2 * units, PAIR_THREADS, PAIR_SMEM, 2, st, tmA, tmB, kblocks, s, e);
 }
 
-template <typename T, Kind KIND, bool READS, bool SETTLE>
+template <typename T, Kind KIND, bool READS, bool EXTRA>
 static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
 {
     const int kblocks = (int)((k + BK - 1) / BK);
     const Plan p = plan_for<KIND>(e.m, e.n, kblocks);
-    return p.pair ? launch_pair<T, KIND, READS, SETTLE>(st, a, b, k, kblocks, e, p.tiles)
-                  : launch_split<T, KIND, READS, SETTLE>(st, a, b, k, kblocks, e, p.split);
+    return p.pair ? launch_pair<T, KIND, READS, EXTRA>(st, a, b, k, kblocks, e, p.tiles)
+                  : launch_split<T, KIND, READS, EXTRA>(st, a, b, k, kblocks, e, p.split);
 }
 
 template <typename T, Kind KIND>
 static int launch_kind(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
 {
-    if constexpr (KIND == kForward)
-        if (settles(KIND, e))
+    if constexpr (KIND != kGradWeight)
+        if (extra(KIND, e))
             return reads(KIND, e) ? launch<T, KIND, true, true>(st, a, b, k, e) : launch<T, KIND, false, true>(st, a, b, k, e);
     return reads(KIND, e) ? launch<T, KIND, true, false>(st, a, b, k, e) : launch<T, KIND, false, false>(st, a, b, k, e);
 }
@@ -752,6 +761,14 @@ static int launch_type(cudaStream_t st, Kind kind, const Operand& a, const Opera
     if (kind == kForward) return launch_kind<T, kForward>(st, a, b, k, e);
     if (kind == kGradInput) return launch_kind<T, kGradInput>(st, a, b, k, e);
     return launch_kind<T, kGradWeight>(st, a, b, k, e);
+}
+
+int64_t sum_parts(int64_t m, int64_t n, int64_t k)
+{
+    if (m == 0 || n == 0) return 0;
+    const Plan p = plan_for<kGradInput>((int)m, (int)n, (int)((k + BK - 1) / BK));
+    if (p.pair) return (int64_t)p.tiles.ntiles * (PAIR_EPI_WARPS / 4);
+    return (n + p.split.bn - 1) / p.split.bn * (p.split.split > 1 ? 8 * p.split.split : 2);
 }
 
 int gemm(cudaStream_t st, int type, Kind kind, const Operand& a, const Operand& b, int64_t k, const Epilogue& e0)

@@ -38,10 +38,11 @@ def forward(x, w1, b1, w2, b2, *, act: str = "gelu", residual: bool = False, sav
 
 def backward(dy, saved: Saved, w1, w2, *, need_dx: bool = True, need_db: bool = True, grad_dtype=None, stream=None):
     """(dx, dw1, db1, dw2, db2) of the block from dy; with need_db=False db1 and db2 are None."""
-    dz, dw2, db2 = linear.backward(dy, saved.z, w2, in_act=saved.act, need_db=need_db, grad_dtype=grad_dtype, stream=stream)
-    dx, dw1, db1 = linear.backward(dz, saved.x, w1, add=dy if saved.residual else None, need_dx=need_dx, need_db=need_db,
-                                   grad_dtype=grad_dtype, stream=stream)
-    return dx, dw1, db1, dw2, db2
+    dz, dw2, db2, *db1 = linear.backward(dy, saved.z, w2, in_act=saved.act, need_db=need_db, dx_sum=need_db,
+                                         grad_dtype=grad_dtype, stream=stream)
+    dx, dw1, _ = linear.backward(dz, saved.x, w1, add=dy if saved.residual else None, need_dx=need_dx, need_db=False,
+                                 grad_dtype=grad_dtype, stream=stream)
+    return dx, dw1, db1[0] if db1 else None, dw2, db2
 
 
 class _Block(torch.autograd.Function):

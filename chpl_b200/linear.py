@@ -51,18 +51,20 @@ def forward(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, 
 def backward(dy: torch.Tensor, x, w: torch.Tensor, *, act: str = "none", z=None, in_act: str = "none",
              add: torch.Tensor | None = None, need_dx: bool = True, need_dw: bool = True, need_db: bool = True,
              dx: torch.Tensor | None = None, dw: torch.Tensor | None = None, db: torch.Tensor | None = None,
-             grad_dtype: torch.dtype | None = None, accumulate: bool = False, work=None, stream=None):
+             dx_sum=False, grad_dtype: torch.dtype | None = None, accumulate: bool = False, work=None, stream=None):
     """(dX, dW, db) of Y = act(X w^T + b) + R from dY; dR is dY itself.
 
     x is X, or with in_act the pre-activation that X = in_act(x) came from (dX is then x's gradient); z is the
     layer's own pre-activation, wanted where act is not none.  Either may be a tensor of dY's type or a Ckpt8.
     add is added to dX (the gradient that a skip connection brings); dx may be add itself.  need_*=False leaves an output
-    out (None).  dW and db are of grad_dtype: dY's type, or torch.float32; accumulate adds them to the dw and db given.
+    out (None).  dx_sum=True returns a fourth, the sum of dX over the tokens (with in_act, the db of the layer that made
+    x); a tensor gives the memory for it.  dW, db and that sum are of grad_dtype: dY's type, or torch.float32; accumulate
+    adds them to the dw, db and dx_sum given.
     """
     if stream is not None:
         with on(stream, dy.device):
             return backward(dy, x, w, act=act, z=z, in_act=in_act, add=add, need_dx=need_dx, need_dw=need_dw, need_db=need_db,
-                            dx=dx, dw=dw, db=db, grad_dtype=grad_dtype, accumulate=accumulate, work=work)
+                            dx=dx, dw=dw, db=db, dx_sum=dx_sum, grad_dtype=grad_dtype, accumulate=accumulate, work=work)
     where = "linear.backward"
     code, in_code = _choice(where, "activation", ACTS, act), _choice(where, "activation", ACTS, in_act)
     xc = xs = zc = zs = None
@@ -73,7 +75,10 @@ def backward(dy: torch.Tensor, x, w: torch.Tensor, *, act: str = "none", z=None,
     gt = grad_dtype or (dw.dtype if dw is not None else db.dtype if db is not None else dy.dtype)
     if gt is not dy.dtype and gt is not torch.float32:
         raise _lib.ChplError(_lib.CHPL_ERR_INVALID, where, f"gradients in {gt}: {dy.dtype} or float32 is wanted")
-    if accumulate and ((need_dw and dw is None) or (need_db and db is None)):
-        raise _lib.ChplError(_lib.CHPL_ERR_INVALID, where, "accumulate wants dw and db to add to")
-    return _ops.linear_backward(dy, w, x, xc, xs, z, zc, zs, add, code, in_code, gt is torch.float32, accumulate, need_dx, need_dw,
-                                need_db, dx, dw, db, work)
+    total = dx_sum if isinstance(dx_sum, torch.Tensor) else None
+    if accumulate and ((need_dw and dw is None) or (need_db and db is None) or (dx_sum is True)):
+        raise _lib.ChplError(_lib.CHPL_ERR_INVALID, where, "accumulate wants dw, db and dx_sum to add to")
+    want_sum = dx_sum is True or total is not None
+    out = _ops.linear_backward(dy, w, x, xc, xs, z, zc, zs, add, code, in_code, gt is torch.float32, accumulate, need_dx, need_dw,
+                               need_db, want_sum, dx, dw, db, total, work)
+    return out if want_sum else out[:3]

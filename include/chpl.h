@@ -437,12 +437,14 @@ int chpl_linear_forward(void *stream, const chpl_linear_fwd *a, void *work, size
  * in_act == CHPL_ACT_NONE: Xv is X.  Otherwise X is the pre-activation Xz that
  * the layer's input came from, Xv = in_act(Xz) is recomputed, and dX is the
  * gradient of Xz: the activation between two layers costs no pass of its own.
- * dx, dw and db may each be NULL (not computed; X is needed for dW and, with
- * in_act, for dX).  dX, G and Xv are of `type` (G and Xv are rounded to it to
- * feed the tensor cores; db is summed from the unrounded G).  dW (n x k) and
- * db (n) are of grad_type: `type`, or CHPL_TYPE_F32; accumulate != 0 adds
+ * dx_sum is the sum of dX over the tokens, from its FP32 values: where dX is
+ * the gradient of a layer's pre-activation, that layer's db at no pass of its own.
+ * dx, dw, db and dx_sum may each be NULL (not computed; dx_sum wants dx, and X is
+ * needed for dW and, with in_act, for dX).  dX, G and Xv are of `type` (G and Xv are rounded to it to
+ * feed the tensor cores; db is summed from the unrounded G).  dW (n x k), db (n)
+ * and dx_sum (k) are of grad_type: `type`, or CHPL_TYPE_F32; accumulate != 0 adds
  * to what they hold.  dX may be add (same pointer and ld); no other output may
- * overlap an input.  tokens = 0 gives dW = 0, db = 0 (unchanged if accumulating).
+ * overlap an input.  tokens = 0 gives dW, db and dx_sum = 0 (unchanged if accumulating).
  */
 typedef struct chpl_linear_bwd {
     int type, act, in_act, grad_type, accumulate;
@@ -457,6 +459,7 @@ typedef struct chpl_linear_bwd {
     void *dx; int64_t lddx;
     void *dw; int64_t lddw;
     void *db;
+    void *dx_sum;
 } chpl_linear_bwd;
 
 int chpl_linear_backward_worksize(const chpl_linear_bwd *a, size_t *work_bytes);

@@ -103,7 +103,10 @@ def test_backward(cuda, T, k, n, dt, how):
     dx = D * s_in + (add.double() if add is not None else 0.0)
     slack = e_d * s_in.abs().clamp(min=1) + 2.0 ** -17 * D.abs() + 2.0 ** -24 * dx.abs()
     out, sea = out_like(T, k, dt, pad)
-    got = linear.backward(dy, xa, w, act=name, z=za if name != "none" else None, in_act=inner, add=add, dx=out)
+    got = linear.backward(dy, xa, w, act=name, z=za if name != "none" else None, in_act=inner, add=add, dx=out, dx_sum=True)
+    # the sum over the tokens of dX's FP32 values: its slack without the rounding, and an addition's for each token
+    sums = dx.sum(0)
+    ref.check(got[3], sums, dt, (slack + ref.add_error(T) * dx.abs()).sum(0), "dx_sum", 2)
     ref.check(got[0], dx, dt, slack, "dx", 2)
     assert bool((sea[:, k:] == 7).all())
     e_x = xu * X.abs() + (2.0 ** -18 * xv.abs() + tiny if inner != "none" else 0.0)
@@ -120,6 +123,12 @@ def test_backward(cuda, T, k, n, dt, how):
     assert none is None and a is dw32 and b is db32
     ref.check(dw32, dw0.double() + dw, FP, e_w + 2.0 ** -23 * wabs, "dw in FP32", 1e9)
     ref.check(db32, db0.double() + db, FP, e_b + 2.0 ** -23 * G.abs().sum(0), "db in FP32", 1e9)
+    sum0 = torch.randn(k, device="cuda", generator=g)
+    sum32 = sum0.clone()
+    four = linear.backward(dy, xa if inner != "none" else None, w, act=name, z=za if name != "none" else None, in_act=inner, add=add,
+                           need_dw=False, need_db=False, dx_sum=sum32, grad_dtype=FP, accumulate=True)
+    assert torch.equal(four[0], got[0]) and four[3] is sum32
+    ref.check(sum32, sum0.double() + sums, FP, (slack + ref.add_error(T) * dx.abs()).sum(0) + 1e-6, "dx_sum in FP32", 1e9)
     only = linear.backward(dy, xa if inner != "none" else None, w, act=name, z=za if name != "none" else None, in_act=inner,
                            add=add, need_dw=False, need_db=False)
     assert torch.equal(only[0], got[0]) and only[1] is None and only[2] is None
@@ -164,8 +173,11 @@ def test_empty_and_zero_lengths(cuda, dt):
         dx, dw, db = linear.backward(dy, x, w, add=add)
         if n == 0:
             assert torch.equal(dx, add)
+            ref.check(linear.backward(dy, x, w, add=add, dx_sum=True)[3], add.double().sum(0), dt,
+                      1e-6 * torch.ones(k, dtype=torch.float64, device="cuda"), "dx_sum")
         if T == 0:
             assert bool((dw == 0).all()) and bool((db == 0).all())
+            assert bool((linear.backward(dy, x, w, dx_sum=True)[3] == 0).all())
             dw1, db1 = torch.ones(n, k, dtype=dt, device="cuda"), torch.ones(n, dtype=dt, device="cuda")
             linear.backward(dy, x, w, dw=dw1, db=db1, accumulate=True)
             assert bool((dw1 == 1).all()) and bool((db1 == 1).all())
@@ -291,7 +303,8 @@ def test_refusals(cuda):
            lambda: linear.forward(x[:1].expand(4, 16), w),
            lambda: linear.backward(dy, x, w, act="gelu"), lambda: linear.backward(dy, None, w),
            lambda: linear.backward(dy, x[:3], w), lambda: linear.backward(dy, x, w, grad_dtype=HF),
-           lambda: linear.backward(dy, x, w, accumulate=True), lambda: linear.backward(dy, x, w[:, :8]),
+           lambda: linear.backward(dy, x, w, accumulate=True), lambda: linear.backward(dy, x, w, need_dx=False, dx_sum=True),
+           lambda: linear.backward(dy, x, w, dx_sum=torch.zeros(15, dtype=BF, device="cuda")), lambda: linear.backward(dy, x, w[:, :8]),
            lambda: linear.backward(dy, x, w, act="gelu", z=x),
            lambda: linear.backward(dy, ckpt8.Ckpt8(x.to(torch.int8), x.to(torch.uint8), BF), w)]
     for i, f in enumerate(bad):
