@@ -58,6 +58,37 @@ def test_backward_refuses(kw, code):
     assert L.chpl_last_error_string().startswith(b"linear_backward")
 
 
+def test_c_program_calls_the_worksize_functions(tmp_path):
+    """A C program fills the argument structures by name and links against libchpl.so."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "lin.c"
+    src.write_text(r"""
+#include "chpl.h"
+int main(void) {
+    chpl_linear_fwd f = {0};
+    chpl_linear_bwd g = {0};
+    chpl_ckpt8 c = {0, 0, 32, 1};
+    size_t need = 1;
+    f.type = CHPL_TYPE_BF16; f.act = CHPL_ACT_GELU; f.tokens = 8; f.n = 64; f.k = 32; f.ldx = 32; f.ldw = 32; f.ldy = 64;
+    if (chpl_linear_forward_worksize(&f, &need) != CHPL_OK || need != 0) return 2;
+    f.ldx = 33;
+    if (chpl_linear_forward_worksize(&f, &need) != CHPL_OK || need < 8 * 32 * 2) return 3;
+    g.type = CHPL_TYPE_F16; g.grad_type = CHPL_TYPE_F32; g.in_act = CHPL_ACT_SILU; g.tokens = 8; g.n = 64; g.k = 32;
+    if (chpl_linear_backward_worksize(&g, &need) != CHPL_OK || need != 0) return 4;
+    if (chpl_linear_backward(0, &g, 0, 0) != CHPL_OK) return 5;   /* no output wanted */
+    if (chpl_ckpt8_pack(0, CHPL_TYPE_F32, -1, 32, 0, 32, &c) != CHPL_ERR_INVALID) return 6;
+    return 0;
+}
+""")
+    exe, libdir = tmp_path / "lin", os.path.dirname(_lib.LIB_PATH)
+    cc = subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(root, "include"), str(src), "-o", str(exe), "-L",
+                         libdir, "-lchpl", f"-Wl,-rpath,{libdir}"], capture_output=True, text=True)
+    assert cc.returncode == 0, cc.stderr
+    assert subprocess.run([str(exe)], timeout=60).returncode == 0
+
+
 def test_null_arguments():
     L, need = _lib.load(), ctypes.c_size_t()
     assert L.chpl_linear_forward(None, None, None, 0) == INVALID
@@ -107,3 +138,18 @@ def test_checkpoint_rule_on_known_values():
     codes, scales = ref.pack(x)
     assert scales.tolist() == [[127, 133]] and codes[0, :4].tolist() == [64, -32, 127, 0] and codes[0, 32] == 100
     assert ref.unpack(codes, scales)[0, 0] == 1.0 and ref.unpack(codes, scales)[0, 32] == 100.0
+
+
+def test_python_entry_points_refuse_without_a_gpu():
+    """The torch binding loads without a GPU and refuses what is not on one, as ChplError with the C ABI's code."""
+    from chpl_b200 import ckpt8, ffn, linear
+    x, w = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16)
+    bad = [lambda: linear.forward(x, w), lambda: linear.forward(x, w, act="swish"), lambda: linear.forward(x, w, save="16"),
+           lambda: linear.forward(None, w), lambda: linear.forward(x[0], w), lambda: linear.backward(x, x, w),
+           lambda: linear.backward(x, x, w, grad_dtype=torch.float64), lambda: linear.backward(x, x, w, accumulate=True),
+           lambda: ckpt8.pack(x), lambda: ckpt8.unpack(ckpt8.empty(4, 16, torch.bfloat16, "cpu")),
+           lambda: ffn.forward(x, w, None, w, None), lambda: _lib.torch_ops().linear_forward(x, w)]
+    for i, f in enumerate(bad):
+        with pytest.raises(_lib.ChplError) as err:
+            f()
+        assert err.value.code == INVALID, i
