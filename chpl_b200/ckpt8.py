@@ -19,7 +19,8 @@ GROUP = 32
 
 
 class Ckpt8(NamedTuple):
-    """codes: int8 rows x cols; scales: uint8 rows x ceil(cols / 32); dtype: the type of what was coded."""
+    """codes: int8 rows x cols (rows may lie apart: new ones start every 16 bytes); scales: uint8 rows x ceil(cols / 32);
+    dtype: the type of what was coded."""
     codes: torch.Tensor
     scales: torch.Tensor
     dtype: torch.dtype
@@ -34,7 +35,7 @@ class Ckpt8(NamedTuple):
 
 def empty(rows: int, cols: int, dtype: torch.dtype, device) -> Ckpt8:
     """Memory for the checkpoint of a rows x cols matrix."""
-    return Ckpt8(torch.empty(rows, cols, dtype=torch.int8, device=device),
+    return Ckpt8(torch.empty(rows, -(-cols // 16) * 16, dtype=torch.int8, device=device)[:, :cols],
                  torch.empty(rows, -(-cols // GROUP), dtype=torch.uint8, device=device), dtype)
 
 

@@ -134,15 +134,17 @@ struct Call {
     }
 };
 
-// a new checkpoint's tensors
+// a new checkpoint's tensors; rows of codes a multiple of 16 bytes apart, which
+// the kernels read and write in whole pieces
 struct NewCkpt {
     at::Tensor codes, scales;
     chpl_ckpt8 make(const Call& call, int64_t rows, int64_t cols)
     {
-        const int64_t groups = (cols + kGroup - 1) / kGroup;
-        codes = call.empty(rows, cols, at::kChar);
+        const int64_t groups = (cols + kGroup - 1) / kGroup, ld = (cols + 15) / 16 * 16;
+        codes = call.empty(rows, ld, at::kChar);
+        if (ld != cols) codes = codes.as_strided({rows, cols}, {ld, 1});
         scales = call.empty(rows, groups, at::kByte);
-        return {static_cast<int8_t*>(codes.data_ptr()), static_cast<uint8_t*>(scales.data_ptr()), cols, groups};
+        return {static_cast<int8_t*>(codes.data_ptr()), static_cast<uint8_t*>(scales.data_ptr()), ld, groups};
     }
 };
 

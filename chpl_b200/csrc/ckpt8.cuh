@@ -259,18 +259,35 @@ struct RowsOut {
     __device__ __forceinline__ void put(int64_t t, int j, int cols, const float (&v)[8]) const
     {
         T* at = p + t * ld + j;
-        if (vec && j + 8 <= cols) {
-            uint4 w[sizeof(T) / 2];
-            T* e = reinterpret_cast<T*>(w);
+        uint4 w[sizeof(T) / 2];
+        T* e = reinterpret_cast<T*>(w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+        for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+        if (vec && j + 8 <= cols) {
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(at)[i] = w[i];
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (j + i < cols) at[i] = from_f32<T>(v[i]);
+                if (j + i < cols) at[i] = e[i];
         }
+    }
+    // the same for a whole warp, whose lanes hold 256 consecutive elements: rows
+    // that pieces cannot start on are turned about in shared memory (`turn`, 256
+    // elements of the warp's own), so that a store covers 32 elements in a row
+    __device__ __forceinline__ void put_warp(int64_t t, int j, int cols, const float (&v)[8], void* turn) const
+    {
+        if (vec) return put(t, j, cols, v);
+        T* buf = static_cast<T*>(turn);
+        const int lane = lane_id(), j0 = j - lane * 8;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) buf[lane * 8 + i] = from_f32<T>(v[i]);
+        __syncwarp();
+        T* row = p + t * ld + j0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (j0 + i * 32 + lane < cols) row[i * 32 + lane] = buf[i * 32 + lane];
     }
 };
 
@@ -351,7 +368,9 @@ struct RowsJob {
     template <int UNITS>
     __device__ __forceinline__ void run(unsigned block) const
     {
+        __shared__ uint4 turns[kRowsThreads / 32][64];  // 256 elements of up to 4 bytes for each warp
         const int lane = lane_id();
+        uint4* turn = turns[warp_id()];
         const int64_t step = (int64_t)blocks * (kRowsThreads / 32);
         for (int64_t i = (int64_t)block * (kRowsThreads / 32) + warp_id(); i < items; i += step) {
             const int64_t t = items < 0xffffffffll ? (int64_t)((uint32_t)i / segs) : i / segs;
@@ -365,7 +384,7 @@ struct RowsJob {
                 in.value(raw[u], v);
                 f(v);
                 if constexpr (std::is_same<Out, CkptOut>::value) out.put(t, j0 + u * 256, cols, v, in.top(raw[u]));
-                else out.put(t, j0 + u * 256, cols, v);
+                else out.put_warp(t, j0 + u * 256, cols, v, turn);
             }
         }
     }
