@@ -612,7 +612,7 @@ static int num_sms()
 // shorter below 128 rows) and the epilogue, which a pair runs under the next
 // tile; the join of a split comes on top.  The constants are fitted to 3000
 // timings of 150 products (each kind, 1 to 8000 tokens, 64 to 16384 features): the
-// choice is 2.5 % slower than the best candidate in the mean, a third at worst; one
+// choice is 1.2 % slower than the best candidate in the mean, a sixth at worst; one
 // fixed tile was up to 5 times slower.  E.g. 512 x 4096 x 4096: a lone CTA's 128
 // rows 17 us, a pair's 128 rows 19, 256 rows 26, split in two 25.
 //
@@ -657,11 +657,10 @@ static Plan plan_for(int m, int n, int kblocks)
         const double stage = std::max(0.18, 0.0090 / 1024 * stage_bytes<KIND>(bn)), rest = 0.0068 * bn;
         for (int split = 1; split <= 8 && (split == 1 || split <= kblocks); split *= 2) {
             const double ctas = (double)tiles * split;
-            // CTAs on an SM, which share its memory: two where one each does not hold them all
+            // CTAs on an SM, two where one each does not hold them all: the SMs that hold two are the last to end
             const int resident = bn <= 64 && ctas > slots(split, 1, sms) ? 2 : 1;
             const double waves = std::ceil(ctas / slots(split, resident, sms));
-            const double share = waves > 1 ? resident : std::max(1.0, std::min((double)resident, ctas / sms));
-            const double t = 2.2 + waves * (share * ((kblocks + split - 1) / split * stage + rest) + 0.48) +
+            const double t = 2.2 + waves * (resident * ((kblocks + split - 1) / split * stage + rest) + 0.48) +
                              (split > 1 ? 1.3 + 0.0174 * bn : 0.0);
             if (t < least) {
                 least = t;
