@@ -620,15 +620,15 @@ static int num_sms()
 
 // Which kernel, tile and split: the candidate of least estimated time.  The
 // estimate, in us, is a start-up time and, for each wave of tiles that the SMs
-// run, the staging of A and B per k-block (what a stage of 128 features and bn
-// rows weighs, 16 + bn / 8 KB, at the rate each kernel was seen to stage it; for
-// a lone CTA no less than four MMAs of 128 features take, which do not get
-// shorter below 128 rows) and the epilogue, which a pair runs under the next
-// tile; the join of a split comes on top.  The constants are fitted to 3000
-// timings of 150 products (each kind, 1 to 8000 tokens, 64 to 16384 features): the
-// choice is 1.2 % slower than the best candidate in the mean, a sixth at worst; one
-// fixed tile was up to 5 times slower.  E.g. 512 x 4096 x 4096: a lone CTA's 128
-// rows 17 us, a pair's 128 rows 19, 256 rows 26, split in two 25.
+// run, the staging of A and B per k-block (what a stage weighs, 16 + bn / 8 KB for
+// a lone CTA, at the rate each kernel was seen to stage it with the GPU full; an
+// SM by itself reaches 200 GB/s, its ring of 216 KB over the latency of L2) and the
+// epilogue, which a pair runs under the next tile; the join of a split comes on
+// top.  The constants are fitted to 3000 timings of 150 products (each kind, 1 to
+// 8000 tokens, 64 to 16384 features): the choice is 1.5 % slower than the best
+// candidate in the mean, a fifth at worst; one fixed tile was up to 5 times slower.
+// E.g. 512 x 4096 x 4096: a lone CTA's 128 rows 16.7 us, a pair's 128 rows 16.9,
+// 256 rows 25.2, split in two 23.
 //
 // Large products run at the board's power limit, where traffic costs clock: a
 // pair's tiles are walked in groups of features whose A, 32 MB of it, stays in
@@ -668,7 +668,7 @@ static Plan plan_for(int m, int n, int kblocks)
         if (size >= 2 * n && least < 1e300) break;  // half the size holds every row
         const int bn = fit_rows(n, size, Major<KIND>::b ? 16 : 64);
         const int64_t tiles = (int64_t)((m + BM - 1) / BM) * ((n + bn - 1) / bn);
-        const double stage = std::max(0.18, 0.0090 / 1024 * stage_bytes<KIND>(bn)), rest = 0.0068 * bn;
+        const double stage = 0.0090 / 1024 * stage_bytes<KIND>(bn), rest = 0.0068 * bn;
         for (int split = 1; split <= 8 && (split == 1 || split <= kblocks); split *= 2) {
             const double ctas = (double)tiles * split;
             // CTAs on an SM, two where one each does not hold them all: the SMs that hold two are the last to end
