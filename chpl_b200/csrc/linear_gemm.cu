@@ -620,15 +620,15 @@ static int num_sms()
 
 // Which kernel, tile and split: the candidate of least estimated time.  The
 // estimate, in us, is a start-up time and, for each wave of tiles that the SMs
-// run, the staging of A and B per k-block (what a stage weighs, 16 + bn / 8 KB for
-// a lone CTA, at the rate each kernel was seen to stage it with the GPU full; an
-// SM by itself reaches 200 GB/s, its ring of 216 KB over the latency of L2) and the
-// epilogue, which a pair runs under the next tile; the join of a split comes on
-// top.  The constants are fitted to 3000 timings of 150 products (each kind, 1 to
-// 8000 tokens, 64 to 16384 features): the choice is 1.5 % slower than the best
-// candidate in the mean, a fifth at worst; one fixed tile was up to 5 times slower.
-// E.g. 512 x 4096 x 4096: a lone CTA's 128 rows 16.7 us, a pair's 128 rows 16.9,
-// 256 rows 25.2, split in two 23.
+// run, the staging of A and B per k-block and the epilogue, which a pair runs
+// under the next tile; the join of a split comes on top.  A stage costs its
+// bytes, 16 + bn / 8 KB for a lone CTA, at the rate of the SM (its ring of 216 KB
+// over the latency of L2) or at that of L2 where all SMs stage; a pair's k-block
+// also no less than its MMAs.  The constants are fitted to 6000 timings of 210
+// products (each kind, 1 to 8000 tokens, 64 to 16384 features): the choice is
+// 1.1 % slower than the best candidate in the mean, a fifth at worst; one fixed
+// tile was up to 5 times slower.  E.g. 512 x 4096 x 4096: a lone CTA's 128 rows
+// 16.7 us, a pair's 128 rows 16.9, 256 rows 25.2, split in two 23.
 //
 // Large products run at the board's power limit, where traffic costs clock: a
 // pair's tiles are walked in groups of features whose A, 32 MB of it, stays in
@@ -664,18 +664,20 @@ static Plan plan_for(int m, int n, int kblocks)
     Plan best;
     std::memset(&best, 0, sizeof(best));
     double least = 1e300;
-    for (int size = Major<KIND>::b ? 16 : 64; size <= 256; size *= 2) {
+    const int unit = Major<KIND>::b ? 16 : 64;  // rows: B's whole boxes where it is MN-major
+    for (const int size : {16, 32, 48, 64, 96, 128, 192, 256}) {
+        if (size % unit) continue;
         if (size >= 2 * n && least < 1e300) break;  // half the size holds every row
-        const int bn = fit_rows(n, size, Major<KIND>::b ? 16 : 64);
+        const int bn = fit_rows(n, size, unit);
         const int64_t tiles = (int64_t)((m + BM - 1) / BM) * ((n + bn - 1) / bn);
-        const double stage = 0.0090 / 1024 * stage_bytes<KIND>(bn), rest = 0.0068 * bn;
+        const double kbytes = stage_bytes<KIND>(bn) / 1024.0, rest = 0.0078 * bn;
         for (int split = 1; split <= 8 && (split == 1 || split <= kblocks); split *= 2) {
             const double ctas = (double)tiles * split;
             // CTAs on an SM, two where one each does not hold them all: the SMs that hold two are the last to end
-            const int resident = bn <= 64 && ctas > slots(split, 1, sms) ? 2 : 1;
-            const double waves = std::ceil(ctas / slots(split, resident, sms));
-            const double t = 2.2 + waves * (resident * ((kblocks + split - 1) / split * stage + rest) + 0.48) +
-                             (split > 1 ? 1.3 + 0.0174 * bn : 0.0);
+            const int resident = bn <= 64 && ctas > slots(split, 1, sms) ? 2 : 1, places = slots(split, resident, sms);
+            const double stage = kbytes * std::max(0.0075, 0.0085 * std::min(1.0, ctas / places));
+            const double t = 2.26 + std::ceil(ctas / places) * (resident * ((kblocks + split - 1) / split * stage + rest) + 0.7) +
+                             (split > 1 ? 0.95 + 0.0147 * bn : 0.0);
             if (t < least) {
                 least = t;
                 best.pair = false;
@@ -690,8 +692,10 @@ static Plan plan_for(int m, int n, int kblocks)
     for (int size = Major<KIND>::b ? ROUND : 128; size <= 256 && kblocks > 0 && n > size / 2; size += step) {
         const int bn = std::max(ROUND, fit_rows(n, size, step));
         const int64_t mt = (m + 2 * BM - 1) / (2 * BM), nt = (n + bn - 1) / bn;
-        const double products = kblocks * 0.0078 / 1024 * (A_BYTES + 2 * b_bytes<KIND>(bn / 2)), rest = 0.006 * bn;
-        const double t = 2.95 + std::ceil((double)mt * nt / (sms / 2)) * (std::max(products, rest) + 0.47) + std::min(products, rest);
+        const double pairs = sms / 2, kbytes = (A_BYTES + 2 * b_bytes<KIND>(bn / 2)) / 1024.0, rest = 0.0072 * bn;
+        const double stage = kbytes * std::max(0.0063, 0.0076 * std::min(1.0, (double)mt * nt / pairs));
+        const double products = kblocks * std::max(stage, 0.0013 * bn);
+        const double t = 3.1 + std::ceil((double)mt * nt / pairs) * (std::max(products, rest) + 0.42) + std::min(products, rest);
         if (t < least && mt * nt < 0x7fffffff) {
             least = t;
             best.pair = true;
