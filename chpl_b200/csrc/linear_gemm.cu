@@ -52,7 +52,7 @@ constexpr int SMEM_LIMIT = 227 * 1024;
 // one MMA and stage to the next: one thread issues them all, another all copies,
 // and with narrow tiles their instructions bound the kernel.  With descriptors
 // put together for each MMA and addresses multiplied out for each stage,
-// 64 x 4096 x 1024 without a split takes 12.8 us, like this 9.2.
+// 64 x 4096 x 1024 in tiles of 16 rows takes 12.7 us, like this 8.9.
 constexpr uint32_t DESC_HI = 1024u >> 4 | 1u << 14 | 2u << 29;
 
 // (in a cluster an address carries the CTA's rank above the 18 bits of shared memory)
