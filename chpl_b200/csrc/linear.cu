@@ -353,7 +353,8 @@ static int check(const char* who, const chpl_linear_bwd* a, bool pointers)
             else CHPL_TRY(check_operand(who, "z", a->z, a->ldz, a->n, 2));
         }
     }
-    if (a->tokens > 0 && a->k > 0 && (a->dw ? a->n > 0 : a->dx && a->in_act != CHPL_ACT_NONE)) {
+    // dW's operand; with in_act dX's epilogue reads it, of outputs of the layer or of none (n = 0)
+    if (a->tokens > 0 && a->k > 0 && ((a->dw && a->n > 0) || (a->dx && a->in_act != CHPL_ACT_NONE))) {
         if (a->x8.codes) CHPL_TRY(check_ckpt(who, "x8", a->x8, a->k));
         else CHPL_TRY(check_operand(who, "x", a->x, a->ldx, a->k, 2));
     }
