@@ -14,6 +14,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ckpt8, linear
 
@@ -54,6 +55,7 @@ class _Block(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable  # the kernels' gradients carry no graph: a second differentiation raises
     def backward(ctx, dy):
         xc, xs, zc, zs, w1, w2 = ctx.saved_tensors
         dt, act, residual, has1, has2 = ctx.how
@@ -64,5 +66,6 @@ class _Block(torch.autograd.Function):
 
 
 def block(x, w1, b1, w2, b2, act: str = "gelu", residual: bool = False):
-    """The block as a function that torch's autograd differentiates through."""
+    """The block as a function that torch's autograd differentiates through, once: its gradients cannot be differentiated
+    again (create_graph and a second backward pass raise)."""
     return _Block.apply(x, w1, b1, w2, b2, act, residual)
