@@ -14,9 +14,8 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import ckpt8, linear
+from . import _lib, ckpt8, linear
 
 
 class Saved(NamedTuple):
@@ -46,6 +45,19 @@ def backward(dy, saved: Saved, w1, w2, *, need_dx: bool = True, need_db: bool = 
     return dx, dw1, db1[0] if db1 else None, dw2, db2
 
 
+class _Once(torch.autograd.Function):
+    """Gradients that cannot be differentiated again.  torch's once_differentiable raises only where dy carries a graph;
+    the block's gradients depend on its weights and input too."""
+
+    @staticmethod
+    def forward(ctx, *grads):
+        return tuple(v if v is None else v.view_as(v) for v in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise _lib.ChplError(_lib.CHPL_ERR_UNSUPPORTED, "ffn.block", "its gradients cannot be differentiated again")
+
+
 class _Block(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w1, b1, w2, b2, act, residual):
@@ -55,14 +67,17 @@ class _Block(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable  # the kernels' gradients carry no graph: a second differentiation raises
     def backward(ctx, dy):
         xc, xs, zc, zs, w1, w2 = ctx.saved_tensors
         dt, act, residual, has1, has2 = ctx.how
         s = Saved(ckpt8.Ckpt8(xc, xs, dt), ckpt8.Ckpt8(zc, zs, dt), act, residual)
-        dx, dw1, db1, dw2, db2 = backward(dy.contiguous(), s, w1, w2, need_dx=ctx.needs_input_grad[0],
-                                          need_db=has1 or has2)
-        return dx, dw1, db1 if has1 else None, dw2, db2 if has2 else None, None, None
+        with torch.no_grad():
+            dx, dw1, db1, dw2, db2 = backward(dy.contiguous(), s, w1, w2, need_dx=ctx.needs_input_grad[0],
+                                              need_db=has1 or has2)
+        grads = [dx, dw1, db1 if has1 else None, dw2, db2 if has2 else None]
+        if torch.is_grad_enabled():  # create_graph
+            grads = _Once.apply(*(v if v is None else v.requires_grad_() for v in grads))
+        return *grads, None, None
 
 
 def block(x, w1, b1, w2, b2, act: str = "gelu", residual: bool = False):

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from chpl_b200 import ckpt8, ffn
+from chpl_b200 import _lib, ckpt8, ffn
 
 
 class Passes:
@@ -61,9 +61,18 @@ def test_first_gradients(passes):
 
 
 def test_a_second_differentiation_raises(passes):
-    """The block's backward is not differentiable: a gradient penalty raises instead of losing the block's share."""
+    """The block's backward is not differentiable: a gradient penalty raises instead of losing the block's share, also
+    where dy carries no graph of its own."""
+    for weight in (1.0, torch.ones((), dtype=torch.float64, requires_grad=True)):
+        t = leaves()
+        y = ffn.block(*t.values(), "gelu", True)
+        dx, = torch.autograd.grad((y * weight).sum() + (t["x"] ** 2).sum(), t["x"], create_graph=True)
+        with pytest.raises(_lib.ChplError, match="differentiated again"):
+            (y.sum() + dx.square().sum()).backward()
+    # with the graph kept but no second differentiation, the gradients are those without
     t = leaves()
+    dy = torch.randn(5, 3, dtype=torch.float64)
     y = ffn.block(*t.values(), "gelu", True)
-    dx, = torch.autograd.grad(y.sum() + (t["x"] ** 2).sum(), t["x"], create_graph=True)
-    with pytest.raises(RuntimeError, match="differentiate twice"):
-        (y.sum() + dx.square().sum()).backward()
+    want = torch.autograd.grad(y, list(t.values()), dy, retain_graph=True)
+    got = torch.autograd.grad(y, list(t.values()), dy, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
