@@ -76,3 +76,38 @@ def test_a_second_differentiation_raises(passes):
     want = torch.autograd.grad(y, list(t.values()), dy, retain_graph=True)
     got = torch.autograd.grad(y, list(t.values()), dy, create_graph=True)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_frozen_weights_cost_no_product(passes):
+    """Only the gradients that autograd asks for are formed; dW of a frozen weight is left out."""
+    for frozen in (("w1",), ("w2",), ("w1", "w2"), ("x",), ("b1", "b2"), ("x", "w1", "b1", "w2")):
+        t = leaves(frozen)
+        dy = torch.randn(5, 3, dtype=torch.float64)
+        wanted = [v for v in t.values() if v.requires_grad]
+        want = torch.autograd.grad(plain(**t), wanted, dy)
+        got = torch.autograd.grad(ffn.block(*t.values(), "gelu", True), wanted, dy)
+        assert all(torch.allclose(a, b) for a, b in zip(got, want)), frozen
+        _, dx, dw1, dw2, db = passes.calls[-1]
+        assert (dx, dw1, dw2, db) == ("x" not in frozen, "w1" not in frozen, "w2" not in frozen, not {"b1", "b2"} <= set(frozen))
+
+
+def test_nothing_is_held_where_nothing_is_differentiated(passes):
+    t = leaves()
+    with torch.no_grad():
+        y = ffn.block(*t.values(), "gelu", True)
+    assert passes.calls == [("forward", False)] and not y.requires_grad and torch.allclose(y, plain(**t))
+    t = leaves(("x", "w1", "b1", "w2", "b2"))
+    ffn.block(*t.values(), "gelu", True)
+    assert passes.calls[1:] == [("forward", False)]
+
+
+@pytest.mark.parametrize("lead", [(), (5,), (2, 3), (1, 1, 4), (0, 3)])
+def test_leading_dimensions(passes, lead):
+    """X of any leading dimensions, as batch x sequence x features; Y and dX have its shape."""
+    t = leaves(lead=lead)
+    y = ffn.block(*t.values(), "gelu", True)
+    want = plain(**t)
+    assert y.shape == want.shape and torch.allclose(y, want)
+    dy = torch.randn(want.shape, dtype=torch.float64)
+    for a, b in zip(torch.autograd.grad(y, list(t.values()), dy), torch.autograd.grad(want, list(t.values()), dy)):
+        assert a.shape == b.shape and torch.allclose(a, b)
