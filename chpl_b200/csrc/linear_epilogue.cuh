@@ -632,11 +632,13 @@ __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float 
                 v[frag<NCB>(g >> 1, cb, g & 1, 1)] += two.y;
             }
     }
-    if (KIND == kGradInput && EXTRA) {  // rows past the end are zero
+    if (KIND == kGradInput && EXTRA) {  // rows past the end are 0 x W: NaN where W is infinite
+        const bool whole = t0 + 8 * NCB <= e.n;
 #pragma unroll
         for (int g = 0; g < 4; ++g)
 #pragma unroll
-            for (int i = 0; i < 2 * NCB; ++i) sums[g] += v[frag<NCB>(g >> 1, i >> 1, g & 1, i & 1)];
+            for (int i = 0; i < 2 * NCB; ++i)
+                sums[g] += whole || t0 + 8 * (i >> 1) + 2 * (lane & 3) + (i & 1) < e.n ? v[frag<NCB>(g >> 1, i >> 1, g & 1, i & 1)] : 0.0f;
     }
     put16<T, NCB>(e, e.out, e.ldo, e.vec_out, f0, t0, stage, v);
     if (KIND == kForward && EXTRA && __any_sync(0xffffffffu, near != 0)) settle<T, false>(e, f0, t0, near);
