@@ -7,7 +7,7 @@ activation checkpoints (linear, ckpt8, ffn).
 All compute runs in the in-tree CUDA library libchpl.so (C ABI: include/chpl.h);
 importing a submodule that needs it raises if the library is missing.
 """
-from ._lib import ChplError, load  # noqa: F401
+from ._lib import ChplError, check_device, load  # noqa: F401
 
-__all__ = ["ChplError", "load", "oz2", "hpl", "linear", "ckpt8", "ffn"]
+__all__ = ["ChplError", "check_device", "load", "oz2", "hpl", "linear", "ckpt8", "ffn"]
 __version__ = "0.1"

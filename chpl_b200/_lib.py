@@ -82,6 +82,7 @@ SIGNATURES = {
     "chpl_version": (ctypes.c_char_p, []),
     "chpl_device_status": (_int, [ctypes.POINTER(_int)]),
     "chpl_diag_bounded_wait": (_int, [_vp, _int, ctypes.c_uint64]),
+    "chpl_diag_linear_wait": (_int, [_vp, ctypes.c_uint64]),
     "chpl_host_alloc": (_int, [_sz, ctypes.POINTER(_vp)]),
     "chpl_host_free": (_int, [_vp]),
     "chpl_oz2_worksize": (_int, [_sz, _sz, _sz, _uint, _int, _int, ctypes.POINTER(_sz), ctypes.POINTER(_sz),
@@ -168,3 +169,17 @@ def check(code: int, where: str) -> None:
     if code != CHPL_OK:
         msg = load().chpl_last_error_string().decode(errors="replace")
         raise ChplError(code, where, msg)
+
+
+def check_device(device=None) -> None:
+    """Raise ChplError(CHPL_ERR_TIMEOUT) if a wait inside a kernel of this library has run out on the current CUDA device
+    (or on `device`, as torch names it) since the last call: the outputs of the calls since then are undefined.  Waits
+    for the device; a program calls it where it synchronizes anyway, once a step or a request."""
+    if device is not None:
+        import torch
+        with torch.cuda.device(device):
+            return check_device()
+    status = _int()
+    check(load().chpl_device_status(ctypes.byref(status)), "chpl_device_status")
+    if status.value != CHPL_OK:
+        raise ChplError(status.value, "check_device", "a wait inside a kernel ran out; outputs since the last check are undefined")

@@ -807,6 +807,19 @@ int gemm(cudaStream_t st, int type, Kind kind, const Operand& a, const Operand& 
                                   : launch_type<__half>(st, kind, a, b, k, e);
 }
 
+// a wait on a phase that nothing completes, recorded as the kernels above record theirs
+__global__ void diag_linear_wait_kernel(uint64_t limit_ns)
+{
+    __shared__ __align__(8) uint64_t bar;
+    __shared__ int abort_flag;
+    if (threadIdx.x != 0) return;
+    mbar_init(&bar, 1);
+    abort_flag = 0;
+    fence_barrier_init();
+    mbar_wait(&bar, 0, &abort_flag, limit_ns);
+    if (*static_cast<volatile int*>(&abort_flag)) atomicExch(&g_status, CHPL_ERR_TIMEOUT);
+}
+
 int read_clear_status(int* st)
 {
     int v = 0, z = 0;
@@ -818,3 +831,11 @@ int read_clear_status(int* st)
 
 }  // namespace linear
 }  // namespace chpl
+
+extern "C" int chpl_diag_linear_wait(void* stream, uint64_t limit_ns)
+{
+    if (limit_ns == 0 || limit_ns > chpl::kWaitLimitNs) { chpl::set_error("limit_ns must be in (0, 2 s]"); return CHPL_ERR_INVALID; }
+    chpl::linear::diag_linear_wait_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(limit_ns);
+    CHPL_CUDA(cudaGetLastError());
+    return CHPL_OK;
+}

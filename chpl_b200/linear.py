@@ -6,7 +6,8 @@
 X is tokens x k, W is n x k, Y is tokens x n: CUDA tensors of BF16 or F16 whose rows are contiguous; rows may lie
 any distance apart (include/chpl.h has the rules, and which copies unaligned rows cost).  Calls are asynchronous on torch's
 current stream, or on `stream`, on which the inputs have to be ready; outputs that are not given and the workspace are
-allocated from that stream's memory.  Errors raise ChplError.  Everything runs in libchpl.so on the GPU; there is no
+allocated from that stream's memory.  Errors raise ChplError; a wait inside a kernel that runs out is reported by
+chpl_b200.check_device(), which waits for the GPU (these calls do not).  Everything runs in libchpl.so on the GPU; there is no
 host implementation here.
 """
 from __future__ import annotations

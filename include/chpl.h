@@ -269,6 +269,10 @@ int chpl_residual_matrix(void *stream, int64_t N, const double *Ab, size_t ldab,
  * usable.  Synchronizes the stream.
  */
 int chpl_diag_bounded_wait(void *stream, int kind, uint64_t limit_ns);
+/* The same for the products of the linear layers: queues one wait on an mbarrier phase that nothing completes, which
+ * leaves, after limit_ns (<= 2 s), what a product's wait leaves when it runs out: CHPL_ERR_TIMEOUT for
+ * chpl_device_status.  Does not synchronize. */
+int chpl_diag_linear_wait(void *stream, uint64_t limit_ns);
 
 /* ------------------------------------------------------------------------ */
 /* HPL solver                                                                */
