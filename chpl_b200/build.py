@@ -1,4 +1,5 @@
-"""Build libchpl.so (and the chpl_single / chpl_p2 executables) in-tree for sm_100a.
+"""Build libchpl.so, the chpl_single / chpl_p2 executables and, where torch imports, the Python module _torch.so, in-tree
+for sm_100a.
 
     python -m chpl_b200.build [--force] [--verbose]
 
@@ -90,6 +91,26 @@ def _torch_ext_command(src: str) -> list[str]:
             "-lc10", "-lc10_cuda", "-Wl,-rpath," + libs]
 
 
+def _build_torch_ext(force: bool, verbose: bool, hdrs: list[str]) -> None:
+    """_torch.so, where there is a torch: the library and the executables do without.  Built again for another torch or
+    Python, whose C++ interfaces it is compiled against."""
+    try:
+        import torch
+    except (ImportError, OSError) as e:
+        sys.stderr.write(f"chpl_b200: {os.path.basename(TORCH_EXT)} is not built, torch does not import ({e}); linear, ckpt8 and ffn need it\n")
+        return
+    src, stamp = os.path.join(CSRC, "bindings.cpp"), os.path.join(BUILD, "_torch.version")
+    version = f"torch {torch.__version__}, Python {sys.version}"
+    built_for = ""
+    if os.path.exists(stamp):
+        with open(stamp) as f:
+            built_for = f.read()
+    if force or built_for != version or _newer(TORCH_EXT, [src, LIB] + hdrs):
+        _run(_torch_ext_command(src), verbose)
+        with open(stamp, "w") as f:
+            f.write(version)
+
+
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None) -> str:
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(BIN, exist_ok=True)
@@ -108,9 +129,6 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
             list(ex.map(lambda c: _run(c, verbose), jobs))
     if force or _newer(LIB, objs):
         _run([NVCC] + ARCH + ["-shared", "-o", LIB] + objs + LINK, verbose)
-    s = os.path.join(CSRC, "bindings.cpp")
-    if force or _newer(TORCH_EXT, [s, LIB] + hdrs):
-        _run(_torch_ext_command(s), verbose)
     for exe, src in EXES.items():
         s = os.path.join(CSRC, src)
         out = os.path.join(BIN, exe)
@@ -119,6 +137,7 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
                   "-Wl,-rpath,$ORIGIN/..", "-Wl,-rpath," + os.path.join(CUDA, "lib64"),
                   "-I", os.path.join(CUDA, "include"), "-L" + os.path.join(CUDA, "lib64"), "-lcublas", "-lcudart", "-lpthread",
                   "-ldl", "-Wall"], verbose)
+    _build_torch_ext(force, verbose, hdrs)
     return LIB
 
 
