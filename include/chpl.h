@@ -412,9 +412,14 @@ int chpl_ckpt8_unpack(void *stream, int type, int64_t rows, int64_t cols, const 
  * Y = act(Z) + R,  Z = X W^T + b.  X is tokens x k, W n x k, Y, R and Z
  * tokens x n, b n; all of `type` (BF16 or F16).  b and R may be NULL.  Z is
  * kept for the backward pass where z (16 bits) or z8.codes (8 bits, coded from
- * the FP32 value; with ReLU, quotients near +-1/2 from a product formed again, so
- * that the slope at the code is the slope at Z) is given.  Y may be R (same pointer and ld); no other output
- * may overlap an input.  k = 0 gives act(b) + R.
+ * the FP32 value) is given.  With ReLU, whose slope at a checkpoint is 1 for a
+ * positive code and 0 for code 0, quotients near +-1/2 are formed again from X
+ * and W, at most eight for the rows that a warp finishes together, so that
+ * these codes are the exact Z's and do not follow the tiling; more than eight,
+ * and sums whose terms cancel to far less than their size, may still follow it.
+ * A positive Z of at most half a step codes to 0 all the same: its slope is 1
+ * at Z and 0 at the checkpoint.  Y may be R (same pointer and ld); no other
+ * output may overlap an input.  k = 0 gives act(b) + R.
  */
 typedef struct chpl_linear_fwd {
     int type, act;
