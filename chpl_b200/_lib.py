@@ -83,6 +83,7 @@ SIGNATURES = {
     "chpl_device_status": (_int, [ctypes.POINTER(_int)]),
     "chpl_diag_bounded_wait": (_int, [_vp, _int, ctypes.c_uint64]),
     "chpl_diag_linear_wait": (_int, [_vp, ctypes.c_uint64]),
+    "chpl_diag_linear_plan": (_int, [_int, _i64, _i64, _i64, ctypes.POINTER(_i64)]),
     "chpl_host_alloc": (_int, [_sz, ctypes.POINTER(_vp)]),
     "chpl_host_free": (_int, [_vp]),
     "chpl_oz2_worksize": (_int, [_sz, _sz, _sz, _uint, _int, _int, ctypes.POINTER(_sz), ctypes.POINTER(_sz),

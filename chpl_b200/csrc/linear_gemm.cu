@@ -839,3 +839,25 @@ extern "C" int chpl_diag_linear_wait(void* stream, uint64_t limit_ns)
     CHPL_CUDA(cudaGetLastError());
     return CHPL_OK;
 }
+
+extern "C" int chpl_diag_linear_plan(int product, int64_t features, int64_t rows, int64_t contraction, int64_t plan[4])
+{
+    using namespace chpl::linear;
+    const char* who = "diag_linear_plan";
+    CHPL_TRY(check_size(who, "features", features));
+    CHPL_TRY(check_size(who, "rows", rows));
+    CHPL_TRY(check_size(who, "contraction", contraction));
+    if (product < kForward || product > kGradWeight || !features || !rows || !plan) {
+        chpl::set_error("%s: product 0, 1 or 2, features and rows above 0 and a plan are wanted", who);
+        return CHPL_ERR_INVALID;
+    }
+    const int m = (int)features, n = (int)rows, kblocks = (int)((contraction + BK - 1) / BK);
+    const Plan p = product == kForward     ? plan_for<kForward>(m, n, kblocks)
+                   : product == kGradInput ? plan_for<kGradInput>(m, n, kblocks)
+                                           : plan_for<kGradWeight>(m, n, kblocks);
+    plan[0] = p.pair;
+    plan[1] = p.pair ? p.tiles.bn : p.split.bn;
+    plan[2] = p.pair ? 1 : p.split.split;
+    plan[3] = p.pair ? (int64_t)p.tiles.mtiles * p.tiles.ntiles : (int64_t)((m + BM - 1) / BM) * ((n + p.split.bn - 1) / p.split.bn);
+    return CHPL_OK;
+}

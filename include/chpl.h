@@ -273,6 +273,12 @@ int chpl_diag_bounded_wait(void *stream, int kind, uint64_t limit_ns);
  * leaves, after limit_ns (<= 2 s), what a product's wait leaves when it runs out: CHPL_ERR_TIMEOUT for
  * chpl_device_status.  Does not synchronize. */
 int chpl_diag_linear_wait(void *stream, uint64_t limit_ns);
+/* Which kernel, tile and split a product of the linear layers takes on the current device (148 SMs where there is
+ * none), for tests that have to reach each: product 0 is forward (features = n of the layer, contraction = k), 1 dX
+ * (features = k, contraction = n), both of tokens rows, 2 dW (features = k, rows = n, contraction = tokens).
+ * plan[0]: 1 for pairs of CTAs, 0 for clusters; plan[1]: rows of a tile; plan[2]: CTAs that split the contraction (1
+ * with pairs); plan[3]: tiles. */
+int chpl_diag_linear_plan(int product, int64_t features, int64_t rows, int64_t contraction, int64_t plan[4]);
 
 /* ------------------------------------------------------------------------ */
 /* HPL solver                                                                */
