@@ -28,7 +28,7 @@ struct Epilogue {
     int act;
     int out_f32;     // out is FP32 (kGradWeight), else of the operands' type
     float* sums;     // kGradInput: sums of out's columns over parts of its rows, [sum_parts()][m]
-    // the product's operands, and how near to 1/2 a quotient has to be taken from them (SETTLE); set by gemm()
+    // the product's operands, and how near to +-1/2 a quotient is taken from them (SETTLE); set by gemm() and launch()
     const void *w, *x;
     int64_t ldw, ldx;
     int k;

@@ -363,95 +363,169 @@ __device__ __forceinline__ void put16(const Epilogue& e, void* out, int64_t ld, 
     }
 }
 
-// ReLU's slope at a checkpoint hangs on whether a code is 0 or 1.  tcgen05 adds
-// into FP32 accumulators by cutting, so its sums are off by some 2^-24 for each
-// 16 elements of the contraction, several times an FP32 sum's rounding, and a
-// quotient that near to a half would let the tiling decide over a gradient (777
-// x 1024 x 4096: 28 slopes in 40 calls, an FP32 product 7).  With ReLU those few
-// quotients, one in 100000, are formed again from the operands (SETTLE): products
-// exact in FP32, eight added there, the eights in FP64, by the whole warp, about
-// 2 us each; at most kSettled of a warp's rows at a time, so that data made of
-// ties costs no more than a few times the product.  "Near" (e.tie) is ten times
-// the error seen on random operands, which grows with the contraction, and no
-// bound: a sum whose terms cancel to far less than their size can be off by
-// more, and its code then follows the tiling, as codes past kSettled do.  A large
-// forward product with ReLU and codes takes 10 % longer for it.
+// ReLU's slope at a checkpoint hangs on whether a code is 0 or 1, and a quotient
+// near to +-1/2 would let the tiling decide over it: the tensor cores' sums are off
+// by several times what an FP32 sum is.  With ReLU those quotients are formed again
+// from the operands (SETTLE): products exact in FP32, eight added there, the eights
+// in FP64.  Of 4100 x 16384 x 4200's slopes 38 are off without it, 2 with it, and 4
+// of an FP32 product.
+//
+// How near (tie_width): the tensor cores add 16 products at a time into an FP32
+// accumulator by cutting, toward zero, half a unit in the last place or 0.36 2^-23
+// of the partial sum in the mean.  The mean of the partial sums of random terms
+// whose sum ends near zero has 0.29 s as its standard deviation, s = sqrt(sum x^2
+// w^2): over a contraction of 16384, 1.3e-5 s (measured: 0.9 to 1.0e-5 s, in
+// proportion to the contraction of one CTA, so 1/8 of it split in 8).  The largest
+// of a group's 32 is below 1.2 s once in 4000 groups, so s is at most 107 steps
+// else, and 2e-5 steps for each k-block of 64 are five of the measured deviations;
+// short contractions, whose error hangs on single products, have 5e-5 on top.
+// Random operands settle that way; sums whose terms cancel to far less than their
+// group's others can be off by more, and then follow the tiling.
+//
+// A warp lists what is near in the half of its staging memory that NCB = 2 leaves
+// free, kSettled of 8 rows of 32 features at most (so that data made of ties costs
+// no more than a few times the product), and a CTA's warps settle all lists at its
+// end; what no list takes up becomes 0, which is what a quotient at a tie rounds
+// to.  8192 x 4096 x 16384: 855 us, 790 without settling; 4096 x 16384 x 4096: 489,
+// 410; 777 x 1024 x 4096: 17.6, 14.3; one token x 4096 x 16384: 25.6, 23.8.  Settled
+// by a warp where they turn up, they hold up the tiles behind: 957, 488, 17.0 and
+// 25.1 us with a width a quarter of this.
 constexpr int kSettled = 8;
+constexpr int kListed = 126;
+// Outputs of a product, for each warp that lists them, of which random operands leave
+// eight near: 1/2 is met by 0.05 of the quotients for each unit of width (32 normal
+// values under a common step); values beside outliers come nearer to eight times that.
+inline double settle_share(float tie) { return 8.0 / (0.05 * tie); }
 
+struct SettleList {
+    int count, unused;
+    int2 at[kListed];  // t, f
+};
+static_assert(sizeof(SettleList) <= kStageBytes / 2, "list");
+
+inline float tie_width(int kblocks, int split) { return fminf(0.25f, 5e-5f + 2e-5f * (float)((kblocks + split - 1) / split)); }
+
+// the products of c .. c + 7; rows lie on 16-byte boundaries, as TMA wants them
 template <typename T>
-__device__ __noinline__ double exact_z(const T* __restrict__ a, const T* __restrict__ b, int k, double bias)
+__device__ __forceinline__ float eight(const T* __restrict__ a, const T* __restrict__ b, const uint4& u, const uint4& v, int c, int k)
 {
-    constexpr int kAhead = 4;
-    double sum = 0.0;
-    for (int c0 = lane_id() * 8; c0 < k; c0 += kAhead * 256) {
-        uint4 u[kAhead], v[kAhead];  // rows lie on 16-byte boundaries, as TMA wants them
+    float part = 0.0f;
+    if (c + 8 <= k) {
+        const T *p = reinterpret_cast<const T*>(&u), *q = reinterpret_cast<const T*>(&v);
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-            if (c0 + i * 256 + 8 <= k) {
-                u[i] = *reinterpret_cast<const uint4*>(a + c0 + i * 256);
-                v[i] = *reinterpret_cast<const uint4*>(b + c0 + i * 256);
-            }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int c = c0 + i * 256;
-            float part = 0.0f;
-            if (c + 8 <= k) {
-                const T *p = reinterpret_cast<const T*>(&u[i]), *q = reinterpret_cast<const T*>(&v[i]);
-#pragma unroll
-                for (int h = 0; h < 8; ++h) part = fmaf(to_f32(p[h]), to_f32(q[h]), part);
-            } else {
-                for (int h = c; h < k; ++h) part = fmaf(to_f32(a[h]), to_f32(b[h]), part);
-            }
-            sum += (double)part;
-        }
+        for (int h = 0; h < 8; ++h) part = fmaf(to_f32(p[h]), to_f32(q[h]), part);
+    } else {
+        for (int h = c; h < k; ++h) part = fmaf(to_f32(a[h]), to_f32(b[h]), part);
     }
+    return part;
+}
+
+// a warp's memory: its staging and, with SETTLE, its list behind that
+__device__ __forceinline__ SettleList& list_of(uint8_t* areas, int warp)
+{
+    return *reinterpret_cast<SettleList*>(areas + warp * kStageBytes + kStageBytes / 2);
+}
+
+// Settles the lists of WARPS warps, after a barrier of these; sync() is that
+// barrier.  All of them form two quotients at a time, so that one alone takes
+// little; a thread finishes each.
+template <typename T, int WARPS, typename Sync>
+__device__ __forceinline__ void settle_all(const Epilogue& e, uint8_t* areas, int thread, Sync&& sync)
+{
+    constexpr int kBatch = 64, kStride = WARPS * 32 * 8;
+    static_assert(kBatch * sizeof(double) <= kStageBytes / 2 && kBatch <= WARPS * 32, "partial sums");
+    const int lane = lane_id();
+    int w = 0, at = 0, left = 0;
+    for (int v = 0; v < WARPS; ++v) left += list_of(areas, v).count;
+    for (int batch; left > 0; left -= batch) {
+        batch = min(kBatch, left);
+        int2 mine = make_int2(0, 0);
+        for (int i = 0; i < batch; i += 2) {
+            const T *a[2], *b[2];
+            double sum[2] = {0.0, 0.0};
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    return sum + bias;
-}
-
-template <typename T>
-__device__ __forceinline__ double exact_z(const Epilogue& e, int f, int t)
-{
-    return exact_z<T>(static_cast<const T*>(e.w) + (int64_t)f * e.ldw, static_cast<const T*>(e.x) + (int64_t)t * e.ldx, e.k,
-                      e.bias ? (double)to_f32(static_cast<const T*>(e.bias)[f]) : 0.0);
-}
-
-// Settles the codes of a warp's near quotients (bit i of `near`: element i of
-// the lane, in the order of put_ckpt, or four features of one row with ROW) in
-// global memory, after the codes and scales have been written there.
-template <typename T, bool ROW>
-__device__ __noinline__ void settle(const Epilogue& e, int f0, int t0, uint32_t near)
-{
-    __syncwarp();  // orders the warp's stores before these
-    int settled = 0;
-    for (uint32_t lanes = __ballot_sync(0xffffffffu, near != 0); lanes; lanes &= lanes - 1) {
-        const int src = __ffs(lanes) - 1;
-        for (uint32_t bits = __shfl_sync(0xffffffffu, near, src); bits && settled < kSettled; bits &= bits - 1) {
-            const int i = __ffs(bits) - 1, r = i >> 2;
-            const int f = ROW ? f0 + 4 * src + i : f0 + 8 * (i & 3) + (src >> 2);
-            const int t = ROW ? t0 : t0 + 8 * (r >> 1) + 2 * (src & 3) + (r & 1);
-            if (f >= e.m || t >= e.n) continue;
-            ++settled;
-            const double z = exact_z<T>(e, f, t);
+            for (int h = 0; h < 2; ++h) {
+                if (i + h < batch) {
+                    while (at == list_of(areas, w).count) {
+                        ++w;
+                        at = 0;
+                    }
+                    const int2 p = list_of(areas, w).at[at++];
+                    if (thread == i + h) mine = p;
+                    a[h] = static_cast<const T*>(e.w) + (int64_t)p.y * e.ldw;
+                    b[h] = static_cast<const T*>(e.x) + (int64_t)p.x * e.ldx;
+                } else {
+                    a[h] = a[0];
+                    b[h] = b[0];
+                }
+            }
+            for (int c = thread * 8; c < e.k; c += 2 * kStride) {
+                uint4 u[2][2], v[2][2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (c + r * kStride + 8 <= e.k) {
+                            u[h][r] = *reinterpret_cast<const uint4*>(a[h] + c + r * kStride);
+                            v[h][r] = *reinterpret_cast<const uint4*>(b[h] + c + r * kStride);
+                        }
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) sum[h] += (double)eight<T>(a[h], b[h], u[h][r], v[h][r], c + r * kStride, e.k);
+            }
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) {
+                sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], d);
+                sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], d);
+            }
+            if (lane < 2) reinterpret_cast<double*>(areas + (thread >> 5) * kStageBytes)[i + lane] = lane ? sum[1] : sum[0];
+        }
+        sync();
+        if (thread < batch) {
+            const int t = mine.x, f = mine.y;
             const uint32_t s = *const_cast<volatile uint8_t*>(e.z8.scales + (int64_t)t * e.z8.lds + f / kCkptGroup);
-            if (lane_id() == src)
-                e.z8.codes[(int64_t)t * e.z8.ldc + f] = (int8_t)max(-127, min(127, __double2int_rn(z * (double)ckpt_inv_step(s))));
+            double z = e.bias ? (double)to_f32(static_cast<const T*>(e.bias)[f]) : 0.0;
+#pragma unroll
+            for (int v = 0; v < WARPS; ++v) z += reinterpret_cast<const double*>(areas + v * kStageBytes)[thread];
+            e.z8.codes[(int64_t)t * e.z8.ldc + f] = (int8_t)max(-127, min(127, __double2int_rn(z * (double)ckpt_inv_step(s))));
         }
+        sync();
     }
 }
 
-// bit 0, 1: whether a quotient of the two lies within e.tie of +-1/2
-__device__ __forceinline__ uint32_t near_half(Two v, Two inv, float tie)
+// how far the nearer of two quotients is from +-1/2
+__device__ __forceinline__ float from_half(Two v, Two inv)
 {
     const float2 q = apart(v * inv);
-    return (fabsf(fabsf(q.x) - 0.5f) < tie ? 1u : 0u) | (fabsf(fabsf(q.y) - 0.5f) < tie ? 2u : 0u);
+    return fminf(fabsf(fabsf(q.x) - 0.5f), fabsf(fabsf(q.y) - 0.5f));
+}
+__device__ __forceinline__ bool is_near(float v, float inv, float tie) { return fabsf(fabsf(v * inv) - 0.5f) < tie; }
+
+// Puts the lanes' near quotients (bits of `near`; at(i, f, t): where the i-th is)
+// on the warp's list, kSettled of them at most.  Every lane calls it.
+template <typename At>
+__device__ __forceinline__ void list_near(SettleList& list, uint32_t near, At&& at)
+{
+    const int from = list.count, to = min(kListed, from + kSettled);
+    int count = from;
+    for (uint32_t lanes = __ballot_sync(0xffffffffu, near != 0); lanes && count < to; lanes = __ballot_sync(0xffffffffu, near != 0)) {
+        int f = 0, t = 0;
+        if (near) at(__ffs(near) - 1, f, t);
+        const int slot = count + __popc(lanes & ((1u << lane_id()) - 1u));
+        if (near && slot < to) list.at[slot] = make_int2(t, f);
+        near &= near - 1;
+        count = min(to, count + __popc(lanes));
+    }
+    __syncwarp();
+    if (lane_id() == 0) list.count = count;
+    __syncwarp();
 }
 
-// Codes and scales of v, through `at` (shared, 32-byte rows).  Returns, with
-// SETTLE, which of the lane's quotients are near +-1/2: bit 8 cb + 4 p + g.
+// Codes and scales of v, through `at` (shared, 32-byte rows); with SETTLE the
+// quotients near +-1/2 go on the warp's list.
 template <bool SETTLE, int NCB>
-__device__ __forceinline__ uint32_t put_ckpt(const Epilogue& e, int f0, int t0, uint32_t at, const float (&v)[8 * NCB])
+__device__ __forceinline__ void put_ckpt(const Epilogue& e, int f0, int t0, uint32_t at, const float (&v)[8 * NCB], SettleList* list)
 {
     const int lane = lane_id();
     const bool whole = f0 + 32 <= e.m;
@@ -480,21 +554,26 @@ __device__ __forceinline__ uint32_t put_ckpt(const Epilogue& e, int f0, int t0, 
     // two rows at a time
     constexpr int kZero = 0x4B400000;  // 3 * 2^22
     int code[8 * NCB];
-    uint32_t near = 0;
+    float nearest = 1.0f;
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
         const Two inv = two(ckpt_inv_step(scale[2 * cb]), ckpt_inv_step(scale[2 * cb + 1]));
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int i = frag<NCB>(g >> 1, cb, g & 1, 0);
-            if (SETTLE) {
-                const uint32_t n2 = near_half(two(v[i], v[i + 1]), inv, e.tie);
-                near |= (n2 & 1u) << (8 * cb + g) | (n2 >> 1) << (8 * cb + 4 + g);
-            }
+            if (SETTLE) nearest = fminf(nearest, from_half(two(v[i], v[i + 1]), inv));
             const float2 q = apart(fma2(two(v[i], v[i + 1]), inv, both(12582912.0f)));
             code[8 * cb + g] = min(max(__float_as_int(q.x), kZero - 127), kZero + 127);
             code[8 * cb + 4 + g] = min(max(__float_as_int(q.y), kZero - 127), kZero + 127);
         }
+    }
+    const bool some = SETTLE && __any_sync(0xffffffffu, nearest < e.tie);
+    if (SETTLE && nearest < e.tie) {
+#pragma unroll
+        for (int r = 0; r < 2 * NCB; ++r)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (is_near(v[frag<NCB>(g >> 1, r >> 1, g & 1, r & 1)], ckpt_inv_step(scale[r]), e.tie)) code[4 * r + g] = -128;  // no code
     }
     __syncwarp();
 #pragma unroll
@@ -530,6 +609,17 @@ __device__ __forceinline__ uint32_t put_ckpt(const Epilogue& e, int f0, int t0, 
         const int t = 8 * cb + (lane >> 2), f = 8 * (lane & 3);
         uint2 w;
         asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "r"(at + t * 32 + f) : "memory");
+        if (SETTLE && some) {  // 0 for the time being, which is what a quotient at a tie rounds to
+            const uint32_t lo = __vcmpeq4(w.x, 0x80808080u), hi = __vcmpeq4(w.y, 0x80808080u);
+            w.x &= ~lo;
+            w.y &= ~hi;
+            uint32_t near = ((lo & 0x08040201u) * 0x01010101u >> 24 & 0xfu) | (hi & 0x08040201u) * 0x01010101u >> 24 << 4;
+            near &= t0 + t < e.n && f0 + f < e.m ? (1u << min(8, e.m - f0 - f)) - 1u : 0u;
+            list_near(*list, near, [&](int i, int& at_f, int& at_t) {
+                at_f = f0 + f + i;
+                at_t = t0 + t;
+            });
+        }
         if (t0 + t >= e.n) continue;
         if (e.vec_codes && whole) {
             *reinterpret_cast<uint2*>(o + t * e.z8.ldc + f) = w;
@@ -539,22 +629,20 @@ __device__ __forceinline__ uint32_t put_ckpt(const Epilogue& e, int f0, int t0, 
                 if (f0 + f + i < e.m) o[t * e.z8.ldc + f + i] = (int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
         }
     }
-    return near;
 }
 
 // Every lane of the warp calls it.  bias[2 h + rr]; `stage`: kStageBytes of
 // shared memory of the warp's own (shared-space address, 128-byte aligned).
 // READS: x holds what these rows read, and what the rows `next` do on return.
-// EXTRA: kForward settles codes, kGradInput adds the rows into sums (features
-// f0 + 8 g + l / 4).
+// EXTRA: kForward lists the codes to settle, kGradInput adds the rows into sums
+// (features f0 + 8 g + l / 4).
 template <typename T, Kind KIND, bool READS, bool EXTRA, int NCB>
 __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float (&v)[8 * NCB], const float (&bias)[4],
-                                       Fetched<NCB>& x, Next next, uint32_t stage, float (&sums)[4])
+                                       Fetched<NCB>& x, Next next, uint32_t stage, float (&sums)[4], SettleList* list)
 {
-    static_assert(NCB * 8 * 64 <= kStageBytes, "stage");
+    static_assert(NCB * 8 * 64 <= kStageBytes / (KIND == kForward && EXTRA ? 2 : 1), "stage");
     const int lane = lane_id();
     const bool here = f0 < e.m && t0 < e.n;
-    uint32_t near = 0;
     uint32_t add[4 * NCB], zf[4 * NCB];
     if (READS && here) {
         if (KIND == kGradWeight && e.out_f32) {
@@ -599,7 +687,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float 
 #pragma unroll
         for (int i = 0; i < 8 * NCB; ++i) v[i] += bias[(i / (4 * NCB)) * 2 + ((i >> 1) & 1)];
         if (e.z) put16<T, NCB>(e, e.z, e.ldz, e.vec_z, f0, t0, stage, v);
-        if (e.z8.codes) near = put_ckpt<EXTRA, NCB>(e, f0, t0, stage, v);
+        if (e.z8.codes) put_ckpt<EXTRA, NCB>(e, f0, t0, stage, v, list);
         with_act(e.act, [&](auto tag) {
 #pragma unroll
             for (int i = 0; i < 8 * NCB; i += 2) activate<decltype(tag)::value>(v[i], v[i + 1]);
@@ -645,7 +733,6 @@ __device__ __forceinline__ void finish(const Epilogue& e, int f0, int t0, float 
                 sums[g] += whole || t0 + 8 * (i >> 1) + 2 * (lane & 3) + (i & 1) < e.n ? v[frag<NCB>(g >> 1, i >> 1, g & 1, i & 1)] : 0.0f;
     }
     put16<T, NCB>(e, e.out, e.ldo, e.vec_out, f0, t0, stage, v);
-    if (KIND == kForward && EXTRA && __any_sync(0xffffffffu, near != 0)) settle<T, false>(e, f0, t0, near);
 }
 
 // ----------------------------------------------------------------------------
@@ -722,9 +809,8 @@ __device__ __forceinline__ void put_row16(void* out, int64_t ld, bool vec, int f
 // Every lane of the warp calls it; t < e.n; bias of the four features.
 template <typename T, Kind KIND, bool READS, bool EXTRA>
 __device__ __forceinline__ void finish_row(const Epilogue& e, int f, int t, float (&v)[4], const float (&bias)[4], const RowFetched& x,
-                                           float (&sums)[4])
+                                           float (&sums)[4], SettleList* list)
 {
-    uint32_t near = 0;
     if (KIND == kGradWeight && e.out_f32) {
         float* o = static_cast<float*>(e.out) + (int64_t)t * e.ldo + f;
         if (READS && e.add) {
@@ -751,7 +837,22 @@ __device__ __forceinline__ void finish_row(const Epilogue& e, int f, int t, floa
             s = ckpt_scale(s);
             const float inv = ckpt_inv_step(s);
             uint32_t w = ckpt_codes4(v, inv);
-            if (EXTRA) near = near_half(two(v[0], v[1]), both(inv), e.tie) | near_half(two(v[2], v[3]), both(inv), e.tie) << 2;
+            if (EXTRA) {
+                const float nearest = fminf(from_half(two(v[0], v[1]), both(inv)), from_half(two(v[2], v[3]), both(inv)));
+                if (__any_sync(0xffffffffu, nearest < e.tie)) {
+                    uint32_t near = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (f + i < e.m && is_near(v[i], inv, e.tie)) {
+                            near |= 1u << i;
+                            w &= ~(0xffu << (8 * i));
+                        }
+                    list_near(*list, near, [&](int i, int& at_f, int& at_t) {
+                        at_f = f + i;
+                        at_t = t;
+                    });
+                }
+            }
             if (s == kCkptBadScale) w = 0;
             int8_t* c = e.z8.codes + (int64_t)t * e.z8.ldc + f;
             if (e.vec_codes && f + 4 <= e.m) {
@@ -802,7 +903,6 @@ __device__ __forceinline__ void finish_row(const Epilogue& e, int f, int t, floa
         for (int i = 0; i < 4; ++i) sums[i] += v[i];
     }
     put_row16<T>(e.out, e.ldo, e.vec_out, f, t, e.m, v);
-    if (KIND == kForward && EXTRA && __any_sync(0xffffffffu, near != 0)) settle<T, true>(e, f - 4 * lane_id(), t, near);
 }
 
 // sums of a warp's rows into part `part` of e.sums

@@ -298,12 +298,20 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
 
+    // the warps' memory: the ring's first, or behind the partial sums
+    uint8_t* areas = smem + (joined ? sh.bn * JOIN_LD * 4 : 0);
+    SettleList* list = &list_of(areas, warp);
+    if (KIND == kForward && EXTRA) {
+        if (lane == 0) list->count = 0;
+        __syncwarp();
+    }
+
     if (!joined) {
         const uint32_t stage = smem_u32(smem) + warp * kStageBytes;
         for (int c = half * 16; ok && c < rows; c += 32) {
             float v[16] = {};
             if (kblocks > 0) tmem_ld_frag<2>(tmem + lanes + c, v);
-            finish<T, KIND, READS, EXTRA, 2>(e, fq, t0 + c, v, bias, ahead, {c + 32 < rows ? fq : -1, t0 + c + 32}, stage, sums);
+            finish<T, KIND, READS, EXTRA, 2>(e, fq, t0 + c, v, bias, ahead, {c + 32 < rows ? fq : -1, t0 + c + 32}, stage, sums, list);
         }
         if (KIND == kGradInput && EXTRA) put_sums(e, tile / mtiles * 2 + half, fq, sums);
     } else {
@@ -336,7 +344,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
             }
 #pragma unroll
             for (int u = 0; u < JOIN; ++u)
-                if (ok && row + u * deal < rows) finish_row<T, KIND, READS, EXTRA>(e, f4, t0 + row + u * deal, v[u], bias, ahead_rows[u], sums);
+                if (ok && row + u * deal < rows) finish_row<T, KIND, READS, EXTRA>(e, f4, t0 + row + u * deal, v[u], bias, ahead_rows[u], sums, list);
             if (READS) {
 #pragma unroll
                 for (int u = 0; u < JOIN; ++u)
@@ -350,6 +358,10 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
                 if (f4 + i < e.m) o[i] = sums[i];
         }
         cluster_sync();  // no CTA leaves while another still reads its sums
+    }
+    if (KIND == kForward && EXTRA) {
+        // every warp's codes and list are written; after a wait that ran out copies may still land on the lists
+        if (__syncthreads_and(ok)) settle_all<T, SPLIT_THREADS / 32>(e, areas, threadIdx.x, [] { __syncthreads(); });
     }
     __syncwarp();
     tc_fence_before();
@@ -533,6 +545,11 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         const int f_in = (int)rank * BM + quarter * 32;  // the warp's features within a tile
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t stage = smem_u32(stages) + (warp - 2) * kStageBytes;
+        SettleList* list = &list_of(stages, warp - 2);
+        if (KIND == kForward && EXTRA) {
+            if (lane == 0) list->count = 0;
+            __syncwarp();
+        }
         uint32_t acc = 0;
         float sums[4] = {};
         int mt, nt;
@@ -560,9 +577,15 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive_peer(lead_acc_empty + buf * 8);
                 }
-                finish<T, KIND, READS, EXTRA, PAIR_NCB>(e, f, t0 + c, v, bias, ahead, last ? after : Next{f, t0 + c + ROUND}, stage, sums);
+                finish<T, KIND, READS, EXTRA, PAIR_NCB>(e, f, t0 + c, v, bias, ahead, last ? after : Next{f, t0 + c + ROUND}, stage, sums,
+                                                       list);
             }
             if (KIND == kGradInput && EXTRA) put_sums(e, t0 / sh.bn * (PAIR_EPI_WARPS / 4) + part, f, sums);
+        }
+        if (KIND == kForward && EXTRA) {
+            const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(PAIR_EPI_WARPS * 32) : "memory"); };
+            sync();  // every epilogue warp's codes and list are written
+            settle_all<T, PAIR_EPI_WARPS>(e, stages, threadIdx.x - 64, sync);
         }
     }
     __syncwarp();
@@ -755,16 +778,17 @@ static int launch_pair(cudaStream_t st, const Operand& a, const Operand& b, int6
 }
 
 template <typename T, Kind KIND, bool READS, bool EXTRA>
-static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
+static int launch(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, Epilogue& e)
 {
     const int kblocks = (int)((k + BK - 1) / BK);
     const Plan p = plan_for<KIND>(e.m, e.n, kblocks);
+    e.tie = tie_width(kblocks, p.pair ? 1 : p.split.split);
     return p.pair ? launch_pair<T, KIND, READS, EXTRA>(st, a, b, k, kblocks, e, p.tiles)
                   : launch_split<T, KIND, READS, EXTRA>(st, a, b, k, kblocks, e, p.split);
 }
 
 template <typename T, Kind KIND>
-static int launch_kind(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
+static int launch_kind(cudaStream_t st, const Operand& a, const Operand& b, int64_t k, Epilogue& e)
 {
     if constexpr (KIND != kGradWeight)
         if (extra(KIND, e))
@@ -773,7 +797,7 @@ static int launch_kind(cudaStream_t st, const Operand& a, const Operand& b, int6
 }
 
 template <typename T>
-static int launch_type(cudaStream_t st, Kind kind, const Operand& a, const Operand& b, int64_t k, const Epilogue& e)
+static int launch_type(cudaStream_t st, Kind kind, const Operand& a, const Operand& b, int64_t k, Epilogue& e)
 {
     if (kind == kForward) return launch_kind<T, kForward>(st, a, b, k, e);
     if (kind == kGradInput) return launch_kind<T, kGradInput>(st, a, b, k, e);
@@ -788,10 +812,8 @@ int64_t sum_parts(int64_t m, int64_t n, int64_t k)
     return (n + p.split.bn - 1) / p.split.bn * (p.split.split > 1 ? 8 * p.split.split : 2);
 }
 
-int gemm(cudaStream_t st, int type, Kind kind, const Operand& a, const Operand& b, int64_t k, const Epilogue& e0)
+static int gemm_rows(cudaStream_t st, int type, Kind kind, const Operand& a, const Operand& b, int64_t k, Epilogue& e)
 {
-    if (e0.m == 0 || e0.n == 0) return CHPL_OK;
-    Epilogue e = e0;
     const int elt = e.out_f32 ? 4 : 2;
     e.vec_out = aligned(e.out, e.ldo * elt, 16);
     e.vec_add = aligned(e.add, e.ldadd * elt, 16);
@@ -802,9 +824,38 @@ int gemm(cudaStream_t st, int type, Kind kind, const Operand& a, const Operand& 
     e.x = b.p;
     e.ldx = b.ld;
     e.k = (int)k;
-    e.tie = 5e-6f * (float)((k + BK - 1) / BK);  // some 10 times the error seen, of quotients up to 128
     return type == CHPL_TYPE_BF16 ? launch_type<__nv_bfloat16>(st, kind, a, b, k, e)
                                   : launch_type<__half>(st, kind, a, b, k, e);
+}
+
+// p, rows further
+template <typename P>
+static P* skip(P* p, int64_t rows, int64_t ld, int elt)
+{
+    return p ? reinterpret_cast<P*>(reinterpret_cast<uintptr_t>(p) + (size_t)(rows * ld * elt)) : p;
+}
+
+int gemm(cudaStream_t st, int type, Kind kind, const Operand& a, const Operand& b, int64_t k, const Epilogue& e0)
+{
+    if (e0.m == 0 || e0.n == 0) return CHPL_OK;
+    int64_t rows = e0.n;
+    if (kind == kForward && extra(kind, e0)) {  // as many at a time as the warps' lists of codes to settle are made for
+        const double outputs = settle_share(tie_width((int)((k + BK - 1) / BK), 1)) * PAIR_EPI_WARPS * num_sms();
+        rows = std::min(rows, std::max<int64_t>(256, (int64_t)(outputs / e0.m)));
+    }
+    for (int64_t t = 0; t < e0.n; t += rows) {
+        Epilogue e = e0;
+        e.n = (int)std::min(rows, e0.n - t);
+        e.out = skip(e.out, t, e.ldo, e.out_f32 ? 4 : 2);
+        e.add = skip(e.add, t, e.ldadd, e.out_f32 ? 4 : 2);
+        e.z = skip(e.z, t, e.ldz, 2);
+        e.z8.codes = skip(e.z8.codes, t, e.z8.ldc, 1);
+        e.z8.scales = skip(e.z8.scales, t, e.z8.lds, 1);
+        Operand bt = b;
+        if (t > 0) bt.p = skip(b.p, t, b.ld, 2);
+        CHPL_TRY(gemm_rows(st, type, kind, a, bt, k, e));
+    }
+    return CHPL_OK;
 }
 
 // a wait on a phase that nothing completes, recorded as the kernels above record theirs

@@ -420,9 +420,11 @@ int chpl_ckpt8_unpack(void *stream, int type, int64_t rows, int64_t cols, const 
  * kept for the backward pass where z (16 bits) or z8.codes (8 bits, coded from
  * the FP32 value) is given.  With ReLU, whose slope at a checkpoint is 1 for a
  * positive code and 0 for code 0, quotients near +-1/2 are formed again from X
- * and W, at most eight for the rows that a warp finishes together, so that
- * these codes are the exact Z's and do not follow the tiling; more than eight,
- * and sums whose terms cancel to far less than their size, may still follow it.
+ * and W, so that these codes are the exact Z's and do not follow the tiling.
+ * Near is five standard deviations of the products' error on random operands:
+ * sums whose terms cancel to far less than their size may still follow it.  Of
+ * some 200 neighbouring quotients eight at most are formed again; others that
+ * near take code 0, which a quotient at a tie rounds to.
  * A positive Z of at most half a step codes to 0 all the same: its slope is 1
  * at Z and 0 at the checkpoint.  Y may be R (same pointer and ld); no other
  * output may overlap an input.  k = 0 gives act(b) + R.

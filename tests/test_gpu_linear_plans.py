@@ -144,3 +144,84 @@ def test_gradients_in_fp32_and_accumulated(cuda, T, k, n, dt):
     ref.check(held16, want, dt, ref.add_error(T) * Wabs + 2.0 ** -24 * want.abs(), "dw added in 16 bits")
     new16 = linear.backward(dy, x, w, need_dx=False, need_db=False)[1]
     ref.check(new16, W, dt, ref.add_error(T) * Wabs, "dw in 16 bits")
+
+
+PAIRS = [(4100, 16384, 4200), (2300, 16383, 4200), (3000, 8200, 4200)]
+
+
+@pytest.mark.parametrize("T,k,n", PAIRS)
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_relu_codes_of_pairs_settle_at_the_exact_code(cuda, T, k, n, dt):
+    """Products on pairs of CTAs: with ReLU a quotient near 1/2 has the code that the exact Z has, unless it is nearer
+    than what settling can tell: its FP32 sums of eight products round by 2^-24 of a partial sum for each term, of random
+    signs, a standard deviation of at most 1.3 2^-24 sqrt(sum x^2 w^2); six of them are held off.  Without ReLU the longest
+    contraction's own error (some 10^-4 of a step) decides over a few of them.  A warp's 16 rows of 32 features hold
+    0.02 quotients within the settled width, eight or more never."""
+    assert lp.plan(0, n, T, k)[0] == 1
+    g = gen(41)
+    x, w = mk(g, T, k, dt=dt), mk(g, n, k, dt=dt, scale=k ** -0.5)
+    z = x.double() @ w.double().t()
+    size = (x.double().square() @ w.double().square().t()).sqrt()
+    codes, scales = ref.pack(z)
+    step = torch.ldexp(torch.ones_like(scales, dtype=torch.float64), scales.int() - 133).repeat_interleave(32, 1)[:, :n]
+    q = z.abs() / step
+    sure = (q - 0.5).abs() > 8 * 2.0 ** -24 * size / step
+
+    def wrong(c):
+        same = (c.scales == scales).repeat_interleave(32, 1)[:, :n]
+        return int((((c.codes != 0) != (q > 0.5)) & sure & same).sum())
+
+    for res in (None, mk(g, T, n, dt=dt)):
+        assert wrong(linear.forward(x, w, residual=res, act="relu", save="z8")[1]) == 0
+    if k == 16384:
+        assert wrong(linear.forward(x, w, act="silu", save="z8")[1]) > 0
+
+
+@pytest.mark.parametrize("T,k,n", [(1, 512, 1000), (40, 1024, 300), (333, 256, 1100), (2300, 320, 4200)])
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_relu_codes_of_data_made_of_ties(cuda, T, k, n, dt):
+    """Whole numbers whose sums are exact, one feature of each group far above the rest: most quotients are 1/2 or 3/2 to
+    the last bit, more than a warp's list holds, and every code is the rule's."""
+    g = gen(7)
+    x = torch.randint(-1, 2, (T, k), device="cuda", generator=g).to(dt)
+    w = torch.zeros(n, k, dtype=dt, device="cuda")
+    w[torch.arange(n, device="cuda"), torch.randint(0, k - 1, (n,), device="cuda", generator=g)] = 1  # z in -1, 0, 1
+    x[:, -1] = 1
+    w[::32, :] = 0
+    w[::32, -1] = 128                                                                                   # step 2
+    z = x.double() @ w.double().t()
+    codes, scales = ref.pack(z)
+    for b in (None, torch.ones(n, dtype=dt, device="cuda")):
+        want = (codes, scales) if b is None else ref.pack(z + 1)
+        one = linear.forward(x, w, b, act="relu", save="z8")[1]
+        assert torch.equal(one.scales, want[1]) and torch.equal(one.codes, want[0])
+        two = linear.forward(x, w, b, act="relu", save="z8")[1]
+        assert torch.equal(one.codes, two.codes)
+
+
+def test_relu_codes_of_more_rows_than_the_lists_are_made_for(cuda):
+    """A product in several launches: Y, the addend and the codes of all of them, rows apart."""
+    T, k, n, dt = 24000, 16384, 4096, BF
+    g = gen(43)
+    x, w, b = mk(g, T, k, dt=dt), mk(g, n, k, dt=dt, scale=k ** -0.5), mk(g, n, dt=dt)
+    r = mk(g, T, n + 8, dt=dt)[:, :n]
+    held = ckpt8.Ckpt8(torch.empty(T, n + 32, dtype=torch.int8, device="cuda")[:, :n],
+                       torch.empty(T, n // 32 + 1, dtype=torch.uint8, device="cuda")[:, : n // 32], dt)
+    y, z8 = linear.forward(x, w, b, residual=r, act="relu", save="z8", z=held)
+    assert z8 is held
+    wrong = 0
+    for t0 in range(0, T, 4000):
+        rows = slice(t0, t0 + 4000)
+        z = x[rows].double() @ w.double().t() + b.double()
+        want = ref.act(z, "relu") + r[rows].double()
+        size = (x[rows].double().square() @ w.double().square().t()).sqrt()
+        # random operands: cut sums are off by 1e-5 of their size in the standard deviation, ten of them allowed
+        ref.check(y[rows], want, dt, 1e-4 * size + 2.0 ** -24 * want.abs(), "y")
+        codes, scales = ref.pack(z)
+        step = torch.ldexp(torch.ones_like(scales, dtype=torch.float64), scales.int() - 133).repeat_interleave(32, 1)
+        q = z.abs() / step
+        sure = (q - 0.5).abs() > 8 * 2.0 ** -24 * size / step
+        same = (held.scales[rows] == scales).repeat_interleave(32, 1)
+        assert float(same.double().mean()) > 0.999
+        wrong += int((((held.codes[rows] != 0) != (q > 0.5)) & sure & same).sum())
+    assert wrong == 0
