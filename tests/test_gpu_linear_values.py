@@ -24,3 +24,26 @@ def test_an_infinite_weight_in_the_sum_over_tokens(cuda, T, k, n, dt):
         keep = torch.ones(k, dtype=torch.bool, device="cuda")
         keep[k // 3] = keep[k - 1] = False
         assert torch.equal(was[:, keep], now[:, keep])
+
+
+@pytest.mark.parametrize("T,k,n", [(200003, 40, 72), (70001, 264, 33), (8192, 100, 9000)])
+@pytest.mark.parametrize("grad", [torch.float32, torch.bfloat16])
+def test_sums_over_many_tokens(cuda, T, k, n, grad):
+    """db and dX's sum of more chunks than a block has warps: an FP32 sum's error of 2^-24 of a partial sum for each of
+    a run's terms, of random signs, and the result's rounding."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(T)
+    dy = torch.empty(T, n, device="cuda").normal_(generator=g).bfloat16()
+    w = torch.empty(n, k, device="cuda").normal_(0.0, n ** -0.5, generator=g).bfloat16()
+    dx, _, db, total = linear.backward(dy, None, w, need_dw=False, grad_dtype=grad, dx_sum=True)
+    D = torch.cat([part.double() @ w.double() for part in dy.split(20000)])
+    for got, v in ((db, dy.double()), (total, D)):
+        want, size = v.sum(0), v.square().sum(0).sqrt()
+        lim = 2.0 ** -23 * (n / 16 + T ** 0.5) * size.norm() + (2.0 ** -8 if grad is torch.bfloat16 else 2.0 ** -24) * want.norm()
+        assert (got.double() - want).norm() <= lim
+    held = [db.clone(), total.clone()]
+    linear.backward(dy, None, w, need_dw=False, db=held[0], dx_sum=held[1], grad_dtype=grad, accumulate=True)
+    again = linear.backward(dy, None, w, need_dw=False, grad_dtype=grad, dx_sum=True)
+    assert torch.equal(again[2], db) and torch.equal(again[3], total) and torch.equal(again[0], dx)
+    if grad is torch.float32:
+        assert torch.equal(held[0], db + db) and torch.equal(held[1], total + total)
