@@ -647,11 +647,13 @@ static int num_sms()
 // under the next tile; the join of a split comes on top.  A stage costs its
 // bytes, 16 + bn / 8 KB for a lone CTA, at the rate of the SM (its ring of 216 KB
 // over the latency of L2) or at that of L2 where all SMs stage; a pair's k-block
-// also no less than its MMAs.  The constants are fitted to 6000 timings of 210
-// products (each kind, 1 to 8000 tokens, 64 to 16384 features): the choice is
-// 1.1 % slower than the best candidate in the mean, a fifth at worst; one fixed
-// tile was up to 5 times slower.  E.g. 512 x 4096 x 4096: a lone CTA's 128 rows
-// 16.7 us, a pair's 128 rows 16.9, 256 rows 25.2, split in two 23.
+// also no less than its MMAs.  The constants are fitted to 3553 timings of 210
+// products (profiles/linear_plan_timings.json; each kind, 1 to 8000 tokens, 64 to
+// 16384 features): the choice is 2 % slower than the best candidate in the mean,
+// a quarter at worst but for dW of some 30 tokens and fewer, one k-block a tile
+// (1.4 to 1.6 times the best in three of them); one fixed tile was up to 5 times
+// slower.  E.g. 512 x 4096 x 4096: a lone CTA's 128 rows 16.7 us, a pair's 128 rows
+// 16.9, 256 rows 25.2, split in two 23.
 //
 // Large products run at the board's power limit, where traffic costs clock: a
 // pair's tiles are walked in groups of features whose A, 32 MB of it, stays in
