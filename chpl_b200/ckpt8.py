@@ -4,7 +4,8 @@ A checkpoint codes a matrix (rows x cols, BF16, F16 or FP32) in 8 bits per eleme
 consecutive features 32g..32g+31 of a row share a power-of-two step, and each is stored as a signed code of 7 bits
 (the OCP Microscaling MXINT8 elements and scales; include/chpl.h has the exact rule).  ``linear.forward`` writes
 one from its epilogue, ``linear.backward`` reads it in its products; ``pack`` and ``unpack`` convert whole tensors.
-Everything runs in libchpl.so on the GPU; there is no host implementation here.
+Everything runs in libchpl.so on the GPU; there is no host implementation here.  Autograd does not see these functions:
+a gradient does not pass a checkpoint.
 """
 from __future__ import annotations
 

@@ -43,7 +43,9 @@ constexpr float kGeluA = 0.044715f;
 // Phi(z), the normal distribution function, and E = exp(-z^2 / 2) by the way:
 // Abramowitz and Stegun 7.1.26 (Hastings), erfc(x) = t (a1 + ... + a5 t^4) E
 // with t = 1 / (1 + p x), x = |z| / sqrt(2), absolute error below 1.5e-7.  One
-// exponential and one reciprocal, and the slope's density is E again.
+// exponential and one reciprocal, and the slope's density is E again.  In the left
+// tail the error is in E's proportion: relative 5e-5 at -3, 5e-4 at -4 (F16's unit),
+// 1.6e-3 at -5 and 3.6e-3 at -6 (BF16's), where 1 + erf has cancelled in FP32.
 __device__ __forceinline__ Two normal_cdf(Two z, Two& E)
 {
     const float2 s = apart(z);

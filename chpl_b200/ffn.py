@@ -7,7 +7,7 @@ backward ones take act(Z), act'(Z) and X from the codes.  The gradients are thos
     y, saved = ffn.forward(x, w1, b1, w2, b2, act="gelu", residual=True, save=True)
     dx, dw1, db1, dw2, db2 = ffn.backward(dy, saved, w1, w2)
 
-``block`` wraps the two for torch's autograd.
+``block`` wraps the two for torch's autograd; the two themselves it does not see.
 """
 from __future__ import annotations
 

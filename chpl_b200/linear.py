@@ -9,6 +9,9 @@ current stream, or on `stream`, on which the inputs have to be ready; outputs th
 allocated from that stream's memory.  Errors raise ChplError; a wait inside a kernel that runs out is reported by
 chpl_b200.check_device(), which waits for the GPU (these calls do not).  Everything runs in libchpl.so on the GPU; there is no
 host implementation here.
+
+Autograd does not see these functions: what they return carries no graph and no tangents, whatever the inputs require.
+A program calls ``backward`` for the gradients, or uses ``ffn.block``.
 """
 from __future__ import annotations
 
