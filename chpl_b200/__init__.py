@@ -9,5 +9,5 @@ importing a submodule that needs it raises if the library is missing.
 """
 from ._lib import ChplError, check_device, load  # noqa: F401
 
-__all__ = ["ChplError", "check_device", "load", "oz2", "hpl", "linear", "ckpt8", "ffn"]
+__all__ = ["ChplError", "check_device", "load", "oz2", "hpl", "linear", "ckpt8", "ffn", "norm", "mx4"]
 __version__ = "0.1"

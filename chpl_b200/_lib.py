@@ -31,6 +31,10 @@ CHPL_TYPE_BF16 = 0
 CHPL_TYPE_F16 = 1
 CHPL_TYPE_F32 = 2
 
+CHPL_NORM_NONE = 0
+CHPL_NORM_RMS = 1
+CHPL_NORM_LAYER = 2
+
 CHPL_ACT_NONE = 0
 CHPL_ACT_RELU = 1
 CHPL_ACT_GELU = 2
@@ -74,6 +78,33 @@ class LinearBwd(ctypes.Structure):
                 ("tokens", _i64), ("n", _i64), ("k", _i64), ("dy", _vp), ("lddy", _i64), ("w", _vp), ("ldw", _i64),
                 ("x", _vp), ("ldx", _i64), ("x8", Ckpt8), ("z", _vp), ("ldz", _i64), ("z8", Ckpt8), ("add", _vp),
                 ("ldadd", _i64), ("dx", _vp), ("lddx", _i64), ("dw", _vp), ("lddw", _i64), ("db", _vp), ("dx_sum", _vp)]
+
+
+class Norm(ctypes.Structure):
+    _fields_ = [("kind", _int), ("eps", ctypes.c_float), ("weight", _vp), ("bias", _vp)]
+
+
+class NormFwd(ctypes.Structure):
+    _fields_ = [("type", _int), ("join", _int), ("tokens", _i64), ("n", _i64), ("scale", ctypes.c_float), ("residual_scale", ctypes.c_float),
+                ("x", _vp), ("ldx", _i64), ("y", _vp), ("ldy", _i64), ("gate", _vp), ("ldgate", _i64), ("post", Norm), ("pre", Norm),
+                ("r", _vp), ("ldr", _i64), ("h", _vp), ("ldh", _i64), ("post_stats", _vp), ("pre_stats", _vp)]
+
+
+class NormBwd(ctypes.Structure):
+    _fields_ = [("type", _int), ("join", _int), ("grad_type", _int), ("accumulate", _int), ("tokens", _i64), ("n", _i64),
+                ("scale", ctypes.c_float), ("residual_scale", ctypes.c_float), ("dr", _vp), ("lddr", _i64), ("dh", _vp), ("lddh", _i64),
+                ("r", _vp), ("ldr", _i64), ("y", _vp), ("ldy", _i64), ("gate", _vp), ("ldgate", _i64), ("post", Norm), ("pre", Norm),
+                ("post_stats", _vp), ("pre_stats", _vp), ("dx", _vp), ("lddx", _i64), ("dy", _vp), ("lddy", _i64), ("dgate", _vp),
+                ("lddgate", _i64), ("dpost_weight", _vp), ("dpost_bias", _vp), ("dpre_weight", _vp), ("dpre_bias", _vp)]
+
+
+class Mx4(ctypes.Structure):
+    _fields_ = [("codes", _vp), ("scales", _vp), ("ldc", _i64)]
+
+
+class Mx4Fwd(ctypes.Structure):
+    _fields_ = [("type", _int), ("act", _int), ("tokens", _i64), ("n", _i64), ("k", _i64), ("x", _vp), ("ldx", _i64), ("x4", Mx4), ("w4", Mx4),
+                ("bias", _vp), ("residual", _vp), ("ldr", _i64), ("y", _vp), ("ldy", _i64)]
 
 
 # name -> (restype, argtypes); every function declared in include/chpl.h
@@ -123,6 +154,14 @@ SIGNATURES = {
     "chpl_linear_forward": (_int, [_vp, ctypes.POINTER(LinearFwd), _vp, _sz]),
     "chpl_linear_backward_worksize": (_int, [ctypes.POINTER(LinearBwd), ctypes.POINTER(_sz)]),
     "chpl_linear_backward": (_int, [_vp, ctypes.POINTER(LinearBwd), _vp, _sz]),
+    "chpl_norm_forward": (_int, [_vp, ctypes.POINTER(NormFwd)]),
+    "chpl_norm_backward_worksize": (_int, [ctypes.POINTER(NormBwd), ctypes.POINTER(_sz)]),
+    "chpl_norm_backward": (_int, [_vp, ctypes.POINTER(NormBwd), _vp, _sz]),
+    "chpl_mx4_scale_bytes": (_int, [_i64, _i64, ctypes.POINTER(_i64)]),
+    "chpl_mx4_pack": (_int, [_vp, _int, _i64, _i64, _vp, _i64, ctypes.POINTER(Mx4)]),
+    "chpl_mx4_unpack": (_int, [_vp, _int, _i64, _i64, ctypes.POINTER(Mx4), _vp, _i64]),
+    "chpl_mx4_linear_worksize": (_int, [ctypes.POINTER(Mx4Fwd), ctypes.POINTER(_sz)]),
+    "chpl_mx4_linear": (_int, [_vp, ctypes.POINTER(Mx4Fwd), _vp, _sz]),
     "chpl_grid_unique_id": (_int, [_vp, _sz]),
     "chpl_grid_create": (_int, [_int, _int, _int, _vp, _sz, _dbl, ctypes.POINTER(_vp)]),
     "chpl_grid_run": (_int, [_vp, ctypes.POINTER(HplConfig), ctypes.POINTER(HplResult), _vp]),
@@ -156,7 +195,7 @@ def load() -> ctypes.CDLL:
 
 
 def torch_ops():
-    """The module chpl_b200._torch: the linear-layer entry points for torch tensors (raises if it is missing)."""
+    """The module chpl_b200._torch: the entry points of a model's layers for torch tensors (raises if it is missing)."""
     try:
         import torch  # noqa: F401  (its libraries first)
 

@@ -4,6 +4,7 @@
 
 #include "common.cuh"
 #include "linear.h"
+#include "mx4.h"
 #include "oz2.h"
 
 namespace chpl {
@@ -35,11 +36,12 @@ extern "C" const char* chpl_version(void) { return "chpl_b200 0.1 (sm_100a)"; }
 extern "C" int chpl_device_status(int* status)
 {
     CHPL_CUDA(cudaDeviceSynchronize());
-    int a = 0, b = 0, c = 0;
+    int a = 0, b = 0, c = 0, d = 0;
     CHPL_TRY(chpl::oz2::read_clear_status(&a));
     CHPL_TRY(chpl::hpl_read_clear_status(&b));
     CHPL_TRY(chpl::linear::read_clear_status(&c));
-    if (status) *status = a ? a : b ? b : c;
+    CHPL_TRY(chpl::mx4::read_clear_status(&d));
+    if (status) *status = a ? a : b ? b : c ? c : d;
     return CHPL_OK;
 }
 

@@ -11,6 +11,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 #include <utility>
@@ -50,6 +51,19 @@ int launch_kernel(void (*kernel)(P...), int64_t grid, int threads, int smem, int
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
     CHPL_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
+    return CHPL_OK;
+}
+
+// lets a kernel use `bytes` of shared memory, once per device (bit d of ready: done on device d < 64)
+template <typename K>
+int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& ready)
+{
+    int dev = 0;
+    CHPL_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (bit & ready.load(std::memory_order_relaxed)) return CHPL_OK;
+    CHPL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    ready.fetch_or(bit, std::memory_order_relaxed);
     return CHPL_OK;
 }
 
@@ -253,6 +267,7 @@ struct CkptIn {
 
 template <typename T>
 struct RowsOut {
+    static constexpr bool kCodes = false;
     T* p;
     int64_t ld;
     bool vec;
@@ -292,6 +307,7 @@ struct RowsOut {
 };
 
 struct CkptOut {
+    static constexpr bool kCodes = true;
     chpl_ckpt8 c;
     bool vec;
     // v and the largest magnitude's bits among them; every lane of a group's four
@@ -383,7 +399,7 @@ struct RowsJob {
                 float v[8];
                 in.value(raw[u], v);
                 f(v);
-                if constexpr (std::is_same<Out, CkptOut>::value) out.put(t, j0 + u * 256, cols, v, in.top(raw[u]));
+                if constexpr (Out::kCodes) out.put(t, j0 + u * 256, cols, v, in.top(raw[u]));
                 else out.put_warp(t, j0 + u * 256, cols, v, turn);
             }
         }

@@ -54,7 +54,7 @@ static int check_act(const char* who, int act)
     return CHPL_ERR_INVALID;
 }
 
-static int check_work(const char* who, const void* work, size_t have, size_t need)
+int check_work(const char* who, const void* work, size_t have, size_t need)
 {
     if (have < need || (need && !work)) { set_error("%s: workspace of %zu bytes, %zu are needed", who, work ? have : (size_t)0, need); return CHPL_ERR_WORKSPACE; }
     if (need && reinterpret_cast<uintptr_t>(work) % 256) { set_error("%s: workspace is not 256-byte aligned", who); return CHPL_ERR_INVALID; }

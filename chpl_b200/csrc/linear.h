@@ -63,6 +63,12 @@ int64_t sum_parts(int64_t m, int64_t n, int64_t k);
 int check_size(const char* who, const char* what, int64_t v);
 int check_operand(const char* who, const char* what, const void* p, int64_t ld, int64_t width, int elt);
 int check_ckpt(const char* who, const char* what, const chpl_ckpt8& c, int64_t width);
+int check_work(const char* who, const void* work, size_t have, size_t need);
+
+// of the products' plans and tensor maps
+int num_sms();
+int slots(int split, int resident, int sms);
+int fit_rows(int n, int bn, int step);
 
 int read_clear_status(int* st);
 

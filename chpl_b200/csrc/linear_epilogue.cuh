@@ -163,6 +163,44 @@ __device__ __forceinline__ void with_act(int act, F&& f)
 // as soon as the rows before have taken theirs out of the registers.  READS is
 // false where there is nothing to read.
 // ----------------------------------------------------------------------------
+// accumulators of 32 lanes (features) and NCB x 8 columns (rows t), as the
+// fragments that the epilogue takes
+template <int NCB>
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&v)[8 * NCB])
+{
+    uint32_t r[8 * NCB];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < NCB / 2; ++c) {
+            uint32_t* q = r + (h * NCB + 2 * c) * 4;
+            asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                         : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7])
+                         : "r"(taddr + ((uint32_t)(16 * h) << 16) + 16 * c));
+        }
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 8 * NCB; ++j) v[j] = __uint_as_float(r[j]);
+}
+
+// Arrival on the even CTA's barrier that this warp has read its accumulators
+// (ordered by tcgen05.fence, not by the memory model: the default CTA-scope
+// release does not wait for the stores under way, as a cluster-scope one would).
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
 constexpr int kStageBytes = 2048;  // a warp's shared memory: 32 rows of 64 bytes
 
 template <int NCB>

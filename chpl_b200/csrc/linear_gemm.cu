@@ -96,44 +96,6 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint32_t a_lo, uin
         : "memory");
 }
 
-// accumulators of 32 lanes (features) and NCB x 8 columns (rows t), as the
-// fragments that the epilogue takes
-template <int NCB>
-__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&v)[8 * NCB])
-{
-    uint32_t r[8 * NCB];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int c = 0; c < NCB / 2; ++c) {
-            uint32_t* q = r + (h * NCB + 2 * c) * 4;
-            asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                         : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7])
-                         : "r"(taddr + ((uint32_t)(16 * h) << 16) + 16 * c));
-        }
-    tmem_wait_ld();
-#pragma unroll
-    for (int j = 0; j < 8 * NCB; ++j) v[j] = __uint_as_float(r[j]);
-}
-
-// Arrival on the even CTA's barrier that this warp has read its accumulators
-// (ordered by tcgen05.fence, not by the memory model: the default CTA-scope
-// release does not wait for the stores under way, as a cluster-scope one would).
-__device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr)
-{
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr)
-{
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
-}
-
 template <Kind KIND>
 struct Major {
     static constexpr bool a = KIND == kForward;      // A is K-major
@@ -601,7 +563,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 // ----------------------------------------------------------------------------
 // host side
 // ----------------------------------------------------------------------------
-static PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
 {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
@@ -633,7 +595,7 @@ static int make_tmap(CUtensorMap* tm, const Operand& o, int64_t extent, int64_t 
     return CHPL_OK;
 }
 
-static int num_sms()
+int num_sms()
 {
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 148;
@@ -669,14 +631,14 @@ struct Plan {
 // CTAs of the split kernel that run at once, one or two to an SM: clusters of 4
 // and 8 do not fill the GPU's processor clusters (132 and 120 of 148 SMs, 284 and
 // 264 of 296 places, by the occupancy calculation for this GPU)
-static int slots(int split, int resident, int sms)
+int slots(int split, int resident, int sms)
 {
     const int lost = split <= 2 ? 0 : resident == 1 ? (split == 4 ? 16 : 28) : (split == 4 ? 12 : 32);
     return std::max(1, sms * resident - lost);
 }
 
 // the narrowest multiple of `step` rows that makes no more tiles of n rows than bn does
-static int fit_rows(int n, int bn, int step)
+int fit_rows(int n, int bn, int step)
 {
     const int tiles = (n + bn - 1) / bn;
     return (int)round_up((size_t)((n + tiles - 1) / tiles), (size_t)step);
@@ -732,19 +694,6 @@ static Plan plan_for(int m, int n, int kblocks)
         }
     }
     return best;
-}
-
-// lets a kernel use `bytes` of shared memory, once per device (bit d of ready: done on device d < 64)
-template <typename K>
-static int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& ready)
-{
-    int dev = 0;
-    CHPL_CUDA(cudaGetDevice(&dev));
-    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
-    if (bit & ready.load(std::memory_order_relaxed)) return CHPL_OK;
-    CHPL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    ready.fetch_or(bit, std::memory_order_relaxed);
-    return CHPL_OK;
 }
 
 template <typename T, Kind KIND, bool READS, bool EXTRA>

@@ -483,6 +483,134 @@ int chpl_linear_backward_worksize(const chpl_linear_bwd *a, size_t *work_bytes);
 int chpl_linear_backward(void *stream, const chpl_linear_bwd *a, void *work, size_t work_bytes);
 
 /* ------------------------------------------------------------------------ */
+/* norms around a model's blocks                                             */
+/* ------------------------------------------------------------------------ */
+
+/* The rules of the linear layers hold here too: row-major, rows ld* apart,
+ * any alignment, nothing allocated or synchronized, results that do not vary
+ * from run to run.  n is at most 16384. */
+#define CHPL_NORM_NONE 0
+#define CHPL_NORM_RMS 1   /* m = 0 */
+#define CHPL_NORM_LAYER 2 /* m = the mean */
+
+/* N(v) = (v - m) s weight + bias, s = 1 / sqrt(mean((v - m)^2) + eps), over the
+ * n features of a row; weight and bias of the operands' type, bias may be NULL.
+ * Statistics are FP32: squares that add up beyond FP32 (values above some 1e18)
+ * give s = 0. */
+typedef struct chpl_norm {
+    int kind;
+    float eps;
+    const void *weight, *bias;
+} chpl_norm;
+
+/*
+ * join == 0: h = Npre(x).
+ * join != 0: r = residual_scale x + scale gate * Npost(y), a block's output y on
+ * the residual stream x, and h = Npre(r) from r before it is rounded; post.kind
+ * NONE: y as it is; gate NULL: none, ldgate 0: a vector of n, else tokens x n;
+ * pre.kind NONE: no h.  post_stats and pre_stats (tokens x 2 floats: m and s of
+ * each row, for the backward pass) may be NULL.  r may be x or y, and h may be x
+ * (without a join) or y (same pointer and ld); no other output may overlap an
+ * input.
+ */
+typedef struct chpl_norm_fwd {
+    int type, join;
+    int64_t tokens, n;
+    float scale, residual_scale;
+    const void *x; int64_t ldx;
+    const void *y; int64_t ldy;
+    const void *gate; int64_t ldgate;
+    chpl_norm post, pre;
+    void *r; int64_t ldr;
+    void *h; int64_t ldh;
+    float *post_stats, *pre_stats;
+} chpl_norm_fwd;
+int chpl_norm_forward(void *stream, const chpl_norm_fwd *a);
+
+/*
+ * Gradients of that.  D = dr + (gradient of Npre at r from dh); without a join
+ * dx = D (r is x, dr what else flows into x; NULL: nothing).  With one,
+ * dx = residual_scale D, and with Do = scale D: dgate = Do * Npost(y), dy the
+ * gradient of Npost at y from Do * gate.  The norms' weights' and biases'
+ * gradients and a vector gate's are sums over the tokens, of grad_type (`type`,
+ * or CHPL_TYPE_F32), added to what they hold where accumulate != 0; a matrix
+ * gate's gradient is of `type`.  Every output may be NULL (not computed).  dx
+ * may be dr or dh (same pointer and ld); no other output may overlap an input.
+ * tokens = 0 gives sums of 0 (unchanged if accumulating).
+ */
+typedef struct chpl_norm_bwd {
+    int type, join, grad_type, accumulate;
+    int64_t tokens, n;
+    float scale, residual_scale;
+    const void *dr; int64_t lddr;
+    const void *dh; int64_t lddh;
+    const void *r; int64_t ldr;
+    const void *y; int64_t ldy;
+    const void *gate; int64_t ldgate;
+    chpl_norm post, pre;
+    const float *post_stats, *pre_stats;
+    void *dx; int64_t lddx;
+    void *dy; int64_t lddy;
+    void *dgate; int64_t lddgate;
+    void *dpost_weight, *dpost_bias, *dpre_weight, *dpre_bias;
+} chpl_norm_bwd;
+int chpl_norm_backward_worksize(const chpl_norm_bwd *a, size_t *work_bytes);
+/* `work`: 256-byte aligned device memory of work_bytes bytes, or NULL when none is needed */
+int chpl_norm_backward(void *stream, const chpl_norm_bwd *a, void *work, size_t work_bytes);
+
+/* ------------------------------------------------------------------------ */
+/* microscaled 4-bit floating point, and linear layers in it                 */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * A row-major matrix (rows x cols) in 4 bits (OCP Microscaling MXFP4: E2M1
+ * elements, E8M0 scales, blocks of 32 along a row).  Features 32g..32g+31 of a
+ * row share the step 2^(s - 127); s = max(e, 7) - 2 for the exponent field e
+ * (FP32, biased by 127) of the group's largest magnitude; a code is x / step
+ * rounded to the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} (codes 0..7, sign in
+ * bit 3), ties to the even code, larger magnitudes to 6.  A group that holds an
+ * infinity or a NaN has s = 255 and codes 0, and reads back as NaN.
+ *   codes  feature j of row t in byte t * ldc + j / 2, the low half for even j;
+ *          rows are whole groups (codes past the last feature are 0), start on 16
+ *          bytes, ldc >= 16 ceil(cols / 32).
+ *   scales as the tensor cores take them: chpl_mx4_scale_bytes() bytes, 16-byte
+ *          aligned; row t's group g is byte ((t / 128) * B + g / 4) * 512 +
+ *          (t % 32) * 16 + (t % 128) / 32 * 4 + g % 4 with B = 2 ceil(cols / 256);
+ *          those of the groups past the last one up to B * 4 are not 255 (pack
+ *          writes 5), those of rows past the last one are not used.
+ */
+typedef struct chpl_mx4 {
+    uint8_t *codes;
+    uint8_t *scales;
+    int64_t ldc;
+} chpl_mx4;
+
+int chpl_mx4_scale_bytes(int64_t rows, int64_t cols, int64_t *bytes);
+/* x (rows x cols, `type` BF16, F16 or F32) -> codes and scales */
+int chpl_mx4_pack(void *stream, int type, int64_t rows, int64_t cols, const void *x, int64_t ldx, const chpl_mx4 *c);
+/* codes and scales -> x of any of the three types (rounded once, to nearest) */
+int chpl_mx4_unpack(void *stream, int type, int64_t rows, int64_t cols, const chpl_mx4 *c, void *x, int64_t ldx);
+
+/*
+ * Y = act(Q(X) W^T + b) + R on the 4-bit tensor cores: W (n x k) in this format,
+ * X (tokens x k) of `type`, coded by the call into `work`, or coded already (x4).
+ * b, R and Y as in chpl_linear_forward; sums are FP32.  Y may be R (same pointer
+ * and ld); no other output may overlap an input.  k = 0 gives act(b) + R.
+ */
+typedef struct chpl_mx4_fwd {
+    int type, act;
+    int64_t tokens, n, k;
+    const void *x; int64_t ldx;
+    chpl_mx4 x4;
+    chpl_mx4 w4;
+    const void *bias;
+    const void *residual; int64_t ldr;
+    void *y; int64_t ldy;
+} chpl_mx4_fwd;
+int chpl_mx4_linear_worksize(const chpl_mx4_fwd *a, size_t *work_bytes);
+int chpl_mx4_linear(void *stream, const chpl_mx4_fwd *a, void *work, size_t work_bytes);
+
+/* ------------------------------------------------------------------------ */
 /* P x Q process grid (one process per GPU, NCCL over NVLink)                */
 /* ------------------------------------------------------------------------ */
 
