@@ -8,12 +8,11 @@
 // that the statistics' passes over it cost no memory traffic and the gradients'
 // sums over the tokens stay in registers, eight a thread, from a CTA's first row
 // to its last.  The rows to come are on their way into shared memory meanwhile,
-// every thread copying what it will itself read: no barrier waits for a copy.
+// every warp copying what it will itself read: no barrier waits for a copy.
 #include <algorithm>
 #include <cmath>
 
-#include "ckpt8.cuh"
-#include "linear.h"
+#include "linear_epilogue.cuh"
 
 namespace chpl {
 namespace norm {
@@ -24,7 +23,7 @@ using linear::check_size;
 constexpr int kMaxThreads = 1024;
 constexpr int kMaxWidth = 2 * 8 * kMaxThreads;  // a cluster of two
 constexpr int kMaxStages = 4;
-constexpr int kStageBudget = 192 * 1024;        // of shared memory on an SM, for the rows under way
+constexpr int kStageBudget = 208 * 1024;        // of shared memory on an SM, for the rows under way
 
 // ----------------------------------------------------------------------------
 // shape of a launch
@@ -35,92 +34,255 @@ struct Shape {
     int cluster;  // CTAs that share a row
     int stages;   // rows of each group that are under way or in use
     int units;    // clusters launched
+    int piece;    // shared memory of a warp's 256 features
+    int turn;     // offset of the memory that unaligned rows are turned about in
     int smem;
 };
 
 // A row's warps are a power of two up to four (several rows to a CTA of eight
 // warps), then as many as it needs.  64 registers a thread leave 1024 threads on
 // an SM.
-static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors)
+static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors, bool inputs_aligned, bool outputs_aligned)
 {
     Shape s;
     s.cluster = n > 8 * kMaxThreads ? 2 : 1;
     const int need = (int)((n + 256 * s.cluster - 1) / (256 * s.cluster));
     s.warps = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : need;
     s.groups = s.warps <= 4 ? 8 / s.warps : 1;
-    const int threads = 32 * s.warps * s.groups, resident = kMaxThreads / threads;
-    const int fixed = vectors * threads * 16;
-    s.stages = std::max(1, std::min(kMaxStages, (kStageBudget / resident - fixed) / std::max(1, tensors * threads * 16)));
-    s.smem = fixed + s.stages * tensors * threads * 16;
+    s.piece = inputs_aligned ? 512 : 544;
+    const int warps = s.warps * s.groups, resident = kMaxThreads / (32 * warps);
+    const int fixed = vectors * warps * 512 + (outputs_aligned ? 0 : warps * 512), row = std::max(1, tensors) * warps * s.piece;
+    s.stages = std::max(1, std::min(kMaxStages, (kStageBudget / resident - fixed) / row));
+    s.turn = vectors * warps * 512 + s.stages * row;
+    s.smem = fixed + s.stages * row;
     const int64_t want = (tokens + s.groups - 1) / s.groups;
     s.units = (int)std::min<int64_t>(want, 148 / s.cluster * resident);
     return s;
 }
 
 // ----------------------------------------------------------------------------
-// eight features of a thread
+// eight consecutive features of a thread
 // ----------------------------------------------------------------------------
-// Features first + (i / E) * stride + i % E of i = 0 .. 7: pieces of E that the
-// rows' alignment allows to access at once.
-template <int E>
-struct Columns {
-    int first, stride, n;
-    __device__ __forceinline__ int at(int i) const { return first + i / E * stride + i % E; }
-    __device__ __forceinline__ bool has(int i) const { return at(i) < n; }
+struct Eight {
+    Two v[4];
 };
 
-// the thread's features of a row (or a vector) into 16 bytes of shared memory,
-// zero past the end; asynchronous where pieces are of 4 bytes at least
-template <int E>
-__device__ __forceinline__ void fetch(uint32_t slot, const void* row, const Columns<E>& c)
+__device__ __forceinline__ Eight zeros()
 {
-    const unsigned short* p = static_cast<const unsigned short*>(row);
-    if constexpr (E == 1) {
-        uint32_t w[4] = {0, 0, 0, 0};
+    Eight r;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c.has(i)) w[i >> 1] |= (uint32_t)p[c.at(i)] << (16 * (i & 1));
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-    } else {
+    for (int i = 0; i < 4; ++i) r.v[i] = both(0.0f);
+    return r;
+}
+__device__ __forceinline__ Eight operator*(const Eight& a, const Eight& b)
+{
+    Eight r;
 #pragma unroll
-        for (int i = 0; i < 8; i += E) {
-            const int left = min(max(c.n - c.at(i), 0), E);
-            const void* src = p + (left ? c.at(i) : 0);
-            if (E == 8) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot), "l"(src), "r"(2 * left) : "memory");
-            else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(slot + 2 * i), "l"(src), "r"(2 * left) : "memory");
-        }
+    for (int i = 0; i < 4; ++i) r.v[i] = a.v[i] * b.v[i];
+    return r;
+}
+__device__ __forceinline__ Eight operator+(const Eight& a, const Eight& b)
+{
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = a.v[i] + b.v[i];
+    return r;
+}
+__device__ __forceinline__ Eight operator*(const Eight& a, float b)
+{
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = a.v[i] * both(b);
+    return r;
+}
+__device__ __forceinline__ Eight operator+(const Eight& a, float b)
+{
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = a.v[i] + both(b);
+    return r;
+}
+__device__ __forceinline__ Eight fma8(const Eight& a, const Eight& b, const Eight& c)
+{
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = fma2(a.v[i], b.v[i], c.v[i]);
+    return r;
+}
+__device__ __forceinline__ Eight fma8(const Eight& a, float b, const Eight& c)
+{
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = fma2(a.v[i], both(b), c.v[i]);
+    return r;
+}
+__device__ __forceinline__ float total_of(const Eight& a)
+{
+    const float2 t = apart((a.v[0] + a.v[1]) + (a.v[2] + a.v[3]));
+    return t.x + t.y;
+}
+__device__ __forceinline__ float dot(const Eight& a, const Eight& b)
+{
+    const float2 t = apart(fma2(a.v[0], b.v[0], a.v[1] * b.v[1]) + fma2(a.v[2], b.v[2], a.v[3] * b.v[3]));
+    return t.x + t.y;
+}
+// zero from the `have`-th on
+__device__ __forceinline__ void clear_tail(Eight& a, int have)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = apart(a.v[i]);
+        a.v[i] = two(2 * i < have ? t.x : 0.0f, 2 * i + 1 < have ? t.y : 0.0f);
     }
 }
 
 template <typename T>
-__device__ __forceinline__ void values(uint32_t slot, float (&v)[8])
+__device__ __forceinline__ Eight expand(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    const uint32_t w[4] = {a, b, c, d};
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = linear::unpack2<T>(w[i]);
+        r.v[i] = two(f.x, f.y);
+    }
+    return r;
+}
+
+// features of a vector that lie in 16 bytes of shared memory of the thread's own
+template <typename T>
+__device__ __forceinline__ Eight vector_at(uint32_t slot)
 {
     uint4 w;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(slot) : "memory");
-    const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+    return expand<T>(w.x, w.y, w.z, w.w);
 }
 
-template <typename T, int E>
-__device__ __forceinline__ void put(void* row, const Columns<E>& c, const float (&v)[8])
+// the thread's `have` features of a vector into its 16 bytes, zero past the end
+__device__ __forceinline__ void fetch_vector(uint32_t slot, const void* v, int first, int have)
 {
-    T* p = static_cast<T*>(row);
-    uint4 w;
-    T* e = reinterpret_cast<T*>(&w);
+    const unsigned short* p = static_cast<const unsigned short*>(v) + first;
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (have == 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+        w[0] = q.x;
+        w[1] = q.y;
+        w[2] = q.z;
+        w[3] = q.w;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
-    const uint32_t* u = &w.x;
+        for (int i = 0; i < 8; ++i)
+            if (i < have) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
+struct Rows {
+    const void* p;
+    int64_t ld;
+    __device__ __forceinline__ const unsigned short* row(int64_t t) const { return static_cast<const unsigned short*>(p) + t * ld; }
+};
+struct RowsTo {
+    void* p;
+    int64_t ld;
+    bool aligned;  // 16-byte stores fit
+    __device__ __forceinline__ unsigned short* row(int64_t t) const { return static_cast<unsigned short*>(p) + t * ld; }
+};
+
+__device__ __forceinline__ void copy16(uint32_t slot, const void* src, int bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot), "l"(src), "r"(bytes) : "memory");
+}
+
+// The warp's 256 features of a row into its piece of shared memory, asynchronously.
+// Aligned rows: the lane's own 16 bytes.  Others: the 16-byte chunks of memory
+// that the features lie in, 33 of them, whose other bytes are the row's (or the
+// rows' beside it); the chunks that reach out of the tensor, in its first and last
+// row, are read by the element.
+template <bool ALIGNED>
+__device__ __forceinline__ void fetch_row(uint32_t piece, const Rows& x, int64_t t, int64_t tokens, int first, int have, int n)
+{
+    const int lane = lane_id();
+    const unsigned short* row = x.row(t);
+    if (ALIGNED) {
+        copy16(piece + lane * 16, row + (have > 0 ? first : 0), 2 * have);
+        return;
+    }
+    const unsigned short* p = row + (first - lane * 8);
+    const char* from = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
+    const char* begin = static_cast<const char*>(x.p);
+    const char* row_end = reinterpret_cast<const char*>(row + n);
+    const char* end = reinterpret_cast<const char*>(x.row(tokens - 1) + n);
+    for (int c = lane; c < 33; c += 32) {
+        const char* at = from + c * 16;
+        if (at >= row_end) break;
+        if (at >= begin && at + 16 <= end) {
+            copy16(piece + c * 16, at, 16);
+        } else {
 #pragma unroll
-    for (int i = 0; i < 8; i += E) {
-        if (E == 8 && c.has(7)) *reinterpret_cast<uint4*>(p + c.at(0)) = w;
-        else if (E == 2 && c.has(i + 1)) *reinterpret_cast<uint32_t*>(p + c.at(i)) = u[i / 2];
-        else {
-#pragma unroll
-            for (int k = 0; k < E; ++k)
-                if (c.has(i + k)) p[c.at(i + k)] = e[i + k];
+            for (int i = 0; i < 8; ++i)
+                if (at + 2 * i >= begin && at + 2 * i < end)
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(piece + c * 16 + 2 * i), "h"(*reinterpret_cast<const unsigned short*>(at + 2 * i)) : "memory");
         }
     }
+}
+
+// the thread's features of that row; zero past its end
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ Eight row_at(uint32_t piece, const Rows& x, int64_t t, int first, int have)
+{
+    const int lane = lane_id();
+    if (ALIGNED) return vector_at<T>(piece + lane * 16);
+    const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(x.row(t) + (first - lane * 8)) & 15u;  // bytes before the first feature
+    const uint32_t at = piece + lane * 16 + (skew & ~3u);
+    uint32_t w[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i)
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i]) : "r"(at + 4 * i) : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (skew & 2u));
+    if (have < 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] &= (2 * i < have ? 0xffffu : 0u) | (2 * i + 1 < have ? 0xffff0000u : 0u);
+    }
+    return expand<T>(w[0], w[1], w[2], w[3]);
+}
+
+// the thread's features into a row; rows that 16-byte stores do not fit go by way
+// of `turn`, 512 bytes of the warp's own, so that a store covers 32 features in a row
+template <typename T>
+__device__ __forceinline__ void put(const RowsTo& out, int64_t t, int first, int have, int n, const Eight& v, uint32_t turn)
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = apart(v.v[i]);
+        w[i] = linear::pack2<T>(f.x, f.y);
+    }
+    unsigned short* p = out.row(t) + first;
+    if (out.aligned) {
+        if (have == 8) {
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < have) p[i] = (unsigned short)(w[i >> 1] >> (16 * (i & 1)));
+        }
+        return;
+    }
+    const int lane = lane_id();
+    __syncwarp();
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(turn + lane * 16), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    __syncwarp();
+    p -= lane * 8;
+    const int left = n - (first - lane * 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i * 32 + lane < left) {
+            unsigned short e;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(e) : "r"(turn + 2 * (i * 32 + lane)) : "memory");
+            p[i * 32 + lane] = e;
+        }
 }
 
 // ----------------------------------------------------------------------------
@@ -128,64 +290,75 @@ __device__ __forceinline__ void put(void* row, const Columns<E>& c, const float 
 // ----------------------------------------------------------------------------
 constexpr int kMaxWarps = kMaxThreads / 32;
 
-// Two sums over the row of a group (of a cluster); every thread of it calls
-// with the same count of calls before.  Warps' sums go through shared memory, two
-// sets of them in turn: who writes a set again has passed the barrier that all
-// readers of its last use reached afterwards.
+__device__ __forceinline__ float warp_sum(float a)
+{
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) a += __shfl_xor_sync(0xffffffffu, a, d);
+    return a;
+}
+
+// Sums over the row of a group (of a cluster); every thread of it calls with the
+// same calls before.  Warps' sums go through shared memory, two sets of them in
+// turn: who writes a set again has passed the barrier that all readers of its last
+// use reached afterwards.
 struct RowSums {
     float2 (*sets)[kMaxWarps];  // [2][warps of the CTA]
     int warps, group, cluster, turn;
 
-    __device__ __forceinline__ float2 operator()(float a, float b)
+    __device__ __forceinline__ void meet() const
     {
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) {
-            a += __shfl_xor_sync(0xffffffffu, a, d);
-            b += __shfl_xor_sync(0xffffffffu, b, d);
+        if (cluster > 1) cluster_sync();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * warps) : "memory");
+    }
+    __device__ __forceinline__ float2 of_lane(const float2* set) const
+    {
+        const int lane = lane_id();
+        float2 sum = make_float2(0.0f, 0.0f);
+        if (lane >= warps) return sum;
+        if (cluster == 1) return set[group * warps + lane];
+        for (int r = 0; r < cluster; ++r) {
+            float2 v;
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(map_to_rank(smem_u32(set + lane), (uint32_t)r)) : "memory");
+            sum.x += v.x;
+            sum.y += v.y;
         }
+        return sum;
+    }
+    __device__ __forceinline__ float one(float a)
+    {
+        a = warp_sum(a);
+        if (warps == 1) return a;
+        float2* set = sets[turn];
+        turn ^= 1;
+        if (lane_id() == 0) set[warp_id()] = make_float2(a, 0.0f);
+        meet();
+        return warp_sum(of_lane(set).x);
+    }
+    __device__ __forceinline__ float2 both_of(float a, float b)
+    {
+        a = warp_sum(a);
+        b = warp_sum(b);
         if (warps == 1) return make_float2(a, b);
         float2* set = sets[turn];
         turn ^= 1;
-        const int lane = lane_id();
-        if (lane == 0) set[warp_id()] = make_float2(a, b);
-        if (cluster > 1) cluster_sync();
-        else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * warps) : "memory");
-        a = b = 0.0f;
-        if (lane < warps) {
-            if (cluster == 1) {
-                const float2 v = set[group * warps + lane];
-                a = v.x;
-                b = v.y;
-            } else {
-                for (int r = 0; r < cluster; ++r) {
-                    float2 v;
-                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(map_to_rank(smem_u32(set + lane), (uint32_t)r)) : "memory");
-                    a += v.x;
-                    b += v.y;
-                }
-            }
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) {
-            a += __shfl_xor_sync(0xffffffffu, a, d);
-            b += __shfl_xor_sync(0xffffffffu, b, d);
-        }
-        return make_float2(a, b);
+        if (lane_id() == 0) set[warp_id()] = make_float2(a, b);
+        meet();
+        const float2 v = of_lane(set);
+        return make_float2(warp_sum(v.x), warp_sum(v.y));
     }
 };
 
 // where a thread stands
-template <int E>
 struct Place {
-    Columns<E> cols;
+    int first, have, n;  // of its features
     int group;
     int64_t row, step;
-    __device__ __forceinline__ Place(const Shape& s, int n)
+    __device__ __forceinline__ Place(const Shape& s, int width) : n(width)
     {
         const int warp = warp_id(), rank = s.cluster > 1 ? (int)cluster_ctarank() : 0;
         group = warp / s.warps;
-        const int thread = (warp - group * s.warps) * 32 + lane_id(), width = 32 * s.warps;
-        cols = {rank * width * 8 + thread * E, width * E, n};
+        first = ((rank * s.warps + warp - group * s.warps) * 32 + lane_id()) * 8;
+        have = min(8, max(0, n - first));
         const int64_t unit = blockIdx.x / s.cluster;
         row = unit * s.groups + group;
         step = (int64_t)s.units * s.groups;
@@ -195,16 +368,17 @@ struct Place {
 // The rows under way: copies of the rows to come, a group of cp.async each,
 // `stages` of them (an empty group where there is no such row).
 struct Ring {
-    uint32_t base;  // of the thread
+    uint32_t base;  // of the warp
     uint32_t tensor, stage_bytes;
     int stages, at;
-    __device__ __forceinline__ Ring(uint32_t smem, int tensors, int nstages)
-        : base(smem + threadIdx.x * 16), tensor(blockDim.x * 16), stage_bytes((uint32_t)tensors * blockDim.x * 16), stages(nstages), at(0)
+    __device__ __forceinline__ Ring(uint32_t mem, int tensors, const Shape& s)
+        : base(mem + warp_id() * s.piece), tensor((blockDim.x >> 5) * s.piece), stage_bytes((uint32_t)tensors * tensor), stages(s.stages), at(0)
     {
     }
-    __device__ __forceinline__ uint32_t slot(int stage, int t) const { return base + stage * stage_bytes + t * tensor; }
+    __device__ __forceinline__ uint32_t piece(int stage, int t) const { return base + stage * stage_bytes + t * tensor; }
     __device__ __forceinline__ static void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-    // the oldest of `stages` groups has arrived
+    // the oldest of `stages` groups has arrived, the whole warp's where a lane reads others' copies
+    template <bool ALIGNED>
     __device__ __forceinline__ void wait() const
     {
         switch (stages) {
@@ -213,6 +387,7 @@ struct Ring {
             case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
             default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
         }
+        if (!ALIGNED) __syncwarp();
     }
     __device__ __forceinline__ void next() { at = at + 1 == stages ? 0 : at + 1; }
 };
@@ -220,17 +395,6 @@ struct Ring {
 // ----------------------------------------------------------------------------
 // forward
 // ----------------------------------------------------------------------------
-struct Rows {
-    const void* p;
-    int64_t ld;
-    __device__ __forceinline__ const void* row(int64_t t) const { return static_cast<const unsigned short*>(p) + t * ld; }
-};
-struct RowsTo {
-    void* p;
-    int64_t ld;
-    __device__ __forceinline__ void* row(int64_t t) const { return static_cast<unsigned short*>(p) + t * ld; }
-};
-
 struct Forward {
     int64_t tokens;
     int n;
@@ -243,99 +407,82 @@ struct Forward {
 };
 
 // slots of the vectors
-enum { kPostW, kPostB, kPreW, kPreB, kGate, kVectors };
+enum { kPreW, kPreB, kPostW, kPostB, kGate, kVectors };
 
-// the norm of v, in place; (mean, 1 / deviation) to *stats.  Mean first, then the
-// squares of what is left: the one pass of squares loses the variance of rows
-// whose mean is large.
-template <typename T, int E>
-__device__ __forceinline__ void normalize(float (&v)[8], const Columns<E>& c, int kind, float eps, float inv_n, uint32_t w, uint32_t b,
-                                          bool has_b, RowSums& sums, float2* stats, bool writes)
+// the norm of v; (mean, 1 / deviation) to *stats.  Mean first, then the squares of
+// what is left: the one pass of squares loses the variance of rows whose mean is
+// large.
+template <typename T>
+__device__ __forceinline__ Eight normalize(Eight v, int have, int kind, float eps, float inv_n, uint32_t w, uint32_t b, bool has_b,
+                                           RowSums& sums, float2* stats, bool writes)
 {
     float mean = 0.0f;
     if (kind == CHPL_NORM_LAYER) {
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += v[i];  // zero past the end
-        mean = sums(s, 0.0f).x * inv_n;
+        mean = sums.one(total_of(v)) * inv_n;  // zero past the end
+        v = v + -mean;
+        if (have < 8) clear_tail(v, have);
     }
-    float q = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v[i] -= mean;
-        q += c.has(i) ? v[i] * v[i] : 0.0f;
-    }
-    const float rstd = rsqrtf(fmaf(sums(q, 0.0f).x, inv_n, eps));
+    const float rstd = rsqrtf(fmaf(sums.one(dot(v, v)), inv_n, eps));
     if (stats && writes) *stats = make_float2(mean, rstd);
-    float wv[8], bv[8] = {};
-    values<T>(w, wv);
-    if (has_b) values<T>(b, bv);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i] * rstd, wv[i], bv[i]);
+    v = v * rstd;
+    return has_b ? fma8(v, vector_at<T>(w), vector_at<T>(b)) : v * vector_at<T>(w);
 }
 
-template <typename T, int E, bool JOIN>
+template <typename T, bool ALIGNED, bool JOIN>
 __global__ void __launch_bounds__(kMaxThreads) forward_kernel(const __grid_constant__ Forward a, const Shape s)
 {
     extern __shared__ uint4 smem[];
     __shared__ float2 sets[2][kMaxWarps];
-    const Place<E> at(s, a.n);
-    const Columns<E>& c = at.cols;
+    const Place at(s, a.n);
     const bool matrix = JOIN && a.gate.p && a.gate.ld;
     const int tensors = JOIN ? 2 + matrix : 1;
-    const uint32_t mem = smem_u32(smem), vec = mem + threadIdx.x * 16, vec_step = blockDim.x * 16;
-    Ring ring(mem + (JOIN ? kVectors : 2) * vec_step, tensors, s.stages);
+    const uint32_t mem = smem_u32(smem), vec = mem + threadIdx.x * 16, vec_step = blockDim.x * 16, turn = mem + s.turn + warp_id() * 512;
+    Ring ring(mem + (JOIN ? kVectors : 2) * vec_step, tensors, s);
     RowSums sums = {sets, s.warps, at.group, s.cluster, 0};
     const float inv_n = 1.0f / (float)a.n;
-    const uint32_t pre_w = vec + (JOIN ? kPreW : 0) * vec_step, pre_b = vec + (JOIN ? kPreB : 1) * vec_step;
     start_of_inputs();
-    if (a.pre) {
-        fetch<E>(pre_w, a.pre_w, c);
-        if (a.pre_b) fetch<E>(pre_b, a.pre_b, c);
-    }
-    if (JOIN) {
-        if (a.post) {
-            fetch<E>(vec + kPostW * vec_step, a.post_w, c);
-            if (a.post_b) fetch<E>(vec + kPostB * vec_step, a.post_b, c);
-        }
-        if (a.gate.p && !matrix) fetch<E>(vec + kGate * vec_step, a.gate.p, c);
-    }
     const auto load = [&](int64_t row, int stage) {
         if (row < a.tokens) {
-            fetch<E>(ring.slot(stage, 0), a.x.row(row), c);
-            if (JOIN) fetch<E>(ring.slot(stage, 1), a.y.row(row), c);
-            if (JOIN && matrix) fetch<E>(ring.slot(stage, 2), a.gate.row(row), c);
+            fetch_row<ALIGNED>(ring.piece(stage, 0), a.x, row, a.tokens, at.first, at.have, a.n);
+            if (JOIN) fetch_row<ALIGNED>(ring.piece(stage, 1), a.y, row, a.tokens, at.first, at.have, a.n);
+            if (JOIN && matrix) fetch_row<ALIGNED>(ring.piece(stage, 2), a.gate, row, a.tokens, at.first, at.have, a.n);
         }
         Ring::commit();
     };
     for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, i);
-    // writes of a row's statistics: one thread of the row
-    const bool writes = c.first == 0;
-    for (int64_t row = at.row; row < a.tokens; row += at.step, ring.next()) {
-        ring.wait();
-        float v[8];
-        if (JOIN) {
-            values<T>(ring.slot(ring.at, 1), v);
-            if (a.post)
-                normalize<T, E>(v, c, a.post, a.post_eps, inv_n, vec + kPostW * vec_step, vec + kPostB * vec_step, a.post_b, sums,
-                                a.post_stats ? a.post_stats + row : nullptr, writes);
-            float u[8];
-            if (a.gate.p) {
-                values<T>(matrix ? ring.slot(ring.at, 2) : vec + kGate * vec_step, u);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= u[i];
-            }
-            values<T>(ring.slot(ring.at, 0), u);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = c.has(i) ? fmaf(a.scale, v[i], a.residual_scale * u[i]) : 0.0f;
-            put<T, E>(a.r.row(row), c, v);
-        } else {
-            values<T>(ring.slot(ring.at, 0), v);
+    if (a.pre) {
+        fetch_vector(vec + kPreW * vec_step, a.pre_w, at.first, at.have);
+        if (a.pre_b) fetch_vector(vec + kPreB * vec_step, a.pre_b, at.first, at.have);
+    }
+    if (JOIN) {
+        if (a.post) {
+            fetch_vector(vec + kPostW * vec_step, a.post_w, at.first, at.have);
+            if (a.post_b) fetch_vector(vec + kPostB * vec_step, a.post_b, at.first, at.have);
         }
+        if (a.gate.p && !matrix) fetch_vector(vec + kGate * vec_step, a.gate.p, at.first, at.have);
+    }
+    const bool writes = at.first == 0;  // the row's statistics
+    for (int64_t row = at.row; row < a.tokens; row += at.step, ring.next()) {
+        ring.template wait<ALIGNED>();
+        Eight v;
+        if (JOIN) {
+            v = row_at<T, ALIGNED>(ring.piece(ring.at, 1), a.y, row, at.first, at.have);
+            if (a.post)
+                v = normalize<T>(v, at.have, a.post, a.post_eps, inv_n, vec + kPostW * vec_step, vec + kPostB * vec_step, a.post_b, sums,
+                                 a.post_stats ? a.post_stats + row : nullptr, writes);
+            if (a.gate.p)
+                v = v * (matrix ? row_at<T, ALIGNED>(ring.piece(ring.at, 2), a.gate, row, at.first, at.have) : vector_at<T>(vec + kGate * vec_step));
+            v = fma8(v, a.scale, row_at<T, ALIGNED>(ring.piece(ring.at, 0), a.x, row, at.first, at.have) * a.residual_scale);
+            put<T>(a.r, row, at.first, at.have, a.n, v, turn);
+        } else {
+            v = row_at<T, ALIGNED>(ring.piece(ring.at, 0), a.x, row, at.first, at.have);
+        }
+        if (!ALIGNED) __syncwarp();
         load(row + s.stages * at.step, ring.at);
         if (a.pre) {
-            normalize<T, E>(v, c, a.pre, a.pre_eps, inv_n, pre_w, pre_b, a.pre_b, sums, a.pre_stats ? a.pre_stats + row : nullptr, writes);
-            put<T, E>(a.h.row(row), c, v);
+            v = normalize<T>(v, at.have, a.pre, a.pre_eps, inv_n, vec + kPreW * vec_step, vec + kPreB * vec_step, a.pre_b, sums,
+                             a.pre_stats ? a.pre_stats + row : nullptr, writes);
+            put<T>(a.h, row, at.first, at.have, a.n, v, turn);
         }
     }
     if (s.cluster > 1) cluster_sync();  // no CTA leaves while another still reads its sums
@@ -349,7 +496,7 @@ struct Backward {
     int n;
     float scale, residual_scale;
     int post, pre;
-    Rows dr, dh, r, y, gate;  // gate.ld 0: a vector; y.p NULL: no join
+    Rows dr, dh, r, y, gate;  // gate.ld 0: a vector; y.p NULL: not wanted
     const void *post_w, *post_b, *pre_w;
     const float2 *post_stats, *pre_stats;
     RowsTo dx, dy, dgate;     // dgate of a matrix
@@ -365,36 +512,33 @@ struct Backward {
 //   3  dh        db_pre
 constexpr int kSums = 4;
 
-template <typename T, int E, bool JOIN, bool BIAS>
+// Rows' tails, which the copies leave zero, need no masks here: every sum over
+// the row has a factor of a zero vector or of a zero row.
+template <typename T, bool ALIGNED, bool JOIN, bool BIAS>
 __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_constant__ Backward a, const Shape s)
 {
     extern __shared__ uint4 smem[];
     __shared__ float2 sets[2][kMaxWarps];
-    const Place<E> at(s, a.n);
-    const Columns<E>& c = at.cols;
+    const Place at(s, a.n);
     const bool matrix = JOIN && a.gate.p && a.gate.ld, has_y = JOIN && a.y.p;
     const int t_dh = a.dr.p ? 1 : 0, t_r = t_dh + 1, t_y = a.pre ? t_r + 1 : t_dh, t_gate = t_y + has_y, tensors = t_gate + matrix;
-    const uint32_t mem = smem_u32(smem), vec = mem + threadIdx.x * 16, vec_step = blockDim.x * 16;
+    const uint32_t mem = smem_u32(smem), vec = mem + threadIdx.x * 16, vec_step = blockDim.x * 16, turn = mem + s.turn + warp_id() * 512;
     const uint32_t pre_w = vec, post_w = vec + vec_step, post_b = post_w + vec_step, gate_v = post_b + vec_step;
-    Ring ring(mem + (JOIN ? 4 : 1) * vec_step, tensors, s.stages);
+    Ring ring(mem + (JOIN ? 4 : 1) * vec_step, tensors, s);
     RowSums sums = {sets, s.warps, at.group, s.cluster, 0};
     const float inv_n = 1.0f / (float)a.n;
+    const auto of = [&](int t, const Rows& x, int64_t row) { return row_at<T, ALIGNED>(ring.piece(ring.at, t), x, row, at.first, at.have); };
     start_of_inputs();
-    if (a.pre) fetch<E>(pre_w, a.pre_w, c);
-    if (JOIN) {
-        if (a.post) fetch<E>(post_w, a.post_w, c);
-        if (a.post && a.post_b) fetch<E>(post_b, a.post_b, c);
-        if (a.gate.p && !matrix) fetch<E>(gate_v, a.gate.p, c);
-    }
     const auto load = [&](int64_t row, int stage) {
         if (row < a.tokens) {
-            if (a.dr.p) fetch<E>(ring.slot(stage, 0), a.dr.row(row), c);
+            const auto fetch = [&](int t, const Rows& x) { fetch_row<ALIGNED>(ring.piece(stage, t), x, row, a.tokens, at.first, at.have, a.n); };
+            if (a.dr.p) fetch(0, a.dr);
             if (a.pre) {
-                fetch<E>(ring.slot(stage, t_dh), a.dh.row(row), c);
-                fetch<E>(ring.slot(stage, t_r), a.r.row(row), c);
+                fetch(t_dh, a.dh);
+                fetch(t_r, a.r);
             }
-            if (has_y) fetch<E>(ring.slot(stage, t_y), a.y.row(row), c);
-            if (matrix) fetch<E>(ring.slot(stage, t_gate), a.gate.row(row), c);
+            if (has_y) fetch(t_y, a.y);
+            if (matrix) fetch(t_gate, a.gate);
         }
         Ring::commit();
     };
@@ -404,120 +548,107 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
         if (a.pre) pre = __ldg(a.pre_stats + row);
         if (JOIN && a.post) post = __ldg(a.post_stats + row);
     };
-    float total[BIAS ? kSums : 2][8] = {};  // without biases sums 0 and 2
-    constexpr int kHat = BIAS ? 2 : 1;
+    for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, i);
+    if (a.pre) fetch_vector(pre_w, a.pre_w, at.first, at.have);
+    if (JOIN) {
+        if (a.post) fetch_vector(post_w, a.post_w, at.first, at.have);
+        if (a.post && a.post_b) fetch_vector(post_b, a.post_b, at.first, at.have);
+        if (a.gate.p && !matrix) fetch_vector(gate_v, a.gate.p, at.first, at.have);
+    }
+    constexpr int kTotals = BIAS ? (JOIN ? 4 : 2) : 2;  // without biases sums 0 and 2, without a join 2 and 3
+    constexpr int kHat = BIAS && JOIN ? 2 : JOIN ? 1 : 0;
+    Eight total[kTotals];
+#pragma unroll
+    for (int k = 0; k < kTotals; ++k) total[k] = zeros();
     float2 pre_next, post_next;
     stats_of(at.row, pre_next, post_next);
-    for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, i);
     for (int64_t row = at.row; row < a.tokens; row += at.step, ring.next()) {
         const float2 pre = pre_next, post = post_next;
         stats_of(row + at.step, pre_next, post_next);
-        ring.wait();
-        float d[8] = {};
+        ring.template wait<ALIGNED>();
+        Eight d;
         if (a.pre) {
-            float g[8], hat[8], w[8];
-            values<T>(ring.slot(ring.at, t_dh), g);
-            values<T>(ring.slot(ring.at, t_r), hat);
-            values<T>(pre_w, w);
-            float sg = 0.0f, sgh = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                hat[i] = c.has(i) ? (hat[i] - pre.x) * pre.y : 0.0f;
-                total[kHat][i] = fmaf(g[i], hat[i], total[kHat][i]);
-                if constexpr (BIAS) total[3][i] += g[i];
-                g[i] *= w[i];
-                sg += g[i];
-                sgh = fmaf(g[i], hat[i], sgh);
+            Eight g = of(t_dh, a.dh, row);
+            const Eight hat = (of(t_r, a.r, row) + -pre.x) * pre.y;
+            total[kHat] = fma8(g, hat, total[kHat]);
+            if constexpr (BIAS) total[kHat + 1] = total[kHat + 1] + g;
+            g = g * vector_at<T>(pre_w);
+            float mg = 0.0f, mgh;
+            if (a.pre == CHPL_NORM_LAYER) {
+                const float2 m = sums.both_of(total_of(g), dot(g, hat));
+                mg = m.x * inv_n;
+                mgh = m.y * inv_n;
+            } else {
+                mgh = sums.one(dot(g, hat)) * inv_n;
             }
-            const float2 m = sums(sg, sgh);
-            const float mg = a.pre == CHPL_NORM_LAYER ? m.x * inv_n : 0.0f, mgh = m.y * inv_n;
-            if (a.dr.p) values<T>(ring.slot(ring.at, 0), d);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = fmaf(pre.y, fmaf(-hat[i], mgh, g[i] - mg), d[i]);
+            d = fma8(hat, -mgh, g + -mg) * pre.y;
+            if (a.dr.p) d = d + of(0, a.dr, row);
         } else {
-            values<T>(ring.slot(ring.at, 0), d);
+            d = of(0, a.dr, row);
         }
-        if (a.dx.p) {
-            float o[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = JOIN ? a.residual_scale * d[i] : d[i];
-            put<T, E>(a.dx.row(row), c, o);
-        }
+        if (a.dx.p) put<T>(a.dx, row, at.first, at.have, a.n, JOIN ? d * a.residual_scale : d, turn);
         if (JOIN) {
-            float y[8] = {}, w[8], u[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = c.has(i) ? a.scale * d[i] : 0.0f;
-            if (has_y) values<T>(ring.slot(ring.at, t_y), y);
-            if (a.post) {
-                values<T>(post_w, w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = c.has(i) ? (y[i] - post.x) * post.y : 0.0f;
-            }
+            d = d * a.scale;
+            Eight y = zeros();
+            if (has_y) y = of(t_y, a.y, row);
+            if (a.post) y = (y + -post.x) * post.y;
             if (matrix) {
-                values<T>(ring.slot(ring.at, t_gate), u);
                 if (a.dgate.p) {
-                    float o[8], b[8] = {};
-                    if (a.post && a.post_b) values<T>(post_b, b);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = d[i] * (a.post ? fmaf(y[i], w[i], b[i]) : y[i]);
-                    put<T, E>(a.dgate.row(row), c, o);
+                    Eight p = y;
+                    if (a.post) p = a.post_b ? fma8(y, vector_at<T>(post_w), vector_at<T>(post_b)) : y * vector_at<T>(post_w);
+                    put<T>(a.dgate, row, at.first, at.have, a.n, d * p, turn);
                 }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] *= u[i];
+                d = d * of(t_gate, a.gate, row);
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                total[0][i] = fmaf(d[i], y[i], total[0][i]);
-                if constexpr (BIAS) total[1][i] += d[i];
-            }
-            if (a.gate.p && !matrix) {
-                values<T>(gate_v, u);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] *= u[i];
-            }
+            total[0] = fma8(d, y, total[0]);
+            if constexpr (BIAS) total[1] = total[1] + d;
+            if (a.gate.p && !matrix) d = d * vector_at<T>(gate_v);
+            if (!ALIGNED) __syncwarp();
             load(row + s.stages * at.step, ring.at);
             if (a.post) {
-                float sg = 0.0f, sgh = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    d[i] *= w[i];
-                    sg += d[i];
-                    sgh = fmaf(d[i], y[i], sgh);
+                d = d * vector_at<T>(post_w);
+                float mg = 0.0f, mgh;
+                if (a.post == CHPL_NORM_LAYER) {
+                    const float2 m = sums.both_of(total_of(d), dot(d, y));
+                    mg = m.x * inv_n;
+                    mgh = m.y * inv_n;
+                } else {
+                    mgh = sums.one(dot(d, y)) * inv_n;
                 }
-                const float2 m = sums(sg, sgh);
-                const float mg = a.post == CHPL_NORM_LAYER ? m.x * inv_n : 0.0f, mgh = m.y * inv_n;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = post.y * fmaf(-y[i], mgh, d[i] - mg);
+                d = fma8(y, -mgh, d + -mg) * post.y;
             }
-            if (a.dy.p) put<T, E>(a.dy.row(row), c, d);
+            if (a.dy.p) put<T>(a.dy, row, at.first, at.have, a.n, d, turn);
         } else {
+            if (!ALIGNED) __syncwarp();
             load(row + s.stages * at.step, ring.at);
         }
     }
     // a CTA's sums: those of its groups, joined in shared memory in order
     if (a.part) {
-        float* turn = reinterpret_cast<float*>(smem);  // [groups][8][threads of a group]
+        float* joined = reinterpret_cast<float*>(smem);  // [groups][8][threads of a group]
         const int width = 32 * s.warps, thread = threadIdx.x - at.group * width;
         const int64_t unit = blockIdx.x / s.cluster;
         asm volatile("cp.async.wait_all;" ::: "memory");
         int slot = 0;
 #pragma unroll
         for (int k = 0; k < kSums; ++k) {
+            if ((!JOIN && k < 2) || (!BIAS && k % 2)) continue;
             if (!(a.sums >> k & 1)) continue;
-            const int have = BIAS ? k : k / 2;
+            constexpr int kSkip = JOIN ? 0 : 2;
+            const Eight& mine = total[BIAS ? k - kSkip : k / 2];
             if (s.groups > 1) {
                 __syncthreads();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) turn[(at.group * 8 + i) * width + thread] = total[have][i];
+                for (int i = 0; i < 8; ++i) joined[(at.group * 8 + i) * width + thread] = i % 2 ? apart(mine.v[i / 2]).y : apart(mine.v[i / 2]).x;
                 __syncthreads();
             }
             if (at.group == 0) {
-                float* out = a.part + ((int64_t)slot * s.units + unit) * a.n;
+                float* out = a.part + ((int64_t)slot * s.units + unit) * a.n + at.first;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    float v = total[have][i];
-                    for (int g = 1; g < s.groups; ++g) v += turn[(g * 8 + i) * width + thread];
-                    if (c.has(i)) out[c.at(i)] = v;
+                    float v = i % 2 ? apart(mine.v[i / 2]).y : apart(mine.v[i / 2]).x;
+                    for (int g = 1; g < s.groups; ++g) v += joined[(g * 8 + i) * width + thread];
+                    if (i < at.have) out[i] = v;
                 }
             }
             ++slot;
@@ -613,16 +744,8 @@ static int check_stats(const char* who, const char* what, const void* p, bool ne
     return CHPL_OK;
 }
 
-// features that all rows can be accessed by at once: 8, 2 or 1
-struct Pieces {
-    int e = 8;
-    void add(const void* p, int64_t ld, int64_t tokens)
-    {
-        if (!p) return;
-        const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (tokens > 1 ? (uintptr_t)(ld * 2) : 0);
-        e = std::min(e, a % 16 == 0 ? 8 : a % 4 == 0 ? 2 : 1);
-    }
-};
+// 16-byte accesses fit
+static bool fits(const void* p, int64_t ld, int64_t tokens) { return !p || aligned(p, tokens > 1 ? ld * 2 : 0, 16); }
 
 static int check(const char* who, const chpl_norm_fwd* a)
 {
@@ -659,14 +782,6 @@ static int launch(cudaStream_t st, const A& a, const Shape& s)
     return launch_kernel(KERNEL, (int64_t)s.units * s.cluster, 32 * s.warps * s.groups, s.smem, s.cluster, st, a, s);
 }
 
-template <typename T, bool JOIN>
-static int forward(cudaStream_t st, int pieces, const Forward& f, const Shape& s)
-{
-    if (pieces == 8) return launch<forward_kernel<T, 8, JOIN>>(st, f, s);
-    if (pieces == 2) return launch<forward_kernel<T, 2, JOIN>>(st, f, s);
-    return launch<forward_kernel<T, 1, JOIN>>(st, f, s);
-}
-
 template <typename T>
 static int forward(cudaStream_t st, const chpl_norm_fwd& a)
 {
@@ -675,44 +790,40 @@ static int forward(cudaStream_t st, const chpl_norm_fwd& a)
     f.n = (int)a.n;
     f.scale = a.scale;
     f.residual_scale = a.residual_scale;
-    f.pre = a.pre.kind;
-    f.pre_eps = a.pre.eps;
     f.x = {a.x, a.ldx};
-    Pieces p;
-    p.add(a.x, a.ldx, a.tokens);
+    bool in = fits(a.x, a.ldx, a.tokens), out = true;
     if (a.join) {
         f.post = a.post.kind;
         f.post_eps = a.post.eps;
         f.y = {a.y, a.ldy};
         f.gate = {a.gate, a.ldgate};
-        f.r = {a.r, a.ldr};
-        p.add(a.y, a.ldy, a.tokens);
-        p.add(a.r, a.ldr, a.tokens);
-        p.add(a.gate, a.ldgate, a.tokens);
+        f.r = {a.r, a.ldr, fits(a.r, a.ldr, a.tokens)};
+        in = in && fits(a.y, a.ldy, a.tokens) && (a.ldgate == 0 || fits(a.gate, a.ldgate, a.tokens));
+        out = f.r.aligned;
         if (f.post) {
             f.post_w = a.post.weight;
             f.post_b = a.post.bias;
             f.post_stats = reinterpret_cast<float2*>(a.post_stats);
-            p.add(f.post_w, 0, 1);
-            p.add(f.post_b, 0, 1);
         }
     }
+    f.pre = a.pre.kind;
     if (f.pre) {
+        f.pre_eps = a.pre.eps;
         f.pre_w = a.pre.weight;
         f.pre_b = a.pre.bias;
-        f.h = {a.h, a.ldh};
+        f.h = {a.h, a.ldh, fits(a.h, a.ldh, a.tokens)};
         f.pre_stats = reinterpret_cast<float2*>(a.pre_stats);
-        p.add(f.pre_w, 0, 1);
-        p.add(f.pre_b, 0, 1);
-        p.add(a.h, a.ldh, a.tokens);
+        out = out && f.h.aligned;
     }
-    const Shape s = shape_for(a.tokens, a.n, a.join ? 2 + (a.gate && a.ldgate) : 1, a.join ? kVectors : 2);
-    return a.join ? forward<T, true>(st, p.e, f, s) : forward<T, false>(st, p.e, f, s);
+    const Shape s = shape_for(a.tokens, a.n, a.join ? 2 + (a.gate && a.ldgate) : 1, a.join ? kVectors : 2, in, out);
+    if (a.join) return in ? launch<forward_kernel<T, true, true>>(st, f, s) : launch<forward_kernel<T, false, true>>(st, f, s);
+    return in ? launch<forward_kernel<T, true, false>>(st, f, s) : launch<forward_kernel<T, false, false>>(st, f, s);
 }
 
 // what a backward call forms
 struct BackwardPlan {
     Shape shape;
+    bool in, out;    // rows that 16-byte accesses fit
     int sums;        // bits
     size_t bytes;
 };
@@ -720,15 +831,17 @@ struct BackwardPlan {
 static BackwardPlan plan(const chpl_norm_bwd& a)
 {
     BackwardPlan p;
-    const bool vector_gate = a.dgate && a.gate && a.ldgate == 0;
+    const bool vector_gate = a.dgate && a.gate && a.ldgate == 0, matrix = a.join && a.gate && a.ldgate, has_y = a.join && (a.post.kind || a.gate);
     p.sums = 0;
     if (a.join && ((a.post.kind && a.dpost_weight) || vector_gate)) p.sums |= 1;
     if (a.join && a.post.kind && (a.dpost_bias || (vector_gate && a.post.bias))) p.sums |= 2;
     if (a.pre.kind && a.dpre_weight) p.sums |= 4;
     if (a.pre.kind && a.dpre_bias) p.sums |= 8;
-    int tensors = (a.dr ? 1 : 0) + (a.pre.kind ? 2 : 0);
-    if (a.join) tensors += (a.post.kind || a.gate ? 1 : 0) + (a.gate && a.ldgate ? 1 : 0);
-    p.shape = shape_for(a.tokens, a.n, tensors, a.join ? 4 : 1);
+    p.in = fits(a.dr, a.lddr, a.tokens) && (!a.pre.kind || (fits(a.dh, a.lddh, a.tokens) && fits(a.r, a.ldr, a.tokens))) &&
+           (!has_y || fits(a.y, a.ldy, a.tokens)) && (!matrix || fits(a.gate, a.ldgate, a.tokens));
+    p.out = fits(a.dx, a.lddx, a.tokens) && (!a.join || fits(a.dy, a.lddy, a.tokens)) && (!matrix || fits(a.dgate, a.lddgate, a.tokens));
+    const int tensors = (a.dr ? 1 : 0) + (a.pre.kind ? 2 : 0) + has_y + matrix;
+    p.shape = shape_for(a.tokens, a.n, tensors, a.join ? 4 : 1, p.in, p.out);
     // the groups' sums are joined where the rows under way were
     p.shape.smem = std::max(p.shape.smem, p.shape.groups > 1 ? 32 * p.shape.warps * p.shape.groups * 8 * 4 : 0);
     int count = 0;
@@ -784,18 +897,10 @@ static int check(const char* who, const chpl_norm_bwd* a, bool pointers)
     return CHPL_OK;
 }
 
-template <typename T, bool JOIN, bool BIAS>
-static int backward(cudaStream_t st, int pieces, const Backward& b, const Shape& s)
-{
-    if (pieces == 8) return launch<backward_kernel<T, 8, JOIN, BIAS>>(st, b, s);
-    if (pieces == 2) return launch<backward_kernel<T, 2, JOIN, BIAS>>(st, b, s);
-    return launch<backward_kernel<T, 1, JOIN, BIAS>>(st, b, s);
-}
-
 template <typename T>
 static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
 {
-    const BackwardPlan plan_ = plan(a);
+    const BackwardPlan p = plan(a);
     const bool matrix = a.join && a.gate && a.ldgate;
     if (a.tokens > 0) {
         Backward b = {};
@@ -803,52 +908,40 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
         b.n = (int)a.n;
         b.scale = a.scale;
         b.residual_scale = a.residual_scale;
-        b.sums = plan_.sums;
-        b.part = plan_.sums ? static_cast<float*>(work) : nullptr;
+        b.sums = p.sums;
+        b.part = p.sums ? static_cast<float*>(work) : nullptr;
         b.dr = {a.dr, a.lddr};
-        b.dx = {a.dx, a.lddx};
-        Pieces p;
-        p.add(a.dr, a.lddr, a.tokens);
-        p.add(a.dx, a.lddx, a.tokens);
+        b.dx = {a.dx, a.lddx, fits(a.dx, a.lddx, a.tokens)};
         if (a.pre.kind) {
             b.pre = a.pre.kind;
             b.dh = {a.dh, a.lddh};
             b.r = {a.r, a.ldr};
             b.pre_w = a.pre.weight;
             b.pre_stats = reinterpret_cast<const float2*>(a.pre_stats);
-            p.add(a.dh, a.lddh, a.tokens);
-            p.add(a.r, a.ldr, a.tokens);
-            p.add(b.pre_w, 0, 1);
         }
         if (a.join) {
             if (a.post.kind || a.gate) b.y = {a.y, a.ldy};
             b.gate = {a.gate, a.ldgate};
-            b.dy = {a.dy, a.lddy};
-            if (matrix) b.dgate = {a.dgate, a.lddgate};
-            p.add(b.y.p, b.y.ld, a.tokens);
-            p.add(a.gate, a.ldgate, a.tokens);
-            p.add(a.dy, a.lddy, a.tokens);
-            p.add(b.dgate.p, b.dgate.ld, a.tokens);
+            b.dy = {a.dy, a.lddy, fits(a.dy, a.lddy, a.tokens)};
+            if (matrix) b.dgate = {a.dgate, a.lddgate, fits(a.dgate, a.lddgate, a.tokens)};
             if (a.post.kind) {
                 b.post = a.post.kind;
                 b.post_w = a.post.weight;
                 b.post_b = a.post.bias;
                 b.post_stats = reinterpret_cast<const float2*>(a.post_stats);
-                p.add(b.post_w, 0, 1);
-                p.add(b.post_b, 0, 1);
             }
         }
-        const bool bias = (plan_.sums & 10) != 0;
-        if (!a.join) CHPL_TRY((backward<T, false, true>(st, p.e, b, plan_.shape)));
-        else if (bias) CHPL_TRY((backward<T, true, true>(st, p.e, b, plan_.shape)));
-        else CHPL_TRY((backward<T, true, false>(st, p.e, b, plan_.shape)));
+        const bool bias = (p.sums & 10) != 0;
+        if (!a.join) CHPL_TRY((p.in ? launch<backward_kernel<T, true, false, true>>(st, b, p.shape) : launch<backward_kernel<T, false, false, true>>(st, b, p.shape)));
+        else if (bias) CHPL_TRY((p.in ? launch<backward_kernel<T, true, true, true>>(st, b, p.shape) : launch<backward_kernel<T, false, true, true>>(st, b, p.shape)));
+        else CHPL_TRY((p.in ? launch<backward_kernel<T, true, true, false>>(st, b, p.shape) : launch<backward_kernel<T, false, true, false>>(st, b, p.shape)));
     }
-    if (!plan_.sums || (a.tokens == 0 && a.accumulate)) return CHPL_OK;
+    if (!p.sums || (a.tokens == 0 && a.accumulate)) return CHPL_OK;
     Parameters q = {};
     q.part = static_cast<const float*>(work);
-    q.units = a.tokens > 0 ? plan_.shape.units : 0;
+    q.units = a.tokens > 0 ? p.shape.units : 0;
     q.n = (int)a.n;
-    q.sums = plan_.sums;
+    q.sums = p.sums;
     q.f32 = a.grad_type == CHPL_TYPE_F32;
     q.accumulate = a.accumulate;
     q.matrix = matrix;
