@@ -4,10 +4,12 @@
 // gate * Npost(y), together with the next block's norm h = Npre(r).
 //
 // Bound: HBM; every row is read and written once.  A row lies in the registers
-// of one CTA (of a cluster above 8192 features), eight features a thread, so
+// of one CTA (of a cluster above 8192 features), sixteen features a thread, so
 // that the statistics' passes over it cost no memory traffic and the gradients'
-// sums over the tokens stay in registers, eight a thread, from a CTA's first row
-// to its last.  The rows to come are on their way into shared memory meanwhile,
+// sums over the tokens stay in registers from a CTA's first row to its last.
+// Sixteen, because what a row costs a thread beside its features (sums over the
+// row, addresses, waits) bounds the kernels with eight: join of 8192 x 4096 68 us,
+// its gradients 136.  The rows to come are on their way into shared memory meanwhile,
 // every warp copying what it will itself read: no barrier waits for a copy.
 #include <algorithm>
 #include <cmath>
@@ -20,10 +22,13 @@ namespace norm {
 using linear::check_operand;
 using linear::check_size;
 
-constexpr int kMaxThreads = 1024;
-constexpr int kMaxWidth = 2 * 8 * kMaxThreads;  // a cluster of two
+constexpr int kHalves = 2;                          // eights of a thread's features, 256 apart
+constexpr int kWarpWidth = 256 * kHalves;
+constexpr int kMaxThreads = 512;
+constexpr int kMaxWidth = 2 * 8 * kHalves * kMaxThreads;  // a cluster of two
 constexpr int kMaxStages = 4;
-constexpr int kStageBudget = 208 * 1024;        // of shared memory on an SM, for the rows under way
+constexpr int kSmem = 227 * 1024;               // of an SM
+constexpr int kSmemApart = 1536;                // of which a CTA takes, beside what it asks for
 
 // ----------------------------------------------------------------------------
 // shape of a launch
@@ -39,21 +44,23 @@ struct Shape {
     int smem;
 };
 
-// A row's warps are a power of two up to four (several rows to a CTA of eight
-// warps), then as many as it needs.  64 registers a thread leave 1024 threads on
-// an SM.
-static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors, bool inputs_aligned, bool outputs_aligned)
+// A row's warps are a power of two up to four (several rows to a CTA of four
+// warps), then as many as it needs.  `on_sm`: threads that an SM has registers for.
+static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors, bool inputs_aligned, bool outputs_aligned, int on_sm)
 {
     Shape s;
-    s.cluster = n > 8 * kMaxThreads ? 2 : 1;
-    const int need = (int)((n + 256 * s.cluster - 1) / (256 * s.cluster));
+    s.cluster = n > kWarpWidth * (kMaxThreads / 32) ? 2 : 1;
+    const int need = (int)((n + kWarpWidth * s.cluster - 1) / (kWarpWidth * s.cluster));
     s.warps = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : need;
-    s.groups = s.warps <= 4 ? 8 / s.warps : 1;
-    s.piece = inputs_aligned ? 512 : 544;
-    const int warps = s.warps * s.groups, resident = kMaxThreads / (32 * warps);
-    const int fixed = vectors * warps * 512 + (outputs_aligned ? 0 : warps * 512), row = std::max(1, tensors) * warps * s.piece;
-    s.stages = std::max(1, std::min(kMaxStages, (kStageBudget / resident - fixed) / row));
-    s.turn = vectors * warps * 512 + s.stages * row;
+    s.groups = s.warps <= 4 ? 4 / s.warps : 1;
+    s.piece = inputs_aligned ? 1024 : 1056;
+    const int warps = s.warps * s.groups, row = std::max(1, tensors) * warps * s.piece;
+    const int fixed = vectors * warps * 1024 + (outputs_aligned ? 0 : warps * 512);
+    // fewer CTAs on an SM rather than one row under way
+    int resident = on_sm / (32 * warps);
+    while (resident > 1 && (kSmem / resident - kSmemApart - fixed) / row < 2) --resident;
+    s.stages = std::max(1, std::min(kMaxStages, (kSmem / resident - kSmemApart - fixed) / row));
+    s.turn = vectors * warps * 1024 + s.stages * row;
     s.smem = fixed + s.stages * row;
     const int64_t want = (tokens + s.groups - 1) / s.groups;
     s.units = (int)std::min<int64_t>(want, 148 / s.cluster * resident);
@@ -61,120 +68,165 @@ static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors, bool
 }
 
 // ----------------------------------------------------------------------------
-// eight consecutive features of a thread
+// a thread's features: eight consecutive ones in each half of its warp's
 // ----------------------------------------------------------------------------
-struct Eight {
-    Two v[4];
+constexpr int kTwos = 4 * kHalves;
+struct Some {
+    Two v[kTwos];
 };
 
-__device__ __forceinline__ Eight zeros()
+__device__ __forceinline__ Some zeros()
 {
-    Eight r;
+    Some r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = both(0.0f);
+    for (int i = 0; i < kTwos; ++i) r.v[i] = both(0.0f);
     return r;
 }
-__device__ __forceinline__ Eight operator*(const Eight& a, const Eight& b)
+__device__ __forceinline__ Some operator*(const Some& a, const Some& b)
 {
-    Eight r;
+    Some r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = a.v[i] * b.v[i];
+    for (int i = 0; i < kTwos; ++i) r.v[i] = a.v[i] * b.v[i];
     return r;
 }
-__device__ __forceinline__ Eight operator+(const Eight& a, const Eight& b)
+__device__ __forceinline__ Some operator+(const Some& a, const Some& b)
 {
-    Eight r;
+    Some r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = a.v[i] + b.v[i];
+    for (int i = 0; i < kTwos; ++i) r.v[i] = a.v[i] + b.v[i];
     return r;
 }
-__device__ __forceinline__ Eight operator*(const Eight& a, float b)
+__device__ __forceinline__ Some operator*(const Some& a, float b)
 {
-    Eight r;
+    Some r;
+    const Two c = both(b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = a.v[i] * both(b);
+    for (int i = 0; i < kTwos; ++i) r.v[i] = a.v[i] * c;
     return r;
 }
-__device__ __forceinline__ Eight operator+(const Eight& a, float b)
+__device__ __forceinline__ Some operator+(const Some& a, float b)
 {
-    Eight r;
+    Some r;
+    const Two c = both(b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = a.v[i] + both(b);
+    for (int i = 0; i < kTwos; ++i) r.v[i] = a.v[i] + c;
     return r;
 }
-__device__ __forceinline__ Eight fma8(const Eight& a, const Eight& b, const Eight& c)
+__device__ __forceinline__ Some fma_of(const Some& a, const Some& b, const Some& c)
 {
-    Eight r;
+    Some r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = fma2(a.v[i], b.v[i], c.v[i]);
+    for (int i = 0; i < kTwos; ++i) r.v[i] = fma2(a.v[i], b.v[i], c.v[i]);
     return r;
 }
-__device__ __forceinline__ Eight fma8(const Eight& a, float b, const Eight& c)
+__device__ __forceinline__ Some fma_of(const Some& a, float b, const Some& c)
 {
-    Eight r;
+    Some r;
+    const Two m = both(b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = fma2(a.v[i], both(b), c.v[i]);
+    for (int i = 0; i < kTwos; ++i) r.v[i] = fma2(a.v[i], m, c.v[i]);
     return r;
 }
-__device__ __forceinline__ float total_of(const Eight& a)
+__device__ __forceinline__ float total_of(const Some& a)
 {
-    const float2 t = apart((a.v[0] + a.v[1]) + (a.v[2] + a.v[3]));
+    Two even = a.v[0], odd = a.v[1];
+#pragma unroll
+    for (int i = 2; i < kTwos; i += 2) {
+        even = even + a.v[i];
+        odd = odd + a.v[i + 1];
+    }
+    const float2 t = apart(even + odd);
     return t.x + t.y;
 }
-__device__ __forceinline__ float dot(const Eight& a, const Eight& b)
+__device__ __forceinline__ float dot(const Some& a, const Some& b)
 {
-    const float2 t = apart(fma2(a.v[0], b.v[0], a.v[1] * b.v[1]) + fma2(a.v[2], b.v[2], a.v[3] * b.v[3]));
+    Two even = a.v[0] * b.v[0], odd = a.v[1] * b.v[1];
+#pragma unroll
+    for (int i = 2; i < kTwos; i += 2) {
+        even = fma2(a.v[i], b.v[i], even);
+        odd = fma2(a.v[i + 1], b.v[i + 1], odd);
+    }
+    const float2 t = apart(even + odd);
     return t.x + t.y;
 }
-// zero from the `have`-th on
-__device__ __forceinline__ void clear_tail(Eight& a, int have)
+__device__ __forceinline__ float feature(const Some& a, int i) { return i % 2 ? apart(a.v[i / 2]).y : apart(a.v[i / 2]).x; }
+
+// where a thread stands: its features first + 256 h + 0 .. 7, of which left - 256 h
+// exist (all eight, some or none)
+struct Place {
+    int first, left;
+    int group;
+    int64_t row, step;
+    __device__ __forceinline__ Place(const Shape& s, int n)
+    {
+        const int warp = warp_id(), rank = s.cluster > 1 ? (int)cluster_ctarank() : 0;
+        group = warp / s.warps;
+        first = (rank * s.warps + warp - group * s.warps) * kWarpWidth + lane_id() * 8;
+        left = n - first;
+        const int64_t unit = blockIdx.x / s.cluster;
+        row = unit * s.groups + group;
+        step = (int64_t)s.units * s.groups;
+    }
+    __device__ __forceinline__ int have(int h) const { return min(8, max(0, left - 256 * h)); }
+    __device__ __forceinline__ bool whole() const { return left >= 256 * (kHalves - 1) + 8; }
+};
+
+// zero past the row's end
+__device__ __forceinline__ void clear_tail(Some& a, const Place& at)
 {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kTwos; ++i) {
         const float2 t = apart(a.v[i]);
-        a.v[i] = two(2 * i < have ? t.x : 0.0f, 2 * i + 1 < have ? t.y : 0.0f);
+        const int left = at.left - 256 * (i / 4) - 2 * (i % 4);
+        a.v[i] = two(left > 0 ? t.x : 0.0f, left > 1 ? t.y : 0.0f);
     }
 }
 
 template <typename T>
-__device__ __forceinline__ Eight expand(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+__device__ __forceinline__ void expand(const uint32_t (&w)[4], int h, Some& r)
 {
-    const uint32_t w[4] = {a, b, c, d};
-    Eight r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 f = linear::unpack2<T>(w[i]);
-        r.v[i] = two(f.x, f.y);
+        r.v[4 * h + i] = two(f.x, f.y);
+    }
+}
+
+// features of a warp's 1024 bytes of shared memory in order, the lane's own
+template <typename T>
+__device__ __forceinline__ Some vector_at(uint32_t piece)
+{
+    Some r;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(piece + h * 512 + lane_id() * 16) : "memory");
+        expand<T>(w, h, r);
     }
     return r;
 }
 
-// features of a vector that lie in 16 bytes of shared memory of the thread's own
-template <typename T>
-__device__ __forceinline__ Eight vector_at(uint32_t slot)
+// the thread's features of a vector into its own bytes there, zero past the end
+__device__ __forceinline__ void fetch_vector(uint32_t piece, const void* v, const Place& at)
 {
-    uint4 w;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(slot) : "memory");
-    return expand<T>(w.x, w.y, w.z, w.w);
-}
-
-// the thread's `have` features of a vector into its 16 bytes, zero past the end
-__device__ __forceinline__ void fetch_vector(uint32_t slot, const void* v, int first, int have)
-{
-    const unsigned short* p = static_cast<const unsigned short*>(v) + first;
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (have == 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-        w[0] = q.x;
-        w[1] = q.y;
-        w[2] = q.z;
-        w[3] = q.w;
-    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < have) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+    for (int h = 0; h < kHalves; ++h) {
+        const unsigned short* p = static_cast<const unsigned short*>(v) + at.first + 256 * h;
+        const int have = at.have(h);
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (have == 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+            const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+            w[0] = q.x;
+            w[1] = q.y;
+            w[2] = q.z;
+            w[3] = q.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < have) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece + h * 512 + lane_id() * 16), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
     }
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
 
 struct Rows {
@@ -194,95 +246,109 @@ __device__ __forceinline__ void copy16(uint32_t slot, const void* src, int bytes
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot), "l"(src), "r"(bytes) : "memory");
 }
 
-// The warp's 256 features of a row into its piece of shared memory, asynchronously.
-// Aligned rows: the lane's own 16 bytes.  Others: the 16-byte chunks of memory
-// that the features lie in, 33 of them, whose other bytes are the row's (or the
-// rows' beside it); the chunks that reach out of the tensor, in its first and last
-// row, are read by the element.
+// The warp's features of a row into its piece of shared memory, asynchronously.
+// Aligned rows: the lane's own 16 bytes of each half.  Others: the 16-byte chunks
+// of memory that the features lie in, one more, whose other bytes are the row's
+// (or the rows' beside it); the chunks that reach out of the tensor, in its first
+// and last row, are read by the element.
 template <bool ALIGNED>
-__device__ __forceinline__ void fetch_row(uint32_t piece, const Rows& x, int64_t t, int64_t tokens, int first, int have, int n)
+__device__ __forceinline__ void fetch_row(uint32_t piece, const Rows& x, int64_t t, int64_t tokens, const Place& at)
 {
     const int lane = lane_id();
     const unsigned short* row = x.row(t);
     if (ALIGNED) {
-        copy16(piece + lane * 16, row + (have > 0 ? first : 0), 2 * have);
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            const int have = at.have(h);
+            copy16(piece + h * 512 + lane * 16, row + (have > 0 ? at.first + 256 * h : 0), 2 * have);
+        }
         return;
     }
-    const unsigned short* p = row + (first - lane * 8);
+    const unsigned short* p = row + (at.first - lane * 8);
     const char* from = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
     const char* begin = static_cast<const char*>(x.p);
+    const int n = at.first + at.left;
     const char* row_end = reinterpret_cast<const char*>(row + n);
     const char* end = reinterpret_cast<const char*>(x.row(tokens - 1) + n);
-    for (int c = lane; c < 33; c += 32) {
-        const char* at = from + c * 16;
-        if (at >= row_end) break;
-        if (at >= begin && at + 16 <= end) {
-            copy16(piece + c * 16, at, 16);
+    for (int c = lane; c < 32 * kHalves + 1; c += 32) {
+        const char* src = from + c * 16;
+        if (src >= row_end) break;
+        if (src >= begin && src + 16 <= end) {
+            copy16(piece + c * 16, src, 16);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (at + 2 * i >= begin && at + 2 * i < end)
-                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(piece + c * 16 + 2 * i), "h"(*reinterpret_cast<const unsigned short*>(at + 2 * i)) : "memory");
+                if (src + 2 * i >= begin && src + 2 * i < end)
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(piece + c * 16 + 2 * i), "h"(*reinterpret_cast<const unsigned short*>(src + 2 * i)) : "memory");
         }
     }
 }
 
 // the thread's features of that row; zero past its end
 template <typename T, bool ALIGNED>
-__device__ __forceinline__ Eight row_at(uint32_t piece, const Rows& x, int64_t t, int first, int have)
+__device__ __forceinline__ Some row_at(uint32_t piece, const Rows& x, int64_t t, const Place& at)
 {
+    if (ALIGNED) return vector_at<T>(piece);
+    Some r;
     const int lane = lane_id();
-    if (ALIGNED) return vector_at<T>(piece + lane * 16);
-    const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(x.row(t) + (first - lane * 8)) & 15u;  // bytes before the first feature
-    const uint32_t at = piece + lane * 16 + (skew & ~3u);
-    uint32_t w[5];
+    const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(x.row(t) + (at.first - lane * 8)) & 15u;  // bytes before the first feature
+    const uint32_t from = piece + lane * 16 + (skew & ~3u);
 #pragma unroll
-    for (int i = 0; i < 5; ++i)
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i]) : "r"(at + 4 * i) : "memory");
+    for (int h = 0; h < kHalves; ++h) {
+        uint32_t u[5], w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (skew & 2u));
-    if (have < 8) {
+        for (int i = 0; i < 5; ++i)
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u[i]) : "r"(from + h * 512 + 4 * i) : "memory");
+        const int have = at.have(h);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] &= (2 * i < have ? 0xffffu : 0u) | (2 * i + 1 < have ? 0xffff0000u : 0u);
+        for (int i = 0; i < 4; ++i) {
+            w[i] = __funnelshift_r(u[i], u[i + 1], 8 * (skew & 2u));
+            if (have < 8) w[i] &= (2 * i < have ? 0xffffu : 0u) | (2 * i + 1 < have ? 0xffff0000u : 0u);
+        }
+        expand<T>(w, h, r);
     }
-    return expand<T>(w[0], w[1], w[2], w[3]);
+    return r;
 }
 
 // the thread's features into a row; rows that 16-byte stores do not fit go by way
 // of `turn`, 512 bytes of the warp's own, so that a store covers 32 features in a row
 template <typename T>
-__device__ __forceinline__ void put(const RowsTo& out, int64_t t, int first, int have, int n, const Eight& v, uint32_t turn)
+__device__ __forceinline__ void put(const RowsTo& out, int64_t t, const Place& at, const Some& v, uint32_t turn)
 {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = apart(v.v[i]);
-        w[i] = linear::pack2<T>(f.x, f.y);
-    }
-    unsigned short* p = out.row(t) + first;
-    if (out.aligned) {
-        if (have == 8) {
-            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < have) p[i] = (unsigned short)(w[i >> 1] >> (16 * (i & 1)));
-        }
-        return;
-    }
+    unsigned short* const row = out.row(t) + at.first;
     const int lane = lane_id();
-    __syncwarp();
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(turn + lane * 16), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-    __syncwarp();
-    p -= lane * 8;
-    const int left = n - (first - lane * 8);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i * 32 + lane < left) {
-            unsigned short e;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(e) : "r"(turn + 2 * (i * 32 + lane)) : "memory");
-            p[i * 32 + lane] = e;
+    for (int h = 0; h < kHalves; ++h) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = apart(v.v[4 * h + i]);
+            w[i] = linear::pack2<T>(f.x, f.y);
         }
+        unsigned short* p = row + 256 * h;
+        const int left = at.left - 256 * h;
+        if (out.aligned) {
+            if (left >= 8) {
+                *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < left) p[i] = (unsigned short)(w[i >> 1] >> (16 * (i & 1)));
+            }
+            continue;
+        }
+        __syncwarp();
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(turn + lane * 16), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        __syncwarp();
+        p -= lane * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i * 32 + lane < left + lane * 8) {
+                unsigned short e;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(e) : "r"(turn + 2 * (i * 32 + lane)) : "memory");
+                p[i * 32 + lane] = e;
+            }
+    }
 }
 
 // ----------------------------------------------------------------------------
@@ -348,23 +414,6 @@ struct RowSums {
     }
 };
 
-// where a thread stands
-struct Place {
-    int first, have, n;  // of its features
-    int group;
-    int64_t row, step;
-    __device__ __forceinline__ Place(const Shape& s, int width) : n(width)
-    {
-        const int warp = warp_id(), rank = s.cluster > 1 ? (int)cluster_ctarank() : 0;
-        group = warp / s.warps;
-        first = ((rank * s.warps + warp - group * s.warps) * 32 + lane_id()) * 8;
-        have = min(8, max(0, n - first));
-        const int64_t unit = blockIdx.x / s.cluster;
-        row = unit * s.groups + group;
-        step = (int64_t)s.units * s.groups;
-    }
-};
-
 // The rows under way: copies of the rows to come, a group of cp.async each,
 // `stages` of them (an empty group where there is no such row).
 struct Ring {
@@ -406,83 +455,85 @@ struct Forward {
     float2 *post_stats, *pre_stats;
 };
 
-// slots of the vectors
-enum { kPreW, kPreB, kPostW, kPostB, kGate, kVectors };
-
 // the norm of v; (mean, 1 / deviation) to *stats.  Mean first, then the squares of
 // what is left: the one pass of squares loses the variance of rows whose mean is
 // large.
 template <typename T>
-__device__ __forceinline__ Eight normalize(Eight v, int have, int kind, float eps, float inv_n, uint32_t w, uint32_t b, bool has_b,
+__device__ __forceinline__ Some normalize(Some v, const Place& at, int kind, float eps, float inv_n, uint32_t w, uint32_t b, bool has_b,
                                            RowSums& sums, float2* stats, bool writes)
 {
     float mean = 0.0f;
     if (kind == CHPL_NORM_LAYER) {
         mean = sums.one(total_of(v)) * inv_n;  // zero past the end
         v = v + -mean;
-        if (have < 8) clear_tail(v, have);
+        if (!at.whole()) clear_tail(v, at);
     }
     const float rstd = rsqrtf(fmaf(sums.one(dot(v, v)), inv_n, eps));
     if (stats && writes) *stats = make_float2(mean, rstd);
     v = v * rstd;
-    return has_b ? fma8(v, vector_at<T>(w), vector_at<T>(b)) : v * vector_at<T>(w);
+    return has_b ? fma_of(v, vector_at<T>(w), vector_at<T>(b)) : v * vector_at<T>(w);
 }
 
 template <typename T, bool ALIGNED, bool JOIN>
-__global__ void __launch_bounds__(kMaxThreads) forward_kernel(const __grid_constant__ Forward a, const Shape s)
+__global__ void __launch_bounds__(kMaxThreads, 2) forward_kernel(const __grid_constant__ Forward a, const Shape s)
 {
     extern __shared__ uint4 smem[];
     __shared__ float2 sets[2][kMaxWarps];
     const Place at(s, a.n);
     const bool matrix = JOIN && a.gate.p && a.gate.ld;
     const int tensors = JOIN ? 2 + matrix : 1;
-    const uint32_t mem = smem_u32(smem), vec = mem + threadIdx.x * 16, vec_step = blockDim.x * 16, turn = mem + s.turn + warp_id() * 512;
-    Ring ring(mem + (JOIN ? kVectors : 2) * vec_step, tensors, s);
+    const uint32_t mem = smem_u32(smem), vec = mem + warp_id() * 1024, vec_step = blockDim.x * 32, turn = mem + s.turn + warp_id() * 512;
+    // the vectors that there are, then the rows
+    uint32_t used = 0;
+    const auto place = [&](const void* v) { return vec + (v ? used++ : 0) * vec_step; };
+    const uint32_t pre_w = place(a.pre_w), pre_b = place(a.pre_b);
+    const uint32_t post_w = JOIN ? place(a.post_w) : 0, post_b = JOIN ? place(a.post_b) : 0, gate_v = JOIN ? place(matrix ? nullptr : a.gate.p) : 0;
+    Ring ring(mem + used * vec_step, tensors, s);
     RowSums sums = {sets, s.warps, at.group, s.cluster, 0};
     const float inv_n = 1.0f / (float)a.n;
     start_of_inputs();
     const auto load = [&](int64_t row, int stage) {
         if (row < a.tokens) {
-            fetch_row<ALIGNED>(ring.piece(stage, 0), a.x, row, a.tokens, at.first, at.have, a.n);
-            if (JOIN) fetch_row<ALIGNED>(ring.piece(stage, 1), a.y, row, a.tokens, at.first, at.have, a.n);
-            if (JOIN && matrix) fetch_row<ALIGNED>(ring.piece(stage, 2), a.gate, row, a.tokens, at.first, at.have, a.n);
+            fetch_row<ALIGNED>(ring.piece(stage, 0), a.x, row, a.tokens, at);
+            if (JOIN) fetch_row<ALIGNED>(ring.piece(stage, 1), a.y, row, a.tokens, at);
+            if (JOIN && matrix) fetch_row<ALIGNED>(ring.piece(stage, 2), a.gate, row, a.tokens, at);
         }
         Ring::commit();
     };
     for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, i);
     if (a.pre) {
-        fetch_vector(vec + kPreW * vec_step, a.pre_w, at.first, at.have);
-        if (a.pre_b) fetch_vector(vec + kPreB * vec_step, a.pre_b, at.first, at.have);
+        fetch_vector(pre_w, a.pre_w, at);
+        if (a.pre_b) fetch_vector(pre_b, a.pre_b, at);
     }
     if (JOIN) {
         if (a.post) {
-            fetch_vector(vec + kPostW * vec_step, a.post_w, at.first, at.have);
-            if (a.post_b) fetch_vector(vec + kPostB * vec_step, a.post_b, at.first, at.have);
+            fetch_vector(post_w, a.post_w, at);
+            if (a.post_b) fetch_vector(post_b, a.post_b, at);
         }
-        if (a.gate.p && !matrix) fetch_vector(vec + kGate * vec_step, a.gate.p, at.first, at.have);
+        if (a.gate.p && !matrix) fetch_vector(gate_v, a.gate.p, at);
     }
     const bool writes = at.first == 0;  // the row's statistics
     for (int64_t row = at.row; row < a.tokens; row += at.step, ring.next()) {
         ring.template wait<ALIGNED>();
-        Eight v;
+        Some v;
         if (JOIN) {
-            v = row_at<T, ALIGNED>(ring.piece(ring.at, 1), a.y, row, at.first, at.have);
+            v = row_at<T, ALIGNED>(ring.piece(ring.at, 1), a.y, row, at);
             if (a.post)
-                v = normalize<T>(v, at.have, a.post, a.post_eps, inv_n, vec + kPostW * vec_step, vec + kPostB * vec_step, a.post_b, sums,
+                v = normalize<T>(v, at, a.post, a.post_eps, inv_n, post_w, post_b, a.post_b, sums,
                                  a.post_stats ? a.post_stats + row : nullptr, writes);
             if (a.gate.p)
-                v = v * (matrix ? row_at<T, ALIGNED>(ring.piece(ring.at, 2), a.gate, row, at.first, at.have) : vector_at<T>(vec + kGate * vec_step));
-            v = fma8(v, a.scale, row_at<T, ALIGNED>(ring.piece(ring.at, 0), a.x, row, at.first, at.have) * a.residual_scale);
-            put<T>(a.r, row, at.first, at.have, a.n, v, turn);
+                v = v * (matrix ? row_at<T, ALIGNED>(ring.piece(ring.at, 2), a.gate, row, at) : vector_at<T>(gate_v));
+            v = fma_of(v, a.scale, row_at<T, ALIGNED>(ring.piece(ring.at, 0), a.x, row, at) * a.residual_scale);
+            put<T>(a.r, row, at, v, turn);
         } else {
-            v = row_at<T, ALIGNED>(ring.piece(ring.at, 0), a.x, row, at.first, at.have);
+            v = row_at<T, ALIGNED>(ring.piece(ring.at, 0), a.x, row, at);
         }
         if (!ALIGNED) __syncwarp();
         load(row + s.stages * at.step, ring.at);
         if (a.pre) {
-            v = normalize<T>(v, at.have, a.pre, a.pre_eps, inv_n, vec + kPreW * vec_step, vec + kPreB * vec_step, a.pre_b, sums,
+            v = normalize<T>(v, at, a.pre, a.pre_eps, inv_n, pre_w, pre_b, a.pre_b, sums,
                              a.pre_stats ? a.pre_stats + row : nullptr, writes);
-            put<T>(a.h, row, at.first, at.have, a.n, v, turn);
+            put<T>(a.h, row, at, v, turn);
         }
     }
     if (s.cluster > 1) cluster_sync();  // no CTA leaves while another still reads its sums
@@ -522,16 +573,19 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
     const Place at(s, a.n);
     const bool matrix = JOIN && a.gate.p && a.gate.ld, has_y = JOIN && a.y.p;
     const int t_dh = a.dr.p ? 1 : 0, t_r = t_dh + 1, t_y = a.pre ? t_r + 1 : t_dh, t_gate = t_y + has_y, tensors = t_gate + matrix;
-    const uint32_t mem = smem_u32(smem), vec = mem + threadIdx.x * 16, vec_step = blockDim.x * 16, turn = mem + s.turn + warp_id() * 512;
-    const uint32_t pre_w = vec, post_w = vec + vec_step, post_b = post_w + vec_step, gate_v = post_b + vec_step;
-    Ring ring(mem + (JOIN ? 4 : 1) * vec_step, tensors, s);
+    const uint32_t mem = smem_u32(smem), vec = mem + warp_id() * 1024, vec_step = blockDim.x * 32, turn = mem + s.turn + warp_id() * 512;
+    uint32_t used = 0;
+    const auto place = [&](const void* v) { return vec + (v ? used++ : 0) * vec_step; };
+    const uint32_t pre_w = place(a.pre_w);
+    const uint32_t post_w = JOIN ? place(a.post_w) : 0, post_b = JOIN ? place(a.post_b) : 0, gate_v = JOIN ? place(matrix ? nullptr : a.gate.p) : 0;
+    Ring ring(mem + used * vec_step, tensors, s);
     RowSums sums = {sets, s.warps, at.group, s.cluster, 0};
     const float inv_n = 1.0f / (float)a.n;
-    const auto of = [&](int t, const Rows& x, int64_t row) { return row_at<T, ALIGNED>(ring.piece(ring.at, t), x, row, at.first, at.have); };
+    const auto of = [&](int t, const Rows& x, int64_t row) { return row_at<T, ALIGNED>(ring.piece(ring.at, t), x, row, at); };
     start_of_inputs();
     const auto load = [&](int64_t row, int stage) {
         if (row < a.tokens) {
-            const auto fetch = [&](int t, const Rows& x) { fetch_row<ALIGNED>(ring.piece(stage, t), x, row, a.tokens, at.first, at.have, a.n); };
+            const auto fetch = [&](int t, const Rows& x) { fetch_row<ALIGNED>(ring.piece(stage, t), x, row, a.tokens, at); };
             if (a.dr.p) fetch(0, a.dr);
             if (a.pre) {
                 fetch(t_dh, a.dh);
@@ -549,15 +603,15 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
         if (JOIN && a.post) post = __ldg(a.post_stats + row);
     };
     for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, i);
-    if (a.pre) fetch_vector(pre_w, a.pre_w, at.first, at.have);
+    if (a.pre) fetch_vector(pre_w, a.pre_w, at);
     if (JOIN) {
-        if (a.post) fetch_vector(post_w, a.post_w, at.first, at.have);
-        if (a.post && a.post_b) fetch_vector(post_b, a.post_b, at.first, at.have);
-        if (a.gate.p && !matrix) fetch_vector(gate_v, a.gate.p, at.first, at.have);
+        if (a.post) fetch_vector(post_w, a.post_w, at);
+        if (a.post && a.post_b) fetch_vector(post_b, a.post_b, at);
+        if (a.gate.p && !matrix) fetch_vector(gate_v, a.gate.p, at);
     }
     constexpr int kTotals = BIAS ? (JOIN ? 4 : 2) : 2;  // without biases sums 0 and 2, without a join 2 and 3
     constexpr int kHat = BIAS && JOIN ? 2 : JOIN ? 1 : 0;
-    Eight total[kTotals];
+    Some total[kTotals];
 #pragma unroll
     for (int k = 0; k < kTotals; ++k) total[k] = zeros();
     float2 pre_next, post_next;
@@ -566,11 +620,11 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
         const float2 pre = pre_next, post = post_next;
         stats_of(row + at.step, pre_next, post_next);
         ring.template wait<ALIGNED>();
-        Eight d;
+        Some d;
         if (a.pre) {
-            Eight g = of(t_dh, a.dh, row);
-            const Eight hat = (of(t_r, a.r, row) + -pre.x) * pre.y;
-            total[kHat] = fma8(g, hat, total[kHat]);
+            Some g = of(t_dh, a.dh, row);
+            const Some hat = (of(t_r, a.r, row) + -pre.x) * pre.y;
+            total[kHat] = fma_of(g, hat, total[kHat]);
             if constexpr (BIAS) total[kHat + 1] = total[kHat + 1] + g;
             g = g * vector_at<T>(pre_w);
             float mg = 0.0f, mgh;
@@ -581,26 +635,26 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
             } else {
                 mgh = sums.one(dot(g, hat)) * inv_n;
             }
-            d = fma8(hat, -mgh, g + -mg) * pre.y;
+            d = fma_of(hat, -mgh, g + -mg) * pre.y;
             if (a.dr.p) d = d + of(0, a.dr, row);
         } else {
             d = of(0, a.dr, row);
         }
-        if (a.dx.p) put<T>(a.dx, row, at.first, at.have, a.n, JOIN ? d * a.residual_scale : d, turn);
+        if (a.dx.p) put<T>(a.dx, row, at, JOIN ? d * a.residual_scale : d, turn);
         if (JOIN) {
             d = d * a.scale;
-            Eight y = zeros();
+            Some y = zeros();
             if (has_y) y = of(t_y, a.y, row);
             if (a.post) y = (y + -post.x) * post.y;
             if (matrix) {
                 if (a.dgate.p) {
-                    Eight p = y;
-                    if (a.post) p = a.post_b ? fma8(y, vector_at<T>(post_w), vector_at<T>(post_b)) : y * vector_at<T>(post_w);
-                    put<T>(a.dgate, row, at.first, at.have, a.n, d * p, turn);
+                    Some p = y;
+                    if (a.post) p = a.post_b ? fma_of(y, vector_at<T>(post_w), vector_at<T>(post_b)) : y * vector_at<T>(post_w);
+                    put<T>(a.dgate, row, at, d * p, turn);
                 }
                 d = d * of(t_gate, a.gate, row);
             }
-            total[0] = fma8(d, y, total[0]);
+            total[0] = fma_of(d, y, total[0]);
             if constexpr (BIAS) total[1] = total[1] + d;
             if (a.gate.p && !matrix) d = d * vector_at<T>(gate_v);
             if (!ALIGNED) __syncwarp();
@@ -615,9 +669,9 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
                 } else {
                     mgh = sums.one(dot(d, y)) * inv_n;
                 }
-                d = fma8(y, -mgh, d + -mg) * post.y;
+                d = fma_of(y, -mgh, d + -mg) * post.y;
             }
-            if (a.dy.p) put<T>(a.dy, row, at.first, at.have, a.n, d, turn);
+            if (a.dy.p) put<T>(a.dy, row, at, d, turn);
         } else {
             if (!ALIGNED) __syncwarp();
             load(row + s.stages * at.step, ring.at);
@@ -625,7 +679,7 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
     }
     // a CTA's sums: those of its groups, joined in shared memory in order
     if (a.part) {
-        float* joined = reinterpret_cast<float*>(smem);  // [groups][8][threads of a group]
+        float* joined = reinterpret_cast<float*>(smem);  // [groups][16][threads of a group]
         const int width = 32 * s.warps, thread = threadIdx.x - at.group * width;
         const int64_t unit = blockIdx.x / s.cluster;
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -635,20 +689,21 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
             if ((!JOIN && k < 2) || (!BIAS && k % 2)) continue;
             if (!(a.sums >> k & 1)) continue;
             constexpr int kSkip = JOIN ? 0 : 2;
-            const Eight& mine = total[BIAS ? k - kSkip : k / 2];
+            const Some& mine = total[BIAS ? k - kSkip : k / 2];
             if (s.groups > 1) {
                 __syncthreads();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) joined[(at.group * 8 + i) * width + thread] = i % 2 ? apart(mine.v[i / 2]).y : apart(mine.v[i / 2]).x;
+                for (int i = 0; i < 2 * kTwos; ++i) joined[(at.group * 2 * kTwos + i) * width + thread] = feature(mine, i);
                 __syncthreads();
             }
             if (at.group == 0) {
                 float* out = a.part + ((int64_t)slot * s.units + unit) * a.n + at.first;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float v = i % 2 ? apart(mine.v[i / 2]).y : apart(mine.v[i / 2]).x;
-                    for (int g = 1; g < s.groups; ++g) v += joined[(g * 8 + i) * width + thread];
-                    if (i < at.have) out[i] = v;
+                for (int i = 0; i < 2 * kTwos; ++i) {
+                    float v = feature(mine, i);
+                    for (int g = 1; g < s.groups; ++g) v += joined[(g * 2 * kTwos + i) * width + thread];
+                    const int j = 256 * (i / 8) + i % 8;
+                    if (j < at.left) out[j] = v;
                 }
             }
             ++slot;
@@ -778,7 +833,7 @@ template <auto KERNEL, typename A>
 static int launch(cudaStream_t st, const A& a, const Shape& s)
 {
     static std::atomic<uint64_t> ready{0};
-    CHPL_TRY(allow_smem(KERNEL, kStageBudget, ready));
+    CHPL_TRY(allow_smem(KERNEL, kSmem - kSmemApart, ready));
     return launch_kernel(KERNEL, (int64_t)s.units * s.cluster, 32 * s.warps * s.groups, s.smem, s.cluster, st, a, s);
 }
 
@@ -815,7 +870,8 @@ static int forward(cudaStream_t st, const chpl_norm_fwd& a)
         f.pre_stats = reinterpret_cast<float2*>(a.pre_stats);
         out = out && f.h.aligned;
     }
-    const Shape s = shape_for(a.tokens, a.n, a.join ? 2 + (a.gate && a.ldgate) : 1, a.join ? kVectors : 2, in, out);
+    const int vectors = (f.pre_w ? 1 : 0) + (f.pre_b ? 1 : 0) + (f.post_w ? 1 : 0) + (f.post_b ? 1 : 0) + (a.join && a.gate && a.ldgate == 0 ? 1 : 0);
+    const Shape s = shape_for(a.tokens, a.n, a.join ? 2 + (a.gate && a.ldgate) : 1, vectors, in, out, 2 * kMaxThreads);
     if (a.join) return in ? launch<forward_kernel<T, true, true>>(st, f, s) : launch<forward_kernel<T, false, true>>(st, f, s);
     return in ? launch<forward_kernel<T, true, false>>(st, f, s) : launch<forward_kernel<T, false, false>>(st, f, s);
 }
@@ -841,9 +897,10 @@ static BackwardPlan plan(const chpl_norm_bwd& a)
            (!has_y || fits(a.y, a.ldy, a.tokens)) && (!matrix || fits(a.gate, a.ldgate, a.tokens));
     p.out = fits(a.dx, a.lddx, a.tokens) && (!a.join || fits(a.dy, a.lddy, a.tokens)) && (!matrix || fits(a.dgate, a.lddgate, a.tokens));
     const int tensors = (a.dr ? 1 : 0) + (a.pre.kind ? 2 : 0) + has_y + matrix;
-    p.shape = shape_for(a.tokens, a.n, tensors, a.join ? 4 : 1, p.in, p.out);
+    const int vectors = (a.pre.kind ? 1 : 0) + (a.join && a.post.kind ? 1 + (a.post.bias ? 1 : 0) : 0) + (a.join && a.gate && a.ldgate == 0 ? 1 : 0);
+    p.shape = shape_for(a.tokens, a.n, tensors, vectors, p.in, p.out, kMaxThreads);
     // the groups' sums are joined where the rows under way were
-    p.shape.smem = std::max(p.shape.smem, p.shape.groups > 1 ? 32 * p.shape.warps * p.shape.groups * 8 * 4 : 0);
+    p.shape.smem = std::max(p.shape.smem, p.shape.groups > 1 ? kWarpWidth * p.shape.warps * p.shape.groups * 4 : 0);
     int count = 0;
     for (int k = 0; k < kSums; ++k) count += p.sums >> k & 1;
     p.bytes = round_up((size_t)count * p.shape.units * a.n * 4, 256);
