@@ -267,7 +267,6 @@ struct CkptIn {
 
 template <typename T>
 struct RowsOut {
-    static constexpr bool kCodes = false;
     T* p;
     int64_t ld;
     bool vec;
@@ -307,7 +306,6 @@ struct RowsOut {
 };
 
 struct CkptOut {
-    static constexpr bool kCodes = true;
     chpl_ckpt8 c;
     bool vec;
     // v and the largest magnitude's bits among them; every lane of a group's four
@@ -399,7 +397,7 @@ struct RowsJob {
                 float v[8];
                 in.value(raw[u], v);
                 f(v);
-                if constexpr (Out::kCodes) out.put(t, j0 + u * 256, cols, v, in.top(raw[u]));
+                if constexpr (std::is_same<Out, CkptOut>::value) out.put(t, j0 + u * 256, cols, v, in.top(raw[u]));
                 else out.put_warp(t, j0 + u * 256, cols, v, turn);
             }
         }

@@ -22,9 +22,9 @@ inline int64_t code_bytes(int64_t cols) { return (cols + kGroup - 1) / kGroup * 
 inline int64_t scale_bytes(int64_t rows, int64_t cols) { return (rows + kBlockRows - 1) / kBlockRows * blocks_of(cols) * kBlockBytes; }
 
 // where row t's groups 4 q .. 4 q + 3 have their scales
-__device__ __forceinline__ int64_t scale_at(int64_t t, int64_t q, int64_t blocks)
+__device__ __forceinline__ int64_t scale_at(uint32_t t, int64_t q, int64_t blocks)
 {
-    return ((t / kBlockRows) * blocks + q) * kBlockBytes + (t % 32) * 16 + (t % kBlockRows) / 32 * 4;
+    return ((int64_t)(t / kBlockRows) * blocks + q) * kBlockBytes + (t % 32) * 16 + (t % kBlockRows) / 32 * 4;
 }
 
 // scale of a group from its largest magnitude's FP32 bits
@@ -41,11 +41,19 @@ __device__ __forceinline__ float step(uint32_t s)
     return s == kBadScale ? __uint_as_float(0x7fffffffu) : s == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(s << 23);
 }
 
-// codes of q[0..7] in nibbles 0..7: rounded to nearest, ties to the even code,
-// magnitudes above 6 to 6
-__device__ __forceinline__ uint32_t codes8(const float* q)
+// codes of v[0..7] times inv in nibbles 0..7: rounded to nearest, ties to the even
+// code, magnitudes above 6 to 6
+__device__ __forceinline__ uint32_t codes8(const float* v, float inv)
 {
     uint32_t w;
+    float q[8];
+    const Two m = both(inv);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float2 p = apart(two(v[i], v[i + 1]) * m);
+        q[i] = p.x;
+        q[i + 1] = p.y;
+    }
     asm("{\n\t.reg .b8 a, b, c, d;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
@@ -92,42 +100,13 @@ struct In {
         Raw r = {0, kMinScale};
         if (j >= cols) return r;
         r.w = __ldg(reinterpret_cast<const uint32_t*>(c.codes + t * c.ldc + j / 2));
-        r.s = c.scales[scale_at(t, j / 128, blocks) + j / kGroup % 4];
+        r.s = c.scales[scale_at((uint32_t)t, j / 128, blocks) + j / kGroup % 4];
         return r;
     }
     __device__ __forceinline__ void value(const Raw& r, float (&v)[8]) const { values8(r.w, step(r.s), v); }
 };
 
-struct Out {
-    static constexpr bool kCodes = true;
-    chpl_mx4 c;
-    int64_t blocks;
-    // every lane of the warp calls it; elements past the row's end are 0
-    __device__ __forceinline__ void put(int64_t t, int j, int cols, const float (&v)[8], uint32_t top) const
-    {
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const uint32_t s = scale_of(top);
-        const float inv = inv_step(s);
-        float q[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = v[i] * inv;
-        uint32_t w = codes8(q);
-        if (s == kBadScale) w = 0;
-        // a block's four scales of this row lie together
-        const int lane = lane_id();
-        uint32_t four = s << (8 * (lane / 4 % 4));
-        four |= __shfl_xor_sync(0xffffffffu, four, 4);
-        four |= __shfl_xor_sync(0xffffffffu, four, 8);
-        const int first = j - lane * 8;
-        if (first >= cols) return;
-        if (j < (cols + kGroup - 1) / kGroup * kGroup) *reinterpret_cast<uint32_t*>(c.codes + t * c.ldc + j / 2) = w;
-        if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(c.scales + scale_at(t, j / 128, blocks)) = four;
-    }
-};
-
 inline In in(const chpl_mx4& c, int64_t cols) { return {c, blocks_of(cols)}; }
-inline Out out(const chpl_mx4& c, int64_t cols) { return {c, blocks_of(cols)}; }
 
 int check_mx4(const char* who, const char* what, const chpl_mx4& c, int64_t rows, int64_t cols);
 int pack(cudaStream_t st, int type, int64_t rows, int64_t cols, const void* x, int64_t ldx, const chpl_mx4& c);

@@ -321,9 +321,18 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
 
 // ----------------------------------------------------------------------------
 // Pair kernel: persistent pairs of CTAs (cta_group::2), one tile of 256 features
-// x bn rows after another, double buffered in TMEM (2 x bn columns and the scales).
-// Each CTA stages its 128 features of W with their scales, half of X's rows, and
-// the scales of all of X's rows, which both CTAs' tensor cores need.
+// x bn rows after another.  Each CTA stages its 128 features of W with their
+// scales, half of X's rows, and the scales of all of X's rows, which both CTAs'
+// tensor cores need.
+//
+// At this rate of products the copies out of L2 bound large tiles, some 11 TB/s
+// over all SMs, so tiles are as wide as an MMA: 256 rows.  Two accumulators of 256
+// columns and the scales do not fit in TMEM's 512 columns; the second one starts
+// at column 192, and a tile's epilogue takes the 64 columns that both share first.
+// The next tile's products start when those have been read (32 arrivals), the
+// other columns are read under them.  A warp that has arrived for a tile has read
+// all it reads of the tile before, whose other columns the next one overwrites.
+// (8192 x 4096 x 16384 with tiles of 192 rows and accumulators apart: 243 us.)
 //
 //   warp 0      TMA producer (both CTAs)
 //   warp 1      TMEM allocation; tcgen05 issue (even CTA)
@@ -334,11 +343,14 @@ constexpr int PAIR_NCB = 2;
 constexpr int PAIR_THREADS = 64 + 32 * PAIR_EPI_WARPS;
 constexpr int ROWS = 8 * PAIR_NCB;                // rows that an epilogue warp takes at a time
 constexpr int ROUND = PAIR_EPI_WARPS / 4 * ROWS;  // rows that all of them do
-constexpr int PAIR_MAX_BN = 192;                  // 2 x 192 columns of sums and 2 x 32 of scales
+constexpr int PAIR_MAX_BN = 256;
+constexpr int ACC_STEP = 192;                     // columns from one accumulator to the next
+constexpr int SCALES_AT = 512 - 2 * SCALE_COLS;   // the second one ends here
+static_assert(ACC_STEP + PAIR_MAX_BN == SCALES_AT && PAIR_MAX_BN - ACC_STEP == ROUND, "TMEM");
 constexpr int PAIR_RING = SMEM_LIMIT - 1024 - PAIR_EPI_WARPS * kStageBytes - 512;
 
 struct PairShape {
-    int bn;              // rows t of a tile: 64, 128 or 192
+    int bn;              // rows t of a tile: 64, 128, 192 or 256
     int mtiles, ntiles;
     int group;           // feature tiles walked before the next row tile
     int stages;
@@ -367,8 +379,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     uint64_t* full = reinterpret_cast<uint64_t*>(stages + PAIR_EPI_WARPS * kStageBytes);
     uint64_t* empty = full + MAX_STAGES;
     uint64_t* acc_full = empty + MAX_STAGES;
-    uint64_t* acc_empty = acc_full + 2;
-    uint64_t* drain = acc_empty + 2;
+    uint64_t* acc_read = acc_full + 2;  // what the next accumulator overwrites
+    uint64_t* drain = acc_read + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -378,7 +390,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     const int total = sh.mtiles * sh.ntiles;
     if (threadIdx.x == 0) {
         for (int s = 0; s < nstages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * PAIR_EPI_WARPS); }
+        for (int b = 0; b < 2; ++b) mbar_init(&acc_full[b], 1);
+        mbar_init(acc_read, 2 * PAIR_EPI_WARPS);
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_barrier_init();
@@ -393,7 +406,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     // barriers of the even CTA, where the MMAs are issued, as shared::cluster addresses
-    const uint32_t lead_full = map_to_rank(smem_u32(full), 0), lead_acc_empty = map_to_rank(smem_u32(acc_empty), 0);
+    const uint32_t lead_full = map_to_rank(smem_u32(full), 0), lead_acc_read = map_to_rank(smem_u32(acc_read), 0);
     start_of_inputs();
 
     if (warp == 0) {
@@ -437,7 +450,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         if (rank == 0 && elect_one()) {
             const uint32_t low = idesc_mxf4(2 * BM, sh.bn, 0), high = idesc_mxf4(2 * BM, sh.bn, 2);
             const uint32_t peer_empty = map_to_rank(smem_u32(empty), 1), peer_acc_full = map_to_rank(smem_u32(acc_full), 1);
-            const uint32_t first = desc_lo(smem_u32(smem)), b_off = (uint32_t)A_BYTES >> 4, scales = tmem + 2 * PAIR_MAX_BN;
+            const uint32_t first = desc_lo(smem_u32(smem)), b_off = (uint32_t)A_BYTES >> 4, scales = tmem + SCALES_AT;
             const uint32_t s_first = smem_u32(smem) + codes;
             int stage = 0;
             uint32_t ph = 0, acc = 0, at = 0, turn = 0;
@@ -446,10 +459,10 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                 int mt, nt;
                 pair_tile(sh, tile, mt, nt);
                 const uint32_t b_shift = (uint32_t)(nt * sh.bn % kBlockRows) / 32;
-                const uint32_t buf = acc & 1u, aph = (acc >> 1) & 1u;
-                if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort_flag)) { ok = false; break; }
+                const uint32_t buf = acc & 1u;
+                if (acc > 0 && !mbar_wait(acc_read, (acc - 1) & 1u, abort_flag)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t d = tmem + buf * PAIR_MAX_BN;
+                const uint32_t d = tmem + buf * ACC_STEP;
                 for (int kb = 0; kb < kblocks; ++kb) {
                     if (!mbar_wait(&full[stage], ph, abort_flag)) { ok = false; break; }
                     tc_fence_after();
@@ -471,9 +484,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                 mma_commit_pair(smem_u32(drain));
                 mbar_wait(drain, 0, &never, 20000000ull);
             } else {
-                // both CTAs' epilogues have released both buffers (their arrivals have landed here)
-                for (int b = 0; b < 2; ++b, ++acc)
-                    if (!mbar_wait(&acc_empty[acc & 1u], ((acc >> 1) & 1u) ^ 1u, abort_flag)) break;
+                // both CTAs' epilogues have arrived for the last tile (the arrivals have landed here)
+                if (acc > 0) mbar_wait(acc_read, (acc - 1) & 1u, abort_flag);
             }
         }
         __syncwarp();
@@ -486,8 +498,15 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         float sums[4] = {};
         int mt, nt;
         pair_tile(sh, unit, mt, nt);
+        // A tile's rounds of 64 rows, the one that lies in both accumulators first: the
+        // first accumulator's from column 192 (if it has them), the second one's from 0.
+        const int rounds = sh.bn / ROUND;
+        const auto rows_of = [&](uint32_t buf, int r) {
+            const int first = buf == 0 && sh.bn > ACC_STEP ? ACC_STEP / ROUND : 0;
+            return (r + first < rounds ? r + first : r + first - rounds) * ROUND + part * ROWS;
+        };
         Fetched<PAIR_NCB> ahead;
-        if (READS) linear::fetch<T, kForward, PAIR_NCB>(e, mt * 2 * BM + f_in, nt * sh.bn + part * ROWS, ahead);
+        if (READS) linear::fetch<T, kForward, PAIR_NCB>(e, mt * 2 * BM + f_in, nt * sh.bn + rows_of(0, 0), ahead);
         for (int tile = unit; tile < total; tile += nunits, ++acc) {
             const int f = mt * 2 * BM + f_in, t0 = nt * sh.bn;
             const uint32_t buf = acc & 1u, aph = (acc >> 1) & 1u;
@@ -496,21 +515,21 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
             Next after = {-1, 0};  // the first rows of the next tile
             if (tile + nunits < total) {
                 pair_tile(sh, tile + nunits, mt, nt);
-                after = {mt * 2 * BM + f_in, nt * sh.bn + part * ROWS};
+                after = {mt * 2 * BM + f_in, nt * sh.bn + rows_of(buf ^ 1u, 0)};
             }
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aph, abort_flag))) break;
             tc_fence_after();
-            for (int c = part * ROWS; c < sh.bn; c += ROUND) {
+            for (int r = 0; r < rounds; ++r) {
+                const int c = rows_of(buf, r);
                 float v[ROWS];
-                linear::tmem_ld_frag<PAIR_NCB>(tmem + lanes + buf * PAIR_MAX_BN + c, v);
-                const bool last = c + ROUND >= sh.bn;
-                if (last) {  // this warp's last columns are in registers
+                linear::tmem_ld_frag<PAIR_NCB>(tmem + lanes + buf * ACC_STEP + c, v);
+                if (r == 0) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) linear::mbar_arrive_peer(lead_acc_empty + buf * 8);
+                    if (lane == 0) linear::mbar_arrive_peer(lead_acc_read);
                 }
-                linear::finish<T, kForward, READS, false, PAIR_NCB>(e, f, t0 + c, v, bias, ahead, last ? after : Next{f, t0 + c + ROUND}, stage,
-                                                                    sums, nullptr);
+                linear::finish<T, kForward, READS, false, PAIR_NCB>(e, f, t0 + c, v, bias, ahead, r + 1 == rounds ? after : Next{f, t0 + rows_of(buf, r + 1)},
+                                                                    stage, sums, nullptr);
             }
         }
     }

@@ -722,7 +722,7 @@ struct Parameters {
     void *dpost_w, *dpost_b, *dgate, *dpre_w, *dpre_b;
 };
 
-constexpr int kJoinWarps = 16;
+constexpr int kJoinWarps = 32;
 
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps) parameters_kernel(const __grid_constant__ Parameters a)
@@ -738,7 +738,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) parameters_kernel(const __gri
         if (!(a.sums >> k & 1)) continue;
         const float* p = a.part + (int64_t)slot++ * a.units * a.n + j;
         if (j < a.n) {
-#pragma unroll 8
+#pragma unroll 16
             for (int u = first; u < last; ++u) sum[k] += p[(int64_t)u * a.n];
         }
         turn[k][warp][lane] = sum[k];
