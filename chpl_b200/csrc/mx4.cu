@@ -102,7 +102,7 @@ int pack(cudaStream_t st, int type, int64_t rows, int64_t cols, const void* x, i
     return pack<float>(st, rows, cols, x, ldx, c);
 }
 
-// the workspace: codes and scales of X, where it comes in 16 bits
+// the workspace: codes and scales of X, where it comes in 16 bits and is coded first
 struct Plan {
     size_t scales = 0, bytes = 0;
 };
@@ -110,7 +110,7 @@ struct Plan {
 static Plan plan(const chpl_mx4_fwd& a)
 {
     Plan p;
-    if (a.x4.codes || a.tokens == 0 || a.n == 0 || a.k == 0) return p;
+    if (a.x4.codes || a.tokens <= kCodedRows || a.n == 0 || a.k == 0) return p;
     p.scales = round_up((size_t)(a.tokens * code_bytes(a.k)), 256);
     p.bytes = p.scales + round_up((size_t)scale_bytes(a.tokens, a.k), 256);
     return p;
@@ -202,5 +202,5 @@ extern "C" int chpl_mx4_linear(void* stream, const chpl_mx4_fwd* a, void* work, 
     e.bias = a->bias;
     e.add = a->residual;
     e.ldadd = a->ldr;
-    return gemm(st, a->type, a->w4, x, a->k, e);
+    return gemm(st, a->type, a->w4, x, x.codes || a->k == 0 ? nullptr : a->x, a->ldx, a->k, e);
 }

@@ -111,8 +111,10 @@ inline In in(const chpl_mx4& c, int64_t cols) { return {c, blocks_of(cols)}; }
 int check_mx4(const char* who, const char* what, const chpl_mx4& c, int64_t rows, int64_t cols);
 int pack(cudaStream_t st, int type, int64_t rows, int64_t cols, const void* x, int64_t ldx, const chpl_mx4& c);
 
-// Y = act(X W^T + b) + R from codes; `type` of b, R and Y
-int gemm(cudaStream_t st, int type, const chpl_mx4& w, const chpl_mx4& x, int64_t k, const linear::Epilogue& e);
+// Y = act(X W^T + b) + R, `type` of b, R and Y.  X comes in codes, or in 16 bits
+// (x16, x.codes NULL), which the product then codes itself: up to kCodedRows rows.
+constexpr int kCodedRows = 8;
+int gemm(cudaStream_t st, int type, const chpl_mx4& w, const chpl_mx4& x, const void* x16, int64_t ldx, int64_t k, const linear::Epilogue& e);
 
 int read_clear_status(int* st);
 

@@ -123,10 +123,18 @@ __device__ __forceinline__ void stage_products(uint32_t d, uint32_t codes_lo, ui
 // each over its share of the contraction, and joins the partial sums through
 // distributed shared memory in rank order, as the linear layers' does.
 //
+// CODES: X comes in 16 bits and every CTA codes its share of it itself, straight
+// into the stages, four rows' 256 features a warp at a time: up to kCodedRows rows
+// that costs less than a launch before (x 4096 x 16384: one token 8.1 us, four 7.9,
+// eight 8.9, twelve 11.1, sixteen 13.4; coded first 10.4 to 12.7).
+//
 //   warp 0     TMA producer          warp 1    TMEM allocation, tcgen05 issue
+//   warps 2-7  CODES: X's codes and scales
 //   warps 0-7  epilogue, once the accumulator is complete
 // ----------------------------------------------------------------------------
 constexpr int SPLIT_THREADS = 256;
+constexpr int CODE_WARPS = SPLIT_THREADS / 32 - 2;
+constexpr int CODE_ROWS = 4;     // that a warp codes at a time
 constexpr int JOIN = 4;          // rows that a warp joins at a time
 constexpr int JOIN_LD = BM + 4;  // row distance of the partial sums: a lane quad's rows in different banks
 
@@ -148,9 +156,10 @@ struct Maps {
     CUtensorMap w, x, sw, sx;  // codes and scales
 };
 
-template <typename T, bool READS>
+template <typename T, bool READS, bool CODES>
 __global__ void __launch_bounds__(SPLIT_THREADS, 2)
-    split_kernel(const __grid_constant__ Maps tm, const int kblocks, const SplitShape sh, const __grid_constant__ Epilogue e)
+    split_kernel(const __grid_constant__ Maps tm, const RowsIn<T> x, const int k, const int kblocks, const SplitShape sh,
+                 const __grid_constant__ Epilogue e)
 {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -168,15 +177,17 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     const int kb0 = (int)((int64_t)kblocks * rank / sh.split), kb1 = (int)((int64_t)kblocks * (rank + 1) / sh.split);
     const uint32_t cols = tmem_cols(sh.bn);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < sh.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < sh.stages; ++s) { mbar_init(&full[s], CODES ? 1 + (e.n + CODE_ROWS - 1) / CODE_ROWS : 1); mbar_init(&empty[s], 1); }
         mbar_init(done, 1);
         *abort_flag = 0;
         fence_barrier_init();
         if (kblocks > 0) {
             tma_prefetch_desc(&tm.w);
-            tma_prefetch_desc(&tm.x);
             tma_prefetch_desc(&tm.sw);
-            tma_prefetch_desc(&tm.sx);
+            if (!CODES) {
+                tma_prefetch_desc(&tm.x);
+                tma_prefetch_desc(&tm.sx);
+            }
         }
     }
     if (warp == 1) { tmem_alloc(tmem_slot, cols); tmem_relinquish(); }
@@ -201,11 +212,13 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
                     }
                     break;
                 }
-                mbar_arrive_expect_tx(&full[stage], sbytes);
+                mbar_arrive_expect_tx(&full[stage], CODES ? A_BYTES + SCALE_BYTES : sbytes);
                 tma_load_2d(sa, &tm.w, &full[stage], kb * ROW_BYTES, f0);
-                tma_load_2d(sa + A_BYTES, &tm.x, &full[stage], kb * ROW_BYTES, t0);
                 tma_load_2d(sa + codes, &tm.sw, &full[stage], kb * (SCALE_BYTES / 4), f0 / kBlockRows);
-                tma_load_2d(sa + codes + SCALE_BYTES, &tm.sx, &full[stage], kb * (SCALE_BYTES / 4), t0 / kBlockRows);
+                if (!CODES) {
+                    tma_load_2d(sa + A_BYTES, &tm.x, &full[stage], kb * ROW_BYTES, t0);
+                    tma_load_2d(sa + codes + SCALE_BYTES, &tm.sx, &full[stage], kb * (SCALE_BYTES / 4), t0 / kBlockRows);
+                }
                 ++started;
                 sa += sbytes;
                 if (++stage == sh.stages) { stage = 0; ph ^= 1u; sa = smem; }
@@ -232,6 +245,55 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
             mma_commit(done);
         }
         __syncwarp();
+    } else if (CODES) {
+        // units of CODE_ROWS rows in one stage, dealt out to the warps in order; the next
+        // unit's rows are read while one is coded
+        using Raw = typename RowsIn<T>::Raw;
+        const int parts = (e.n + CODE_ROWS - 1) / CODE_ROWS, units = (kb1 - kb0) * parts;
+        Raw next[CODE_ROWS];
+        const auto fetch = [&](int unit) {
+            if (unit >= units) return;
+            const int turn = unit / parts, row = (unit - turn * parts) * CODE_ROWS;
+#pragma unroll
+            for (int i = 0; i < CODE_ROWS; ++i)
+                if (row + i < e.n) next[i] = x.raw(row + i, (kb0 + turn) * kPiece + lane * 8, k);
+        };
+        int unit = warp - 2;
+        fetch(unit);
+        for (; unit < units; unit += CODE_WARPS) {
+            const int turn = unit / parts, row = (unit - turn * parts) * CODE_ROWS, stage = turn % sh.stages;
+            Raw raw[CODE_ROWS];
+            uint32_t w[CODE_ROWS], s[CODE_ROWS];
+#pragma unroll
+            for (int i = 0; i < CODE_ROWS; ++i) raw[i] = next[i];
+            fetch(unit + CODE_WARPS);
+#pragma unroll
+            for (int i = 0; i < CODE_ROWS; ++i) {
+                s[i] = x.top(raw[i]);
+                s[i] = max(s[i], __shfl_xor_sync(0xffffffffu, s[i], 1));
+                s[i] = scale_of(max(s[i], __shfl_xor_sync(0xffffffffu, s[i], 2)));
+                float v[8];
+                x.value(raw[i], v);
+                w[i] = codes8(v, inv_step(s[i]));
+                if (s[i] == kBadScale) w[i] = 0;
+            }
+            if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], (uint32_t)(turn / sh.stages & 1) ^ 1u, abort_flag))) break;
+            const uint32_t at = smem_u32(smem) + stage * sbytes;
+#pragma unroll
+            for (int i = 0; i < CODE_ROWS; ++i) {
+                if (row + i >= e.n) break;
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + A_BYTES + (row + i) * ROW_BYTES + (((lane >> 2) ^ (row + i & 7)) << 4) + (lane & 3) * 4),
+                             "r"(w[i])
+                             : "memory");
+                if ((lane & 3) == 0)
+                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(at + codes + SCALE_BYTES + (lane >> 4) * kBlockBytes + (row + i) * 16 + (lane >> 2 & 3)),
+                                 "r"(s[i])
+                                 : "memory");
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[stage]);
+        }
     }
     // One CTA per tile: a warp takes its TMEM quarter's features and every other
     // 16 rows.  Several: the rows are dealt out to the warps of the cluster.
@@ -562,15 +624,17 @@ static int make_tmap(CUtensorMap* tm, CUtensorMapDataType type, int elt, const v
     return CHPL_OK;
 }
 
+// x.codes NULL: X has no maps
 static int make_maps(Maps* tm, const chpl_mx4& w, const chpl_mx4& x, int m, int n, int64_t k, int x_box, int x_blocks)
 {
     const int64_t width = code_bytes(k), scales = blocks_of(k) * kBlockBytes;
     // one row has no distance
     const int64_t ldw = m > 1 ? w.ldc : width, ldx = n > 1 ? x.ldc : width;
     CHPL_TRY(make_tmap(&tm->w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w.codes, width, m, ldw, ROW_BYTES, BM, CU_TENSOR_MAP_SWIZZLE_128B));
-    CHPL_TRY(make_tmap(&tm->x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x.codes, width, n, ldx, ROW_BYTES, x_box, CU_TENSOR_MAP_SWIZZLE_128B));
     CHPL_TRY(make_tmap(&tm->sw, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, w.scales, scales, (m + kBlockRows - 1) / kBlockRows, scales, SCALE_BYTES, 1,
                        CU_TENSOR_MAP_SWIZZLE_NONE));
+    if (!x.codes) return CHPL_OK;
+    CHPL_TRY(make_tmap(&tm->x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x.codes, width, n, ldx, ROW_BYTES, x_box, CU_TENSOR_MAP_SWIZZLE_128B));
     return make_tmap(&tm->sx, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, x.scales, scales, (n + kBlockRows - 1) / kBlockRows, scales, SCALE_BYTES, x_blocks,
                      CU_TENSOR_MAP_SWIZZLE_NONE);
 }
@@ -622,15 +686,26 @@ static Plan plan_for(int m, int n, int kblocks)
             best.tiles.bn = bn;
             best.tiles.mtiles = (int)mt;
             best.tiles.ntiles = (int)nt;
-            best.tiles.group = std::max(8, std::min(16, 1024 / kblocks));
+            best.tiles.group = 16;
             best.tiles.stages = std::min(MAX_STAGES, PAIR_RING / pair_bytes(bn));
         }
     }
     return best;
 }
 
+template <typename T, bool READS, bool CODES>
+static int launch_split(cudaStream_t st, const Maps& tm, const RowsIn<T>& x, int64_t k, int kblocks, const SplitShape& s, const Epilogue& e)
+{
+    const int64_t ctas = (int64_t)((e.m + BM - 1) / BM) * ((e.n + s.bn - 1) / s.bn) * s.split;
+    if (ctas > 0x7fffffff) { set_error("mx4_linear: an output of %d x %d is more than one launch serves", e.n, e.m); return CHPL_ERR_UNSUPPORTED; }
+    static std::atomic<uint64_t> ready{0};
+    CHPL_TRY(allow_smem(split_kernel<T, READS, CODES>, SMEM_LIMIT, ready));
+    return launch_kernel(split_kernel<T, READS, CODES>, ctas, SPLIT_THREADS, 1024 + s.stages * split_bytes(s.bn) + 512, s.split, st, tm, x, (int)k,
+                         kblocks, s, e);
+}
+
 template <typename T, bool READS>
-static int launch(cudaStream_t st, const chpl_mx4& w, const chpl_mx4& x, int64_t k, const Epilogue& e)
+static int launch(cudaStream_t st, const chpl_mx4& w, const chpl_mx4& x, const void* x16, int64_t ldx, int64_t k, const Epilogue& e)
 {
     const int kblocks = (int)((k + kPiece - 1) / kPiece);
     const Plan p = plan_for(e.m, e.n, kblocks);
@@ -645,22 +720,18 @@ static int launch(cudaStream_t st, const chpl_mx4& w, const chpl_mx4& x, int64_t
         return launch_kernel(pair_kernel<T, READS>, 2 * units, PAIR_THREADS, 1024 + s.stages * pair_bytes(s.bn) + PAIR_EPI_WARPS * kStageBytes + 512, 2,
                              st, tm, kblocks, s, e);
     }
-    const SplitShape& s = p.split;
-    const int64_t ctas = (int64_t)((e.m + BM - 1) / BM) * ((e.n + s.bn - 1) / s.bn) * s.split;
-    if (ctas > 0x7fffffff) { set_error("mx4_linear: an output of %d x %d is more than one launch serves", e.n, e.m); return CHPL_ERR_UNSUPPORTED; }
-    if (kblocks > 0) CHPL_TRY(make_maps(&tm, w, x, e.m, e.n, k, s.bn, row_blocks(s.bn)));
-    static std::atomic<uint64_t> ready{0};
-    CHPL_TRY(allow_smem(split_kernel<T, READS>, SMEM_LIMIT, ready));
-    return launch_kernel(split_kernel<T, READS>, ctas, SPLIT_THREADS, 1024 + s.stages * split_bytes(s.bn) + 512, s.split, st, tm, kblocks, s, e);
+    if (kblocks > 0) CHPL_TRY(make_maps(&tm, w, x, e.m, e.n, k, p.split.bn, row_blocks(p.split.bn)));
+    const RowsIn<T> rows = rows_in<T>(x16, ldx);
+    return x16 ? launch_split<T, READS, true>(st, tm, rows, k, kblocks, p.split, e) : launch_split<T, READS, false>(st, tm, rows, k, kblocks, p.split, e);
 }
 
-int gemm(cudaStream_t st, int type, const chpl_mx4& w, const chpl_mx4& x, int64_t k, const Epilogue& e0)
+int gemm(cudaStream_t st, int type, const chpl_mx4& w, const chpl_mx4& x, const void* x16, int64_t ldx, int64_t k, const Epilogue& e0)
 {
     Epilogue e = e0;
     e.vec_out = aligned(e.out, e.ldo * 2, 16);
     e.vec_add = aligned(e.add, e.ldadd * 2, 16);
-    if (type == CHPL_TYPE_BF16) return e.add ? launch<__nv_bfloat16, true>(st, w, x, k, e) : launch<__nv_bfloat16, false>(st, w, x, k, e);
-    return e.add ? launch<__half, true>(st, w, x, k, e) : launch<__half, false>(st, w, x, k, e);
+    if (type == CHPL_TYPE_BF16) return e.add ? launch<__nv_bfloat16, true>(st, w, x, x16, ldx, k, e) : launch<__nv_bfloat16, false>(st, w, x, x16, ldx, k, e);
+    return e.add ? launch<__half, true>(st, w, x, x16, ldx, k, e) : launch<__half, false>(st, w, x, x16, ldx, k, e);
 }
 
 int read_clear_status(int* st)
