@@ -156,16 +156,15 @@ __device__ __forceinline__ float feature(const Some& a, int i) { return i % 2 ? 
 struct Place {
     int first, left;
     int group;
-    int64_t row, step;
+    uint32_t row, step;  // rows and steps past the last row stay far below 2^32
     __device__ __forceinline__ Place(const Shape& s, int n)
     {
         const int warp = warp_id(), rank = s.cluster > 1 ? (int)cluster_ctarank() : 0;
         group = warp / s.warps;
         first = (rank * s.warps + warp - group * s.warps) * kWarpWidth + lane_id() * 8;
         left = n - first;
-        const int64_t unit = blockIdx.x / s.cluster;
-        row = unit * s.groups + group;
-        step = (int64_t)s.units * s.groups;
+        row = blockIdx.x / (uint32_t)s.cluster * s.groups + group;
+        step = (uint32_t)(s.units * s.groups);
     }
     __device__ __forceinline__ int have(int h) const { return min(8, max(0, left - 256 * h)); }
     __device__ __forceinline__ bool whole() const { return left >= 256 * (kHalves - 1) + 8; }
@@ -232,13 +231,13 @@ __device__ __forceinline__ void fetch_vector(uint32_t piece, const void* v, cons
 struct Rows {
     const void* p;
     int64_t ld;
-    __device__ __forceinline__ const unsigned short* row(int64_t t) const { return static_cast<const unsigned short*>(p) + t * ld; }
+    __device__ __forceinline__ const unsigned short* row(uint32_t t) const { return static_cast<const unsigned short*>(p) + (uint64_t)ld * t; }
 };
 struct RowsTo {
     void* p;
     int64_t ld;
     bool aligned;  // 16-byte stores fit
-    __device__ __forceinline__ unsigned short* row(int64_t t) const { return static_cast<unsigned short*>(p) + t * ld; }
+    __device__ __forceinline__ unsigned short* row(uint32_t t) const { return static_cast<unsigned short*>(p) + (uint64_t)ld * t; }
 };
 
 __device__ __forceinline__ void copy16(uint32_t slot, const void* src, int bytes)
@@ -252,15 +251,20 @@ __device__ __forceinline__ void copy16(uint32_t slot, const void* src, int bytes
 // (or the rows' beside it); the chunks that reach out of the tensor, in its first
 // and last row, are read by the element.
 template <bool ALIGNED>
-__device__ __forceinline__ void fetch_row(uint32_t piece, const Rows& x, int64_t t, int64_t tokens, const Place& at)
+__device__ __forceinline__ void fetch_row(uint32_t piece, const Rows& x, uint32_t t, uint32_t tokens, const Place& at)
 {
     const int lane = lane_id();
     const unsigned short* row = x.row(t);
     if (ALIGNED) {
+        if (at.whole()) {
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-            const int have = at.have(h);
-            copy16(piece + h * 512 + lane * 16, row + (have > 0 ? at.first + 256 * h : 0), 2 * have);
+            for (int h = 0; h < kHalves; ++h) copy16(piece + h * 512 + lane * 16, row + at.first + 256 * h, 16);
+        } else {
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+                const int have = at.have(h);
+                copy16(piece + h * 512 + lane * 16, row + (have > 0 ? at.first + 256 * h : 0), 2 * have);
+            }
         }
         return;
     }
@@ -286,7 +290,7 @@ __device__ __forceinline__ void fetch_row(uint32_t piece, const Rows& x, int64_t
 
 // the thread's features of that row; zero past its end
 template <typename T, bool ALIGNED>
-__device__ __forceinline__ Some row_at(uint32_t piece, const Rows& x, int64_t t, const Place& at)
+__device__ __forceinline__ Some row_at(uint32_t piece, const Rows& x, uint32_t t, const Place& at)
 {
     if (ALIGNED) return vector_at<T>(piece);
     Some r;
@@ -313,7 +317,7 @@ __device__ __forceinline__ Some row_at(uint32_t piece, const Rows& x, int64_t t,
 // the thread's features into a row; rows that 16-byte stores do not fit go by way
 // of `turn`, 512 bytes of the warp's own, so that a store covers 32 features in a row
 template <typename T>
-__device__ __forceinline__ void put(const RowsTo& out, int64_t t, const Place& at, const Some& v, uint32_t turn)
+__device__ __forceinline__ void put(const RowsTo& out, uint32_t t, const Place& at, const Some& v, uint32_t turn)
 {
     unsigned short* const row = out.row(t) + at.first;
     const int lane = lane_id();
@@ -328,7 +332,7 @@ __device__ __forceinline__ void put(const RowsTo& out, int64_t t, const Place& a
         unsigned short* p = row + 256 * h;
         const int left = at.left - 256 * h;
         if (out.aligned) {
-            if (left >= 8) {
+            if (at.whole() || left >= 8) {
                 *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
             } else {
 #pragma unroll
@@ -367,85 +371,111 @@ __device__ __forceinline__ float warp_sum(float a)
 // same calls before.  Warps' sums go through shared memory, two sets of them in
 // turn: who writes a set again has passed the barrier that all readers of its last
 // use reached afterwards.
-struct RowSums {
-    float2 (*sets)[kMaxWarps];  // [2][warps of the CTA]
-    int warps, group, cluster, turn;
+struct WarpSums {
+    float2 of[2][kMaxWarps + 1];  // the last one stays zero
+};
 
+struct RowSums {
+    uint32_t mine, from;  // where the warp puts its sums, and where a lane reads one (or the zero)
+    int warps, group, cluster;
+    uint32_t turn;        // from one set to the other
+
+    __device__ __forceinline__ RowSums(WarpSums& sets, const Shape& s, int of_group) : warps(s.warps), group(of_group), cluster(s.cluster), turn(sizeof(sets.of[0]))
+    {
+        const int lane = lane_id();
+        mine = smem_u32(&sets.of[0][warp_id()]);
+        from = smem_u32(&sets.of[0][lane < warps ? group * warps + lane : kMaxWarps]);
+        if (threadIdx.x < 2) sets.of[threadIdx.x][kMaxWarps] = make_float2(0.0f, 0.0f);
+        __syncthreads();
+    }
+    // the sets of both uses follow one another
+    __device__ __forceinline__ void swap()
+    {
+        mine += turn;
+        from += turn;
+        turn = 0u - turn;
+    }
     __device__ __forceinline__ void meet() const
     {
         if (cluster > 1) cluster_sync();
         else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * warps) : "memory");
     }
-    __device__ __forceinline__ float2 of_lane(const float2* set) const
-    {
-        const int lane = lane_id();
-        float2 sum = make_float2(0.0f, 0.0f);
-        if (lane >= warps) return sum;
-        if (cluster == 1) return set[group * warps + lane];
-        for (int r = 0; r < cluster; ++r) {
-            float2 v;
-            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(map_to_rank(smem_u32(set + lane), (uint32_t)r)) : "memory");
-            sum.x += v.x;
-            sum.y += v.y;
-        }
-        return sum;
-    }
     __device__ __forceinline__ float one(float a)
     {
         a = warp_sum(a);
-        if (warps == 1) return a;
-        float2* set = sets[turn];
-        turn ^= 1;
-        if (lane_id() == 0) set[warp_id()] = make_float2(a, 0.0f);
+        if (warps == 1 && cluster == 1) return a;
+        if (lane_id() == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine), "f"(a) : "memory");
         meet();
-        return warp_sum(of_lane(set).x);
+        a = 0.0f;
+        if (cluster == 1) {
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(from) : "memory");
+        } else {
+            for (int r = 0; r < cluster; ++r) {
+                float v;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(from, (uint32_t)r)) : "memory");
+                a += v;
+            }
+        }
+        swap();
+        return warp_sum(a);
     }
     __device__ __forceinline__ float2 both_of(float a, float b)
     {
         a = warp_sum(a);
         b = warp_sum(b);
-        if (warps == 1) return make_float2(a, b);
-        float2* set = sets[turn];
-        turn ^= 1;
-        if (lane_id() == 0) set[warp_id()] = make_float2(a, b);
+        if (warps == 1 && cluster == 1) return make_float2(a, b);
+        if (lane_id() == 0) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(mine), "f"(a), "f"(b) : "memory");
         meet();
-        const float2 v = of_lane(set);
-        return make_float2(warp_sum(v.x), warp_sum(v.y));
+        a = b = 0.0f;
+        if (cluster == 1) {
+            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(a), "=f"(b) : "r"(from) : "memory");
+        } else {
+            for (int r = 0; r < cluster; ++r) {
+                float2 v;
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(map_to_rank(from, (uint32_t)r)) : "memory");
+                a += v.x;
+                b += v.y;
+            }
+        }
+        swap();
+        return make_float2(warp_sum(a), warp_sum(b));
     }
 };
 
 // The rows under way: copies of the rows to come, a group of cp.async each,
 // `stages` of them (an empty group where there is no such row).
 struct Ring {
-    uint32_t base;  // of the warp
-    uint32_t tensor, stage_bytes;
-    int stages, at;
+    uint32_t tensor, bytes, end;  // between tensors, of a stage, behind the last one
+    uint32_t at;                  // the warp's piece of the current row's first tensor
+    int stages;
     __device__ __forceinline__ Ring(uint32_t mem, int tensors, const Shape& s)
-        : base(mem + warp_id() * s.piece), tensor((blockDim.x >> 5) * s.piece), stage_bytes((uint32_t)tensors * tensor), stages(s.stages), at(0)
+        : tensor((blockDim.x >> 5) * s.piece), bytes(tensors * tensor), end(mem + warp_id() * s.piece + s.stages * bytes), at(mem + warp_id() * s.piece),
+          stages(s.stages)
     {
     }
-    __device__ __forceinline__ uint32_t piece(int stage, int t) const { return base + stage * stage_bytes + t * tensor; }
     __device__ __forceinline__ static void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
     // the oldest of `stages` groups has arrived, the whole warp's where a lane reads others' copies
     template <bool ALIGNED>
     __device__ __forceinline__ void wait() const
     {
-        switch (stages) {
-            case 1: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-            case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-            case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-            default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-        }
+        if (stages == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+        else if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+        else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_group 0;" ::: "memory");
         if (!ALIGNED) __syncwarp();
     }
-    __device__ __forceinline__ void next() { at = at + 1 == stages ? 0 : at + 1; }
+    __device__ __forceinline__ void next()
+    {
+        at += bytes;
+        if (at == end) at -= stages * bytes;
+    }
 };
 
 // ----------------------------------------------------------------------------
 // forward
 // ----------------------------------------------------------------------------
 struct Forward {
-    int64_t tokens;
+    uint32_t tokens;
     int n;
     float scale, residual_scale, post_eps, pre_eps;
     int post, pre;          // kinds
@@ -478,7 +508,7 @@ template <typename T, bool ALIGNED, bool JOIN>
 __global__ void __launch_bounds__(kMaxThreads, 2) forward_kernel(const __grid_constant__ Forward a, const Shape s)
 {
     extern __shared__ uint4 smem[];
-    __shared__ float2 sets[2][kMaxWarps];
+    __shared__ WarpSums sets;
     const Place at(s, a.n);
     const bool matrix = JOIN && a.gate.p && a.gate.ld;
     const int tensors = JOIN ? 2 + matrix : 1;
@@ -489,18 +519,18 @@ __global__ void __launch_bounds__(kMaxThreads, 2) forward_kernel(const __grid_co
     const uint32_t pre_w = place(a.pre_w), pre_b = place(a.pre_b);
     const uint32_t post_w = JOIN ? place(a.post_w) : 0, post_b = JOIN ? place(a.post_b) : 0, gate_v = JOIN ? place(matrix ? nullptr : a.gate.p) : 0;
     Ring ring(mem + used * vec_step, tensors, s);
-    RowSums sums = {sets, s.warps, at.group, s.cluster, 0};
+    RowSums sums(sets, s, at.group);
     const float inv_n = 1.0f / (float)a.n;
     start_of_inputs();
-    const auto load = [&](int64_t row, int stage) {
+    const auto load = [&](uint32_t row, uint32_t slot) {
         if (row < a.tokens) {
-            fetch_row<ALIGNED>(ring.piece(stage, 0), a.x, row, a.tokens, at);
-            if (JOIN) fetch_row<ALIGNED>(ring.piece(stage, 1), a.y, row, a.tokens, at);
-            if (JOIN && matrix) fetch_row<ALIGNED>(ring.piece(stage, 2), a.gate, row, a.tokens, at);
+            fetch_row<ALIGNED>(slot + 0 * ring.tensor, a.x, row, a.tokens, at);
+            if (JOIN) fetch_row<ALIGNED>(slot + 1 * ring.tensor, a.y, row, a.tokens, at);
+            if (JOIN && matrix) fetch_row<ALIGNED>(slot + 2 * ring.tensor, a.gate, row, a.tokens, at);
         }
         Ring::commit();
     };
-    for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, i);
+    for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, ring.at + i * ring.bytes);
     if (a.pre) {
         fetch_vector(pre_w, a.pre_w, at);
         if (a.pre_b) fetch_vector(pre_b, a.pre_b, at);
@@ -513,20 +543,20 @@ __global__ void __launch_bounds__(kMaxThreads, 2) forward_kernel(const __grid_co
         if (a.gate.p && !matrix) fetch_vector(gate_v, a.gate.p, at);
     }
     const bool writes = at.first == 0;  // the row's statistics
-    for (int64_t row = at.row; row < a.tokens; row += at.step, ring.next()) {
+    for (uint32_t row = at.row; row < a.tokens; row += at.step, ring.next()) {
         ring.template wait<ALIGNED>();
         Some v;
         if (JOIN) {
-            v = row_at<T, ALIGNED>(ring.piece(ring.at, 1), a.y, row, at);
+            v = row_at<T, ALIGNED>(ring.at + 1 * ring.tensor, a.y, row, at);
             if (a.post)
                 v = normalize<T>(v, at, a.post, a.post_eps, inv_n, post_w, post_b, a.post_b, sums,
                                  a.post_stats ? a.post_stats + row : nullptr, writes);
             if (a.gate.p)
-                v = v * (matrix ? row_at<T, ALIGNED>(ring.piece(ring.at, 2), a.gate, row, at) : vector_at<T>(gate_v));
-            v = fma_of(v, a.scale, row_at<T, ALIGNED>(ring.piece(ring.at, 0), a.x, row, at) * a.residual_scale);
+                v = v * (matrix ? row_at<T, ALIGNED>(ring.at + 2 * ring.tensor, a.gate, row, at) : vector_at<T>(gate_v));
+            v = fma_of(v, a.scale, row_at<T, ALIGNED>(ring.at + 0 * ring.tensor, a.x, row, at) * a.residual_scale);
             put<T>(a.r, row, at, v, turn);
         } else {
-            v = row_at<T, ALIGNED>(ring.piece(ring.at, 0), a.x, row, at);
+            v = row_at<T, ALIGNED>(ring.at + 0 * ring.tensor, a.x, row, at);
         }
         if (!ALIGNED) __syncwarp();
         load(row + s.stages * at.step, ring.at);
@@ -543,7 +573,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) forward_kernel(const __grid_co
 // backward
 // ----------------------------------------------------------------------------
 struct Backward {
-    int64_t tokens;
+    uint32_t tokens;
     int n;
     float scale, residual_scale;
     int post, pre;
@@ -569,7 +599,7 @@ template <typename T, bool ALIGNED, bool JOIN, bool BIAS>
 __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_constant__ Backward a, const Shape s)
 {
     extern __shared__ uint4 smem[];
-    __shared__ float2 sets[2][kMaxWarps];
+    __shared__ WarpSums sets;
     const Place at(s, a.n);
     const bool matrix = JOIN && a.gate.p && a.gate.ld, has_y = JOIN && a.y.p;
     const int t_dh = a.dr.p ? 1 : 0, t_r = t_dh + 1, t_y = a.pre ? t_r + 1 : t_dh, t_gate = t_y + has_y, tensors = t_gate + matrix;
@@ -579,13 +609,13 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
     const uint32_t pre_w = place(a.pre_w);
     const uint32_t post_w = JOIN ? place(a.post_w) : 0, post_b = JOIN ? place(a.post_b) : 0, gate_v = JOIN ? place(matrix ? nullptr : a.gate.p) : 0;
     Ring ring(mem + used * vec_step, tensors, s);
-    RowSums sums = {sets, s.warps, at.group, s.cluster, 0};
+    RowSums sums(sets, s, at.group);
     const float inv_n = 1.0f / (float)a.n;
-    const auto of = [&](int t, const Rows& x, int64_t row) { return row_at<T, ALIGNED>(ring.piece(ring.at, t), x, row, at); };
+    const auto of = [&](int t, const Rows& x, uint32_t row) { return row_at<T, ALIGNED>(ring.at + t * ring.tensor, x, row, at); };
     start_of_inputs();
-    const auto load = [&](int64_t row, int stage) {
+    const auto load = [&](uint32_t row, uint32_t slot) {
         if (row < a.tokens) {
-            const auto fetch = [&](int t, const Rows& x) { fetch_row<ALIGNED>(ring.piece(stage, t), x, row, a.tokens, at); };
+            const auto fetch = [&](int t, const Rows& x) { fetch_row<ALIGNED>(slot + t * ring.tensor, x, row, a.tokens, at); };
             if (a.dr.p) fetch(0, a.dr);
             if (a.pre) {
                 fetch(t_dh, a.dh);
@@ -596,13 +626,13 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
         }
         Ring::commit();
     };
-    const auto stats_of = [&](int64_t row, float2& pre, float2& post) {
+    const auto stats_of = [&](uint32_t row, float2& pre, float2& post) {
         pre = post = make_float2(0.0f, 1.0f);
         if (row >= a.tokens) return;
         if (a.pre) pre = __ldg(a.pre_stats + row);
         if (JOIN && a.post) post = __ldg(a.post_stats + row);
     };
-    for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, i);
+    for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, ring.at + i * ring.bytes);
     if (a.pre) fetch_vector(pre_w, a.pre_w, at);
     if (JOIN) {
         if (a.post) fetch_vector(post_w, a.post_w, at);
@@ -616,7 +646,7 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
     for (int k = 0; k < kTotals; ++k) total[k] = zeros();
     float2 pre_next, post_next;
     stats_of(at.row, pre_next, post_next);
-    for (int64_t row = at.row; row < a.tokens; row += at.step, ring.next()) {
+    for (uint32_t row = at.row; row < a.tokens; row += at.step, ring.next()) {
         const float2 pre = pre_next, post = post_next;
         stats_of(row + at.step, pre_next, post_next);
         ring.template wait<ALIGNED>();
@@ -841,7 +871,7 @@ template <typename T>
 static int forward(cudaStream_t st, const chpl_norm_fwd& a)
 {
     Forward f = {};
-    f.tokens = a.tokens;
+    f.tokens = (uint32_t)a.tokens;
     f.n = (int)a.n;
     f.scale = a.scale;
     f.residual_scale = a.residual_scale;
@@ -961,7 +991,7 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
     const bool matrix = a.join && a.gate && a.ldgate;
     if (a.tokens > 0) {
         Backward b = {};
-        b.tokens = a.tokens;
+        b.tokens = (uint32_t)a.tokens;
         b.n = (int)a.n;
         b.scale = a.scale;
         b.residual_scale = a.residual_scale;
