@@ -26,6 +26,9 @@ int cuda_fail(cudaError_t e, const char* what, const char* file, int line)
 }
 
 int hpl_read_clear_status(int* st);
+namespace norm {
+int read_clear_status(int* st);
+}
 
 }  // namespace chpl
 
@@ -36,12 +39,13 @@ extern "C" const char* chpl_version(void) { return "chpl_b200 0.1 (sm_100a)"; }
 extern "C" int chpl_device_status(int* status)
 {
     CHPL_CUDA(cudaDeviceSynchronize());
-    int a = 0, b = 0, c = 0, d = 0;
+    int a = 0, b = 0, c = 0, d = 0, e = 0;
     CHPL_TRY(chpl::oz2::read_clear_status(&a));
     CHPL_TRY(chpl::hpl_read_clear_status(&b));
     CHPL_TRY(chpl::linear::read_clear_status(&c));
     CHPL_TRY(chpl::mx4::read_clear_status(&d));
-    if (status) *status = a ? a : b ? b : c ? c : d;
+    CHPL_TRY(chpl::norm::read_clear_status(&e));
+    if (status) *status = a ? a : b ? b : c ? c : d ? d : e;
     return CHPL_OK;
 }
 

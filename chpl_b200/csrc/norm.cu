@@ -24,11 +24,16 @@ using linear::check_size;
 
 constexpr int kHalves = 2;                          // eights of a thread's features, 256 apart
 constexpr int kWarpWidth = 256 * kHalves;
-constexpr int kMaxThreads = 512;
-constexpr int kMaxWidth = 2 * 8 * kHalves * kMaxThreads;  // a cluster of two
+constexpr int kForwardThreads = 1024;               // of a CTA, one to an SM: 64 registers each
+constexpr int kBackwardThreads = 512;               // 128
+constexpr int kMaxWarps = kForwardThreads / 32;
+constexpr int kMaxWidth = kForwardThreads * 8 * kHalves;
+constexpr int kMaxCluster = 4;
+constexpr int kClusterGroups = 4;                   // of a CTA in a cluster
 constexpr int kMaxStages = 4;
-constexpr int kSmem = 227 * 1024;               // of an SM
-constexpr int kSmemApart = 1536;                // of which a CTA takes, beside what it asks for
+constexpr int kVectorBytes = 1024 * kHalves;         // of a warp's features as FP32
+constexpr int kSmem = 227 * 1024;                   // of an SM
+constexpr int kSmemApart = 2304;                    // of which a CTA takes, beside what it asks for
 
 // ----------------------------------------------------------------------------
 // shape of a launch
@@ -39,31 +44,53 @@ struct Shape {
     int cluster;  // CTAs that share a row
     int stages;   // rows of each group that are under way or in use
     int units;    // clusters launched
-    int piece;    // shared memory of a warp's 256 features
+    int piece;    // shared memory of a warp's features
     int turn;     // offset of the memory that unaligned rows are turned about in
     int smem;
 };
 
-// A row's warps are a power of two up to four (several rows to a CTA of four
-// warps), then as many as it needs.  `on_sm`: threads that an SM has registers for.
-static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors, bool inputs_aligned, bool outputs_aligned, int on_sm)
+// One CTA to an SM, of as many groups of warps as its registers hold, each with a
+// row of its own: they share the weights in shared memory, and one computes while
+// another waits for its row's sums.  A cluster of two or four CTAs shares a row
+// where that keeps clearly more of the GPU's threads at work (or where a row and
+// the weights do not fit into one CTA's shared memory): gradients of a join with two
+// norms, 13107 x 5120, 223 us alone (one group of ten warps an SM), 192 in clusters of
+// two (three groups of five warps); 8192 x 8192 189 and 192; 5461 x 12288 228 in
+// clusters of two, 245 of four.
+static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors, bool inputs_aligned, bool outputs_aligned, int threads)
 {
-    Shape s;
-    s.cluster = n > kWarpWidth * (kMaxThreads / 32) ? 2 : 1;
-    const int need = (int)((n + kWarpWidth * s.cluster - 1) / (kWarpWidth * s.cluster));
-    s.warps = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : need;
-    s.groups = s.warps <= 4 ? 4 / s.warps : 1;
+    constexpr int kSms = 148, kNamed = 15;  // named barriers, one to a group of several warps
+    Shape s, best = {};
+    double most = 0.0;
+    int row = 0, fixed = 0, turn = 0;
+    const auto sizes = [&] {
+        row = std::max(1, tensors) * s.warps * s.piece;
+        fixed = vectors * s.warps * kVectorBytes;
+        turn = outputs_aligned ? 0 : s.warps * 512;
+    };
     s.piece = inputs_aligned ? 1024 : 1056;
-    const int warps = s.warps * s.groups, row = std::max(1, tensors) * warps * s.piece;
-    const int fixed = vectors * warps * 1024 + (outputs_aligned ? 0 : warps * 512);
-    // fewer CTAs on an SM rather than one row under way
-    int resident = on_sm / (32 * warps);
-    while (resident > 1 && (kSmem / resident - kSmemApart - fixed) / row < 2) --resident;
-    s.stages = std::max(1, std::min(kMaxStages, (kSmem / resident - kSmemApart - fixed) / row));
-    s.turn = vectors * warps * 1024 + s.stages * row;
-    s.smem = fixed + s.stages * row;
+    for (s.cluster = 1; s.cluster <= kMaxCluster; s.cluster *= 2) {
+        s.warps = (int)((n + kWarpWidth * s.cluster - 1) / (kWarpWidth * s.cluster));
+        s.groups = threads / 32 / s.warps;
+        if (s.warps > 1) s.groups = std::min(s.groups, s.cluster > 1 ? kClusterGroups : kNamed);
+        sizes();
+        if (s.groups == 0 || fixed + turn + row > kSmem - kSmemApart) continue;
+        const double work = (double)s.groups * n / s.cluster * linear::slots(s.cluster, 1, kSms);
+        if (work <= 1.1 * most) continue;
+        most = work;
+        best = s;
+    }
+    s = best;
+    sizes();
+    s.groups = (int)std::max<int64_t>(1, std::min<int64_t>(s.groups, (tokens + kSms - 1) / kSms));
+    // fewer groups rather than one row under way
+    const auto stages = [&] { return (kSmem - kSmemApart - fixed - s.groups * turn) / (s.groups * row); };
+    while (s.groups > 1 && stages() < 2) --s.groups;
+    s.stages = std::max(1, std::min(kMaxStages, stages()));
+    s.turn = fixed + s.groups * s.stages * row;
+    s.smem = s.turn + s.groups * turn;
     const int64_t want = (tokens + s.groups - 1) / s.groups;
-    s.units = (int)std::min<int64_t>(want, 148 / s.cluster * resident);
+    s.units = (int)std::min<int64_t>(want, linear::slots(s.cluster, 1, kSms) / s.cluster);
     return s;
 }
 
@@ -193,7 +220,7 @@ __device__ __forceinline__ void expand(const uint32_t (&w)[4], int h, Some& r)
 
 // features of a warp's 1024 bytes of shared memory in order, the lane's own
 template <typename T>
-__device__ __forceinline__ Some vector_at(uint32_t piece)
+__device__ __forceinline__ Some packed_at(uint32_t piece)
 {
     Some r;
 #pragma unroll
@@ -205,27 +232,49 @@ __device__ __forceinline__ Some vector_at(uint32_t piece)
     return r;
 }
 
-// the thread's features of a vector into its own bytes there, zero past the end
-__device__ __forceinline__ void fetch_vector(uint32_t piece, const void* v, const Place& at)
+// Eight features of a vector from the thread's (h-th) first on, zero past the end;
+// all ones where there is no vector
+template <typename T>
+__device__ __forceinline__ void eight_of(const void* v, const Place& at, int h, float (&f)[8])
+{
+    const T* p = static_cast<const T*>(v) + at.first + 256 * h;
+    const int have = at.have(h);
+    if (v && have == 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+        const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = to_f32(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < have ? (v ? to_f32(p[i]) : 1.0f) : 0.0f;
+    }
+}
+
+// A vector, times another (exact in FP32) and a factor, as FP32 in the warp's 2048
+// bytes of shared memory, the lane's own: a row then costs neither conversions nor
+// the products.
+template <typename T>
+__device__ __forceinline__ void put_vector(uint32_t piece, const void* u, const void* v, float factor, const Place& at)
 {
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
-        const unsigned short* p = static_cast<const unsigned short*>(v) + at.first + 256 * h;
-        const int have = at.have(h);
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (have == 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-            const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-            w[0] = q.x;
-            w[1] = q.y;
-            w[2] = q.z;
-            w[3] = q.w;
-        } else {
+        float f[8], g[8];
+        eight_of<T>(u, at, h, f);
+        eight_of<T>(v, at, h, g);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < have) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
-        }
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece + h * 512 + lane_id() * 16), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        for (int i = 0; i < 8; i += 4)
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(piece + h * 1024 + i * 128 + lane_id() * 16), "f"(f[i] * g[i] * factor),
+                         "f"(f[i + 1] * g[i + 1] * factor), "f"(f[i + 2] * g[i + 2] * factor), "f"(f[i + 3] * g[i + 3] * factor)
+                         : "memory");
     }
+}
+__device__ __forceinline__ Some vector_at(uint32_t piece)
+{
+    Some r;
+#pragma unroll
+    for (int i = 0; i < kTwos; i += 2)
+        asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(r.v[i].v), "=l"(r.v[i + 1].v) : "r"(piece + i * 256 + lane_id() * 16) : "memory");
+    return r;
 }
 
 struct Rows {
@@ -292,7 +341,7 @@ __device__ __forceinline__ void fetch_row(uint32_t piece, const Rows& x, uint32_
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ Some row_at(uint32_t piece, const Rows& x, uint32_t t, const Place& at)
 {
-    if (ALIGNED) return vector_at<T>(piece);
+    if (ALIGNED) return packed_at<T>(piece);
     Some r;
     const int lane = lane_id();
     const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(x.row(t) + (at.first - lane * 8)) & 15u;  // bytes before the first feature
@@ -358,8 +407,6 @@ __device__ __forceinline__ void put(const RowsTo& out, uint32_t t, const Place& 
 // ----------------------------------------------------------------------------
 // sums over a row
 // ----------------------------------------------------------------------------
-constexpr int kMaxWarps = kMaxThreads / 32;
-
 __device__ __forceinline__ float warp_sum(float a)
 {
 #pragma unroll
@@ -367,78 +414,88 @@ __device__ __forceinline__ float warp_sum(float a)
     return a;
 }
 
-// Sums over the row of a group (of a cluster); every thread of it calls with the
-// same calls before.  Warps' sums go through shared memory, two sets of them in
-// turn: who writes a set again has passed the barrier that all readers of its last
-// use reached afterwards.
+// Sums over the row of a group; every thread of it calls with the same calls
+// before.  Warps' sums go through shared memory, two sets of them in turn: who
+// writes a set again has passed the barrier that all readers of its last use
+// reached afterwards.  Where a cluster shares the row every warp sends its sums to
+// all CTAs of it, and arrives there on the group's own barrier: groups do not wait
+// for one another.
 struct WarpSums {
-    float2 of[2][kMaxWarps + 1];  // the last one stays zero
+    float2 of[2][kClusterGroups][kMaxWarps + 1];  // the last one stays zero
+    uint64_t bar[2][kClusterGroups];
+    int gave_up;
 };
+
+__device__ int g_status;  // sticky device-side error of this module
+
+// eight bytes to a CTA of the cluster, counted on its barrier.  (A release at
+// cluster scope beside plain stores would wait for the rows' stores under way: a
+// row of 16384 features took 1.7 times as long.)
+__device__ __forceinline__ void send(uint32_t to, uint32_t bar, float a, float b)
+{
+    const Two v = two(a, b);
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to), "l"(v.v), "r"(bar) : "memory");
+}
 
 struct RowSums {
     uint32_t mine, from;  // where the warp puts its sums, and where a lane reads one (or the zero)
+    uint64_t* bar;        // of the group
+    bool leads;           // its first warp
     int warps, group, cluster;
-    uint32_t turn;        // from one set to the other
+    uint32_t set, phase;  // of the next use; the barriers' parity
+    volatile int* gave_up;
 
-    __device__ __forceinline__ RowSums(WarpSums& sets, const Shape& s, int of_group) : warps(s.warps), group(of_group), cluster(s.cluster), turn(sizeof(sets.of[0]))
+    __device__ __forceinline__ RowSums(WarpSums& sets, const Shape& s, int of_group)
+        : warps(s.warps), group(of_group), cluster(s.cluster), set(0), phase(0), gave_up(&sets.gave_up)
     {
-        const int lane = lane_id();
-        mine = smem_u32(&sets.of[0][warp_id()]);
-        from = smem_u32(&sets.of[0][lane < warps ? group * warps + lane : kMaxWarps]);
-        if (threadIdx.x < 2) sets.of[threadIdx.x][kMaxWarps] = make_float2(0.0f, 0.0f);
-        __syncthreads();
-    }
-    // the sets of both uses follow one another
-    __device__ __forceinline__ void swap()
-    {
-        mine += turn;
-        from += turn;
-        turn = 0u - turn;
-    }
-    __device__ __forceinline__ void meet() const
-    {
+        const int lane = lane_id(), warp = warp_id() - group * warps;
+        const int row = cluster > 1 ? group : 0, first = cluster > 1 ? (int)cluster_ctarank() * warps : group * warps;
+        mine = smem_u32(&sets.of[0][row][first + warp]);
+        from = smem_u32(&sets.of[0][row][lane < cluster * warps ? (cluster > 1 ? 0 : first) + lane : kMaxWarps]);
+        bar = &sets.bar[0][row];
+        leads = warp == 0;
+        if (threadIdx.x < 2 * kClusterGroups) {
+            sets.of[threadIdx.x / kClusterGroups][threadIdx.x % kClusterGroups][kMaxWarps] = make_float2(0.0f, 0.0f);
+            mbar_init(&sets.bar[threadIdx.x / kClusterGroups][threadIdx.x % kClusterGroups], 1);
+        }
+        if (threadIdx.x == 0) {
+            sets.gave_up = 0;
+            fence_barrier_init();
+        }
         if (cluster > 1) cluster_sync();
-        else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * warps) : "memory");
+        else __syncthreads();
+    }
+    __device__ __forceinline__ float2 exchange(float a, float b)
+    {
+        const uint32_t other = set ? (uint32_t)sizeof(WarpSums::of[0]) : 0u;
+        if (cluster == 1) {
+            if (lane_id() == 0) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(mine + other), "f"(a), "f"(b) : "memory");
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * warps) : "memory");
+        } else {
+            uint64_t* at = bar + set * kClusterGroups;
+            if (leads && lane_id() == 0) mbar_arrive_expect_tx(at, cluster * warps * 8);
+            if (lane_id() < cluster) send(map_to_rank(mine + other, lane_id()), map_to_rank(smem_u32(at), lane_id()), a, b);
+            if (!mbar_wait(at, phase, gave_up)) atomicExch(&g_status, CHPL_ERR_TIMEOUT);
+            __syncwarp();
+            phase ^= set;
+        }
+        float2 v;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(from + other) : "memory");
+        set ^= 1u;
+        return v;
     }
     __device__ __forceinline__ float one(float a)
     {
         a = warp_sum(a);
-        if (warps == 1 && cluster == 1) return a;
-        if (lane_id() == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine), "f"(a) : "memory");
-        meet();
-        a = 0.0f;
-        if (cluster == 1) {
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(from) : "memory");
-        } else {
-            for (int r = 0; r < cluster; ++r) {
-                float v;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(from, (uint32_t)r)) : "memory");
-                a += v;
-            }
-        }
-        swap();
-        return warp_sum(a);
+        return warps * cluster == 1 ? a : warp_sum(exchange(a, 0.0f).x);
     }
     __device__ __forceinline__ float2 both_of(float a, float b)
     {
         a = warp_sum(a);
         b = warp_sum(b);
-        if (warps == 1 && cluster == 1) return make_float2(a, b);
-        if (lane_id() == 0) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(mine), "f"(a), "f"(b) : "memory");
-        meet();
-        a = b = 0.0f;
-        if (cluster == 1) {
-            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(a), "=f"(b) : "r"(from) : "memory");
-        } else {
-            for (int r = 0; r < cluster; ++r) {
-                float2 v;
-                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(map_to_rank(from, (uint32_t)r)) : "memory");
-                a += v.x;
-                b += v.y;
-            }
-        }
-        swap();
-        return make_float2(warp_sum(a), warp_sum(b));
+        if (warps * cluster == 1) return make_float2(a, b);
+        const float2 v = exchange(a, b);
+        return make_float2(warp_sum(v.x), warp_sum(v.y));
     }
 };
 
@@ -485,12 +542,11 @@ struct Forward {
     float2 *post_stats, *pre_stats;
 };
 
-// the norm of v; (mean, 1 / deviation) to *stats.  Mean first, then the squares of
-// what is left: the one pass of squares loses the variance of rows whose mean is
-// large.
-template <typename T>
+// (v - mean) / deviation, w v + b of it; (mean, 1 / deviation) to *stats.  Mean
+// first, then the squares of what is left: the one pass of squares loses the
+// variance of rows whose mean is large.
 __device__ __forceinline__ Some normalize(Some v, const Place& at, int kind, float eps, float inv_n, uint32_t w, uint32_t b, bool has_b,
-                                           RowSums& sums, float2* stats, bool writes)
+                                          RowSums& sums, float2* stats, bool writes)
 {
     float mean = 0.0f;
     if (kind == CHPL_NORM_LAYER) {
@@ -501,23 +557,24 @@ __device__ __forceinline__ Some normalize(Some v, const Place& at, int kind, flo
     const float rstd = rsqrtf(fmaf(sums.one(dot(v, v)), inv_n, eps));
     if (stats && writes) *stats = make_float2(mean, rstd);
     v = v * rstd;
-    return has_b ? fma_of(v, vector_at<T>(w), vector_at<T>(b)) : v * vector_at<T>(w);
+    return has_b ? fma_of(v, vector_at(w), vector_at(b)) : v * vector_at(w);
 }
 
 template <typename T, bool ALIGNED, bool JOIN>
-__global__ void __launch_bounds__(kMaxThreads, 2) forward_kernel(const __grid_constant__ Forward a, const Shape s)
+__global__ void __launch_bounds__(kForwardThreads) forward_kernel(const __grid_constant__ Forward a, const Shape s)
 {
     extern __shared__ uint4 smem[];
     __shared__ WarpSums sets;
     const Place at(s, a.n);
     const bool matrix = JOIN && a.gate.p && a.gate.ld;
     const int tensors = JOIN ? 2 + matrix : 1;
-    const uint32_t mem = smem_u32(smem), vec = mem + warp_id() * 1024, vec_step = blockDim.x * 32, turn = mem + s.turn + warp_id() * 512;
-    // the vectors that there are, then the rows
+    const uint32_t mem = smem_u32(smem), vec = mem + (warp_id() - at.group * s.warps) * kVectorBytes, vec_step = s.warps * kVectorBytes,
+                   turn = mem + s.turn + warp_id() * 512;
+    // the vectors that there are, then the rows; a vector gate and the scale are in post_w and post_b
     uint32_t used = 0;
-    const auto place = [&](const void* v) { return vec + (v ? used++ : 0) * vec_step; };
-    const uint32_t pre_w = place(a.pre_w), pre_b = place(a.pre_b);
-    const uint32_t post_w = JOIN ? place(a.post_w) : 0, post_b = JOIN ? place(a.post_b) : 0, gate_v = JOIN ? place(matrix ? nullptr : a.gate.p) : 0;
+    const auto place = [&](bool there) { return vec + (there ? used++ : 0) * vec_step; };
+    const bool weighs = JOIN && (a.post || (a.gate.p && !matrix));
+    const uint32_t pre_w = place(a.pre), pre_b = place(a.pre_b), post_w = JOIN ? place(weighs) : 0, post_b = JOIN ? place(a.post_b) : 0;
     Ring ring(mem + used * vec_step, tensors, s);
     RowSums sums(sets, s, at.group);
     const float inv_n = 1.0f / (float)a.n;
@@ -531,17 +588,13 @@ __global__ void __launch_bounds__(kMaxThreads, 2) forward_kernel(const __grid_co
         Ring::commit();
     };
     for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, ring.at + i * ring.bytes);
-    if (a.pre) {
-        fetch_vector(pre_w, a.pre_w, at);
-        if (a.pre_b) fetch_vector(pre_b, a.pre_b, at);
+    if (at.group == 0) {  // the groups' in common
+        if (a.pre) put_vector<T>(pre_w, a.pre_w, nullptr, 1.0f, at);
+        if (a.pre_b) put_vector<T>(pre_b, a.pre_b, nullptr, 1.0f, at);
+        if (JOIN && weighs) put_vector<T>(post_w, a.post_w, matrix ? nullptr : a.gate.p, a.scale, at);
+        if (JOIN && a.post_b) put_vector<T>(post_b, a.post_b, matrix ? nullptr : a.gate.p, a.scale, at);
     }
-    if (JOIN) {
-        if (a.post) {
-            fetch_vector(post_w, a.post_w, at);
-            if (a.post_b) fetch_vector(post_b, a.post_b, at);
-        }
-        if (a.gate.p && !matrix) fetch_vector(gate_v, a.gate.p, at);
-    }
+    __syncthreads();
     const bool writes = at.first == 0;  // the row's statistics
     for (uint32_t row = at.row; row < a.tokens; row += at.step, ring.next()) {
         ring.template wait<ALIGNED>();
@@ -549,11 +602,11 @@ __global__ void __launch_bounds__(kMaxThreads, 2) forward_kernel(const __grid_co
         if (JOIN) {
             v = row_at<T, ALIGNED>(ring.at + 1 * ring.tensor, a.y, row, at);
             if (a.post)
-                v = normalize<T>(v, at, a.post, a.post_eps, inv_n, post_w, post_b, a.post_b, sums,
-                                 a.post_stats ? a.post_stats + row : nullptr, writes);
-            if (a.gate.p)
-                v = v * (matrix ? row_at<T, ALIGNED>(ring.at + 2 * ring.tensor, a.gate, row, at) : vector_at<T>(gate_v));
-            v = fma_of(v, a.scale, row_at<T, ALIGNED>(ring.at + 0 * ring.tensor, a.x, row, at) * a.residual_scale);
+                v = normalize(v, at, a.post, a.post_eps, inv_n, post_w, post_b, a.post_b, sums, a.post_stats ? a.post_stats + row : nullptr, writes);
+            else
+                v = weighs ? v * vector_at(post_w) : v * a.scale;
+            if (matrix) v = v * row_at<T, ALIGNED>(ring.at + 2 * ring.tensor, a.gate, row, at);
+            v = fma_of(row_at<T, ALIGNED>(ring.at + 0 * ring.tensor, a.x, row, at), a.residual_scale, v);
             put<T>(a.r, row, at, v, turn);
         } else {
             v = row_at<T, ALIGNED>(ring.at + 0 * ring.tensor, a.x, row, at);
@@ -561,8 +614,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) forward_kernel(const __grid_co
         if (!ALIGNED) __syncwarp();
         load(row + s.stages * at.step, ring.at);
         if (a.pre) {
-            v = normalize<T>(v, at, a.pre, a.pre_eps, inv_n, pre_w, pre_b, a.pre_b, sums,
-                             a.pre_stats ? a.pre_stats + row : nullptr, writes);
+            v = normalize(v, at, a.pre, a.pre_eps, inv_n, pre_w, pre_b, a.pre_b, sums, a.pre_stats ? a.pre_stats + row : nullptr, writes);
             put<T>(a.h, row, at, v, turn);
         }
     }
@@ -593,21 +645,33 @@ struct Backward {
 //   3  dh        db_pre
 constexpr int kSums = 4;
 
-// Rows' tails, which the copies leave zero, need no masks here: every sum over
-// the row has a factor of a zero vector or of a zero row.
+// With c = v - m the gradient of a norm at v is s (g - mean(g) - c s^2 mean(g c)),
+// g = d weight: g s, mean(g s) and mean(g s c) are formed, which takes one product
+// an element less than the normed value would.  Rows' tails, which the copies leave
+// zero, need no masks: every sum over the row has a factor of a zero weight.
+struct Pull {
+    float mean, along;  // what is taken off: mean + along c
+};
+__device__ __forceinline__ Pull pull(const Some& g, const Some& c, int kind, float s, float inv_n, RowSums& sums)
+{
+    if (kind != CHPL_NORM_LAYER) return {0.0f, sums.one(dot(g, c)) * inv_n * s * s};
+    const float2 t = sums.both_of(total_of(g), dot(g, c));
+    return {t.x * inv_n, t.y * inv_n * s * s};
+}
+
 template <typename T, bool ALIGNED, bool JOIN, bool BIAS>
-__global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_constant__ Backward a, const Shape s)
+__global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid_constant__ Backward a, const Shape s)
 {
     extern __shared__ uint4 smem[];
     __shared__ WarpSums sets;
     const Place at(s, a.n);
-    const bool matrix = JOIN && a.gate.p && a.gate.ld, has_y = JOIN && a.y.p;
+    const bool matrix = JOIN && a.gate.p && a.gate.ld, has_y = JOIN && a.y.p, weighs = JOIN && (a.post || (a.gate.p && !matrix));
     const int t_dh = a.dr.p ? 1 : 0, t_r = t_dh + 1, t_y = a.pre ? t_r + 1 : t_dh, t_gate = t_y + has_y, tensors = t_gate + matrix;
-    const uint32_t mem = smem_u32(smem), vec = mem + warp_id() * 1024, vec_step = blockDim.x * 32, turn = mem + s.turn + warp_id() * 512;
-    uint32_t used = 0;
-    const auto place = [&](const void* v) { return vec + (v ? used++ : 0) * vec_step; };
-    const uint32_t pre_w = place(a.pre_w);
-    const uint32_t post_w = JOIN ? place(a.post_w) : 0, post_b = JOIN ? place(a.post_b) : 0, gate_v = JOIN ? place(matrix ? nullptr : a.gate.p) : 0;
+    const uint32_t mem = smem_u32(smem), vec = mem + (warp_id() - at.group * s.warps) * kVectorBytes, vec_step = s.warps * kVectorBytes,
+                   turn = mem + s.turn + warp_id() * 512;
+    uint32_t used = 0;  // a vector gate is in post_w
+    const auto place = [&](bool there) { return vec + (there ? used++ : 0) * vec_step; };
+    const uint32_t pre_w = place(a.pre), post_w = JOIN ? place(weighs) : 0, post_b = JOIN ? place(matrix && a.post_b) : 0;
     Ring ring(mem + used * vec_step, tensors, s);
     RowSums sums(sets, s, at.group);
     const float inv_n = 1.0f / (float)a.n;
@@ -633,14 +697,14 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
         if (JOIN && a.post) post = __ldg(a.post_stats + row);
     };
     for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, ring.at + i * ring.bytes);
-    if (a.pre) fetch_vector(pre_w, a.pre_w, at);
-    if (JOIN) {
-        if (a.post) fetch_vector(post_w, a.post_w, at);
-        if (a.post && a.post_b) fetch_vector(post_b, a.post_b, at);
-        if (a.gate.p && !matrix) fetch_vector(gate_v, a.gate.p, at);
+    if (at.group == 0) {  // the groups' in common
+        if (a.pre) put_vector<T>(pre_w, a.pre_w, nullptr, 1.0f, at);
+        if (JOIN && weighs) put_vector<T>(post_w, a.post_w, matrix ? nullptr : a.gate.p, 1.0f, at);
+        if (JOIN && matrix && a.post_b) put_vector<T>(post_b, a.post_b, nullptr, 1.0f, at);
     }
-    constexpr int kTotals = BIAS ? (JOIN ? 4 : 2) : 2;  // without biases sums 0 and 2, without a join 2 and 3
-    constexpr int kHat = BIAS && JOIN ? 2 : JOIN ? 1 : 0;
+    __syncthreads();
+    constexpr int kTotals = (BIAS ? 2 : 1) * (JOIN ? 2 : 1);  // without a join sums 2 and 3, without biases 0 and 2
+    constexpr int kHat = JOIN ? (BIAS ? 2 : 1) : 0;
     Some total[kTotals];
 #pragma unroll
     for (int k = 0; k < kTotals; ++k) total[k] = zeros();
@@ -652,54 +716,44 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
         ring.template wait<ALIGNED>();
         Some d;
         if (a.pre) {
-            Some g = of(t_dh, a.dh, row);
-            const Some hat = (of(t_r, a.r, row) + -pre.x) * pre.y;
-            total[kHat] = fma_of(g, hat, total[kHat]);
+            Some c = of(t_r, a.r, row), g = of(t_dh, a.dh, row);
             if constexpr (BIAS) total[kHat + 1] = total[kHat + 1] + g;
-            g = g * vector_at<T>(pre_w);
-            float mg = 0.0f, mgh;
-            if (a.pre == CHPL_NORM_LAYER) {
-                const float2 m = sums.both_of(total_of(g), dot(g, hat));
-                mg = m.x * inv_n;
-                mgh = m.y * inv_n;
-            } else {
-                mgh = sums.one(dot(g, hat)) * inv_n;
-            }
-            d = fma_of(hat, -mgh, g + -mg) * pre.y;
+            if (a.pre == CHPL_NORM_LAYER) c = c + -pre.x;
+            g = g * pre.y;
+            total[kHat] = fma_of(g, c, total[kHat]);
+            g = g * vector_at(pre_w);
+            const Pull p = pull(g, c, a.pre, pre.y, inv_n, sums);
+            d = fma_of(c, -p.along, g);
+            if (a.pre == CHPL_NORM_LAYER) d = d + -p.mean;
             if (a.dr.p) d = d + of(0, a.dr, row);
         } else {
             d = of(0, a.dr, row);
         }
         if (a.dx.p) put<T>(a.dx, row, at, JOIN ? d * a.residual_scale : d, turn);
         if (JOIN) {
-            d = d * a.scale;
             Some y = zeros();
             if (has_y) y = of(t_y, a.y, row);
-            if (a.post) y = (y + -post.x) * post.y;
+            if (a.post == CHPL_NORM_LAYER) y = y + -post.x;
+            // Do, times 1 / deviation of y
+            if (BIAS) d = d * a.scale;
             if (matrix) {
                 if (a.dgate.p) {
-                    Some p = y;
-                    if (a.post) p = a.post_b ? fma_of(y, vector_at<T>(post_w), vector_at<T>(post_b)) : y * vector_at<T>(post_w);
-                    put<T>(a.dgate, row, at, d * p, turn);
+                    Some p = y * post.y;
+                    if (a.post) p = a.post_b ? fma_of(p, vector_at(post_w), vector_at(post_b)) : p * vector_at(post_w);
+                    put<T>(a.dgate, row, at, (BIAS ? d : d * a.scale) * p, turn);
                 }
                 d = d * of(t_gate, a.gate, row);
             }
-            total[0] = fma_of(d, y, total[0]);
             if constexpr (BIAS) total[1] = total[1] + d;
-            if (a.gate.p && !matrix) d = d * vector_at<T>(gate_v);
+            d = d * (BIAS ? post.y : post.y * a.scale);
+            total[0] = fma_of(d, y, total[0]);
+            if (weighs) d = d * vector_at(post_w);
             if (!ALIGNED) __syncwarp();
             load(row + s.stages * at.step, ring.at);
             if (a.post) {
-                d = d * vector_at<T>(post_w);
-                float mg = 0.0f, mgh;
-                if (a.post == CHPL_NORM_LAYER) {
-                    const float2 m = sums.both_of(total_of(d), dot(d, y));
-                    mg = m.x * inv_n;
-                    mgh = m.y * inv_n;
-                } else {
-                    mgh = sums.one(dot(d, y)) * inv_n;
-                }
-                d = fma_of(y, -mgh, d + -mg) * post.y;
+                const Pull p = pull(d, y, a.post, post.y, inv_n, sums);
+                d = fma_of(y, -p.along, d);
+                if (a.post == CHPL_NORM_LAYER) d = d + -p.mean;
             }
             if (a.dy.p) put<T>(a.dy, row, at, d, turn);
         } else {
@@ -718,8 +772,7 @@ __global__ void __launch_bounds__(kMaxThreads) backward_kernel(const __grid_cons
         for (int k = 0; k < kSums; ++k) {
             if ((!JOIN && k < 2) || (!BIAS && k % 2)) continue;
             if (!(a.sums >> k & 1)) continue;
-            constexpr int kSkip = JOIN ? 0 : 2;
-            const Some& mine = total[BIAS ? k - kSkip : k / 2];
+            const Some& mine = total[BIAS ? k - (JOIN ? 0 : 2) : JOIN ? k / 2 : 0];
             if (s.groups > 1) {
                 __syncthreads();
 #pragma unroll
@@ -900,8 +953,8 @@ static int forward(cudaStream_t st, const chpl_norm_fwd& a)
         f.pre_stats = reinterpret_cast<float2*>(a.pre_stats);
         out = out && f.h.aligned;
     }
-    const int vectors = (f.pre_w ? 1 : 0) + (f.pre_b ? 1 : 0) + (f.post_w ? 1 : 0) + (f.post_b ? 1 : 0) + (a.join && a.gate && a.ldgate == 0 ? 1 : 0);
-    const Shape s = shape_for(a.tokens, a.n, a.join ? 2 + (a.gate && a.ldgate) : 1, vectors, in, out, 2 * kMaxThreads);
+    const int vectors = (f.pre_w ? 1 : 0) + (f.pre_b ? 1 : 0) + (a.join && (f.post || (a.gate && a.ldgate == 0)) ? 1 : 0) + (f.post_b ? 1 : 0);
+    const Shape s = shape_for(a.tokens, a.n, a.join ? 2 + (a.gate && a.ldgate) : 1, vectors, in, out, kForwardThreads);
     if (a.join) return in ? launch<forward_kernel<T, true, true>>(st, f, s) : launch<forward_kernel<T, false, true>>(st, f, s);
     return in ? launch<forward_kernel<T, true, false>>(st, f, s) : launch<forward_kernel<T, false, false>>(st, f, s);
 }
@@ -927,8 +980,8 @@ static BackwardPlan plan(const chpl_norm_bwd& a)
            (!has_y || fits(a.y, a.ldy, a.tokens)) && (!matrix || fits(a.gate, a.ldgate, a.tokens));
     p.out = fits(a.dx, a.lddx, a.tokens) && (!a.join || fits(a.dy, a.lddy, a.tokens)) && (!matrix || fits(a.dgate, a.lddgate, a.tokens));
     const int tensors = (a.dr ? 1 : 0) + (a.pre.kind ? 2 : 0) + has_y + matrix;
-    const int vectors = (a.pre.kind ? 1 : 0) + (a.join && a.post.kind ? 1 + (a.post.bias ? 1 : 0) : 0) + (a.join && a.gate && a.ldgate == 0 ? 1 : 0);
-    p.shape = shape_for(a.tokens, a.n, tensors, vectors, p.in, p.out, kMaxThreads);
+    const int vectors = (a.pre.kind ? 1 : 0) + (a.join && (a.post.kind || (a.gate && a.ldgate == 0)) ? 1 : 0) + (matrix && a.post.kind && a.post.bias ? 1 : 0);
+    p.shape = shape_for(a.tokens, a.n, tensors, vectors, p.in, p.out, kBackwardThreads);
     // the groups' sums are joined where the rows under way were
     p.shape.smem = std::max(p.shape.smem, p.shape.groups > 1 ? kWarpWidth * p.shape.warps * p.shape.groups * 4 : 0);
     int count = 0;
@@ -1019,7 +1072,8 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
             }
         }
         const bool bias = (p.sums & 10) != 0;
-        if (!a.join) CHPL_TRY((p.in ? launch<backward_kernel<T, true, false, true>>(st, b, p.shape) : launch<backward_kernel<T, false, false, true>>(st, b, p.shape)));
+        if (!a.join && bias) CHPL_TRY((p.in ? launch<backward_kernel<T, true, false, true>>(st, b, p.shape) : launch<backward_kernel<T, false, false, true>>(st, b, p.shape)));
+        else if (!a.join) CHPL_TRY((p.in ? launch<backward_kernel<T, true, false, false>>(st, b, p.shape) : launch<backward_kernel<T, false, false, false>>(st, b, p.shape)));
         else if (bias) CHPL_TRY((p.in ? launch<backward_kernel<T, true, true, true>>(st, b, p.shape) : launch<backward_kernel<T, false, true, true>>(st, b, p.shape)));
         else CHPL_TRY((p.in ? launch<backward_kernel<T, true, true, false>>(st, b, p.shape) : launch<backward_kernel<T, false, true, false>>(st, b, p.shape)));
     }
@@ -1047,6 +1101,15 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
         q.dpre_b = a.dpre_bias;
     }
     return launch_kernel(parameters_kernel<T>, (a.n + 31) / 32, 32 * kJoinWarps, 0, 1, st, q);
+}
+
+int read_clear_status(int* st)
+{
+    int v = 0, z = 0;
+    CHPL_CUDA(cudaMemcpyFromSymbol(&v, g_status, sizeof(int)));
+    CHPL_CUDA(cudaMemcpyToSymbol(g_status, &z, sizeof(int)));
+    *st = v;
+    return CHPL_OK;
 }
 
 }  // namespace norm
