@@ -89,7 +89,7 @@ def _torch_ext_command(src: str) -> list[str]:
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE] + inc + [
             src, "-o", TORCH_EXT, "-L", HERE, "-lchpl", "-Wl,-rpath,$ORIGIN", "-L", libs, "-ltorch_python", "-ltorch", "-ltorch_cpu",
-            "-lc10", "-lc10_cuda", "-Wl,-rpath," + libs]
+            "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath," + libs]
 
 
 def _build_torch_ext(force: bool, verbose: bool, hdrs: list[str]) -> None:

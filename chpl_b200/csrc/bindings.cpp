@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -97,11 +98,9 @@ struct Call {
         if (device.index() != c10::cuda::current_device()) guard.set_device(device);
     }
     void* stream() const { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
-    at::Tensor empty(int64_t rows, int64_t cols, at::ScalarType t) const
-    {
-        return at::empty({rows, cols}, at::TensorOptions().dtype(t).device(device));
-    }
-    at::Tensor empty(int64_t n, at::ScalarType t) const { return at::empty({n}, at::TensorOptions().dtype(t).device(device)); }
+    // (past the dispatcher, which costs more than the allocation)
+    at::Tensor empty(int64_t rows, int64_t cols, at::ScalarType t) const { return at::detail::empty_cuda({rows, cols}, t, device, c10::nullopt); }
+    at::Tensor empty(int64_t n, at::ScalarType t) const { return at::detail::empty_cuda({n}, t, device, c10::nullopt); }
 
     void same(const char* name, const at::Tensor& t, at::ScalarType type) const
     {

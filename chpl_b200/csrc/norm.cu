@@ -176,7 +176,6 @@ __device__ __forceinline__ float dot(const Some& a, const Some& b)
     const float2 t = apart(even + odd);
     return t.x + t.y;
 }
-__device__ __forceinline__ float feature(const Some& a, int i) { return i % 2 ? apart(a.v[i / 2]).y : apart(a.v[i / 2]).x; }
 
 // where a thread stands: its features first + 256 h + 0 .. 7, of which left - 256 h
 // exist (all eight, some or none)
@@ -633,7 +632,8 @@ struct Backward {
     const void *post_w, *post_b, *pre_w;
     const float2 *post_stats, *pre_stats;
     RowsTo dx, dy, dgate;     // dgate of a matrix
-    float* part;              // [sum][unit][n] of the sums that `sums` names
+    float* part;              // [sum][unit][part_ld] of the sums that `sums` names
+    int part_ld;              // n, up to a multiple of four
     int sums;                 // bit k: sum k
 };
 
@@ -761,35 +761,43 @@ __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid
             load(row + s.stages * at.step, ring.at);
         }
     }
-    // a CTA's sums: those of its groups, joined in shared memory in order
+    // A CTA's sums: every thread's into shared memory, where the rows under way were,
+    // then all threads add up the groups', in order, four features at a time.
     if (a.part) {
-        float* joined = reinterpret_cast<float*>(smem);  // [groups][16][threads of a group]
-        const int width = 32 * s.warps, thread = threadIdx.x - at.group * width;
-        const int64_t unit = blockIdx.x / s.cluster;
+        const int quads = s.warps * (kWarpWidth / 4);  // of a group
         asm volatile("cp.async.wait_all;" ::: "memory");
-        int slot = 0;
+        __syncthreads();
+        uint32_t put_at = mem + ((warp_id() - at.group * s.warps) * (kWarpWidth / 4) + lane_id()) * 16 + at.group * quads * 16;
+        int count = 0;
 #pragma unroll
         for (int k = 0; k < kSums; ++k) {
             if ((!JOIN && k < 2) || (!BIAS && k % 2)) continue;
             if (!(a.sums >> k & 1)) continue;
             const Some& mine = total[BIAS ? k - (JOIN ? 0 : 2) : JOIN ? k / 2 : 0];
-            if (s.groups > 1) {
-                __syncthreads();
 #pragma unroll
-                for (int i = 0; i < 2 * kTwos; ++i) joined[(at.group * 2 * kTwos + i) * width + thread] = feature(mine, i);
-                __syncthreads();
+            for (int i = 0; i < kTwos; i += 2)  // quad i / 2 of the lane's
+                asm volatile("st.shared.v2.b64 [%0], {%1, %2};" ::"r"(put_at + i * 256), "l"(mine.v[i].v), "l"(mine.v[i + 1].v) : "memory");
+            put_at += s.groups * quads * 16;
+            ++count;
+        }
+        __syncthreads();
+        const int rank = s.cluster > 1 ? (int)cluster_ctarank() : 0;
+        const int64_t unit = blockIdx.x / s.cluster;
+        for (int i = threadIdx.x; i < count * quads; i += blockDim.x) {
+            const int k = i / quads, q = i - k * quads, warp = q / (kWarpWidth / 4), in = q % (kWarpWidth / 4);
+            // the in-th four of the warp's features: quad in % 2 of half in / 64 of lane in / 2 % 32
+            const uint32_t from = mem + (uint32_t)(((k * s.groups * s.warps + warp) * (kWarpWidth / 4) + (in / 64 * 2 + in % 2) * 32 + in / 2 % 32) * 16);
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int g = 0; g < s.groups; ++g) {
+                float4 v;
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(from + g * quads * 16) : "memory");
+                sum.x += v.x;
+                sum.y += v.y;
+                sum.z += v.z;
+                sum.w += v.w;
             }
-            if (at.group == 0) {
-                float* out = a.part + ((int64_t)slot * s.units + unit) * a.n + at.first;
-#pragma unroll
-                for (int i = 0; i < 2 * kTwos; ++i) {
-                    float v = feature(mine, i);
-                    for (int g = 1; g < s.groups; ++g) v += joined[(g * 2 * kTwos + i) * width + thread];
-                    const int j = 256 * (i / 8) + i % 8;
-                    if (j < at.left) out[j] = v;
-                }
-            }
-            ++slot;
+            const int j = (rank * s.warps + warp) * kWarpWidth + in * 4;
+            if (j < a.n) *reinterpret_cast<float4*>(a.part + ((int64_t)k * s.units + unit) * a.part_ld + j) = sum;  // past n: padding
         }
     }
     if (s.cluster > 1) cluster_sync();
@@ -799,7 +807,7 @@ __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid
 // warps equal runs of the units, joined in order; bound by the loads' latency.
 struct Parameters {
     const float* part;
-    int units, n, sums;
+    int part_ld, units, n, sums;
     int f32, accumulate, matrix;
     const void *post_w, *post_b, *gate;  // as they were used
     void *dpost_w, *dpost_b, *dgate, *dpre_w, *dpre_b;
@@ -813,26 +821,38 @@ __global__ void __launch_bounds__(32 * kJoinWarps) parameters_kernel(const __gri
     __shared__ float turn[kSums][kJoinWarps][32];
     const int lane = lane_id(), warp = warp_id(), j = blockIdx.x * 32 + lane;
     const int first = (int)((int64_t)a.units * warp / kJoinWarps), last = (int)((int64_t)a.units * (warp + 1) / kJoinWarps);
+    const int count = __popc(a.sums);
+    const int64_t step = (int64_t)a.units * a.part_ld;  // from one sum to the next
     start_of_inputs();
+    const auto of = [&](const void* v, float other) { return v && j < a.n ? to_f32(static_cast<const T*>(v)[j]) : other; };
+    float gate = 1.0f, weight = 1.0f, bias = 0.0f;
+    if (warp == 0) {
+        gate = a.matrix ? 1.0f : of(a.gate, 1.0f);  // a matrix is in the sums
+        weight = of(a.post_w, 1.0f);
+        bias = of(a.post_b, 0.0f);
+    }
     float sum[kSums] = {};
+    if (j < a.n) {
+        const float* p = a.part + j;
+#pragma unroll 4
+        for (int u = first; u < last; ++u)
+#pragma unroll
+            for (int c = 0; c < kSums; ++c)
+                if (c < count) sum[c] += p[c * step + (int64_t)u * a.part_ld];
+    }
+#pragma unroll
+    for (int c = 0; c < kSums; ++c) turn[c][warp][lane] = sum[c];
+    __syncthreads();
+    if (warp > 0 || j >= a.n) return;
+    float all[kSums] = {};
     int slot = 0;
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
         if (!(a.sums >> k & 1)) continue;
-        const float* p = a.part + (int64_t)slot++ * a.units * a.n + j;
-        if (j < a.n) {
-#pragma unroll 16
-            for (int u = first; u < last; ++u) sum[k] += p[(int64_t)u * a.n];
-        }
-        turn[k][warp][lane] = sum[k];
+#pragma unroll 8
+        for (int w = 0; w < kJoinWarps; ++w) all[k] += turn[slot][w][lane];
+        ++slot;
     }
-    __syncthreads();
-    if (warp > 0 || j >= a.n) return;
-#pragma unroll
-    for (int k = 0; k < kSums; ++k)
-        if (a.sums >> k & 1)
-            for (int w = 1; w < kJoinWarps; ++w) sum[k] += turn[k][w][lane];
-    const auto of = [&](const void* v, float other) { return v ? to_f32(static_cast<const T*>(v)[j]) : other; };
     const auto store = [&](void* out, float v) {
         if (!out) return;
         if (a.f32) {
@@ -843,12 +863,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) parameters_kernel(const __gri
             *o = from_f32<T>(a.accumulate ? to_f32(*o) + v : v);
         }
     };
-    const float gate = a.matrix ? 1.0f : of(a.gate, 1.0f);  // a matrix is in the sums
-    store(a.dpost_w, gate * sum[0]);
-    store(a.dpost_b, gate * sum[1]);
-    store(a.dgate, fmaf(of(a.post_w, 1.0f), sum[0], a.post_b ? of(a.post_b, 0.0f) * sum[1] : 0.0f));
-    store(a.dpre_w, sum[2]);
-    store(a.dpre_b, sum[3]);
+    store(a.dpost_w, gate * all[0]);
+    store(a.dpost_b, gate * all[1]);
+    store(a.dgate, a.post_b ? fmaf(weight, all[0], bias * all[1]) : weight * all[0]);
+    store(a.dpre_w, all[2]);
+    store(a.dpre_b, all[3]);
 }
 
 // ----------------------------------------------------------------------------
@@ -964,6 +983,7 @@ struct BackwardPlan {
     Shape shape;
     bool in, out;    // rows that 16-byte accesses fit
     int sums;        // bits
+    int part_ld;
     size_t bytes;
 };
 
@@ -982,11 +1002,12 @@ static BackwardPlan plan(const chpl_norm_bwd& a)
     const int tensors = (a.dr ? 1 : 0) + (a.pre.kind ? 2 : 0) + has_y + matrix;
     const int vectors = (a.pre.kind ? 1 : 0) + (a.join && (a.post.kind || (a.gate && a.ldgate == 0)) ? 1 : 0) + (matrix && a.post.kind && a.post.bias ? 1 : 0);
     p.shape = shape_for(a.tokens, a.n, tensors, vectors, p.in, p.out, kBackwardThreads);
-    // the groups' sums are joined where the rows under way were
-    p.shape.smem = std::max(p.shape.smem, p.shape.groups > 1 ? kWarpWidth * p.shape.warps * p.shape.groups * 4 : 0);
     int count = 0;
     for (int k = 0; k < kSums; ++k) count += p.sums >> k & 1;
-    p.bytes = round_up((size_t)count * p.shape.units * a.n * 4, 256);
+    // the groups' sums are joined where the rows under way were
+    p.shape.smem = std::max(p.shape.smem, count * kWarpWidth * p.shape.warps * p.shape.groups * 4);
+    p.part_ld = (int)round_up((size_t)a.n, 4);
+    p.bytes = round_up((size_t)count * p.shape.units * p.part_ld * 4, 256);
     return p;
 }
 
@@ -1050,6 +1071,7 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
         b.residual_scale = a.residual_scale;
         b.sums = p.sums;
         b.part = p.sums ? static_cast<float*>(work) : nullptr;
+        b.part_ld = p.part_ld;
         b.dr = {a.dr, a.lddr};
         b.dx = {a.dx, a.lddx, fits(a.dx, a.lddx, a.tokens)};
         if (a.pre.kind) {
@@ -1080,6 +1102,7 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
     if (!p.sums || (a.tokens == 0 && a.accumulate)) return CHPL_OK;
     Parameters q = {};
     q.part = static_cast<const float*>(work);
+    q.part_ld = p.part_ld;
     q.units = a.tokens > 0 ? p.shape.units : 0;
     q.n = (int)a.n;
     q.sums = p.sums;

@@ -37,11 +37,17 @@ _NONE = (0, None, None, 0.0)
 
 
 def _of(where: str, v: Norm | None):
-    return _NONE if v is None else (_choice(where, "norm", KINDS, v.kind), v.weight, v.bias, v.eps)
+    if v is None:
+        return _NONE
+    weight, bias, kind, eps = v
+    code = KINDS.get(kind)
+    return _choice(where, "norm", KINDS, kind) if code is None else code, weight, bias, eps
 
 
 def _gradients(where: str, d: torch.Tensor, dtype, given) -> bool:
     """Whether the parameters' gradients are FP32."""
+    if dtype is None and not any(v is not None for v in given):
+        return False
     gt = dtype or next((v.dtype for v in given if v is not None), d.dtype)
     if gt is not d.dtype and gt is not torch.float32:
         raise _lib.ChplError(_lib.CHPL_ERR_INVALID, where, f"gradients in {gt}: {d.dtype} or float32 is wanted")
@@ -100,6 +106,9 @@ class Joined(NamedTuple):
     dpre_bias: torch.Tensor | None
 
 
+_NOWHERE = Joined(*(None,) * 7)
+
+
 def join_backward(dr: torch.Tensor | None, dh: torch.Tensor | None, r: torch.Tensor | None, y: torch.Tensor | None,
                   post_stats: torch.Tensor | None, pre_stats: torch.Tensor | None, *, post: Norm | None = None,
                   gate: torch.Tensor | None = None, scale: float = 1.0, residual_scale: float = 1.0, pre: Norm | None = None,
@@ -117,9 +126,10 @@ def join_backward(dr: torch.Tensor | None, dh: torch.Tensor | None, r: torch.Ten
             return join_backward(dr, dh, r, y, post_stats, pre_stats, post=post, gate=gate, scale=scale, residual_scale=residual_scale,
                                  pre=pre, need_dx=need_dx, need_dy=need_dy, need_dgate=need_dgate, need_dparams=need_dparams, into=into,
                                  grad_dtype=grad_dtype, accumulate=accumulate, work=work)
-    into = into or Joined(*(None,) * 7)
-    sums = into[3:] if gate is None or gate.dim() > 1 else into[2:]
-    f32 = _gradients("norm.join_backward", d, grad_dtype, sums)
-    return Joined(*_ops.norm_backward(True, dr, dh, r, y, gate, scale, residual_scale, *_of("norm.join_backward", post),
+    into = into or _NOWHERE
+    f32 = False
+    if grad_dtype is not None or into is not _NOWHERE:
+        f32 = _gradients("norm.join_backward", d, grad_dtype, into[3:] if gate is None or gate.dim() > 1 else into[2:])
+    return Joined._make(_ops.norm_backward(True, dr, dh, r, y, gate, scale, residual_scale, *_of("norm.join_backward", post),
                                       *_of("norm.join_backward", pre), post_stats, pre_stats, f32, accumulate, need_dx, need_dy, need_dgate,
                                       need_dparams, *into, work))
