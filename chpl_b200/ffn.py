@@ -7,7 +7,8 @@ backward ones take act(Z), act'(Z) and X from the codes.  The gradients are thos
     y, saved = ffn.forward(x, w1, b1, w2, b2, act="gelu", residual=True, save=True)
     dx, dw1, db1, dw2, db2 = ffn.backward(dy, saved, w1, w2)
 
-``block`` wraps the two for torch's autograd; the two themselves it does not see.
+``block`` wraps the two for torch's autograd; the two themselves it does not see.  ``sublayer`` is the block with the norm before
+it and its join with the residual stream.  Where nothing is trained the weights may be 4-bit ones (mx4.pack).
 """
 from __future__ import annotations
 
@@ -15,7 +16,9 @@ from typing import NamedTuple
 
 import torch
 
-from . import _lib, ckpt8, linear
+from . import _lib, ckpt8, linear, mx4
+from . import norm as norms
+from ._once import once
 
 
 class Saved(NamedTuple):
@@ -25,11 +28,17 @@ class Saved(NamedTuple):
     residual: bool
 
 
+def _layer(x, w, b, **how):
+    return mx4.linear(x, w, b, **how) if isinstance(w, mx4.Mx4) else linear.forward(x, w, b, **how)
+
+
 def forward(x, w1, b1, w2, b2, *, act: str = "gelu", residual: bool = False, save: bool = False, stream=None):
-    """Y, or with save=True (Y, what backward needs).  b1 and b2 may be None."""
+    """Y, or with save=True (Y, what backward needs).  b1 and b2 may be None; without save w1 and w2 may be Mx4."""
     if not save:
-        h = linear.forward(x, w1, b1, act=act, stream=stream)
-        return linear.forward(h, w2, b2, residual=x if residual else None, stream=stream)
+        h = _layer(x, w1, b1, act=act, stream=stream)
+        return _layer(h, w2, b2, residual=x if residual else None, stream=stream)
+    if isinstance(w1, mx4.Mx4) or isinstance(w2, mx4.Mx4):
+        raise _lib.ChplError(_lib.CHPL_ERR_UNSUPPORTED, "ffn.forward", "4-bit weights are served, not trained: save=True wants 16-bit ones")
     x8 = ckpt8.pack(x, stream=stream)
     h, z8 = linear.forward(x, w1, b1, act=act, save="z8", stream=stream)
     y = linear.forward(h, w2, b2, residual=x if residual else None, stream=stream)
@@ -50,19 +59,6 @@ def backward(dy, saved: Saved, w1, w2, *, need_dx: bool = True, need_dw1: bool =
     return dx, dw1, db1[0] if db1 else None, dw2, db2
 
 
-class _Once(torch.autograd.Function):
-    """Gradients that cannot be differentiated again.  torch's once_differentiable raises only where dy carries a graph;
-    the block's gradients depend on its weights and input too."""
-
-    @staticmethod
-    def forward(ctx, *grads):
-        return tuple(v if v is None else v.view_as(v) for v in grads)
-
-    @staticmethod
-    def backward(ctx, *_):
-        raise _lib.ChplError(_lib.CHPL_ERR_UNSUPPORTED, "ffn.block", "its gradients cannot be differentiated again")
-
-
 class _Block(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w1, b1, w2, b2, act, residual):
@@ -80,9 +76,7 @@ class _Block(torch.autograd.Function):
         with torch.no_grad():
             dx, dw1, db1, dw2, db2 = backward(dy.contiguous(), s, w1, w2, need_dx=x, need_dw1=n1, need_dw2=n2, need_db=v1 or v2)
         grads = [dx, dw1, db1 if v1 else None, dw2, db2 if v2 else None]
-        if torch.is_grad_enabled():  # create_graph
-            grads = _Once.apply(*(v if v is None else v.requires_grad_() for v in grads))
-        return *grads, None, None
+        return *once("ffn.block", grads), None, None
 
 
 def block(x, w1, b1, w2, b2, act: str = "gelu", residual: bool = False):
@@ -95,3 +89,12 @@ def block(x, w1, b1, w2, b2, act: str = "gelu", residual: bool = False):
     if torch.is_grad_enabled() and any(isinstance(v, torch.Tensor) and v.requires_grad for v in (x, w1, b1, w2, b2)):
         return _Block.apply(x, w1, b1, w2, b2, act, residual)
     return forward(x, w1, b1, w2, b2, act=act, residual=residual)
+
+
+def sublayer(x, norm, w1, b1, w2, b2, *, act: str = "gelu", post=None, gate=None, scale: float = 1.0, residual_scale: float = 1.0,
+             pre=None):
+    """r = residual_scale x + scale gate N_post(Y(N(x))), the block Y between the norm before it and its join with the residual
+    stream (norm, post and pre: norm.Norm); with pre (r, N_pre(r)), the next block's input.  torch's autograd differentiates
+    through it, once; with 4-bit weights it serves."""
+    y = block(norms.normalized(x, norm), w1, b1, w2, b2, act)
+    return norms.joined(x, y, post=post, gate=gate, scale=scale, residual_scale=residual_scale, pre=pre)

@@ -19,6 +19,7 @@ import torch
 
 from . import _lib
 from .ckpt8 import on
+from ._once import once
 from .linear import _choice
 
 _ops = _lib.torch_ops()
@@ -133,3 +134,85 @@ def join_backward(dr: torch.Tensor | None, dh: torch.Tensor | None, r: torch.Ten
     return Joined._make(_ops.norm_backward(True, dr, dh, r, y, gate, scale, residual_scale, *_of("norm.join_backward", post),
                                       *_of("norm.join_backward", pre), post_stats, pre_stats, f32, accumulate, need_dx, need_dy, need_dgate,
                                       need_dparams, *into, work))
+
+
+# ------------------------------------------------------------------------------------------------------- autograd
+def _wanted(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(isinstance(v, torch.Tensor) and v.requires_grad for v in tensors)
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    return x.flatten(0, -2) if x.dim() > 2 else x[None]
+
+
+class _Normalized(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, kind, eps):
+        h, stats = forward(x, Norm(weight, bias, kind, eps), save=True)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.how = kind, eps
+        return h
+
+    @staticmethod
+    def backward(ctx, dh):
+        x, weight, bias, stats = ctx.saved_tensors
+        nx, nw, nb = ctx.needs_input_grad[:3]
+        with torch.no_grad():
+            dx, dw, db = backward(dh.contiguous(), x, stats, Norm(weight, bias, *ctx.how), need_dx=nx, need_dparams=nw or nb)
+        return *once("norm.normalized", (dx, dw if nw else None, db if nb else None)), None, None
+
+
+def normalized(x: torch.Tensor, norm: Norm) -> torch.Tensor:
+    """forward(x, norm) as a function that torch's autograd differentiates through, once (a second differentiation raises).
+    x has any leading dimensions, features last."""
+    if x.dim() not in (0, 2):
+        return normalized(_rows(x), norm).reshape(x.shape)
+    if _wanted(x, norm.weight, norm.bias):
+        return _Normalized.apply(x, *norm)
+    return forward(x, norm)
+
+
+class _Joined(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, gate, post_weight, post_bias, pre_weight, pre_bias, kinds, scales):
+        post = None if post_weight is None else Norm(post_weight, post_bias, *kinds[0])
+        pre = None if pre_weight is None else Norm(pre_weight, pre_bias, *kinds[1])
+        *out, (post_stats, pre_stats) = join(x, y, post=post, gate=gate, scale=scales[0], residual_scale=scales[1], pre=pre, save=True)
+        ctx.save_for_backward(out[0] if pre else None, y if post or gate is not None else None, gate, post_weight, post_bias, pre_weight, pre_bias,
+                              post_stats, pre_stats)
+        ctx.how = kinds, scales
+        ctx.set_materialize_grads(False)
+        return tuple(out) if pre else out[0]
+
+    @staticmethod
+    def backward(ctx, dr, dh=None):
+        r, y, gate, post_weight, post_bias, pre_weight, pre_bias, post_stats, pre_stats = ctx.saved_tensors
+        if dr is None and dh is None:
+            return (None,) * 9
+        kinds, scales = ctx.how
+        post = None if post_weight is None else Norm(post_weight, post_bias, *kinds[0])
+        pre = None if dh is None else Norm(pre_weight, pre_bias, *kinds[1])  # an h that nothing uses brings no gradient
+        nx, ny, ngate, *nparams = ctx.needs_input_grad[:7]
+        with torch.no_grad():
+            g = join_backward(None if dr is None else dr.contiguous(), None if dh is None else dh.contiguous(), r, y, post_stats, pre_stats,
+                              post=post, gate=gate, scale=scales[0], residual_scale=scales[1], pre=pre, need_dx=nx, need_dy=ny,
+                              need_dgate=ngate, need_dparams=any(nparams))
+        return *once("norm.joined", g[:3] + tuple(v if n else None for v, n in zip(g[3:], nparams))), None, None
+
+
+def joined(x: torch.Tensor, y: torch.Tensor, *, post: Norm | None = None, gate: torch.Tensor | None = None, scale: float = 1.0,
+           residual_scale: float = 1.0, pre: Norm | None = None):
+    """join(x, y, ...) as a function that torch's autograd differentiates through, once.  x and y have any leading dimensions,
+    features last; gate is a vector of features or has x's shape."""
+    if x.dim() not in (0, 2):
+        matrix = gate is not None and gate.dim() > 1
+        if y.shape != x.shape or (matrix and gate.shape != x.shape):
+            raise _lib.ChplError(_lib.CHPL_ERR_INVALID, "norm.joined", f"x is {tuple(x.shape)}, y {tuple(y.shape)}"
+                                 + (f", gate {tuple(gate.shape)}" if matrix else ""))
+        out = joined(_rows(x), _rows(y), post=post, gate=_rows(gate) if matrix else gate, scale=scale, residual_scale=residual_scale, pre=pre)
+        return out.reshape(x.shape) if pre is None else tuple(v.reshape(x.shape) for v in out)
+    params = (*(post or (None, None))[:2], *(pre or (None, None))[:2])
+    if _wanted(x, y, gate, *params):
+        kinds = tuple(None if v is None else (v.kind, v.eps) for v in (post, pre))
+        return _Joined.apply(x, y, gate, *params, kinds, (scale, residual_scale))
+    return join(x, y, post=post, gate=gate, scale=scale, residual_scale=residual_scale, pre=pre)
