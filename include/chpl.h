@@ -279,6 +279,8 @@ int chpl_diag_linear_wait(void *stream, uint64_t limit_ns);
  * plan[0]: 1 for pairs of CTAs, 0 for clusters; plan[1]: rows of a tile; plan[2]: CTAs that split the contraction (1
  * with pairs); plan[3]: tiles. */
 int chpl_diag_linear_plan(int product, int64_t features, int64_t rows, int64_t contraction, int64_t plan[4]);
+/* The same for chpl_mx4_linear (features = n, rows = tokens, contraction = k): plan[0] to plan[2] as above. */
+int chpl_diag_mx4_plan(int64_t features, int64_t rows, int64_t contraction, int64_t plan[3]);
 
 /* ------------------------------------------------------------------------ */
 /* HPL solver                                                                */
