@@ -623,6 +623,16 @@ __global__ void __launch_bounds__(kForwardThreads) forward_kernel(const __grid_c
 // ----------------------------------------------------------------------------
 // backward
 // ----------------------------------------------------------------------------
+// What a join has, known to the kernel where its rows are aligned (PARTS < 0: it
+// looks).  Straight code, without branches around what is not there: 8192 x 4096 with
+// two RMS norms 95 -> 89 us.  (The forward kernel gains nothing by it.)
+enum { kPre = 1, kPost = 2, kMatrix = 4, kAnyParts = -1 };
+template <int PARTS>
+__device__ __forceinline__ bool part(int which, bool there)
+{
+    return PARTS < 0 ? there : (PARTS & which) != 0;
+}
+
 struct Backward {
     uint32_t tokens;
     int n;
@@ -659,19 +669,20 @@ __device__ __forceinline__ Pull pull(const Some& g, const Some& c, int kind, flo
     return {t.x * inv_n, t.y * inv_n * s * s};
 }
 
-template <typename T, bool ALIGNED, bool JOIN, bool BIAS>
+template <typename T, bool ALIGNED, bool JOIN, bool BIAS, int PARTS>
 __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid_constant__ Backward a, const Shape s)
 {
+    const bool has_pre = part<PARTS>(kPre, a.pre), has_post = JOIN && part<PARTS>(kPost, a.post);
     extern __shared__ uint4 smem[];
     __shared__ WarpSums sets;
     const Place at(s, a.n);
-    const bool matrix = JOIN && a.gate.p && a.gate.ld, has_y = JOIN && a.y.p, weighs = JOIN && (a.post || (a.gate.p && !matrix));
-    const int t_dh = a.dr.p ? 1 : 0, t_r = t_dh + 1, t_y = a.pre ? t_r + 1 : t_dh, t_gate = t_y + has_y, tensors = t_gate + matrix;
+    const bool matrix = JOIN && part<PARTS>(kMatrix, a.gate.p && a.gate.ld), has_y = JOIN && (has_post || a.y.p), weighs = JOIN && (has_post || (a.gate.p && !matrix));
+    const int t_dh = a.dr.p ? 1 : 0, t_r = t_dh + 1, t_y = has_pre ? t_r + 1 : t_dh, t_gate = t_y + has_y, tensors = t_gate + matrix;
     const uint32_t mem = smem_u32(smem), vec = mem + (warp_id() - at.group * s.warps) * kVectorBytes, vec_step = s.warps * kVectorBytes,
                    turn = mem + s.turn + warp_id() * 512;
     uint32_t used = 0;  // a vector gate is in post_w
     const auto place = [&](bool there) { return vec + (there ? used++ : 0) * vec_step; };
-    const uint32_t pre_w = place(a.pre), post_w = JOIN ? place(weighs) : 0, post_b = JOIN ? place(matrix && a.post_b) : 0;
+    const uint32_t pre_w = place(has_pre), post_w = JOIN ? place(weighs) : 0, post_b = JOIN ? place(matrix && a.post_b) : 0;
     Ring ring(mem + used * vec_step, tensors, s);
     RowSums sums(sets, s, at.group);
     const float inv_n = 1.0f / (float)a.n;
@@ -681,7 +692,7 @@ __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid
         if (row < a.tokens) {
             const auto fetch = [&](int t, const Rows& x) { fetch_row<ALIGNED>(slot + t * ring.tensor, x, row, a.tokens, at); };
             if (a.dr.p) fetch(0, a.dr);
-            if (a.pre) {
+            if (has_pre) {
                 fetch(t_dh, a.dh);
                 fetch(t_r, a.r);
             }
@@ -693,12 +704,12 @@ __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid
     const auto stats_of = [&](uint32_t row, float2& pre, float2& post) {
         pre = post = make_float2(0.0f, 1.0f);
         if (row >= a.tokens) return;
-        if (a.pre) pre = __ldg(a.pre_stats + row);
-        if (JOIN && a.post) post = __ldg(a.post_stats + row);
+        if (has_pre) pre = __ldg(a.pre_stats + row);
+        if (has_post) post = __ldg(a.post_stats + row);
     };
     for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, ring.at + i * ring.bytes);
     if (at.group == 0) {  // the groups' in common
-        if (a.pre) put_vector<T>(pre_w, a.pre_w, nullptr, 1.0f, at);
+        if (has_pre) put_vector<T>(pre_w, a.pre_w, nullptr, 1.0f, at);
         if (JOIN && weighs) put_vector<T>(post_w, a.post_w, matrix ? nullptr : a.gate.p, 1.0f, at);
         if (JOIN && matrix && a.post_b) put_vector<T>(post_b, a.post_b, nullptr, 1.0f, at);
     }
@@ -715,7 +726,7 @@ __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid
         stats_of(row + at.step, pre_next, post_next);
         ring.template wait<ALIGNED>();
         Some d;
-        if (a.pre) {
+        if (has_pre) {
             Some c = of(t_r, a.r, row), g = of(t_dh, a.dh, row);
             if constexpr (BIAS) total[kHat + 1] = total[kHat + 1] + g;
             if (a.pre == CHPL_NORM_LAYER) c = c + -pre.x;
@@ -739,7 +750,7 @@ __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid
             if (matrix) {
                 if (a.dgate.p) {
                     Some p = y * post.y;
-                    if (a.post) p = a.post_b ? fma_of(p, vector_at(post_w), vector_at(post_b)) : p * vector_at(post_w);
+                    if (has_post) p = a.post_b ? fma_of(p, vector_at(post_w), vector_at(post_b)) : p * vector_at(post_w);
                     put<T>(a.dgate, row, at, (BIAS ? d : d * a.scale) * p, turn);
                 }
                 d = d * of(t_gate, a.gate, row);
@@ -750,7 +761,7 @@ __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid
             if (weighs) d = d * vector_at(post_w);
             if (!ALIGNED) __syncwarp();
             load(row + s.stages * at.step, ring.at);
-            if (a.post) {
+            if (has_post) {
                 const Pull p = pull(d, y, a.post, post.y, inv_n, sums);
                 d = fma_of(y, -p.along, d);
                 if (a.post == CHPL_NORM_LAYER) d = d + -p.mean;
@@ -1058,6 +1069,40 @@ static int check(const char* who, const chpl_norm_bwd* a, bool pointers)
     return CHPL_OK;
 }
 
+static int parts_of(const chpl_norm& pre, const chpl_norm& post, const void* gate, int64_t ldgate)
+{
+    return (pre.kind ? kPre : 0) | (post.kind ? kPost : 0) | (gate && ldgate ? kMatrix : 0);
+}
+
+template <int V>
+struct Parts {
+    static constexpr int value = V;
+};
+template <typename F>
+static int with_parts(int parts, F&& f)
+{
+    switch (parts) {
+        case 0: return f(Parts<0>());
+        case 1: return f(Parts<1>());
+        case 2: return f(Parts<2>());
+        case 3: return f(Parts<3>());
+        case 4: return f(Parts<4>());
+        case 5: return f(Parts<5>());
+        case 6: return f(Parts<6>());
+        default: return f(Parts<7>());
+    }
+}
+
+template <typename T, bool BIAS>
+static int launch_backward(cudaStream_t st, const chpl_norm_bwd& a, const Backward& b, const BackwardPlan& p)
+{
+    if (!a.join)
+        return p.in ? launch<backward_kernel<T, true, false, BIAS, kPre>>(st, b, p.shape) : launch<backward_kernel<T, false, false, BIAS, kPre>>(st, b, p.shape);
+    if (!p.in) return launch<backward_kernel<T, false, true, BIAS, kAnyParts>>(st, b, p.shape);
+    return with_parts(parts_of(a.pre, a.post, a.gate, a.ldgate),
+                      [&](auto parts) { return launch<backward_kernel<T, true, true, BIAS, decltype(parts)::value>>(st, b, p.shape); });
+}
+
 template <typename T>
 static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
 {
@@ -1094,10 +1139,7 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
             }
         }
         const bool bias = (p.sums & 10) != 0;
-        if (!a.join && bias) CHPL_TRY((p.in ? launch<backward_kernel<T, true, false, true>>(st, b, p.shape) : launch<backward_kernel<T, false, false, true>>(st, b, p.shape)));
-        else if (!a.join) CHPL_TRY((p.in ? launch<backward_kernel<T, true, false, false>>(st, b, p.shape) : launch<backward_kernel<T, false, false, false>>(st, b, p.shape)));
-        else if (bias) CHPL_TRY((p.in ? launch<backward_kernel<T, true, true, true>>(st, b, p.shape) : launch<backward_kernel<T, false, true, true>>(st, b, p.shape)));
-        else CHPL_TRY((p.in ? launch<backward_kernel<T, true, true, false>>(st, b, p.shape) : launch<backward_kernel<T, false, true, false>>(st, b, p.shape)));
+        CHPL_TRY((bias ? launch_backward<T, true>(st, a, b, p) : launch_backward<T, false>(st, a, b, p)));
     }
     if (!p.sums || (a.tokens == 0 && a.accumulate)) return CHPL_OK;
     Parameters q = {};
