@@ -98,7 +98,7 @@ def _build_torch_ext(force: bool, verbose: bool, hdrs: list[str]) -> None:
     try:
         import torch
     except (ImportError, OSError) as e:
-        sys.stderr.write(f"chpl_b200: {os.path.basename(TORCH_EXT)} is not built, torch does not import ({e}); linear, ckpt8 and ffn need it\n")
+        sys.stderr.write(f"chpl_b200: {os.path.basename(TORCH_EXT)} is not built, torch does not import ({e}); linear, ckpt8, ffn, norm and mx4 need it\n")
         return
     src, stamp = os.path.join(CSRC, "bindings.cpp"), os.path.join(BUILD, "_torch.version")
     version = f"torch {torch.__version__}, Python {sys.version}"
