@@ -231,41 +231,55 @@ __device__ __forceinline__ Some packed_at(uint32_t piece)
     return r;
 }
 
-// Eight features of a vector from the thread's (h-th) first on, zero past the end;
-// all ones where there is no vector
+// The thread's features of a vector as they are in memory, zero past the end; all
+// ones where there is no vector.
 template <typename T>
-__device__ __forceinline__ void eight_of(const void* v, const Place& at, int h, float (&f)[8])
+struct Raw {
+    uint32_t w[kHalves][4];
+};
+template <typename T>
+__device__ __forceinline__ Raw<T> raw_vector(const void* v, bool there, const Place& at)
 {
-    const T* p = static_cast<const T*>(v) + at.first + 256 * h;
-    const int have = at.have(h);
-    if (v && have == 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-        const T* e = reinterpret_cast<const T*>(&q);
+    constexpr uint32_t one = std::is_same<T, __half>::value ? 0x3C00u : 0x3F80u;
+    Raw<T> r;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_f32(e[i]);
-    } else {
+    for (int h = 0; h < kHalves; ++h) {
+        const unsigned short* p = static_cast<const unsigned short*>(v) + at.first + 256 * h;
+        const int have = at.have(h);
+        if (there && have == 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+            const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+            r.w[h][0] = q.x;
+            r.w[h][1] = q.y;
+            r.w[h][2] = q.z;
+            r.w[h][3] = q.w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = i < have ? (v ? to_f32(p[i]) : 1.0f) : 0.0f;
+            for (int i = 0; i < 8; i += 2) {
+                const uint32_t lo = i < have ? (there ? __ldg(p + i) : one) : 0u, hi = i + 1 < have ? (there ? __ldg(p + i + 1) : one) : 0u;
+                r.w[h][i / 2] = lo | hi << 16;
+            }
+        }
     }
+    return r;
 }
 
 // A vector, times another (exact in FP32) and a factor, as FP32 in the warp's 2048
 // bytes of shared memory, the lane's own: a row then costs neither conversions nor
-// the products.
+// the products.  (All of a kernel's vectors are read before the first is put: one
+// latency, not one for each, which a single row waits for.)
 template <typename T>
-__device__ __forceinline__ void put_vector(uint32_t piece, const void* u, const void* v, float factor, const Place& at)
+__device__ __forceinline__ void put_vector(uint32_t piece, const Raw<T>& u, const Raw<T>& v, float factor)
 {
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-        float f[8], g[8];
-        eight_of<T>(u, at, h, f);
-        eight_of<T>(v, at, h, g);
+    for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-        for (int i = 0; i < 8; i += 4)
-            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(piece + h * 1024 + i * 128 + lane_id() * 16), "f"(f[i] * g[i] * factor),
-                         "f"(f[i + 1] * g[i + 1] * factor), "f"(f[i + 2] * g[i + 2] * factor), "f"(f[i + 3] * g[i + 3] * factor)
+        for (int i = 0; i < 4; i += 2) {
+            const float2 a = linear::unpack2<T>(u.w[h][i]), b = linear::unpack2<T>(u.w[h][i + 1]), c = linear::unpack2<T>(v.w[h][i]),
+                         d = linear::unpack2<T>(v.w[h][i + 1]);
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(piece + h * 1024 + i * 256 + lane_id() * 16), "f"(a.x * c.x * factor),
+                         "f"(a.y * c.y * factor), "f"(b.x * d.x * factor), "f"(b.y * d.y * factor)
                          : "memory");
-    }
+        }
 }
 __device__ __forceinline__ Some vector_at(uint32_t piece)
 {
@@ -588,10 +602,15 @@ __global__ void __launch_bounds__(kForwardThreads) forward_kernel(const __grid_c
     };
     for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, ring.at + i * ring.bytes);
     if (at.group == 0) {  // the groups' in common
-        if (a.pre) put_vector<T>(pre_w, a.pre_w, nullptr, 1.0f, at);
-        if (a.pre_b) put_vector<T>(pre_b, a.pre_b, nullptr, 1.0f, at);
-        if (JOIN && weighs) put_vector<T>(post_w, a.post_w, matrix ? nullptr : a.gate.p, a.scale, at);
-        if (JOIN && a.post_b) put_vector<T>(post_b, a.post_b, matrix ? nullptr : a.gate.p, a.scale, at);
+        const Raw<T> none = raw_vector<T>(nullptr, false, at), w1 = raw_vector<T>(a.pre_w, a.pre, at), b1 = raw_vector<T>(a.pre_b, a.pre_b, at);
+        if (JOIN) {
+            const Raw<T> w0 = raw_vector<T>(a.post_w, a.post, at), b0 = raw_vector<T>(a.post_b, a.post_b, at),
+                         g0 = raw_vector<T>(a.gate.p, a.gate.p && !matrix, at);
+            if (weighs) put_vector<T>(post_w, w0, g0, a.scale);
+            if (a.post_b) put_vector<T>(post_b, b0, g0, a.scale);
+        }
+        if (a.pre) put_vector<T>(pre_w, w1, none, 1.0f);
+        if (a.pre_b) put_vector<T>(pre_b, b1, none, 1.0f);
     }
     __syncthreads();
     const bool writes = at.first == 0;  // the row's statistics
@@ -709,9 +728,14 @@ __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid
     };
     for (int i = 0; i < s.stages; ++i) load(at.row + i * at.step, ring.at + i * ring.bytes);
     if (at.group == 0) {  // the groups' in common
-        if (has_pre) put_vector<T>(pre_w, a.pre_w, nullptr, 1.0f, at);
-        if (JOIN && weighs) put_vector<T>(post_w, a.post_w, matrix ? nullptr : a.gate.p, 1.0f, at);
-        if (JOIN && matrix && a.post_b) put_vector<T>(post_b, a.post_b, nullptr, 1.0f, at);
+        const Raw<T> none = raw_vector<T>(nullptr, false, at), w1 = raw_vector<T>(a.pre_w, has_pre, at);
+        if (JOIN) {
+            const Raw<T> w0 = raw_vector<T>(a.post_w, has_post, at), b0 = raw_vector<T>(a.post_b, matrix && a.post_b, at),
+                         g0 = raw_vector<T>(a.gate.p, a.gate.p && !matrix, at);
+            if (weighs) put_vector<T>(post_w, w0, g0, 1.0f);
+            if (matrix && a.post_b) put_vector<T>(post_b, b0, none, 1.0f);
+        }
+        if (has_pre) put_vector<T>(pre_w, w1, none, 1.0f);
     }
     __syncthreads();
     constexpr int kTotals = (BIAS ? 2 : 1) * (JOIN ? 2 : 1);  // without a join sums 2 and 3, without biases 0 and 2
@@ -824,14 +848,14 @@ struct Parameters {
     void *dpost_w, *dpost_b, *dgate, *dpre_w, *dpre_b;
 };
 
-constexpr int kJoinWarps = 32;
+constexpr int kJoinWarps = 32;  // at most: one to four units
 
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps) parameters_kernel(const __grid_constant__ Parameters a)
 {
     __shared__ float turn[kSums][kJoinWarps][32];
-    const int lane = lane_id(), warp = warp_id(), j = blockIdx.x * 32 + lane;
-    const int first = (int)((int64_t)a.units * warp / kJoinWarps), last = (int)((int64_t)a.units * (warp + 1) / kJoinWarps);
+    const int lane = lane_id(), warp = warp_id(), warps = blockDim.x / 32, j = blockIdx.x * 32 + lane;
+    const int first = (int)((int64_t)a.units * warp / warps), last = (int)((int64_t)a.units * (warp + 1) / warps);
     const int count = __popc(a.sums);
     const int64_t step = (int64_t)a.units * a.part_ld;  // from one sum to the next
     start_of_inputs();
@@ -861,7 +885,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) parameters_kernel(const __gri
     for (int k = 0; k < kSums; ++k) {
         if (!(a.sums >> k & 1)) continue;
 #pragma unroll 8
-        for (int w = 0; w < kJoinWarps; ++w) all[k] += turn[slot][w][lane];
+        for (int w = 0; w < warps; ++w) all[k] += turn[slot][w][lane];
         ++slot;
     }
     const auto store = [&](void* out, float v) {
@@ -1165,7 +1189,7 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
         q.dpre_w = a.dpre_weight;
         q.dpre_b = a.dpre_bias;
     }
-    return launch_kernel(parameters_kernel<T>, (a.n + 31) / 32, 32 * kJoinWarps, 0, 1, st, q);
+    return launch_kernel(parameters_kernel<T>, (a.n + 31) / 32, 32 * std::max(1, std::min(kJoinWarps, (q.units + 3) / 4)), 0, 1, st, q);
 }
 
 int read_clear_status(int* st)
