@@ -75,24 +75,61 @@ __global__ void __launch_bounds__(kRowsThreads) pack_kernel(const RowsIn<T> in, 
     }
 }
 
+// The way back, in the same pieces: the words of scales of all units are read by
+// eight lanes and dealt out (8192 x 16384 to BF16: 65 us with a byte read for each
+// lane and unit).
+template <typename T, int UNITS>
+__global__ void __launch_bounds__(kRowsThreads) unpack_kernel(const chpl_mx4 c, const RowsOut<T> out, const int64_t items, const uint32_t segs,
+                                                              const int cols)
+{
+    __shared__ uint4 turns[kRowsThreads / 32][64];  // 256 elements of up to 4 bytes for each warp
+    start_of_inputs();
+    const int lane = lane_id();
+    const int64_t blocks = blocks_of(cols), step_items = (int64_t)gridDim.x * (kRowsThreads / 32);
+    for (int64_t i = (int64_t)blockIdx.x * (kRowsThreads / 32) + warp_id(); i < items; i += step_items) {
+        const uint32_t t = items < 0xffffffffll ? (uint32_t)i / segs : (uint32_t)(i / segs);
+        const int seg = (int)(i - (int64_t)t * segs), j0 = seg * (UNITS * kPiece) + lane * 8, block = seg * (2 * UNITS) + lane;
+        const uint8_t* codes = c.codes + (int64_t)t * c.ldc + j0 / 2;
+        uint32_t w[UNITS], four = 0;  // lane 2 u + h: the four scales of half h of unit u
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) w[u] = j0 + u * kPiece < cols ? __ldg(reinterpret_cast<const uint32_t*>(codes + u * (kPiece / 2))) : 0;
+        if (lane < 2 * UNITS && block < blocks) four = __ldg(reinterpret_cast<const uint32_t*>(c.scales + scale_at(t, block, blocks)));
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const uint32_t s = __shfl_sync(0xffffffffu, four, 2 * u + (lane >> 4)) >> (lane >> 2 & 3) * 8 & 0xffu;
+            float v[8];
+            values8(w[u], step(s), v);
+            out.put_warp(t, j0 + u * kPiece, cols, v, turns[warp_id()]);
+        }
+    }
+}
+
+// A launch over `rows` rows, in pieces of four units where rows are long and that
+// leaves every warp a piece, else of one
+template <typename L>
+static int in_pieces(int64_t rows, int64_t cols, L&& launch)
+{
+    constexpr int64_t kWarps = kRowsThreads / 32, kBlocks = 148 * 8;  // eight resident blocks per SM, then a grid stride
+    const int units = cols > kPiece && rows * ((cols + 4 * kPiece - 1) / (4 * kPiece)) >= kBlocks * kWarps ? 4 : 1;
+    const int64_t segs = (cols + units * kPiece - 1) / (units * kPiece), items = rows * segs;
+    return launch(units, std::min((items + kWarps - 1) / kWarps, kBlocks), items, (uint32_t)segs);
+}
+
 template <typename T>
 static int pack(cudaStream_t st, int64_t rows, int64_t cols, const void* x, int64_t ldx, const chpl_mx4& c)
 {
-    constexpr int64_t kWarps = kRowsThreads / 32, kBlocks = 148 * 8;  // eight resident blocks per SM, then a grid stride
-    const auto launch = [&](auto kernel, int units) {
-        const int64_t segs = (cols + units * kPiece - 1) / (units * kPiece), items = rows * segs;
-        return launch_kernel(kernel, std::min((items + kWarps - 1) / kWarps, kBlocks), kRowsThreads, 0, 1, st, rows_in<T>(x, ldx), c, items, (uint32_t)segs,
-                             (int)cols);
-    };
-    // long rows in pieces of four units, as long as that leaves every warp a piece
-    if (cols > kPiece && rows * ((cols + 4 * kPiece - 1) / (4 * kPiece)) >= kBlocks * kWarps) return launch(pack_kernel<T, 4>, 4);
-    return launch(pack_kernel<T, 1>, 1);
+    return in_pieces(rows, cols, [&](int units, int64_t blocks, int64_t items, uint32_t segs) {
+        return launch_kernel(units == 4 ? pack_kernel<T, 4> : pack_kernel<T, 1>, blocks, kRowsThreads, 0, 1, st, rows_in<T>(x, ldx), c, items, segs, (int)cols);
+    });
 }
 
 template <typename T>
 static int unpack(cudaStream_t st, int64_t rows, int64_t cols, void* x, int64_t ldx, const chpl_mx4& c)
 {
-    return run_rows(st, RowsJob<In, RowsOut<T>, Keep>(in(c, cols), rows_out<T>(x, ldx), Keep(), rows, cols));
+    return in_pieces(rows, cols, [&](int units, int64_t blocks, int64_t items, uint32_t segs) {
+        return launch_kernel(units == 4 ? unpack_kernel<T, 4> : unpack_kernel<T, 1>, blocks, kRowsThreads, 0, 1, st, c, rows_out<T>(x, ldx), items, segs,
+                             (int)cols);
+    });
 }
 
 int pack(cudaStream_t st, int type, int64_t rows, int64_t cols, const void* x, int64_t ldx, const chpl_mx4& c)

@@ -85,29 +85,6 @@ __device__ __forceinline__ void values8(uint32_t w, float st, float* v)
     }
 }
 
-// ----------------------------------------------------------------------------
-// eight consecutive elements of a row in this format, as one lane of rows_kernel
-// holds them: a warp's 256 are one piece
-// ----------------------------------------------------------------------------
-struct In {
-    chpl_mx4 c;
-    int64_t blocks;
-    struct Raw {
-        uint32_t w, s;
-    };
-    __device__ __forceinline__ Raw raw(int64_t t, int j, int cols) const
-    {
-        Raw r = {0, kMinScale};
-        if (j >= cols) return r;
-        r.w = __ldg(reinterpret_cast<const uint32_t*>(c.codes + t * c.ldc + j / 2));
-        r.s = c.scales[scale_at((uint32_t)t, j / 128, blocks) + j / kGroup % 4];
-        return r;
-    }
-    __device__ __forceinline__ void value(const Raw& r, float (&v)[8]) const { values8(r.w, step(r.s), v); }
-};
-
-inline In in(const chpl_mx4& c, int64_t cols) { return {c, blocks_of(cols)}; }
-
 int check_mx4(const char* who, const char* what, const chpl_mx4& c, int64_t rows, int64_t cols);
 int pack(cudaStream_t st, int type, int64_t rows, int64_t cols, const void* x, int64_t ldx, const chpl_mx4& c);
 
