@@ -420,10 +420,11 @@ __device__ __forceinline__ void put(const RowsTo& out, uint32_t t, const Place& 
 // ----------------------------------------------------------------------------
 // sums over a row
 // ----------------------------------------------------------------------------
+template <int LANES = 32>
 __device__ __forceinline__ float warp_sum(float a)
 {
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2) a += __shfl_xor_sync(0xffffffffu, a, d);
+    for (int d = LANES / 2; d > 0; d /= 2) a += __shfl_xor_sync(0xffffffffu, a, d);
     return a;
 }
 
@@ -454,6 +455,7 @@ struct RowSums {
     uint32_t mine, from;  // where the warp puts its sums, and where a lane reads one (or the zero)
     uint64_t* bar;        // of the group
     bool leads;           // its first warp
+    bool few;             // up to eight warps share the row: every eight lanes read all of their sums
     int warps, group, cluster;
     uint32_t set, phase;  // of the next use; the barriers' parity
     volatile int* gave_up;
@@ -464,7 +466,9 @@ struct RowSums {
         const int lane = lane_id(), warp = warp_id() - group * warps;
         const int row = cluster > 1 ? group : 0, first = cluster > 1 ? (int)cluster_ctarank() * warps : group * warps;
         mine = smem_u32(&sets.of[0][row][first + warp]);
-        from = smem_u32(&sets.of[0][row][lane < cluster * warps ? (cluster > 1 ? 0 : first) + lane : kMaxWarps]);
+        few = cluster * warps <= 8;
+        const int entry = few ? lane % 8 : lane;
+        from = smem_u32(&sets.of[0][row][entry < cluster * warps ? (cluster > 1 ? 0 : first) + entry : kMaxWarps]);
         bar = &sets.bar[0][row];
         leads = warp == 0;
         if (threadIdx.x < 2 * kClusterGroups) {
@@ -500,7 +504,9 @@ struct RowSums {
     __device__ __forceinline__ float one(float a)
     {
         a = warp_sum(a);
-        return warps * cluster == 1 ? a : warp_sum(exchange(a, 0.0f).x);
+        if (warps * cluster == 1) return a;
+        a = exchange(a, 0.0f).x;
+        return few ? warp_sum<8>(a) : warp_sum(a);
     }
     __device__ __forceinline__ float2 both_of(float a, float b)
     {
@@ -508,7 +514,7 @@ struct RowSums {
         b = warp_sum(b);
         if (warps * cluster == 1) return make_float2(a, b);
         const float2 v = exchange(a, b);
-        return make_float2(warp_sum(v.x), warp_sum(v.y));
+        return few ? make_float2(warp_sum<8>(v.x), warp_sum<8>(v.y)) : make_float2(warp_sum(v.x), warp_sum(v.y));
     }
 };
 
