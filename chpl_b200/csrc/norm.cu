@@ -217,17 +217,19 @@ __device__ __forceinline__ void expand(const uint32_t (&w)[4], int h, Some& r)
     }
 }
 
-// features of a warp's 1024 bytes of shared memory in order, the lane's own
+// features of a warp's 1024 bytes of shared memory in order; at: the lane's first
+// (one address register for all of an operand's accesses, here and below: join of
+// 16384 x 4096 99.5 -> 97.9 us)
+static_assert(kHalves == 2, "the accesses below");
 template <typename T>
-__device__ __forceinline__ Some packed_at(uint32_t piece)
+__device__ __forceinline__ Some packed_at(uint32_t at)
 {
     Some r;
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-        uint32_t w[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(piece + h * 512 + lane_id() * 16) : "memory");
-        expand<T>(w, h, r);
-    }
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    expand<T>(w, 0, r);
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4 + 512];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    expand<T>(w, 1, r);
     return r;
 }
 
@@ -268,7 +270,7 @@ __device__ __forceinline__ Raw<T> raw_vector(const void* v, bool there, const Pl
 // the products.  (All of a kernel's vectors are read before the first is put: one
 // latency, not one for each, which a single row waits for.)
 template <typename T>
-__device__ __forceinline__ void put_vector(uint32_t piece, const Raw<T>& u, const Raw<T>& v, float factor)
+__device__ __forceinline__ void put_vector(uint32_t at, const Raw<T>& u, const Raw<T>& v, float factor)
 {
 #pragma unroll
     for (int h = 0; h < kHalves; ++h)
@@ -276,30 +278,32 @@ __device__ __forceinline__ void put_vector(uint32_t piece, const Raw<T>& u, cons
         for (int i = 0; i < 4; i += 2) {
             const float2 a = linear::unpack2<T>(u.w[h][i]), b = linear::unpack2<T>(u.w[h][i + 1]), c = linear::unpack2<T>(v.w[h][i]),
                          d = linear::unpack2<T>(v.w[h][i + 1]);
-            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(piece + h * 1024 + i * 256 + lane_id() * 16), "f"(a.x * c.x * factor),
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + h * 1024 + i * 256), "f"(a.x * c.x * factor),
                          "f"(a.y * c.y * factor), "f"(b.x * d.x * factor), "f"(b.y * d.y * factor)
                          : "memory");
         }
 }
-__device__ __forceinline__ Some vector_at(uint32_t piece)
+__device__ __forceinline__ Some vector_at(uint32_t at)
 {
     Some r;
-#pragma unroll
-    for (int i = 0; i < kTwos; i += 2)
-        asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(r.v[i].v), "=l"(r.v[i + 1].v) : "r"(piece + i * 256 + lane_id() * 16) : "memory");
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(r.v[0].v), "=l"(r.v[1].v) : "r"(at) : "memory");
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2 + 512];" : "=l"(r.v[2].v), "=l"(r.v[3].v) : "r"(at) : "memory");
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2 + 1024];" : "=l"(r.v[4].v), "=l"(r.v[5].v) : "r"(at) : "memory");
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2 + 1536];" : "=l"(r.v[6].v), "=l"(r.v[7].v) : "r"(at) : "memory");
     return r;
 }
 
+// rows of 16-bit features, `ld` bytes apart
 struct Rows {
     const void* p;
     int64_t ld;
-    __device__ __forceinline__ const unsigned short* row(uint32_t t) const { return static_cast<const unsigned short*>(p) + (uint64_t)ld * t; }
+    __device__ __forceinline__ const char* row(uint32_t t) const { return static_cast<const char*>(p) + (uint64_t)ld * t; }
 };
 struct RowsTo {
     void* p;
     int64_t ld;
     bool aligned;  // 16-byte stores fit
-    __device__ __forceinline__ unsigned short* row(uint32_t t) const { return static_cast<unsigned short*>(p) + (uint64_t)ld * t; }
+    __device__ __forceinline__ char* row(uint32_t t) const { return static_cast<char*>(p) + (uint64_t)ld * t; }
 };
 
 __device__ __forceinline__ void copy16(uint32_t slot, const void* src, int bytes)
@@ -315,27 +319,25 @@ __device__ __forceinline__ void copy16(uint32_t slot, const void* src, int bytes
 template <bool ALIGNED>
 __device__ __forceinline__ void fetch_row(uint32_t piece, const Rows& x, uint32_t t, uint32_t tokens, const Place& at)
 {
-    const int lane = lane_id();
-    const unsigned short* row = x.row(t);
-    if (ALIGNED) {
+    const char* row = x.row(t);
+    if (ALIGNED) {  // piece: of the lane
         if (at.whole()) {
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h) copy16(piece + h * 512 + lane * 16, row + at.first + 256 * h, 16);
+            asm volatile(
+                "cp.async.cg.shared.global [%0], [%1], 16;\n\t"
+                "cp.async.cg.shared.global [%0 + 512], [%1 + 512], 16;" ::"r"(piece), "l"(row + 2u * (uint32_t)at.first)
+                : "memory");
         } else {
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
                 const int have = at.have(h);
-                copy16(piece + h * 512 + lane * 16, row + (have > 0 ? at.first + 256 * h : 0), 2 * have);
+                copy16(piece + h * 512, row + (have > 0 ? 2 * (at.first + 256 * h) : 0), 2 * have);
             }
         }
         return;
     }
-    const unsigned short* p = row + (at.first - lane * 8);
-    const char* from = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
-    const char* begin = static_cast<const char*>(x.p);
-    const int n = at.first + at.left;
-    const char* row_end = reinterpret_cast<const char*>(row + n);
-    const char* end = reinterpret_cast<const char*>(x.row(tokens - 1) + n);
+    const int lane = lane_id(), n = at.first + at.left;
+    const char* from = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(row + 2 * (at.first - lane * 8)) & ~(uintptr_t)15);
+    const char *begin = static_cast<const char*>(x.p), *row_end = row + 2 * n, *end = x.row(tokens - 1) + 2 * n;
     for (int c = lane; c < 32 * kHalves + 1; c += 32) {
         const char* src = from + c * 16;
         if (src >= row_end) break;
@@ -357,7 +359,7 @@ __device__ __forceinline__ Some row_at(uint32_t piece, const Rows& x, uint32_t t
     if (ALIGNED) return packed_at<T>(piece);
     Some r;
     const int lane = lane_id();
-    const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(x.row(t) + (at.first - lane * 8)) & 15u;  // bytes before the first feature
+    const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(x.row(t) + 2 * (at.first - lane * 8)) & 15u;  // bytes before the first feature
     const uint32_t from = piece + lane * 16 + (skew & ~3u);
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
@@ -381,7 +383,7 @@ __device__ __forceinline__ Some row_at(uint32_t piece, const Rows& x, uint32_t t
 template <typename T>
 __device__ __forceinline__ void put(const RowsTo& out, uint32_t t, const Place& at, const Some& v, uint32_t turn)
 {
-    unsigned short* const row = out.row(t) + at.first;
+    unsigned short* const row = reinterpret_cast<unsigned short*>(out.row(t) + 2 * at.first);
     const int lane = lane_id();
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
@@ -522,11 +524,10 @@ struct RowSums {
 // `stages` of them (an empty group where there is no such row).
 struct Ring {
     uint32_t tensor, bytes, end;  // between tensors, of a stage, behind the last one
-    uint32_t at;                  // the warp's piece of the current row's first tensor
+    uint32_t at;                  // the warp's (the lane's, where rows are aligned) piece of the current row's first tensor
     int stages;
-    __device__ __forceinline__ Ring(uint32_t mem, int tensors, const Shape& s)
-        : tensor((blockDim.x >> 5) * s.piece), bytes(tensors * tensor), end(mem + warp_id() * s.piece + s.stages * bytes), at(mem + warp_id() * s.piece),
-          stages(s.stages)
+    __device__ __forceinline__ Ring(uint32_t mine, int tensors, const Shape& s)
+        : tensor((blockDim.x >> 5) * s.piece), bytes(tensors * tensor), end(mine + s.stages * bytes), at(mine), stages(s.stages)
     {
     }
     __device__ __forceinline__ static void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -587,14 +588,14 @@ __global__ void __launch_bounds__(kForwardThreads) forward_kernel(const __grid_c
     const Place at(s, a.n);
     const bool matrix = JOIN && a.gate.p && a.gate.ld;
     const int tensors = JOIN ? 2 + matrix : 1;
-    const uint32_t mem = smem_u32(smem), vec = mem + (warp_id() - at.group * s.warps) * kVectorBytes, vec_step = s.warps * kVectorBytes,
+    const uint32_t mem = smem_u32(smem), vec = mem + (warp_id() - at.group * s.warps) * kVectorBytes + lane_id() * 16, vec_step = s.warps * kVectorBytes,
                    turn = mem + s.turn + warp_id() * 512;
     // the vectors that there are, then the rows; a vector gate and the scale are in post_w and post_b
     uint32_t used = 0;
     const auto place = [&](bool there) { return vec + (there ? used++ : 0) * vec_step; };
     const bool weighs = JOIN && (a.post || (a.gate.p && !matrix));
     const uint32_t pre_w = place(a.pre), pre_b = place(a.pre_b), post_w = JOIN ? place(weighs) : 0, post_b = JOIN ? place(a.post_b) : 0;
-    Ring ring(mem + used * vec_step, tensors, s);
+    Ring ring(mem + used * vec_step + warp_id() * s.piece + (ALIGNED ? lane_id() * 16 : 0), tensors, s);
     RowSums sums(sets, s, at.group);
     const float inv_n = 1.0f / (float)a.n;
     start_of_inputs();
@@ -702,13 +703,13 @@ __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid
     __shared__ WarpSums sets;
     const Place at(s, a.n);
     const bool matrix = JOIN && part<PARTS>(kMatrix, a.gate.p && a.gate.ld), has_y = JOIN && (has_post || a.y.p), weighs = JOIN && (has_post || (a.gate.p && !matrix));
-    const int t_dh = a.dr.p ? 1 : 0, t_r = t_dh + 1, t_y = has_pre ? t_r + 1 : t_dh, t_gate = t_y + has_y, tensors = t_gate + matrix;
-    const uint32_t mem = smem_u32(smem), vec = mem + (warp_id() - at.group * s.warps) * kVectorBytes, vec_step = s.warps * kVectorBytes,
+    const int t_dh = 0, t_r = 1, t_y = has_pre ? 2 : 0, t_gate = t_y + has_y, t_dr = t_gate + matrix, tensors = t_dr + (a.dr.p ? 1 : 0);
+    const uint32_t mem = smem_u32(smem), vec = mem + (warp_id() - at.group * s.warps) * kVectorBytes + lane_id() * 16, vec_step = s.warps * kVectorBytes,
                    turn = mem + s.turn + warp_id() * 512;
     uint32_t used = 0;  // a vector gate is in post_w
     const auto place = [&](bool there) { return vec + (there ? used++ : 0) * vec_step; };
     const uint32_t pre_w = place(has_pre), post_w = JOIN ? place(weighs) : 0, post_b = JOIN ? place(matrix && a.post_b) : 0;
-    Ring ring(mem + used * vec_step, tensors, s);
+    Ring ring(mem + used * vec_step + warp_id() * s.piece + (ALIGNED ? lane_id() * 16 : 0), tensors, s);
     RowSums sums(sets, s, at.group);
     const float inv_n = 1.0f / (float)a.n;
     const auto of = [&](int t, const Rows& x, uint32_t row) { return row_at<T, ALIGNED>(ring.at + t * ring.tensor, x, row, at); };
@@ -716,7 +717,7 @@ __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid
     const auto load = [&](uint32_t row, uint32_t slot) {
         if (row < a.tokens) {
             const auto fetch = [&](int t, const Rows& x) { fetch_row<ALIGNED>(slot + t * ring.tensor, x, row, a.tokens, at); };
-            if (a.dr.p) fetch(0, a.dr);
+            if (a.dr.p) fetch(t_dr, a.dr);
             if (has_pre) {
                 fetch(t_dh, a.dh);
                 fetch(t_r, a.r);
@@ -766,9 +767,9 @@ __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid
             const Pull p = pull(g, c, a.pre, pre.y, inv_n, sums);
             d = fma_of(c, -p.along, g);
             if (a.pre == CHPL_NORM_LAYER) d = d + -p.mean;
-            if (a.dr.p) d = d + of(0, a.dr, row);
+            if (a.dr.p) d = d + of(t_dr, a.dr, row);
         } else {
-            d = of(0, a.dr, row);
+            d = of(t_dr, a.dr, row);
         }
         if (a.dx.p) put<T>(a.dx, row, at, JOIN ? d * a.residual_scale : d, turn);
         if (JOIN) {
@@ -988,14 +989,14 @@ static int forward(cudaStream_t st, const chpl_norm_fwd& a)
     f.n = (int)a.n;
     f.scale = a.scale;
     f.residual_scale = a.residual_scale;
-    f.x = {a.x, a.ldx};
+    f.x = {a.x, a.ldx * 2};
     bool in = fits(a.x, a.ldx, a.tokens), out = true;
     if (a.join) {
         f.post = a.post.kind;
         f.post_eps = a.post.eps;
-        f.y = {a.y, a.ldy};
-        f.gate = {a.gate, a.ldgate};
-        f.r = {a.r, a.ldr, fits(a.r, a.ldr, a.tokens)};
+        f.y = {a.y, a.ldy * 2};
+        f.gate = {a.gate, a.ldgate * 2};
+        f.r = {a.r, a.ldr * 2, fits(a.r, a.ldr, a.tokens)};
         in = in && fits(a.y, a.ldy, a.tokens) && (a.ldgate == 0 || fits(a.gate, a.ldgate, a.tokens));
         out = f.r.aligned;
         if (f.post) {
@@ -1009,7 +1010,7 @@ static int forward(cudaStream_t st, const chpl_norm_fwd& a)
         f.pre_eps = a.pre.eps;
         f.pre_w = a.pre.weight;
         f.pre_b = a.pre.bias;
-        f.h = {a.h, a.ldh, fits(a.h, a.ldh, a.tokens)};
+        f.h = {a.h, a.ldh * 2, fits(a.h, a.ldh, a.tokens)};
         f.pre_stats = reinterpret_cast<float2*>(a.pre_stats);
         out = out && f.h.aligned;
     }
@@ -1147,20 +1148,20 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
         b.sums = p.sums;
         b.part = p.sums ? static_cast<float*>(work) : nullptr;
         b.part_ld = p.part_ld;
-        b.dr = {a.dr, a.lddr};
-        b.dx = {a.dx, a.lddx, fits(a.dx, a.lddx, a.tokens)};
+        b.dr = {a.dr, a.lddr * 2};
+        b.dx = {a.dx, a.lddx * 2, fits(a.dx, a.lddx, a.tokens)};
         if (a.pre.kind) {
             b.pre = a.pre.kind;
-            b.dh = {a.dh, a.lddh};
-            b.r = {a.r, a.ldr};
+            b.dh = {a.dh, a.lddh * 2};
+            b.r = {a.r, a.ldr * 2};
             b.pre_w = a.pre.weight;
             b.pre_stats = reinterpret_cast<const float2*>(a.pre_stats);
         }
         if (a.join) {
-            if (a.post.kind || a.gate) b.y = {a.y, a.ldy};
-            b.gate = {a.gate, a.ldgate};
-            b.dy = {a.dy, a.lddy, fits(a.dy, a.lddy, a.tokens)};
-            if (matrix) b.dgate = {a.dgate, a.lddgate, fits(a.dgate, a.lddgate, a.tokens)};
+            if (a.post.kind || a.gate) b.y = {a.y, a.ldy * 2};
+            b.gate = {a.gate, a.ldgate * 2};
+            b.dy = {a.dy, a.lddy * 2, fits(a.dy, a.lddy, a.tokens)};
+            if (matrix) b.dgate = {a.dgate, a.lddgate * 2, fits(a.dgate, a.lddgate, a.tokens)};
             if (a.post.kind) {
                 b.post = a.post.kind;
                 b.post_w = a.post.weight;
