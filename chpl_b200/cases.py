@@ -104,8 +104,9 @@ def fp64_case(what: str, m: int, n: int, k: int, reps: int) -> dict:
 
 def ffn_case(tokens: int, d: int, hidden: int, act: str, steps: int) -> dict:
     """A few steps of gradient descent on Y = act(X W1^T + b1) W2^T + b2 + X (BF16, X in hand, a target made by another
-    random block), holding 8-bit checkpoints between the passes; then one token through it."""
-    from . import ffn
+    random block), holding 8-bit checkpoints between the passes; then one token through it, from 16-bit and from 4-bit
+    weights, and through the sublayer of it (the norm before, the join with the residual stream)."""
+    from . import ffn, mx4, norm
     g = torch.Generator(device="cuda")
     g.manual_seed(3)
 
@@ -131,18 +132,27 @@ def ffn_case(tokens: int, d: int, hidden: int, act: str, steps: int) -> dict:
         ms.append(e0.elapsed_time(e1))
     flops = 12.0 * tokens * d * hidden
     one = x[:1]
-    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-    for _ in range(3):
-        ffn.forward(one, *w, act=act, residual=True)
-    e0.record()
-    for _ in range(20):
-        ffn.forward(one, *w, act=act, residual=True)
-    e1.record()
-    torch.cuda.synchronize()
+
+    def timed(f):
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        for _ in range(3):
+            f()
+        e0.record()
+        for _ in range(20):
+            f()
+        e1.record()
+        torch.cuda.synchronize()
+        return e0.elapsed_time(e1) / 20 * 1e3
+
+    us = timed(lambda: ffn.forward(one, *w, act=act, residual=True))
+    coded = [mx4.pack(w[0]), w[1], mx4.pack(w[2]), w[3]]
+    n = norm.Norm(torch.ones(d, dtype=torch.bfloat16, device="cuda"))
+    us4 = timed(lambda: ffn.forward(one, *coded, act=act, residual=True))
+    us_layer = timed(lambda: ffn.sublayer(one, n, *coded, act=act, post=n, pre=n))
     return {"case": "ffn", "tokens": tokens, "d": d, "hidden": hidden, "act": act, "loss": loss, "step_ms": min(ms),
             "tflops": flops / min(ms) / 1e9, "held_bytes": saved.x.nbytes() + saved.z.nbytes(),
-            "held_bytes_16bit": 2 * tokens * (d + 2 * hidden), "one_token_us": e0.elapsed_time(e1) / 20 * 1e3,
-            "one_token_gbs": 4.0 * d * hidden / (e0.elapsed_time(e1) / 20 * 1e-3) / 1e9}
+            "held_bytes_16bit": 2 * tokens * (d + 2 * hidden), "one_token_us": us,
+            "one_token_gbs": 4.0 * d * hidden / us / 1e3, "one_token_4bit_us": us4, "one_token_4bit_sublayer_us": us_layer}
 
 
 def panel_case(m: int, n: int, reps: int) -> dict:

@@ -394,7 +394,8 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
 // The next tile's products start when those have been read (32 arrivals), the
 // other columns are read under them.  A warp that has arrived for a tile has read
 // all it reads of the tile before, whose other columns the next one overwrites.
-// (8192 x 4096 x 16384 with tiles of 192 rows and accumulators apart: 243 us.)
+// 8192 x 4096 x 16384 with GELU: 220 us, 5.0 PFLOP/s (243 with tiles of 192 rows and
+// accumulators apart); without copies into the stages 174, without outputs 167.
 //
 //   warp 0      TMA producer (both CTAs)
 //   warp 1      TMEM allocation; tcgen05 issue (even CTA)

@@ -4,13 +4,20 @@
 // gate * Npost(y), together with the next block's norm h = Npre(r).
 //
 // Bound: HBM; every row is read and written once.  A row lies in the registers
-// of one CTA (of a cluster above 8192 features), sixteen features a thread, so
-// that the statistics' passes over it cost no memory traffic and the gradients'
-// sums over the tokens stay in registers from a CTA's first row to its last.
-// Sixteen, because what a row costs a thread beside its features (sums over the
-// row, addresses, waits) bounds the kernels with eight: join of 8192 x 4096 68 us,
-// its gradients 136.  The rows to come are on their way into shared memory meanwhile,
-// every warp copying what it will itself read: no barrier waits for a copy.
+// of one CTA (a wide one of a cluster), sixteen features a thread, so that the
+// statistics' passes over it cost no memory traffic and the gradients' sums over
+// the tokens stay in registers from a CTA's first row to its last.  Sixteen,
+// because what a row costs a thread beside its features (sums over the row,
+// addresses, waits) bounds the kernels with eight: join of 8192 x 4096 68 -> 59 us,
+// its gradients 136 -> 101 by that step.  The rows to come are on their way into
+// shared memory meanwhile, every warp copying what it will itself read: no barrier
+// waits for a copy.
+//
+// Measured (BF16, from launch to launch): 8192 x 4096 with two RMS norms and a
+// vector gate 53 us (5.1 TB/s), its gradients 84 (4.8); layer norm's gradients with
+// a skip's 62 (4.3, the launch for the parameters in it); a copy by torch 6.05 TB/s.
+// What is left is the latency of the sums over a row beside issue slots 50 to 60 %
+// busy: rows of 512 features, a warp's own, run at 5.6 to 6.0 TB/s.
 #include <algorithm>
 #include <cmath>
 
@@ -31,7 +38,7 @@ constexpr int kMaxWidth = kForwardThreads * 8 * kHalves;
 constexpr int kMaxCluster = 4;
 constexpr int kClusterGroups = 4;                   // of a CTA in a cluster
 constexpr int kMaxStages = 4;
-constexpr int kVectorBytes = 1024 * kHalves;         // of a warp's features as FP32
+constexpr int kVectorBytes = 1024 * kHalves;        // of a warp's features as FP32
 constexpr int kSmem = 227 * 1024;                   // of an SM
 constexpr int kSmemApart = 2304;                    // of which a CTA takes, beside what it asks for
 
@@ -54,9 +61,9 @@ struct Shape {
 // another waits for its row's sums.  A cluster of two or four CTAs shares a row
 // where that keeps clearly more of the GPU's threads at work (or where a row and
 // the weights do not fit into one CTA's shared memory): gradients of a join with two
-// norms, 13107 x 5120, 223 us alone (one group of ten warps an SM), 192 in clusters of
-// two (three groups of five warps); 8192 x 8192 189 and 192; 5461 x 12288 228 in
-// clusters of two, 245 of four.
+// norms, 13107 x 5120, take 14 % less in clusters of two (three groups of five warps)
+// than alone (one of ten), 8192 x 8192 the same, 5461 x 12288 7 % more in clusters of
+// four than of two.
 static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors, bool inputs_aligned, bool outputs_aligned, int threads)
 {
     constexpr int kSms = 148, kNamed = 15;  // named barriers, one to a group of several warps
@@ -476,11 +483,9 @@ struct RowSums {
         if (threadIdx.x < 2 * kClusterGroups) {
             sets.of[threadIdx.x / kClusterGroups][threadIdx.x % kClusterGroups][kMaxWarps] = make_float2(0.0f, 0.0f);
             mbar_init(&sets.bar[threadIdx.x / kClusterGroups][threadIdx.x % kClusterGroups], 1);
-        }
-        if (threadIdx.x == 0) {
-            sets.gave_up = 0;
             fence_barrier_init();
         }
+        if (threadIdx.x == 0) sets.gave_up = 0;
         if (cluster > 1) cluster_sync();
         else __syncthreads();
     }
@@ -643,7 +648,7 @@ __global__ void __launch_bounds__(kForwardThreads) forward_kernel(const __grid_c
             put<T>(a.h, row, at, v, turn);
         }
     }
-    if (s.cluster > 1) cluster_sync();  // no CTA leaves while another still reads its sums
+    if (s.cluster > 1) cluster_sync();  // no CTA leaves while another still sends to it
 }
 
 // ----------------------------------------------------------------------------
