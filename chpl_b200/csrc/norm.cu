@@ -14,10 +14,10 @@
 // waits for a copy.
 //
 // Measured (BF16, from launch to launch): 8192 x 4096 with two RMS norms and a
-// vector gate 53 us (5.1 TB/s), its gradients 84 (4.8); layer norm's gradients with
-// a skip's 62 (4.3, the launch for the parameters in it); a copy by torch 6.05 TB/s.
-// What is left is the latency of the sums over a row beside issue slots 50 to 60 %
-// busy: rows of 512 features, a warp's own, run at 5.6 to 6.0 TB/s.
+// vector gate 47.5 us (5.7 TB/s), its gradients 71.5 (5.6); layer norm's gradients
+// with a skip's 51.7 (5.2, the launch for the parameters in it); a copy by torch 6.05
+// TB/s.  What is left is the latency of the sums over a row, and rows below 512
+// features, of which a warp takes as long as for 512.
 #include <algorithm>
 #include <cmath>
 
@@ -37,10 +37,10 @@ constexpr int kMaxWarps = kForwardThreads / 32;
 constexpr int kMaxWidth = kForwardThreads * 8 * kHalves;
 constexpr int kMaxCluster = 4;
 constexpr int kClusterGroups = 4;                   // of a CTA in a cluster
-constexpr int kMaxStages = 4;
+constexpr int kMaxStages = 2;                       // four: gradients of 8192 x 4096 53.8 us, not 51.7
 constexpr int kVectorBytes = 1024 * kHalves;        // of a warp's features as FP32
 constexpr int kSmem = 227 * 1024;                   // of an SM
-constexpr int kSmemApart = 2304;                    // of which a CTA takes, beside what it asks for
+constexpr int kSmemApart = 2304;                    // of which a CTA takes, beside what it asks for, in whole lines
 
 // ----------------------------------------------------------------------------
 // shape of a launch
@@ -526,7 +526,10 @@ struct RowSums {
 };
 
 // The rows under way: copies of the rows to come, a group of cp.async each,
-// `stages` of them (an empty group where there is no such row).
+// `stages` of them (an empty group where there is no such row).  Aligned rows' pieces start on
+// 128 bytes, so that a warp's access touches no more lines than it has bytes for (16
+// bytes off: join of 8192 x 4096 53 us instead of 47.4, its gradients 84 instead of
+// 73.5).
 struct Ring {
     uint32_t tensor, bytes, end;  // between tensors, of a stage, behind the last one
     uint32_t at;                  // the warp's (the lane's, where rows are aligned) piece of the current row's first tensor
@@ -540,9 +543,8 @@ struct Ring {
     template <bool ALIGNED>
     __device__ __forceinline__ void wait() const
     {
-        if (stages == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
-        else if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-        else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        static_assert(kMaxStages == 2, "the groups waited for");
+        if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
         else asm volatile("cp.async.wait_group 0;" ::: "memory");
         if (!ALIGNED) __syncwarp();
     }
@@ -588,7 +590,7 @@ __device__ __forceinline__ Some normalize(Some v, const Place& at, int kind, flo
 template <typename T, bool ALIGNED, bool JOIN>
 __global__ void __launch_bounds__(kForwardThreads) forward_kernel(const __grid_constant__ Forward a, const Shape s)
 {
-    extern __shared__ uint4 smem[];
+    extern __shared__ __align__(128) uint4 smem[];
     __shared__ WarpSums sets;
     const Place at(s, a.n);
     const bool matrix = JOIN && a.gate.p && a.gate.ld;
@@ -704,7 +706,7 @@ template <typename T, bool ALIGNED, bool JOIN, bool BIAS, int PARTS>
 __global__ void __launch_bounds__(kBackwardThreads) backward_kernel(const __grid_constant__ Backward a, const Shape s)
 {
     const bool has_pre = part<PARTS>(kPre, a.pre), has_post = JOIN && part<PARTS>(kPost, a.post);
-    extern __shared__ uint4 smem[];
+    extern __shared__ __align__(128) uint4 smem[];
     __shared__ WarpSums sets;
     const Place at(s, a.n);
     const bool matrix = JOIN && part<PARTS>(kMatrix, a.gate.p && a.gate.ld), has_y = JOIN && (has_post || a.y.p), weighs = JOIN && (has_post || (a.gate.p && !matrix));
