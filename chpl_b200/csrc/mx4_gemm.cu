@@ -134,7 +134,7 @@ __device__ __forceinline__ void stage_products(uint32_t d, uint32_t codes_lo, ui
 // ----------------------------------------------------------------------------
 constexpr int SPLIT_THREADS = 256;
 constexpr int CODE_WARPS = SPLIT_THREADS / 32 - 2;
-constexpr int CODE_ROWS = 4;     // that a warp codes at a time
+constexpr int CODE_ROWS = 4;     // that a warp codes at a time, a unit
 constexpr int JOIN = 4;          // rows that a warp joins at a time
 constexpr int JOIN_LD = BM + 4;  // row distance of the partial sums: a lane quad's rows in different banks
 
@@ -143,6 +143,19 @@ struct SplitShape {
     int split;   // CTAs per tile
     int stages;
 };
+
+// The units of a stage, and the warps that all units are dealt out to in order.  A
+// warp waits for a stage by the parity of its use, which tells a turn of the ring from
+// the one before but not from the one before that.  With no more warps than one turn
+// has units, a warp's next unit is at most one turn further; its last wait saw the
+// stage of a turn before that read, so the use before the last of the stage that it
+// comes to has been read, and the parity names the last one.  (Two CTAs to an SM have
+// rings of five stages: five warps for up to four rows.)
+__host__ __device__ constexpr int code_units(int rows) { return (rows + CODE_ROWS - 1) / CODE_ROWS; }
+__host__ __device__ constexpr int code_warps(int stages, int rows)
+{
+    return CODE_WARPS < stages * code_units(rows) ? CODE_WARPS : stages * code_units(rows);
+}
 
 // blocks of scales that a tile's rows lie in: tiles start on multiples of 64
 __host__ __device__ constexpr int row_blocks(int bn) { return bn <= 128 ? 1 : 2; }
@@ -177,7 +190,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
     const int kb0 = (int)((int64_t)kblocks * rank / sh.split), kb1 = (int)((int64_t)kblocks * (rank + 1) / sh.split);
     const uint32_t cols = tmem_cols(sh.bn);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < sh.stages; ++s) { mbar_init(&full[s], CODES ? 1 + (e.n + CODE_ROWS - 1) / CODE_ROWS : 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < sh.stages; ++s) { mbar_init(&full[s], CODES ? 1 + code_units(e.n) : 1); mbar_init(&empty[s], 1); }
         mbar_init(done, 1);
         *abort_flag = 0;
         fence_barrier_init();
@@ -245,11 +258,11 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
             mma_commit(done);
         }
         __syncwarp();
-    } else if (CODES) {
+    } else if (CODES && warp - 2 < code_warps(sh.stages, e.n)) {
         // units of CODE_ROWS rows in one stage, dealt out to the warps in order; the next
         // unit's rows are read while one is coded
         using Raw = typename RowsIn<T>::Raw;
-        const int parts = (e.n + CODE_ROWS - 1) / CODE_ROWS, units = (kb1 - kb0) * parts;
+        const int parts = code_units(e.n), units = (kb1 - kb0) * parts, coders = code_warps(sh.stages, e.n);
         Raw next[CODE_ROWS];
         const auto fetch = [&](int unit) {
             if (unit >= units) return;
@@ -260,13 +273,13 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 2)
         };
         int unit = warp - 2;
         fetch(unit);
-        for (; unit < units; unit += CODE_WARPS) {
+        for (; unit < units; unit += coders) {
             const int turn = unit / parts, row = (unit - turn * parts) * CODE_ROWS, stage = turn % sh.stages;
             Raw raw[CODE_ROWS];
             uint32_t w[CODE_ROWS], s[CODE_ROWS];
 #pragma unroll
             for (int i = 0; i < CODE_ROWS; ++i) raw[i] = next[i];
-            fetch(unit + CODE_WARPS);
+            fetch(unit + coders);
 #pragma unroll
             for (int i = 0; i < CODE_ROWS; ++i) {
                 s[i] = x.top(raw[i]);
@@ -750,6 +763,22 @@ int read_clear_status(int* st)
 
 }  // namespace mx4
 }  // namespace chpl
+
+extern "C" int chpl_diag_mx4_ring(int64_t features, int64_t rows, int64_t contraction, int64_t ring[3])
+{
+    using namespace chpl::mx4;
+    const char* who = "diag_mx4_ring";
+    CHPL_TRY(chpl::linear::check_size(who, "features", features));
+    CHPL_TRY(chpl::linear::check_size(who, "rows", rows));
+    CHPL_TRY(chpl::linear::check_size(who, "contraction", contraction));
+    if (!ring || !features || !rows) { chpl::set_error("%s: nothing to plan", who); return CHPL_ERR_INVALID; }
+    const Plan p = plan_for((int)features, (int)rows, (int)((contraction + kPiece - 1) / kPiece));
+    const bool coded = rows <= kCodedRows;
+    ring[0] = p.pair ? p.tiles.stages : p.split.stages;
+    ring[1] = coded ? code_units((int)rows) : 0;
+    ring[2] = coded ? code_warps(p.split.stages, (int)rows) : 0;
+    return CHPL_OK;
+}
 
 extern "C" int chpl_diag_mx4_plan(int64_t features, int64_t rows, int64_t contraction, int64_t plan[3])
 {

@@ -281,6 +281,9 @@ int chpl_diag_linear_wait(void *stream, uint64_t limit_ns);
 int chpl_diag_linear_plan(int product, int64_t features, int64_t rows, int64_t contraction, int64_t plan[4]);
 /* The same for chpl_mx4_linear (features = n, rows = tokens, contraction = k): plan[0] to plan[2] as above. */
 int chpl_diag_mx4_plan(int64_t features, int64_t rows, int64_t contraction, int64_t plan[3]);
+/* And its ring in shared memory: ring[0]: stages; where the product codes X itself (up to eight rows), ring[1]: units of
+ * work in a stage, ring[2]: warps that they are dealt out to (0 elsewhere). */
+int chpl_diag_mx4_ring(int64_t features, int64_t rows, int64_t contraction, int64_t ring[3]);
 
 /* ------------------------------------------------------------------------ */
 /* HPL solver                                                                */
