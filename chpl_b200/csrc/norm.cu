@@ -39,6 +39,7 @@ constexpr int kMaxCluster = 4;
 constexpr int kClusterGroups = 4;                   // of a CTA in a cluster
 constexpr int kMaxStages = 2;                       // four: gradients of 8192 x 4096 53.8 us, not 51.7
 constexpr int kVectorBytes = 1024 * kHalves;        // of a warp's features as FP32
+constexpr int kSms = 148;                           // what launches and the workspace are laid out for
 constexpr int kSmem = 227 * 1024;                   // of an SM
 constexpr int kSmemApart = 2304;                    // of which a CTA takes, beside what it asks for, in whole lines
 
@@ -66,7 +67,7 @@ struct Shape {
 // four than of two.
 static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors, bool inputs_aligned, bool outputs_aligned, int threads)
 {
-    constexpr int kSms = 148, kNamed = 15;  // named barriers, one to a group of several warps
+    constexpr int kNamed = 15;  // named barriers, one to a group of several warps
     Shape s, best = {};
     double most = 0.0;
     int row = 0, fixed = 0, turn = 0;
@@ -1056,7 +1057,9 @@ static BackwardPlan plan(const chpl_norm_bwd& a)
     // the groups' sums are joined where the rows under way were
     p.shape.smem = std::max(p.shape.smem, count * kWarpWidth * p.shape.warps * p.shape.groups * 4);
     p.part_ld = (int)round_up((size_t)a.n, 4);
-    p.bytes = round_up((size_t)count * p.shape.units * p.part_ld * 4, 256);
+    // as many units as any launch of so many tokens has (fewer where a CTA holds several rows or shares one), so that
+    // what serves a batch serves every smaller one, wherever its operands lie
+    p.bytes = round_up((size_t)count * std::min<int64_t>(a.tokens, kSms) * p.part_ld * 4, 256);
     return p;
 }
 

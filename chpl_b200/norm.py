@@ -69,7 +69,8 @@ def backward(dh: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, norm: Norm,
              dbias: torch.Tensor | None = None, grad_dtype: torch.dtype | None = None, accumulate: bool = False, work=None, stream=None):
     """(dx, dweight, dbias) of h = N(x) from dh; dbias is None where there is no bias.  add is added to dx (the gradient that a
     skip connection brings); dx may be add or dh.  dweight and dbias are of grad_dtype: dh's type, or torch.float32;
-    accumulate adds them to the ones given."""
+    accumulate adds them to the ones given.  work: a uint8 CUDA tensor to use as workspace instead of allocating one; what
+    serves a batch serves every smaller one."""
     if stream is not None:
         with on(stream, dh.device):
             return backward(dh, x, stats, norm, add=add, need_dx=need_dx, need_dparams=need_dparams, dx=dx, dweight=dweight, dbias=dbias,
@@ -118,7 +119,7 @@ def join_backward(dr: torch.Tensor | None, dh: torch.Tensor | None, r: torch.Ten
     """Gradients of a join from those of r (None: nothing but h uses it) and of h (None where there is no pre).  r is wanted
     with pre, y with post or gate.  into gives the memory for any of them; its dx may be dr or dh.  A vector gate's and the
     norms' parameters' gradients are of grad_dtype: the tensors' type, or torch.float32; accumulate adds them to the ones
-    given.  need_*=False leaves outputs out (None)."""
+    given.  need_*=False leaves outputs out (None).  work: as backward's."""
     d = dh if dh is not None else dr
     if d is None:
         raise _lib.ChplError(_lib.CHPL_ERR_INVALID, "norm.join_backward", "neither dr nor dh")

@@ -559,6 +559,8 @@ typedef struct chpl_norm_bwd {
     void *dgate; int64_t lddgate;
     void *dpost_weight, *dpost_bias, *dpre_weight, *dpre_bias;
 } chpl_norm_bwd;
+/* The size depends on which norms, biases, gate and outputs there are, but on no address or row distance, and never falls as
+ * tokens, n or the outputs grow: a workspace for a batch serves every smaller one. */
 int chpl_norm_backward_worksize(const chpl_norm_bwd *a, size_t *work_bytes);
 /* `work`: 256-byte aligned device memory of work_bytes bytes, or NULL when none is needed */
 int chpl_norm_backward(void *stream, const chpl_norm_bwd *a, void *work, size_t work_bytes);
