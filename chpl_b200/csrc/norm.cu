@@ -1085,7 +1085,6 @@ static int check(const char* who, const chpl_norm_bwd* a, bool pointers)
         if (a->dpost_weight) CHPL_TRY(check_operand(who, "dweight of y's norm", a->dpost_weight, a->n, a->n, ge));
         if (a->dpost_bias) CHPL_TRY(check_operand(who, "dbias of y's norm", a->dpost_bias, a->n, a->n, ge));
         if (a->dgate && !a->ldgate) CHPL_TRY(check_operand(who, "dgate", a->dgate, a->n, a->n, ge));
-        // without tokens the parameters' gradients still follow from these
         if (a->join && a->gate && !a->ldgate) CHPL_TRY(check_operand(who, "gate", a->gate, a->n, a->n, 2));
     }
     if (!any) return CHPL_OK;
@@ -1192,12 +1191,13 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
     q.f32 = a.grad_type == CHPL_TYPE_F32;
     q.accumulate = a.accumulate;
     q.matrix = matrix;
+    const bool any = a.tokens > 0;  // without tokens sums of nothing, not 0 times what a gate or a weight may hold
     if (a.join) {
-        q.gate = a.gate;
+        if (any) q.gate = a.gate;
         if (!matrix) q.dgate = a.dgate;
         if (a.post.kind) {
-            q.post_w = a.post.weight;
-            q.post_b = a.post.bias;
+            if (any) q.post_w = a.post.weight;
+            if (any) q.post_b = a.post.bias;
             q.dpost_w = a.dpost_weight;
             q.dpost_b = a.dpost_bias;
         }
