@@ -486,10 +486,10 @@ PyObject* norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
     if (join) {
         b.post = norm_of(call, "post", a + 8, b.n);
         b.gate = gate_of(call, a[5], b.tokens, b.n, &b.ldgate);
-        if (b.post.kind || b.gate) b.y = call.matrix("y", a[4], call.type, b.tokens, b.n, &b.ldy).data_ptr();
+        const bool gate_wanted = given(a[5]) && PyObject_IsTrue(a[22]);
+        if (b.post.kind || gate_wanted) b.y = call.matrix("y", a[4], call.type, b.tokens, b.n, &b.ldy).data_ptr();
         if (b.post.kind) b.post_stats = statistics(call, "post_stats", a[16], b.tokens);
         rows_to("dy", PyObject_IsTrue(a[21]), a[25], dy, b.dy, b.lddy);
-        const bool gate_wanted = given(a[5]) && PyObject_IsTrue(a[22]);
         if (b.ldgate) rows_to("dgate", gate_wanted, a[26], dgate, b.dgate, b.lddgate);
         else sum_to("dgate", gate_wanted, a[26], dgate, b.dgate);
         sum_to("dpost.weight", params && b.post.kind, a[27], sums[0], b.dpost_weight);

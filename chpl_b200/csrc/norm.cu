@@ -1037,10 +1037,13 @@ struct BackwardPlan {
     size_t bytes;
 };
 
+// y, or what is left of it after its mean, is a factor of the norm's gradients and of the gate's
+static bool wants_y(const chpl_norm_bwd& a) { return a.join && (a.post.kind || a.dgate); }
+
 static BackwardPlan plan(const chpl_norm_bwd& a)
 {
     BackwardPlan p;
-    const bool vector_gate = a.dgate && a.gate && a.ldgate == 0, matrix = a.join && a.gate && a.ldgate, has_y = a.join && (a.post.kind || a.gate);
+    const bool vector_gate = a.dgate && a.gate && a.ldgate == 0, matrix = a.join && a.gate && a.ldgate, has_y = wants_y(a);
     p.sums = 0;
     if (a.join && ((a.post.kind && a.dpost_weight) || vector_gate)) p.sums |= 1;
     if (a.join && a.post.kind && (a.dpost_bias || (vector_gate && a.post.bias))) p.sums |= 2;
@@ -1101,7 +1104,7 @@ static int check(const char* who, const chpl_norm_bwd* a, bool pointers)
     if (a->dx && ((a->dx == a->dr && a->lddx != a->lddr) || (a->pre.kind && a->dx == a->dh && a->lddx != a->lddh))) { set_error("%s: dx is an input with another row distance", who); return CHPL_ERR_INVALID; }
     if (a->join) {
         if (a->gate && a->ldgate) CHPL_TRY(check_operand(who, "gate", a->gate, a->ldgate, a->n, 2));
-        if (a->post.kind || a->gate) CHPL_TRY(check_operand(who, "y", a->y, a->ldy, a->n, 2));
+        if (wants_y(*a)) CHPL_TRY(check_operand(who, "y", a->y, a->ldy, a->n, 2));
         if (a->post.kind) CHPL_TRY(check_stats(who, "statistics of y", a->post_stats, true));
         if (a->dy) CHPL_TRY(check_operand(who, "dy", a->dy, a->lddy, a->n, 2));
         if (a->dgate && a->ldgate) CHPL_TRY(check_operand(who, "dgate", a->dgate, a->lddgate, a->n, 2));
@@ -1167,7 +1170,7 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
             b.pre_stats = reinterpret_cast<const float2*>(a.pre_stats);
         }
         if (a.join) {
-            if (a.post.kind || a.gate) b.y = {a.y, a.ldy * 2};
+            if (wants_y(a)) b.y = {a.y, a.ldy * 2};
             b.gate = {a.gate, a.ldgate * 2};
             b.dy = {a.dy, a.lddy * 2, fits(a.dy, a.lddy, a.tokens)};
             if (matrix) b.dgate = {a.dgate, a.lddgate * 2, fits(a.dgate, a.lddgate, a.tokens)};

@@ -117,9 +117,9 @@ def join_backward(dr: torch.Tensor | None, dh: torch.Tensor | None, r: torch.Ten
                   need_dx: bool = True, need_dy: bool = True, need_dgate: bool = True, need_dparams: bool = True,
                   into: Joined | None = None, grad_dtype: torch.dtype | None = None, accumulate: bool = False, work=None, stream=None) -> Joined:
     """Gradients of a join from those of r (None: nothing but h uses it) and of h (None where there is no pre).  r is wanted
-    with pre, y with post or gate.  into gives the memory for any of them; its dx may be dr or dh.  A vector gate's and the
-    norms' parameters' gradients are of grad_dtype: the tensors' type, or torch.float32; accumulate adds them to the ones
-    given.  need_*=False leaves outputs out (None).  work: as backward's."""
+    with pre, y with post or where the gate's gradient is.  into gives the memory for any of them; its dx may be dr or dh.  A
+    vector gate's and the norms' parameters' gradients are of grad_dtype: the tensors' type, or torch.float32; accumulate adds
+    them to the ones given.  need_*=False leaves outputs out (None).  work: as backward's."""
     d = dh if dh is not None else dr
     if d is None:
         raise _lib.ChplError(_lib.CHPL_ERR_INVALID, "norm.join_backward", "neither dr nor dh")
@@ -179,7 +179,8 @@ class _Joined(torch.autograd.Function):
         post = None if post_weight is None else Norm(post_weight, post_bias, *kinds[0])
         pre = None if pre_weight is None else Norm(pre_weight, pre_bias, *kinds[1])
         *out, (post_stats, pre_stats) = join(x, y, post=post, gate=gate, scale=scales[0], residual_scale=scales[1], pre=pre, save=True)
-        ctx.save_for_backward(out[0] if pre else None, y if post or gate is not None else None, gate, post_weight, post_bias, pre_weight, pre_bias,
+        keep_y = post is not None or ctx.needs_input_grad[2]  # a frozen gate's gradients do without it
+        ctx.save_for_backward(out[0] if pre else None, y if keep_y else None, gate, post_weight, post_bias, pre_weight, pre_bias,
                               post_stats, pre_stats)
         ctx.how = kinds, scales
         ctx.set_materialize_grads(False)

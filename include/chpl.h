@@ -539,7 +539,8 @@ int chpl_norm_forward(void *stream, const chpl_norm_fwd *a);
  * gradient of Npost at y from Do * gate.  The norms' weights' and biases'
  * gradients and a vector gate's are sums over the tokens, of grad_type (`type`,
  * or CHPL_TYPE_F32), added to what they hold where accumulate != 0; a matrix
- * gate's gradient is of `type`.  Every output may be NULL (not computed).  dx
+ * gate's gradient is of `type`.  Every output may be NULL (not computed); dh and
+ * r are wanted with a norm of the sum, y with a norm of y or with dgate.  dx
  * may be dr or dh (same pointer and ld); no other output may overlap an input.
  * tokens = 0 gives sums of 0 (unchanged if accumulating).
  */
