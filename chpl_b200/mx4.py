@@ -40,7 +40,8 @@ class Mx4(NamedTuple):
 
 
 def pack(x: torch.Tensor, out: Mx4 | None = None, stream=None) -> Mx4:
-    """x (rows x cols, BF16, F16 or FP32) in 4 bits, on torch's current stream or on `stream`."""
+    """x (rows x cols, BF16, F16 or FP32) in 4 bits, on torch's current stream or on `stream`.  out gives the memory; what is
+    returned is in it and of x's type, out itself where that is its type already."""
     if stream is not None:
         with on(stream, x.device):
             return pack(x, out)
@@ -48,7 +49,7 @@ def pack(x: torch.Tensor, out: Mx4 | None = None, stream=None) -> Mx4:
         if out.shape != x.shape:
             raise _lib.ChplError(_lib.CHPL_ERR_INVALID, "mx4.pack", f"out is {tuple(out.shape)}, x {tuple(x.shape)}")
         _ops.mx4_pack(x, out.codes, out.scales)
-        return out
+        return out if out.dtype is x.dtype else out._replace(dtype=x.dtype)
     return Mx4(*_ops.mx4_pack(x, None, None), x.shape[1], x.dtype)
 
 
