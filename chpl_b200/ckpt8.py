@@ -47,13 +47,14 @@ def on(stream, device: torch.device):
 
 
 def pack(x: torch.Tensor, out: Ckpt8 | None = None, stream=None) -> Ckpt8:
-    """The checkpoint of x (rows x cols), on torch's current stream or on `stream`."""
+    """The checkpoint of x (rows x cols), on torch's current stream or on `stream`.  out gives the memory; what is returned is
+    in it and of x's type, out itself where that is its type already."""
     if stream is not None:
         with on(stream, x.device):
             return pack(x, out)
     if out is not None:
         _ops.ckpt8_pack(x, out.codes, out.scales)
-        return out
+        return out if out.dtype is x.dtype else out._replace(dtype=x.dtype)
     return Ckpt8(*_ops.ckpt8_pack(x, None, None), x.dtype)
 
 

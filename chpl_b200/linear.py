@@ -48,7 +48,7 @@ def forward(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, 
     if how == 2:
         codes, scales = (None, None) if z is None else (z.codes, z.scales)
         y, codes, scales = _ops.linear_forward(x, w, bias, residual, code, how, out, None, codes, scales, work)
-        return y, Ckpt8(codes, scales, x.dtype) if z is None else z
+        return y, Ckpt8(codes, scales, x.dtype) if z is None else z if z.dtype is x.dtype else z._replace(dtype=x.dtype)
     return _ops.linear_forward(x, w, bias, residual, code, how, out, z, None, None, work)
 
 
