@@ -66,12 +66,12 @@ def linear(x, w: Mx4, bias: torch.Tensor | None = None, *, residual: torch.Tenso
     """act(Q(x) w^T + bias) + residual, of x's type.  x: tokens x k in BF16 or F16, coded by this call, or an Mx4 of such a
     tensor.  out may give the memory for the result and may be residual itself; work: a uint8 CUDA tensor to use as
     workspace instead of allocating one."""
+    if not isinstance(w, Mx4):
+        raise _lib.ChplError(_lib.CHPL_ERR_INVALID, "mx4.linear", "w is not an Mx4")
     if stream is not None:
         with on(stream, w.codes.device):
             return linear(x, w, bias, residual=residual, act=act, out=out, work=work)
     code = _choice("mx4.linear", "activation", ACTS, act)
-    if not isinstance(w, Mx4):
-        raise _lib.ChplError(_lib.CHPL_ERR_INVALID, "mx4.linear", "w is not an Mx4")
     if isinstance(x, Mx4):
         return _ops.mx4_linear(None, x.codes, x.scales, x.cols, x.dtype, w.codes, w.scales, w.cols, bias, residual, code, out, work)
     return _ops.mx4_linear(x, None, None, None, None, w.codes, w.scales, w.cols, bias, residual, code, out, work)
