@@ -159,6 +159,8 @@ SIGNATURES = {
     "chpl_norm_forward": (_int, [_vp, ctypes.POINTER(NormFwd)]),
     "chpl_norm_backward_worksize": (_int, [ctypes.POINTER(NormBwd), ctypes.POINTER(_sz)]),
     "chpl_norm_backward": (_int, [_vp, ctypes.POINTER(NormBwd), _vp, _sz]),
+    "chpl_diag_norm_forward_plan": (_int, [ctypes.POINTER(NormFwd), ctypes.POINTER(_i64)]),
+    "chpl_diag_norm_backward_plan": (_int, [ctypes.POINTER(NormBwd), ctypes.POINTER(_i64)]),
     "chpl_mx4_scale_bytes": (_int, [_i64, _i64, ctypes.POINTER(_i64)]),
     "chpl_mx4_pack": (_int, [_vp, _int, _i64, _i64, _vp, _i64, ctypes.POINTER(Mx4)]),
     "chpl_mx4_unpack": (_int, [_vp, _int, _i64, _i64, ctypes.POINTER(Mx4), _vp, _i64]),

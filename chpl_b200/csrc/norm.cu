@@ -90,7 +90,11 @@ static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors, bool
     }
     s = best;
     sizes();
-    s.groups = (int)std::max<int64_t>(1, std::min<int64_t>(s.groups, (tokens + kSms - 1) / kSms));
+    // no more groups than hold all rows at once, over the units that run at once: 74
+    // clusters of two, 33 of four (join's gradients of 148 x 5120 11.0 us, of 148 x 9216
+    // 13.8; 14.2 and 20.4 with the rows dealt out as if to 148 units, one after another)
+    const int places = linear::slots(s.cluster, 1, kSms) / s.cluster;
+    s.groups = (int)std::max<int64_t>(1, std::min<int64_t>(s.groups, (tokens + places - 1) / places));
     // fewer groups rather than one row under way
     const auto stages = [&] { return (kSmem - kSmemApart - fixed - s.groups * turn) / (s.groups * row); };
     while (s.groups > 1 && stages() < 2) --s.groups;
@@ -98,7 +102,7 @@ static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors, bool
     s.turn = fixed + s.groups * s.stages * row;
     s.smem = s.turn + s.groups * turn;
     const int64_t want = (tokens + s.groups - 1) / s.groups;
-    s.units = (int)std::min<int64_t>(want, linear::slots(s.cluster, 1, kSms) / s.cluster);
+    s.units = (int)std::min<int64_t>(want, places);
     return s;
 }
 
@@ -989,24 +993,39 @@ static int launch(cudaStream_t st, const A& a, const Shape& s)
     return launch_kernel(KERNEL, (int64_t)s.units * s.cluster, 32 * s.warps * s.groups, s.smem, s.cluster, st, a, s);
 }
 
+// what a forward call is launched as
+struct ForwardPlan {
+    Shape shape;
+    bool in;  // rows that 16-byte accesses fit
+};
+
+static ForwardPlan plan(const chpl_norm_fwd& a)
+{
+    const bool post = a.join && a.post.kind, matrix = a.join && a.gate && a.ldgate;
+    ForwardPlan p;
+    p.in = fits(a.x, a.ldx, a.tokens) && (!a.join || fits(a.y, a.ldy, a.tokens)) && (!matrix || fits(a.gate, a.ldgate, a.tokens));
+    const bool out = (!a.join || fits(a.r, a.ldr, a.tokens)) && (!a.pre.kind || fits(a.h, a.ldh, a.tokens));
+    const int vectors = (a.pre.kind ? 1 + (a.pre.bias != nullptr) : 0) + (post || (a.join && a.gate && !matrix) ? 1 : 0) + (post && a.post.bias ? 1 : 0);
+    p.shape = shape_for(a.tokens, a.n, a.join ? 2 + matrix : 1, vectors, p.in, out, kForwardThreads);
+    return p;
+}
+
 template <typename T>
 static int forward(cudaStream_t st, const chpl_norm_fwd& a)
 {
+    const ForwardPlan p = plan(a);
     Forward f = {};
     f.tokens = (uint32_t)a.tokens;
     f.n = (int)a.n;
     f.scale = a.scale;
     f.residual_scale = a.residual_scale;
     f.x = {a.x, a.ldx * 2};
-    bool in = fits(a.x, a.ldx, a.tokens), out = true;
     if (a.join) {
         f.post = a.post.kind;
         f.post_eps = a.post.eps;
         f.y = {a.y, a.ldy * 2};
         f.gate = {a.gate, a.ldgate * 2};
         f.r = {a.r, a.ldr * 2, fits(a.r, a.ldr, a.tokens)};
-        in = in && fits(a.y, a.ldy, a.tokens) && (a.ldgate == 0 || fits(a.gate, a.ldgate, a.tokens));
-        out = f.r.aligned;
         if (f.post) {
             f.post_w = a.post.weight;
             f.post_b = a.post.bias;
@@ -1020,12 +1039,9 @@ static int forward(cudaStream_t st, const chpl_norm_fwd& a)
         f.pre_b = a.pre.bias;
         f.h = {a.h, a.ldh * 2, fits(a.h, a.ldh, a.tokens)};
         f.pre_stats = reinterpret_cast<float2*>(a.pre_stats);
-        out = out && f.h.aligned;
     }
-    const int vectors = (f.pre_w ? 1 : 0) + (f.pre_b ? 1 : 0) + (a.join && (f.post || (a.gate && a.ldgate == 0)) ? 1 : 0) + (f.post_b ? 1 : 0);
-    const Shape s = shape_for(a.tokens, a.n, a.join ? 2 + (a.gate && a.ldgate) : 1, vectors, in, out, kForwardThreads);
-    if (a.join) return in ? launch<forward_kernel<T, true, true>>(st, f, s) : launch<forward_kernel<T, false, true>>(st, f, s);
-    return in ? launch<forward_kernel<T, true, false>>(st, f, s) : launch<forward_kernel<T, false, false>>(st, f, s);
+    if (a.join) return p.in ? launch<forward_kernel<T, true, true>>(st, f, p.shape) : launch<forward_kernel<T, false, true>>(st, f, p.shape);
+    return p.in ? launch<forward_kernel<T, true, false>>(st, f, p.shape) : launch<forward_kernel<T, false, false>>(st, f, p.shape);
 }
 
 // what a backward call forms
@@ -1212,6 +1228,13 @@ static int backward(cudaStream_t st, const chpl_norm_bwd& a, void* work)
     return launch_kernel(parameters_kernel<T>, (a.n + 31) / 32, 32 * std::max(1, std::min(kJoinWarps, (q.units + 3) / 4)), 0, 1, st, q);
 }
 
+static void describe(const Shape& s, int64_t plan[3])
+{
+    plan[0] = s.cluster;
+    plan[1] = s.groups;
+    plan[2] = s.units;
+}
+
 int read_clear_status(int* st)
 {
     int v = 0, z = 0;
@@ -1251,4 +1274,22 @@ extern "C" int chpl_norm_backward(void* stream, const chpl_norm_bwd* a, void* wo
     CHPL_TRY(chpl::linear::check_work("norm_backward", work, work_bytes, need));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return a->type == CHPL_TYPE_BF16 ? backward<__nv_bfloat16>(st, *a, work) : backward<__half>(st, *a, work);
+}
+
+extern "C" int chpl_diag_norm_forward_plan(const chpl_norm_fwd* a, int64_t plan[3])
+{
+    const char* who = "diag_norm_forward_plan";
+    CHPL_TRY(chpl::norm::check(who, a));
+    if (!plan || !a->tokens || !a->n) { chpl::set_error("%s: nothing to plan", who); return CHPL_ERR_INVALID; }
+    chpl::norm::describe(chpl::norm::plan(*a).shape, plan);
+    return CHPL_OK;
+}
+
+extern "C" int chpl_diag_norm_backward_plan(const chpl_norm_bwd* a, int64_t plan[3])
+{
+    const char* who = "diag_norm_backward_plan";
+    CHPL_TRY(chpl::norm::check(who, a, true));
+    if (!plan || !a->tokens || !a->n) { chpl::set_error("%s: nothing to plan", who); return CHPL_ERR_INVALID; }
+    chpl::norm::describe(chpl::norm::plan(*a).shape, plan);
+    return CHPL_OK;
 }

@@ -566,6 +566,11 @@ int chpl_norm_backward_worksize(const chpl_norm_bwd *a, size_t *work_bytes);
 /* `work`: 256-byte aligned device memory of work_bytes bytes, or NULL when none is needed */
 int chpl_norm_backward(void *stream, const chpl_norm_bwd *a, void *work, size_t work_bytes);
 
+/* Diagnostic, host only: what a call is launched as.  plan[0]: CTAs that share a row; plan[1]: rows that they hold at once;
+ * plan[2]: how many such CTAs or clusters. */
+int chpl_diag_norm_forward_plan(const chpl_norm_fwd *a, int64_t plan[3]);
+int chpl_diag_norm_backward_plan(const chpl_norm_bwd *a, int64_t plan[3]);
+
 /* ------------------------------------------------------------------------ */
 /* microscaled 4-bit floating point, and linear layers in it                 */
 /* ------------------------------------------------------------------------ */
