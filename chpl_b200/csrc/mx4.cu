@@ -140,13 +140,13 @@ int pack(cudaStream_t st, int type, int64_t rows, int64_t cols, const void* x, i
 }
 
 // the workspace: codes and scales of X, where it comes in 16 bits and is coded first
-struct Plan {
+struct CodedInput {
     size_t scales = 0, bytes = 0;
 };
 
-static Plan plan(const chpl_mx4_fwd& a)
+static CodedInput coded_input(const chpl_mx4_fwd& a)
 {
-    Plan p;
+    CodedInput p;
     if (a.x4.codes || a.tokens <= kCodedRows || a.n == 0 || a.k == 0) return p;
     p.scales = round_up((size_t)(a.tokens * code_bytes(a.k)), 256);
     p.bytes = p.scales + round_up((size_t)scale_bytes(a.tokens, a.k), 256);
@@ -211,7 +211,7 @@ extern "C" int chpl_mx4_linear_worksize(const chpl_mx4_fwd* a, size_t* work_byte
     using namespace chpl::mx4;
     CHPL_TRY(check("mx4_linear_worksize", a, false));
     if (!work_bytes) { chpl::set_error("mx4_linear_worksize: work_bytes is NULL"); return CHPL_ERR_INVALID; }
-    *work_bytes = plan(*a).bytes;
+    *work_bytes = coded_input(*a).bytes;
     return CHPL_OK;
 }
 
@@ -220,7 +220,7 @@ extern "C" int chpl_mx4_linear(void* stream, const chpl_mx4_fwd* a, void* work, 
     using namespace chpl::mx4;
     CHPL_TRY(check("mx4_linear", a, true));
     if (a->tokens == 0 || a->n == 0) return CHPL_OK;
-    const Plan p = plan(*a);
+    const CodedInput p = coded_input(*a);
     CHPL_TRY(chpl::linear::check_work("mx4_linear", work, work_bytes, p.bytes));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     chpl_mx4 x = a->x4;
