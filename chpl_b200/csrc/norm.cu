@@ -80,7 +80,7 @@ static Shape shape_for(int64_t tokens, int64_t n, int tensors, int vectors, bool
     for (s.cluster = 1; s.cluster <= kMaxCluster; s.cluster *= 2) {
         s.warps = (int)((n + kWarpWidth * s.cluster - 1) / (kWarpWidth * s.cluster));
         s.groups = threads / 32 / s.warps;
-        if (s.warps > 1) s.groups = std::min(s.groups, s.cluster > 1 ? kClusterGroups : kNamed);
+        if (s.cluster > 1 || s.warps > 1) s.groups = std::min(s.groups, s.cluster > 1 ? kClusterGroups : kNamed);
         sizes();
         if (s.groups == 0 || fixed + turn + row > kSmem - kSmemApart) continue;
         const double work = (double)s.groups * n / s.cluster * linear::slots(s.cluster, 1, kSms);

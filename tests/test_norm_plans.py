@@ -49,6 +49,16 @@ def test_rows_wait_only_for_room(of, join, pad):
     assert clusters >= {1, 2}
 
 
+@pytest.mark.parametrize("of", [forward, backward], ids=["forward", "backward"])
+def test_every_width_has_a_shape(of):
+    """A cluster exchanges the sums of four rows at most, and a row's warps fit into its CTAs."""
+    for n in range(1, 16385, 5):
+        for join in (0, 1):
+            cluster, rows, units = plan(of(1 << 20, n, join, n % 3))
+            assert cluster in (1, 2, 4) and (cluster == 1 or rows <= 4) and rows * -(-n // (512 * cluster)) <= (32 if of is forward else 16)
+            assert units == {1: 148, 2: 74, 4: 33}[cluster]
+
+
 def test_refusals():
     p = (ctypes.c_int64 * 3)()
     L = _lib.load()
