@@ -69,6 +69,16 @@ int check_work(const char* who, const void* work, size_t have, size_t need);
 int num_sms();
 int slots(int split, int resident, int sms);
 int fit_rows(int n, int bn, int step);
+// Estimated time in us (linear_gemm.cu says where it comes from) of `tiles` tiles of
+// bn rows, a stage of the contraction taking stage_bytes of each: by clusters of
+// `split` CTAs, one or two of them resident on an SM, and by pairs, whose stage is
+// the even CTA's with all of the rows.
+struct SplitTime {
+    double us;
+    int resident;
+};
+SplitTime split_time(int stage_bytes, int bn, int64_t tiles, int split, int kblocks, int sms);
+double pair_time(int stage_bytes, int bn, int64_t tiles, int kblocks, int sms);
 
 int read_clear_status(int* st);
 

@@ -644,6 +644,24 @@ int fit_rows(int n, int bn, int step)
     return (int)round_up((size_t)((n + tiles - 1) / tiles), (size_t)step);
 }
 
+SplitTime split_time(int stage_bytes, int bn, int64_t tiles, int split, int kblocks, int sms)
+{
+    const double ctas = (double)tiles * split, kbytes = stage_bytes / 1024.0, rest = 0.0078 * bn;
+    // CTAs on an SM, two where one each does not hold them all: the SMs that hold two are the last to end
+    const int resident = bn <= 64 && ctas > slots(split, 1, sms) ? 2 : 1, places = slots(split, resident, sms);
+    const double stage = kbytes * std::max(0.0075, 0.0085 * std::min(1.0, ctas / places));
+    return {2.26 + std::ceil(ctas / places) * (resident * ((kblocks + split - 1) / split * stage + rest) + 0.7) + (split > 1 ? 0.95 + 0.0147 * bn : 0.0),
+            resident};
+}
+
+double pair_time(int stage_bytes, int bn, int64_t tiles, int kblocks, int sms)
+{
+    const double pairs = sms / 2, kbytes = stage_bytes / 1024.0, rest = 0.0072 * bn;
+    const double stage = kbytes * std::max(0.0063, 0.0076 * std::min(1.0, tiles / pairs));
+    const double products = kblocks * std::max(stage, 0.0013 * bn);
+    return 3.1 + std::ceil(tiles / pairs) * (std::max(products, rest) + 0.42) + std::min(products, rest);
+}
+
 template <Kind KIND>
 static Plan plan_for(int m, int n, int kblocks)
 {
@@ -657,20 +675,14 @@ static Plan plan_for(int m, int n, int kblocks)
         if (size >= 2 * n && least < 1e300) break;  // half the size holds every row
         const int bn = fit_rows(n, size, unit);
         const int64_t tiles = (int64_t)((m + BM - 1) / BM) * ((n + bn - 1) / bn);
-        const double kbytes = stage_bytes<KIND>(bn) / 1024.0, rest = 0.0078 * bn;
         for (int split = 1; split <= 8 && (split == 1 || split <= kblocks); split *= 2) {
-            const double ctas = (double)tiles * split;
-            // CTAs on an SM, two where one each does not hold them all: the SMs that hold two are the last to end
-            const int resident = bn <= 64 && ctas > slots(split, 1, sms) ? 2 : 1, places = slots(split, resident, sms);
-            const double stage = kbytes * std::max(0.0075, 0.0085 * std::min(1.0, ctas / places));
-            const double t = 2.26 + std::ceil(ctas / places) * (resident * ((kblocks + split - 1) / split * stage + rest) + 0.7) +
-                             (split > 1 ? 0.95 + 0.0147 * bn : 0.0);
-            if (t < least) {
-                least = t;
+            const SplitTime e = split_time(stage_bytes<KIND>(bn), bn, tiles, split, kblocks, sms);
+            if (e.us < least) {
+                least = e.us;
                 best.pair = false;
                 best.split.bn = bn;
                 best.split.split = split;
-                best.split.stages = std::min(MAX_STAGES, (SMEM_LIMIT / resident - 2048) / stage_bytes<KIND>(bn));
+                best.split.stages = std::min(MAX_STAGES, (SMEM_LIMIT / e.resident - 2048) / stage_bytes<KIND>(bn));
             }
         }
     }
@@ -679,10 +691,7 @@ static Plan plan_for(int m, int n, int kblocks)
     for (int size = Major<KIND>::b ? ROUND : 128; size <= 256 && kblocks > 0 && n > size / 2; size += step) {
         const int bn = std::max(ROUND, fit_rows(n, size, step));
         const int64_t mt = (m + 2 * BM - 1) / (2 * BM), nt = (n + bn - 1) / bn;
-        const double pairs = sms / 2, kbytes = (A_BYTES + 2 * b_bytes<KIND>(bn / 2)) / 1024.0, rest = 0.0072 * bn;
-        const double stage = kbytes * std::max(0.0063, 0.0076 * std::min(1.0, (double)mt * nt / pairs));
-        const double products = kblocks * std::max(stage, 0.0013 * bn);
-        const double t = 3.1 + std::ceil((double)mt * nt / pairs) * (std::max(products, rest) + 0.42) + std::min(products, rest);
+        const double t = pair_time(A_BYTES + 2 * b_bytes<KIND>(bn / 2), bn, mt * nt, kblocks, sms);
         if (t < least && mt * nt < 0x7fffffff) {
             least = t;
             best.pair = true;

@@ -675,29 +675,20 @@ static Plan plan_for(int m, int n, int kblocks)
         if (n > size && size % 64) continue;        // several tiles start on multiples of 64
         const int bn = linear::fit_rows(n, size, n > size ? 64 : 16);
         const int64_t tiles = (int64_t)((m + BM - 1) / BM) * ((n + bn - 1) / bn);
-        const double kbytes = split_bytes(bn) / 1024.0, rest = 0.0078 * bn;
         for (int split = 1; split <= 8 && (split == 1 || split <= kblocks); split *= 2) {
-            const int64_t ctas = tiles * split;
-            const int resident = bn <= 64 && ctas > linear::slots(split, 1, sms) ? 2 : 1, places = linear::slots(split, resident, sms);
-            const double stage = kbytes * std::max(0.0075, 0.0085 * std::min(1.0, (double)ctas / places));
-            const double t = 2.26 + (double)((ctas + places - 1) / places) * (resident * ((kblocks + split - 1) / split * stage + rest) + 0.7) +
-                             (split > 1 ? 0.95 + 0.0147 * bn : 0.0);
-            if (t < least) {
-                least = t;
+            const linear::SplitTime e = linear::split_time(split_bytes(bn), bn, tiles, split, kblocks, sms);
+            if (e.us < least) {
+                least = e.us;
                 best.pair = false;
                 best.split.bn = bn;
                 best.split.split = split;
-                best.split.stages = std::min(MAX_STAGES, (SMEM_LIMIT / resident - 2048) / split_bytes(bn));
+                best.split.stages = std::min(MAX_STAGES, (SMEM_LIMIT / e.resident - 2048) / split_bytes(bn));
             }
         }
     }
     for (int bn = 64; bn <= PAIR_MAX_BN && kblocks > 0 && n > bn / 2; bn += 64) {
         const int64_t mt = (m + 2 * BM - 1) / (2 * BM), nt = (n + bn - 1) / bn;
-        const int pairs = sms / 2;
-        const double kbytes = (A_BYTES + bn * ROW_BYTES + 3 * SCALE_BYTES) / 1024.0, rest = 0.0072 * bn;
-        const double stage = kbytes * std::max(0.0063, 0.0076 * std::min(1.0, (double)mt * nt / pairs));
-        const double products = kblocks * std::max(stage, 0.0013 * bn);
-        const double t = 3.1 + (double)((mt * nt + pairs - 1) / pairs) * (std::max(products, rest) + 0.42) + std::min(products, rest);
+        const double t = linear::pair_time(A_BYTES + bn * ROW_BYTES + 3 * SCALE_BYTES, bn, mt * nt, kblocks, sms);
         if (t < least && mt * nt < 0x7fffffff) {
             least = t;
             best.pair = true;
