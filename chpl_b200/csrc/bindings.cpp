@@ -98,7 +98,8 @@ struct Call {
         if (device.index() != c10::cuda::current_device()) guard.set_device(device);
     }
     void* stream() const { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
-    // (past the dispatcher, which costs more than the allocation)
+    // (past the dispatcher, which costs more than the allocation; a TorchDispatchMode does not see these, and
+    // torch.utils.deterministic.fill_uninitialized_memory does not fill them: every element is written by the call)
     at::Tensor empty(int64_t rows, int64_t cols, at::ScalarType t) const { return at::detail::empty_cuda({rows, cols}, t, device, c10::nullopt); }
     at::Tensor empty(int64_t n, at::ScalarType t) const { return at::detail::empty_cuda({n}, t, device, c10::nullopt); }
 

@@ -125,8 +125,11 @@ __device__ __forceinline__ void stage_products(uint32_t d, uint32_t codes_lo, ui
 //
 // CODES: X comes in 16 bits and every CTA codes its share of it itself, straight
 // into the stages, four rows' 256 features a warp at a time: up to kCodedRows rows
-// that costs less than a launch before (x 4096 x 16384: one token 8.1 us, four 7.9,
-// eight 8.9, twelve 11.1, sixteen 13.4; coded first 10.4 to 12.7).
+// that needs no workspace and no launch before.  x 4096 x 16384, weights out of HBM,
+// with GELU: one token 8.8 us, four 9.5, eight 10.8, coded first 10.2 to 10.4; x 4096
+// x 28672 (two CTAs to an SM) 13.4, 13.2 and 13.8, coded first 14.8 to 15.0.  (Five to
+// eight tokens, two units a stage, gain no GPU time on layers of up to 18944 features;
+// the host launches once.)
 //
 //   warp 0     TMA producer          warp 1    TMEM allocation, tcgen05 issue
 //   warps 2-7  CODES: X's codes and scales

@@ -501,7 +501,9 @@ int chpl_linear_backward(void *stream, const chpl_linear_bwd *a, void *work, siz
 /* N(v) = (v - m) s weight + bias, s = 1 / sqrt(mean((v - m)^2) + eps), over the
  * n features of a row; weight and bias of the operands' type, bias may be NULL.
  * Statistics are FP32: squares that add up beyond FP32 (values above some 1e18)
- * give s = 0. */
+ * give s = 0; where eps is below some 1e-37, rows of values below some 1e-19,
+ * whose squares and s^2 leave FP32, have no statistics and no gradients that mean
+ * anything. */
 typedef struct chpl_norm {
     int kind;
     float eps;
