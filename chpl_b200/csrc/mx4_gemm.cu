@@ -148,12 +148,12 @@ struct SplitShape {
 };
 
 // The units of a stage, and the warps that all units are dealt out to in order.  A
-// warp waits for a stage by the parity of its use, which tells a turn of the ring from
-// the one before but not from the one before that.  With no more warps than one turn
-// has units, a warp's next unit is at most one turn further; its last wait saw the
-// stage of a turn before that read, so the use before the last of the stage that it
-// comes to has been read, and the parity names the last one.  (Two CTAs to an SM have
-// rings of five stages: five warps for up to four rows.)
+// warp waits until a stage's last use has been read by the parity of that use, which
+// tells it from the use before, but not from the one before that.  With no more warps
+// than one turn of the ring has units, a warp's units lie at most one turn apart.
+// Stages are read in order, so what its last wait saw read covers the use before the
+// last of the stage that it comes to: the parity can only mean the last one.  (Two
+// CTAs to an SM have rings of five stages: five warps for up to four rows.)
 __host__ __device__ constexpr int code_units(int rows) { return (rows + CODE_ROWS - 1) / CODE_ROWS; }
 __host__ __device__ constexpr int code_warps(int stages, int rows)
 {
